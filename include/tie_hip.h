@@ -28,8 +28,10 @@ extern "C" {
 
 /* GGML type ids as in gguf.h:8-36 */
 #define TIE_GGML_F32 0
+#define TIE_GGML_F16 1
 #define TIE_GGML_Q4_K 12
 #define TIE_GGML_Q6_K 14
+#define TIE_GGML_I8 24
 #define TIE_GGML_BF16 30
 
 #define TIE_HIP_OK 0
@@ -226,6 +228,135 @@ void tie_hip_matrix_destroy(tie_hip_matrix *m);
  * TIE_HIP_PATH_MFMA on an unsupported matrix is an error.  Enqueued on `stream`.  The attention projections, the dense FFN and the LM
  * head of transformer_layer_qwen3 / main.c use it. */
 int tie_hip_mat_mat(tie_hip_matrix *m, const float *x_dev, int T, float *out_dev, int flags, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* The attention half for drafted tokens: a paged key/value cache        */
+/* ------------------------------------------------------------------ */
+/* What lies between a layer's projections (tie_hip_mat_mat) and its FFN half
+ * (tie_hip_moe_forward_residual), and behind the LM head: the norms of queries
+ * and keys for each head, the rotation and the cache write (tie_hip_kv_append),
+ * the attention of a tree of drafted tokens, a prompt's chunk or single tokens
+ * (tie_hip_tree_attention), the accepted path (tie_hip_verify_tree) and its
+ * rows (tie_hip_kv_keep).  Everything is on device pointers, enqueued on
+ * `stream` (NULL: the library stream) and captures into HIP graphs.  No call
+ * here reproduces TIE's arithmetic bit for bit: they are held to 64-bit
+ * results (F32 outputs to about 1e-6 relative).
+ *
+ * The caller owns the cache's memory, in pages of TIE_HIP_PAGE_ROWS rows (a
+ * row: one token) that the layers share the numbering of:
+ *   k  [n_layers][n_pages][kv_heads][64][head_dim]
+ *   v  [n_layers][n_pages][kv_heads][head_dim][64]
+ * as f16, or as int8 codes with F32 scales [n_layers][n_pages][kv_heads][64]
+ * (value = code * scale; scale = largest magnitude of the row's head / 127,
+ * code = the nearest whole number to value / scale, ties to even).  Values
+ * beyond the f16 range are held as the largest f16; an int8 row with a value
+ * that is not finite has scale NaN.  Pages need no clearing. */
+#define TIE_HIP_PAGE_ROWS 64
+
+typedef struct tie_hip_kv_cache {
+	int type;     /* TIE_GGML_F16 or TIE_GGML_I8 */
+	int n_layers; /* layers in the arrays */
+	int n_pages;  /* pages of a layer */
+	int kv_heads;
+	int head_dim; /* 64 or 128 */
+	void *k, *v;  /* 16-byte aligned */
+	float *k_scale, *v_scale; /* TIE_GGML_I8; else NULL */
+} tie_hip_kv_cache;
+
+/* The sequences of a call, as device arrays.  Sequence b has `len[b]` rows in
+ * the cache (committed: every token of it sees them) and the token rows
+ * first[b] .. first[b + 1] - 1 of the activations; its token j is cache row
+ * len[b] + j, on page pages[b][(len[b] + j) / 64].  Rows that belong to no
+ * sequence are left as they are.  The arrays are read on the device, so no call
+ * can refuse what they say; it is checked there: where a length, a range of
+ * rows or a page lies outside the call's sizes, nothing is written to the
+ * cache, and the outputs that would need it are NaN. */
+typedef struct tie_hip_kv_seqs {
+	int n_seqs;           /* at most 65535 */
+	int max_pages;        /* columns of the page table */
+	int n_tokens;         /* token rows of the activations */
+	const int32_t *pages; /* [n_seqs][max_pages] */
+	const int32_t *len;   /* [n_seqs] */
+	const int32_t *first; /* [n_seqs + 1], ascending; NULL: one token for each sequence */
+} tie_hip_kv_seqs;
+
+/* Norm, rotation and cache write of the sequences' tokens in one layer, one
+ * launch.  q, k, v: F32 rows of the projections, `*_stride` floats from a
+ * token to the next (all three may lie in one matrix); q has n_heads heads (a
+ * multiple of kv_heads), k and v kv_heads.
+ *   norm      x * w / sqrt(mean(x^2) + eps) over each head, q_norm and k_norm
+ *             F32 [head_dim] (NULL: none)
+ *   rotation  the pair (x[i], x[i + head_dim / 2]) by pos * theta^(-2 i /
+ *             head_dim); pos [n_tokens] (a tree's nodes at one depth share a
+ *             position), NULL: the token's cache row
+ * in 64 bits, rounded once.  The queries go to q_out (which may be q, with the
+ * same stride), keys and values to the cache. */
+int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q, size_t q_stride,
+		      const float *k, size_t k_stride, const float *v, size_t v_stride, int n_heads, const float *q_norm,
+		      const float *k_norm, float eps, float theta, const int32_t *pos, float *q_out, size_t q_out_stride,
+		      void *stream);
+
+/* The cache rows of the sequences' tokens as F32, of n_layers layers from
+ * `layer` on: k_out and v_out [n_layers][n_tokens][kv_heads][head_dim].  (len
+ * of zeros and first over whole lengths reads whole sequences.) */
+int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_layers, const tie_hip_kv_seqs *seqs, float *k_out,
+		    float *v_out, void *stream);
+
+/* Attention of the sequences' tokens over their committed rows and, of their
+ * own tokens, those that `mask` names: bit j % 64 of mask[t][j / 64] says that
+ * token row t sees token j of its sequence ([n_tokens][mask_words]; tokens past
+ * the words are not seen).  mask NULL: token i sees tokens 0 .. i (a prompt's
+ * chunk, a chain, a single token).  A row that sees nothing gives 0.
+ *   q    [n_tokens] rows of n_heads heads (as tie_hip_kv_append leaves them)
+ *   out  the same shape (may be q, with the same stride)
+ *   work work_bytes of device memory, 16-byte aligned, at least
+ *        tie_hip_tree_attention_work_bytes; NULL: the stream's workspace, which
+ *        all calls on the stream share and which grows as needed, but not
+ *        during HIP graph capture (run the largest call once before, or pass
+ *        memory).  Graphs that may run at the same time need memory of their own.
+ * A row's result is the same whatever else the call holds only up to F32
+ * rounding: how the rows are cut follows the lengths.  Two equal calls give
+ * equal bits. */
+size_t tie_hip_tree_attention_work_bytes(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, int n_heads);
+int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
+			   size_t q_stride, int n_heads, float scale, const uint64_t *mask, int mask_words, float *out,
+			   size_t out_stride, void *work, size_t work_bytes, void *stream);
+
+/* Keep the accepted path of each sequence: cache row len + path[b][j] becomes
+ * row len + j for j < n_keep[b], in all layers, and len_out[b] = len[b] +
+ * n_keep[b] (len_out may be len; NULL: not wanted).  path [n_seqs][max_path]
+ * holds tokens of the sequence, ascending; an entry that does not ascend or
+ * is no token of it ends the path there. */
+int tie_hip_kv_keep(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, const int32_t *path, int max_path,
+		    const int32_t *n_keep, int32_t *len_out, void *stream);
+
+/* Which drafted tokens the target accepts, and the token after them, so that
+ * tokens follow the target's distribution whatever the draft proposed.  Token
+ * rows first[b] .. first[b + 1] - 1 are a tree: row 0 of a sequence is its root
+ * (a token that already stands), parent[t] the node's parent as an index in its
+ * sequence (below its own; -1: none, the root), tokens[t] its token.
+ *   logits    [n_tokens] rows of `vocab` (the LM head's, for each node)
+ *   draft     [n_tokens] rows of `vocab`: the distribution that a node's
+ *             children were drawn from, each on its own; NULL: proposed without
+ *             probabilities (looked up, or a draft's best)
+ *   u_accept, u_sample  F32 [n_tokens] random numbers in [0, 1): for taking the
+ *             node, and for the token after it
+ * With p = softmax(logits / temperature) of a node and q its draft row, its
+ * first max_children children are tried in order: child x is taken when
+ * u_accept q(x) M < max(0, p(x) - c q(x)) (c = 0, M = 1 at first); otherwise c
+ * += M and M = sum of max(0, p - c q).  Without draft rows: taken when u_accept M
+ * < p(x); otherwise x leaves p, and M is what is left.  Where no child is taken, or
+ * the path holds max_path nodes, next[b] is the first token whose running sum of
+ * the residual (at the path's full length: of p) exceeds u_sample times the
+ * whole.  temperature 0: the largest logit (the lowest of equals) alone counts.
+ *   path   [n_seqs][max_path] accepted nodes, the root first; -1 behind them
+ *   n_keep [n_seqs] how many; next [n_seqs] (0 and -1 for a sequence of no rows)
+ * All sums in 64 bits.  work as for tie_hip_tree_attention. */
+size_t tie_hip_verify_tree_work_bytes(int vocab, int n_tokens, int max_children, int with_draft);
+int tie_hip_verify_tree(const float *logits, size_t logits_stride, const float *draft, size_t draft_stride, int vocab,
+			int n_seqs, int n_tokens, const int32_t *first, const int32_t *tokens, const int32_t *parent,
+			const float *u_accept, const float *u_sample, float temperature, int max_children, int max_path,
+			int32_t *path, int32_t *n_keep, int32_t *next, void *work, size_t work_bytes, void *stream);
 
 /* ------------------------------------------------------------------ */
 /* GGUF models: every MoE layer uploaded once                           */

@@ -1,0 +1,193 @@
+"""Acceptance of drafted tokens and the token after them, against a plain
+64-bit form: whole numbers, so equal.  (The kernels' sums and the form's are
+both in 64 bits; a random number within 1e-12 of a border would fall on either
+side, and none of these does.)"""
+import numpy as np
+import pytest
+
+import kv_ref
+import tie_amd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    import torch
+    assert torch.cuda.is_available(), "GPU test without a GPU"
+    tie_amd.init(0)
+    yield
+    tie_amd.shutdown()
+
+
+def cuda(x):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(x)).cuda()
+
+
+class Case:
+    def __init__(self, seed, counts, V, draft, branch=2, peaked=2.5, parent=None, off=0.7):
+        rng = np.random.default_rng(seed)
+        self.counts, self.V = counts, V
+        N = sum(counts)
+        self.logits = (rng.standard_normal((N, V)) * peaked).astype(np.float32)
+        d = self.logits + off * rng.standard_normal((N, V)).astype(np.float32)
+        d = np.exp(d - d.max(1, keepdims=True))
+        d = (d / d.sum(1, keepdims=True)).astype(np.float32)
+        self.parent = np.concatenate([parent or [(j - 1) // branch for j in range(n)] for n in counts] + [[]]).astype(np.int32)
+        self.first = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        self.tokens = np.zeros(N, np.int32)
+        t0 = 0
+        for n in counts:
+            for j in range(n):
+                row = d[t0 + max(0, self.parent[t0 + j])].astype(np.float64)
+                self.tokens[t0 + j] = rng.choice(V, p=row / row.sum())
+            t0 += n
+        self.draft = d if draft else None
+        self.ua, self.us = rng.random(N).astype(np.float32), rng.random(N).astype(np.float32)
+
+    def want(self, temperature, kids, most):
+        paths, n, nxt = np.full((len(self.counts), most), -1, np.int32), [], []
+        for b in range(len(self.counts)):
+            s = slice(self.first[b], self.first[b + 1])
+            if s.stop == s.start:
+                n.append(0)
+                nxt.append(-1)
+                continue
+            p, x = kv_ref.verify(self.logits[s], self.draft[s] if self.draft is not None else None, self.tokens[s],
+                                 self.parent[s], self.ua[s], self.us[s], temperature, kids, most)
+            paths[b, : len(p)] = p
+            n.append(len(p))
+            nxt.append(x)
+        return paths, np.array(n, np.int32), np.array(nxt, np.int32)
+
+    def run(self, temperature, kids, most, stride=0, **kw):
+        import torch
+        N, V = self.logits.shape
+        def rows(x):
+            if x is None:
+                return None
+            b = torch.full((N, V + stride), float("nan"), device="cuda")
+            b[:, :V] = cuda(x)
+            return b[:, :V]
+        B = len(self.counts)
+        path = torch.full((B, most), 99, dtype=torch.int32, device="cuda")
+        n, nxt = (torch.full((B,), 99, dtype=torch.int32, device="cuda") for _ in range(2))
+        args = [rows(self.logits), cuda(self.first), cuda(self.tokens), cuda(self.parent), cuda(self.ua), cuda(self.us)]
+        d = rows(self.draft)
+        torch.cuda.synchronize()
+        tie_amd.verify_tree(*args, path, n, nxt, temperature=temperature, draft=d, max_children=kids, **kw)
+        torch.cuda.synchronize()
+        return path.cpu().numpy(), n.cpu().numpy(), nxt.cpu().numpy()
+
+    def check(self, temperature, kids, most, **kw):
+        for g, w, what in zip(self.run(temperature, kids, most, **kw), self.want(temperature, kids, most), ("path", "n_keep", "next")):
+            np.testing.assert_array_equal(g, w, what)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("temperature", [0.0, 0.3, 1.0, 5.0])
+@pytest.mark.parametrize("V", [1, 2, 64, 4096, 4097, 32001])
+def test_trees(draft, temperature, V):
+    for seed in range(4):
+        Case(seed, [5, 1, 13, 8], V, draft, branch=1 + seed % 3).check(temperature, 3, 13, stride=seed % 2 * 3)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_large_vocabulary(draft):
+    Case(3, [9, 7], 151936, draft, branch=2).check(0.8, 2, 9)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_many_children_and_cut_paths(draft):
+    """16 children of one node, fewer tried than there are, paths cut at the
+    outputs' depth, sequences of one node and of none, siblings of one token."""
+    c = Case(11, [17, 0, 1, 40], 300, draft, branch=16)
+    for kids in (1, 2, 16):
+        for most in (1, 2, 5):
+            c.check(0.9, kids, most)
+    c = Case(12, [20, 20], 50, draft, branch=4, peaked=0.5)
+    c.tokens[1:5] = c.tokens[1]
+    c.tokens[21:25] = 7
+    for s in range(6):
+        c.ua[:] = np.random.default_rng(s).random(40).astype(np.float32)
+        c.check(1.0, 4, 6)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_long_chains(draft):
+    c = Case(13, [150, 70], 97, draft, branch=1, off=0.05)
+    c.ua[:] *= 0.2  # most are taken
+    c.check(1.0, 1, 200)
+    c.ua[:] = 0.0  # all whose probability is not 0 are
+    c.check(1.0, 1, 200)
+    assert c.run(1.0, 1, 200)[1].tolist() == [150, 70]
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_random_numbers_at_their_ends(draft):
+    """0 and the largest below 1, logits of minus infinity, tokens that are
+    none, equal largest logits."""
+    c = Case(14, [7, 7, 7], 5000, draft, branch=2)
+    c.logits[:, 100:4500] = -np.inf
+    c.logits[3, :] = -np.inf
+    c.logits[3, 4999] = 1.0
+    c.logits[:, 7] = c.logits[:, 4700] = 20.0
+    c.tokens[2], c.tokens[9] = -1, 5000
+    for a in (0.0, 1 - 2.0 ** -24):
+        for s in (0.0, 1 - 2.0 ** -24):
+            c.ua[:], c.us[:] = a, s
+            c.check(0.7, 2, 7)
+            c.check(0.0, 2, 7)
+
+
+def test_tokens_follow_the_target():
+    """The first token after the root over many draws has the target's
+    distribution, whatever the draft's: counts of 8 tokens in 20000 draws
+    within 5 standard deviations."""
+    V, n = 8, 20000
+    rng = np.random.default_rng(15)
+    logits = rng.standard_normal(V).astype(np.float32) * 1.5
+    q = np.exp(rng.standard_normal(V) * 1.5)
+    q = (q / q.sum()).astype(np.float32)
+    c = Case(16, [3] * n, V, True, parent=[-1, 0, 0])
+    c.logits[:], c.draft[:] = logits, q
+    c.tokens[:] = rng.choice(V, size=3 * n, p=q.astype(np.float64) / q.astype(np.float64).sum())
+    p = np.exp(logits.astype(np.float64))
+    p /= p.sum()
+    for draft in (c.draft, None):
+        c.draft = draft
+        path, kept, nxt = c.run(1.0, 2, 2)
+        first = np.where(kept == 2, c.tokens[3 * np.arange(n) + np.clip(path[:, 1], 0, 2)], nxt)
+        got = np.bincount(first, minlength=V)
+        assert (np.abs(got - n * p) <= 5 * np.sqrt(n * p * (1 - p))).all(), (got, n * p)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_repeats_work_streams_and_graphs(draft):
+    import torch
+    c = Case(17, [9, 12], 20000, draft, branch=3)
+    want = c.want(0.8, 3, 12)
+    need = tie_amd.verify_tree_work_bytes(20000, 21, 3, draft)
+    work = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    for kw in ({}, dict(work=work), dict(stream=torch.cuda.Stream().cuda_stream)):
+        for g, w in zip(c.run(0.8, 3, 12, **kw), want):
+            np.testing.assert_array_equal(g, w)
+    with pytest.raises(tie_amd.TieError):
+        c.run(0.8, 3, 12, work=work[: need - 16])
+    args = [cuda(x) for x in (c.logits, c.first, c.tokens, c.parent, c.ua, c.us)]
+    d = cuda(c.draft) if draft else None
+    path, n, nxt = torch.zeros(2, 12, dtype=torch.int32, device="cuda"), *(torch.zeros(2, dtype=torch.int32, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        tie_amd.verify_tree(*args, path, n, nxt, temperature=0.8, draft=d, max_children=3, work=work,
+                            stream=torch.cuda.current_stream().cuda_stream)
+    for rep in range(3):
+        path.zero_()
+        n.zero_()
+        nxt.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        for a, w in zip((path, n, nxt), want):
+            np.testing.assert_array_equal(a.cpu().numpy(), w, str(rep))

@@ -16,6 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TIE_AMD_LIB") or os.path.join(HERE, "libtie_hip.so")
 
 F32, Q4_K, Q6_K, BF16 = 0, 12, 14, 30
+F16, I8 = 1, 24  # cache types
+PAGE_ROWS = 64
 OK, EINVAL, EHIP, ENOMEM, ENOINIT = 0, -1, -2, -3, -4
 PATH_AUTO, PATH_EXACT, PATH_MFMA = 0, 1, 2
 ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
@@ -32,6 +34,8 @@ EXPORTS = (
     "tie_hip_debug_fail_alloc", "tie_hip_host_expf", "tie_hip_profile_enable", "tie_hip_profile_read",
     "tie_hip_moe_forward_noalloc", "tie_hip_stream_status", "tie_hip_debug_decode_give_up", "tie_hip_debug_decode_form",
     "tie_hip_stream_release", "tie_hip_debug_layer_shifts",
+    "tie_hip_kv_append", "tie_hip_kv_read", "tie_hip_kv_keep", "tie_hip_tree_attention",
+    "tie_hip_tree_attention_work_bytes", "tie_hip_verify_tree", "tie_hip_verify_tree_work_bytes",
 )
 
 
@@ -62,6 +66,21 @@ class ModelInfo(ctypes.Structure):
         ("d", ctypes.c_int), ("F", ctypes.c_int), ("E", ctypes.c_int), ("k", ctypes.c_int),
         ("n_layers", ctypes.c_int), ("first_moe_layer", ctypes.c_int),
         ("norm_eps", ctypes.c_float), ("routing", ctypes.c_int),
+    ]
+
+
+class KVCacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int), ("n_layers", ctypes.c_int), ("n_pages", ctypes.c_int), ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+    ]
+
+
+class KVSeqsDesc(ctypes.Structure):
+    _fields_ = [
+        ("n_seqs", ctypes.c_int), ("max_pages", ctypes.c_int), ("n_tokens", ctypes.c_int),
+        ("pages", ctypes.c_void_p), ("len", ctypes.c_void_p), ("first", ctypes.c_void_p),
     ]
 
 
@@ -143,6 +162,21 @@ def lib():
         L.tie_hip_profile_enable.restype = I
         L.tie_hip_profile_read.argtypes = [ctypes.c_char_p, ctypes.c_size_t, P, P, I]
         L.tie_hip_profile_read.restype = I
+        Z, F = ctypes.c_size_t, ctypes.c_float
+        L.tie_hip_kv_append.argtypes = [P, I, P, P, Z, P, Z, P, Z, I, P, P, F, F, P, P, Z, P]
+        L.tie_hip_kv_append.restype = I
+        L.tie_hip_kv_read.argtypes = [P, I, I, P, P, P, P]
+        L.tie_hip_kv_read.restype = I
+        L.tie_hip_kv_keep.argtypes = [P, P, P, I, P, P, P]
+        L.tie_hip_kv_keep.restype = I
+        L.tie_hip_tree_attention.argtypes = [P, I, P, P, Z, I, F, P, I, P, Z, P, Z, P]
+        L.tie_hip_tree_attention.restype = I
+        L.tie_hip_tree_attention_work_bytes.argtypes = [P, P, I]
+        L.tie_hip_tree_attention_work_bytes.restype = Z
+        L.tie_hip_verify_tree.argtypes = [P, Z, P, Z, I, I, I, P, P, P, P, P, F, I, I, P, P, P, P, Z, P]
+        L.tie_hip_verify_tree.restype = I
+        L.tie_hip_verify_tree_work_bytes.argtypes = [I, I, I, I]
+        L.tie_hip_verify_tree_work_bytes.restype = Z
         _lib = L
     return _lib
 
@@ -421,3 +455,134 @@ class Layer:
             self.close()
         except Exception:
             pass
+
+
+def _rows(a, what, width=None):
+    """(pointer, row stride, values of a row) of F32 rows: a 2-D tensor, or one
+    of [rows][heads][head_dim] whose rows are contiguous."""
+    st, sh = a.stride(), a.shape
+    if str(a.dtype) != "torch.float32" or len(sh) not in (2, 3):
+        raise ValueError("%s: rows of float32 values are wanted (got %s, %d dimensions)" % (what, a.dtype, len(sh)))
+    n = sh[1] if len(sh) == 2 else sh[1] * sh[2]
+    inner = (st[-1] == 1 or sh[-1] == 1) and (len(sh) == 2 or st[1] == sh[2] or sh[1] == 1)
+    if not inner or (width is not None and n != width):
+        raise ValueError("%s: rows of %s contiguous values are wanted (got shape %s, strides %s)" % (what, width or "", tuple(sh), st))
+    return a.data_ptr(), (st[0] if sh[0] > 1 else max(n, st[0])), n
+
+
+def _array(a, dtype, shape, what):
+    """The pointer of a contiguous device array of this type and shape (None for None)."""
+    if a is None:
+        return None
+    if str(a.dtype) != "torch." + dtype or tuple(a.shape) != tuple(shape) or not a.is_contiguous():
+        raise ValueError("%s: a contiguous %s array of shape %s is wanted (got %s, %s)" % (what, dtype, tuple(shape), a.dtype,
+                                                                                           tuple(a.shape)))
+    return a.data_ptr()
+
+
+class KVSeqs:
+    """The sequences of a call (tie_hip_kv_seqs): device int32 tensors `pages`
+    [n_seqs][max_pages], `lens` [n_seqs] and `first` [n_seqs + 1] (None: one
+    token each), read when the kernels run; n_tokens rows of activations."""
+
+    def __init__(self, pages, lens, first=None, n_tokens=None):
+        n_seqs, max_pages = pages.shape
+        if n_tokens is None:
+            n_tokens = n_seqs if first is None else int(first[-1])
+        self.n_seqs, self.n_tokens, self.keep = n_seqs, n_tokens, (pages, lens, first)
+        self.desc = KVSeqsDesc(n_seqs, max_pages, n_tokens, _array(pages, "int32", pages.shape, "pages"),
+                               _array(lens, "int32", (n_seqs,), "lens"), _array(first, "int32", (n_seqs + 1,), "first"))
+        self.ref = ctypes.byref(self.desc)
+
+
+class KVCache:
+    """A paged cache in the caller's tensors (tie_hip_kv_cache): k [n_layers]
+    [n_pages][kv_heads][64][head_dim] and v [n_layers][n_pages][kv_heads]
+    [head_dim][64], float16, or int8 with float32 scales [n_layers][n_pages]
+    [kv_heads][64]."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        kind = {"torch.float16": F16, "torch.int8": I8}.get(str(k.dtype))
+        if kind is None or len(k.shape) != 5 or k.shape[3] != PAGE_ROWS:
+            raise ValueError("k: [layers][pages][kv heads][%d][head_dim] of float16 or int8 is wanted (got %s, %s)"
+                             % (PAGE_ROWS, k.dtype, tuple(k.shape)))
+        nl, npg, kvh, _, hd = k.shape
+        name = str(k.dtype)[6:]
+        if kind == I8 and (k_scale is None or v_scale is None):
+            raise ValueError("an int8 cache needs k_scale and v_scale")
+        self.kv_heads, self.head_dim, self.n_layers, self.keep_alive = kvh, hd, nl, (k, v, k_scale, v_scale)
+        self.desc = KVCacheDesc(kind, nl, npg, kvh, hd, _array(k, name, k.shape, "k"),
+                                _array(v, name, (nl, npg, kvh, hd, PAGE_ROWS), "v"),
+                                _array(k_scale, "float32", k.shape[:4], "k_scale"),
+                                _array(v_scale, "float32", k.shape[:4], "v_scale"))
+        self.ref = ctypes.byref(self.desc)
+
+    def _heads(self, width, what):
+        if width % self.head_dim:
+            raise ValueError("%s: rows of %d values are no whole heads of %d" % (what, width, self.head_dim))
+        return width // self.head_dim
+
+    def _q(self, q, out, seqs, what):
+        pq, sq, w = _rows(q, "q")
+        po, so, _ = _rows(out, what, w)
+        if q.shape[0] < seqs.n_tokens or out.shape[0] < seqs.n_tokens:
+            raise ValueError("q/%s: %d rows are wanted (got %d, %d)" % (what, seqs.n_tokens, q.shape[0], out.shape[0]))
+        return pq, sq, po, so, self._heads(w, "q")
+
+    def append(self, layer, seqs, q, k, v, q_out, pos=None, q_norm=None, k_norm=None, eps=1e-6, theta=1e6, stream=None):
+        """tie_hip_kv_append: norm and rotation of q and k, cache write of k and v."""
+        pq, sq, po, so, heads = self._q(q, q_out, seqs, "q_out")
+        w = self.kv_heads * self.head_dim
+        pk, sk, _ = _rows(k, "k", w)
+        pv, sv, _ = _rows(v, "v", w)
+        if min(k.shape[0], v.shape[0]) < seqs.n_tokens:
+            raise ValueError("k/v: %d rows are wanted" % seqs.n_tokens)
+        check(lib().tie_hip_kv_append(self.ref, layer, seqs.ref, pq, sq, pk, sk, pv, sv, heads,
+                                      _array(q_norm, "float32", (self.head_dim,), "q_norm"),
+                                      _array(k_norm, "float32", (self.head_dim,), "k_norm"), eps, theta,
+                                      _array(pos, "int32", (seqs.n_tokens,), "pos"), po, so, stream))
+
+    def read(self, seqs, k_out, v_out, layer=0, n_layers=1, stream=None):
+        """tie_hip_kv_read: rows of the cache as float32 [n_layers][n_tokens][kv_heads][head_dim]."""
+        shape = (n_layers, seqs.n_tokens, self.kv_heads, self.head_dim)
+        check(lib().tie_hip_kv_read(self.ref, layer, n_layers, seqs.ref, _array(k_out, "float32", shape, "k_out"),
+                                    _array(v_out, "float32", shape, "v_out"), stream))
+
+    def attention(self, layer, seqs, q, out, scale, mask=None, work=None, stream=None):
+        """tie_hip_tree_attention; mask: int64 [n_tokens][words] (bit patterns), None: causal; work: a uint8 tensor."""
+        pq, sq, po, so, heads = self._q(q, out, seqs, "out")
+        words = 0 if mask is None else mask.shape[1]
+        check(lib().tie_hip_tree_attention(self.ref, layer, seqs.ref, pq, sq, heads, scale,
+                                           _array(mask, "int64", (seqs.n_tokens, words), "mask"), words, po, so, _p(work),
+                                           0 if work is None else work.numel() * work.element_size(), stream))
+
+    def attention_work_bytes(self, seqs, n_heads):
+        return lib().tie_hip_tree_attention_work_bytes(self.ref, seqs.ref, n_heads)
+
+    def keep(self, seqs, path, n_keep, len_out=None, stream=None):
+        """tie_hip_kv_keep: the accepted paths' rows moved down in every layer."""
+        check(lib().tie_hip_kv_keep(self.ref, seqs.ref, _array(path, "int32", (seqs.n_seqs, path.shape[1]), "path"),
+                                    path.shape[1], _array(n_keep, "int32", (seqs.n_seqs,), "n_keep"),
+                                    _array(len_out, "int32", (seqs.n_seqs,), "len_out"), stream))
+
+
+def verify_tree_work_bytes(vocab, n_tokens, max_children, with_draft):
+    return lib().tie_hip_verify_tree_work_bytes(vocab, n_tokens, max_children, int(with_draft))
+
+
+def verify_tree(logits, first, tokens, parent, u_accept, u_sample, path, n_keep, next_token, temperature=1.0, draft=None,
+                max_children=1, work=None, stream=None):
+    """tie_hip_verify_tree: the accepted path [n_seqs][max_path], its length and the next token of each sequence."""
+    n, n_seqs = tokens.shape[0], n_keep.shape[0]
+    pl, sl, vocab = _rows(logits, "logits")
+    pd, sd, _ = (None, 0, 0) if draft is None else _rows(draft, "draft", vocab)
+    if logits.shape[0] < n or (draft is not None and draft.shape[0] < n):
+        raise ValueError("logits/draft: %d rows are wanted" % n)
+    check(lib().tie_hip_verify_tree(pl, sl, pd, sd, vocab, n_seqs, n, _array(first, "int32", (n_seqs + 1,), "first"),
+                                    _array(tokens, "int32", (n,), "tokens"), _array(parent, "int32", (n,), "parent"),
+                                    _array(u_accept, "float32", (n,), "u_accept"),
+                                    _array(u_sample, "float32", (n,), "u_sample"), temperature, max_children, path.shape[1],
+                                    _array(path, "int32", (n_seqs, path.shape[1]), "path"),
+                                    _array(n_keep, "int32", (n_seqs,), "n_keep"),
+                                    _array(next_token, "int32", (n_seqs,), "next_token"), _p(work),
+                                    0 if work is None else work.numel() * work.element_size(), stream))

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <map>
 #include <string>
 #include <mutex>
@@ -13,6 +14,7 @@
 
 #include "common.h"
 #include "gguf.h"
+#include "kv.h"
 
 namespace tie {
 int set_error(int code, const char *fmt, ...);
@@ -320,9 +322,15 @@ static int ensure_workspace(hipStream_t s, int T, int k, int d, int F, int E, Wo
 		// caller chained to it) may read the old buffer: drain the device
 		HIP_TRY(hipDeviceSynchronize());
 		HIP_TRY(hipFree(w.alloc));
-		int32_t *status = w.one_status; // (a given-up wait not yet reported survives the growth)
-		w = Workspace();
-		w.one_status = status;
+		// (a given-up wait not yet reported and the attention's scratch survive
+		// the growth)
+		Workspace kept;
+		kept.one_status = w.one_status;
+		kept.aux = w.aux;
+		kept.aux_bytes = w.aux_bytes;
+		memcpy(kept.aux_old, w.aux_old, sizeof kept.aux_old);
+		kept.n_aux_old = w.n_aux_old;
+		w = kept;
 	}
 	int rc = dev_malloc(&mem, bytes, "workspace");
 	if (rc)
@@ -354,6 +362,17 @@ static int take_stream_status(hipStream_t s)
 	*st = 0;
 	return set_error(TIE_HIP_EHIP, "one-token forward: a wait between workgroups gave up (the GPU did not run "
 				       "them together); that call's outputs are NaN");
+}
+
+static void free_aux(Workspace &w)
+{
+	if (w.aux)
+		(void)hipFree(w.aux);
+	for (int i = 0; i < w.n_aux_old; i++)
+		(void)hipFree(w.aux_old[i]);
+	w.aux = nullptr;
+	w.aux_bytes = 0;
+	w.n_aux_old = 0;
 }
 
 static void free_layer(tie_hip_layer *l)
@@ -770,6 +789,7 @@ extern "C" void tie_hip_shutdown(void)
 			(void)hipFree(kv.second.alloc);
 		if (kv.second.one_status)
 			(void)hipHostFree(kv.second.one_status);
+		free_aux(kv.second);
 	}
 	g.ws.clear();
 	if (g.pin)
@@ -1305,6 +1325,360 @@ extern "C" int tie_hip_qwen3_ffn(float *hidden, int T, int d, int F, int E, int 
 			    eps);
 }
 
+// ---------------------------------------------------- the attention half
+namespace tie {
+
+// `need` bytes of scratch: the caller's, or the stream's own, grown.
+static int aux_scratch(hipStream_t s, void *work, size_t work_bytes, size_t need, void **out)
+{
+	if (work) {
+		if ((uintptr_t)work & 15)
+			return set_error(TIE_HIP_EINVAL, "work is not 16-byte aligned");
+		if (work_bytes < need)
+			return set_error(TIE_HIP_EINVAL, "work of %zu bytes, %zu needed", work_bytes, need);
+		*out = work;
+		return TIE_HIP_OK;
+	}
+	Workspace &w = g.ws[s];
+	if (need > w.aux_bytes) {
+		if (capturing(s))
+			return set_error(TIE_HIP_EINVAL,
+					 "the stream's workspace would have to grow to %zu bytes during graph capture: run the "
+					 "call once before, or pass work",
+					 need);
+		if (w.n_aux_old == (int)(sizeof w.aux_old / sizeof *w.aux_old))
+			return set_error(TIE_HIP_ENOMEM, "the stream's workspace has grown too often");
+		size_t bytes = need > 2 * w.aux_bytes ? need : 2 * w.aux_bytes;
+		bytes = bytes > ((size_t)1 << 20) ? align256(bytes) : (size_t)1 << 20;
+		void *mem = nullptr;
+		int rc = dev_malloc(&mem, bytes, "attention workspace");
+		if (rc)
+			return rc;
+		if (w.aux)
+			w.aux_old[w.n_aux_old++] = w.aux;
+		w.aux = mem;
+		w.aux_bytes = bytes;
+	}
+	*out = w.aux;
+	return TIE_HIP_OK;
+}
+
+static int check_cache(const tie_hip_kv_cache *c, int layer, int n_layers, KvLayer &l)
+{
+	if (!c)
+		return set_error(TIE_HIP_EINVAL, "null cache");
+	if (c->type != TIE_GGML_F16 && c->type != TIE_GGML_I8)
+		return set_error(TIE_HIP_EINVAL, "cache type %d unsupported (F16, I8)", c->type);
+	if (c->head_dim != 64 && c->head_dim != 128)
+		return set_error(TIE_HIP_EINVAL, "head_dim=%d unsupported (64, 128)", c->head_dim);
+	if (c->kv_heads < 1 || c->kv_heads > 1024 || c->n_layers < 1 || c->n_layers > 4096 || c->n_pages < 1)
+		return set_error(TIE_HIP_EINVAL, "bad cache: kv_heads=%d n_layers=%d n_pages=%d", c->kv_heads, c->n_layers,
+				 c->n_pages);
+	if (layer < 0 || n_layers < 1 || layer >= c->n_layers || n_layers > c->n_layers - layer)
+		return set_error(TIE_HIP_EINVAL, "layer %d (%d of them) outside [0, %d)", layer, n_layers, c->n_layers);
+	l.i8 = c->type == TIE_GGML_I8;
+	if (!c->k || !c->v || (l.i8 && (!c->k_scale || !c->v_scale)))
+		return set_error(TIE_HIP_EINVAL, "null cache array");
+	if (((uintptr_t)c->k | (uintptr_t)c->v | (l.i8 ? (uintptr_t)c->k_scale | (uintptr_t)c->v_scale : 0)) & 15)
+		return set_error(TIE_HIP_EINVAL, "cache arrays must be 16-byte aligned");
+	l.n_pages = c->n_pages;
+	l.kvh = c->kv_heads;
+	l.hd = c->head_dim;
+	l.layer_scales = (size_t)c->n_pages * c->kv_heads * PAGE;
+	l.layer_bytes = l.layer_scales * c->head_dim * (l.i8 ? 1 : 2);
+	l.k = (uint8_t *)c->k + layer * l.layer_bytes;
+	l.v = (uint8_t *)c->v + layer * l.layer_bytes;
+	l.ks = l.i8 ? c->k_scale + layer * l.layer_scales : nullptr;
+	l.vs = l.i8 ? c->v_scale + layer * l.layer_scales : nullptr;
+	return TIE_HIP_OK;
+}
+
+static int check_seqs(const tie_hip_kv_seqs *q, KvSeqs &s)
+{
+	if (!q)
+		return set_error(TIE_HIP_EINVAL, "null seqs");
+	if (q->n_seqs < 0 || q->n_seqs > 65535 || q->n_tokens < 0)
+		return set_error(TIE_HIP_EINVAL, "n_seqs=%d outside [0, 65535] or n_tokens=%d < 0", q->n_seqs, q->n_tokens);
+	if (q->max_pages < 1 || q->max_pages > 0x7fffffff / PAGE)
+		return set_error(TIE_HIP_EINVAL, "max_pages=%d outside [1, %d]", q->max_pages, 0x7fffffff / PAGE);
+	if (q->n_seqs > 0 && (!q->pages || !q->len))
+		return set_error(TIE_HIP_EINVAL, "null pages/len");
+	if (!q->first && q->n_tokens != q->n_seqs)
+		return set_error(TIE_HIP_EINVAL, "without first, n_tokens=%d must be n_seqs=%d", q->n_tokens, q->n_seqs);
+	s.pages = q->pages;
+	s.len = q->len;
+	s.first = q->first;
+	s.n_seqs = q->n_seqs;
+	s.max_pages = q->max_pages;
+	s.n_tokens = q->n_tokens;
+	return TIE_HIP_OK;
+}
+
+static int check_heads(const KvLayer &l, int n_heads)
+{
+	if (n_heads < 1 || n_heads > 65536 || n_heads % l.kvh)
+		return set_error(TIE_HIP_EINVAL, "n_heads=%d must be a multiple of kv_heads=%d up to 65536", n_heads, l.kvh);
+	return TIE_HIP_OK;
+}
+
+// the bytes from the first to the last of T rows
+static size_t row_span(int T, size_t stride, size_t width)
+{
+	return T > 0 ? ((size_t)(T - 1) * stride + width) * 4 : 0;
+}
+
+} // namespace tie
+
+#define TIE_TRY(expr)                     \
+	do {                              \
+		const int rc_ = (expr);   \
+		if (rc_ != TIE_HIP_OK)    \
+			return rc_;       \
+	} while (0)
+
+extern "C" int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
+				 size_t q_stride, const float *k, size_t k_stride, const float *v, size_t v_stride, int n_heads,
+				 const float *q_norm, const float *k_norm, float eps, float theta, const int32_t *pos,
+				 float *q_out, size_t q_out_stride, void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	KvLayer l;
+	KvSeqs s;
+	TIE_TRY(check_cache(cache, layer, 1, l));
+	TIE_TRY(check_seqs(seqs, s));
+	TIE_TRY(check_heads(l, n_heads));
+	if (!(theta > 0.0f) || !(theta <= 3.4e38f) || !(eps >= 0.0f))
+		return set_error(TIE_HIP_EINVAL, "theta=%g must be positive and finite, eps=%g not negative", theta, eps);
+	const size_t wq = (size_t)n_heads * l.hd, wk = (size_t)l.kvh * l.hd;
+	if (q_stride < wq || k_stride < wk || v_stride < wk || q_out_stride < wq)
+		return set_error(TIE_HIP_EINVAL, "a row stride is below its row's width (%zu, %zu)", wq, wk);
+	const bool none = s.n_tokens == 0 || s.n_seqs == 0;
+	if (!none && (!q || !k || !v || !q_out))
+		return set_error(TIE_HIP_EINVAL, "null q/k/v/q_out");
+	const int T = s.n_tokens;
+	const size_t no = row_span(T, q_out_stride, wq);
+	if (!(q_out == q && q_out_stride == q_stride) &&
+	    (overlap(q_out, no, q, row_span(T, q_stride, wq)) || overlap(q_out, no, k, row_span(T, k_stride, wk)) ||
+	     overlap(q_out, no, v, row_span(T, v_stride, wk))))
+		return set_error(TIE_HIP_EINVAL, "q_out overlaps an input (it may be q itself, with q's stride)");
+	TIE_TRY(ensure_init());
+	if (none)
+		return TIE_HIP_OK;
+	AppendArgs a;
+	a.q = q;
+	a.k = k;
+	a.v = v;
+	a.q_stride = q_stride;
+	a.k_stride = k_stride;
+	a.v_stride = v_stride;
+	a.q_out = q_out;
+	a.qo_stride = q_out_stride;
+	a.q_norm = q_norm;
+	a.k_norm = k_norm;
+	a.pos = pos;
+	a.n_heads = n_heads;
+	a.eps = eps;
+	a.log2_theta = log2((double)theta);
+	hipStream_t st = stream ? (hipStream_t)stream : g.stream;
+	prof_begin("kv_append", st);
+	const hipError_t e = launch_kv_append(l, s, a, st);
+	prof_end(st);
+	HIP_TRY(e);
+	return TIE_HIP_OK;
+}
+
+extern "C" int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_layers, const tie_hip_kv_seqs *seqs,
+			       float *k_out, float *v_out, void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	KvLayer l;
+	KvSeqs s;
+	TIE_TRY(check_cache(cache, layer, n_layers, l));
+	TIE_TRY(check_seqs(seqs, s));
+	const bool none = s.n_tokens == 0 || s.n_seqs == 0;
+	if (!none && (!k_out || !v_out))
+		return set_error(TIE_HIP_EINVAL, "null k_out/v_out");
+	const size_t n = (size_t)n_layers * s.n_tokens * l.kvh * l.hd * 4;
+	if (overlap(k_out, n, v_out, n))
+		return set_error(TIE_HIP_EINVAL, "k_out and v_out overlap");
+	TIE_TRY(ensure_init());
+	if (none)
+		return TIE_HIP_OK;
+	hipStream_t st = stream ? (hipStream_t)stream : g.stream;
+	prof_begin("kv_read", st);
+	const hipError_t e = launch_kv_read(l, n_layers, s, k_out, v_out, st);
+	prof_end(st);
+	HIP_TRY(e);
+	return TIE_HIP_OK;
+}
+
+extern "C" int tie_hip_kv_keep(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, const int32_t *path, int max_path,
+			       const int32_t *n_keep, int32_t *len_out, void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	KvLayer l;
+	KvSeqs s;
+	TIE_TRY(check_cache(cache, 0, cache ? cache->n_layers : 1, l));
+	TIE_TRY(check_seqs(seqs, s));
+	if (max_path < 1)
+		return set_error(TIE_HIP_EINVAL, "max_path=%d < 1", max_path);
+	if (s.n_seqs > 0 && (!path || !n_keep))
+		return set_error(TIE_HIP_EINVAL, "null path/n_keep");
+	const size_t nb = (size_t)s.n_seqs * 4;
+	if (len_out && ((len_out != s.len && overlap(len_out, nb, s.len, nb)) || overlap(len_out, nb, n_keep, nb) ||
+			overlap(len_out, nb, path, nb * max_path) || overlap(len_out, nb, s.first, nb + 4) ||
+			overlap(len_out, nb, s.pages, nb * s.max_pages)))
+		return set_error(TIE_HIP_EINVAL, "len_out overlaps an input (it may be len itself)");
+	TIE_TRY(ensure_init());
+	if (s.n_seqs == 0)
+		return TIE_HIP_OK;
+	hipStream_t st = stream ? (hipStream_t)stream : g.stream;
+	prof_begin("kv_keep", st);
+	const hipError_t e = launch_kv_keep(l, cache->n_layers, s, path, max_path, n_keep, len_out, st);
+	prof_end(st);
+	HIP_TRY(e);
+	return TIE_HIP_OK;
+}
+
+extern "C" size_t tie_hip_tree_attention_work_bytes(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, int n_heads)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	KvLayer l;
+	KvSeqs s;
+	if (check_cache(cache, 0, 1, l) || check_seqs(seqs, s) || check_heads(l, n_heads) || s.n_seqs == 0)
+		return 0;
+	AttnArgs a = {};
+	a.n_heads = n_heads;
+	return attention_work_bytes(l, s, a);
+}
+
+extern "C" int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
+				      size_t q_stride, int n_heads, float scale, const uint64_t *mask, int mask_words,
+				      float *out, size_t out_stride, void *work, size_t work_bytes, void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	KvLayer l;
+	KvSeqs s;
+	TIE_TRY(check_cache(cache, layer, 1, l));
+	TIE_TRY(check_seqs(seqs, s));
+	TIE_TRY(check_heads(l, n_heads));
+	const size_t w = (size_t)n_heads * l.hd;
+	if (q_stride < w || out_stride < w)
+		return set_error(TIE_HIP_EINVAL, "a row stride is below the row's width %zu", w);
+	if (mask && mask_words < 1)
+		return set_error(TIE_HIP_EINVAL, "mask_words=%d < 1", mask_words);
+	if (((uintptr_t)mask & 7) != 0)
+		return set_error(TIE_HIP_EINVAL, "mask is not 8-byte aligned");
+	if (!(scale - scale == 0.0f))
+		return set_error(TIE_HIP_EINVAL, "scale is not finite");
+	const bool none = s.n_tokens == 0 || s.n_seqs == 0;
+	if (!none && (!q || !out))
+		return set_error(TIE_HIP_EINVAL, "null q/out");
+	if (!(out == q && out_stride == q_stride) &&
+	    overlap(out, row_span(s.n_tokens, out_stride, w), q, row_span(s.n_tokens, q_stride, w)))
+		return set_error(TIE_HIP_EINVAL, "out overlaps q (it may be q itself, with q's stride)");
+	TIE_TRY(ensure_init());
+	if (none)
+		return TIE_HIP_OK;
+	AttnArgs a;
+	a.q = q;
+	a.q_stride = q_stride;
+	a.out = out;
+	a.o_stride = out_stride;
+	a.mask = mask;
+	a.mask_words = mask ? mask_words : 0;
+	a.n_heads = n_heads;
+	a.scale = scale;
+	hipStream_t st = stream ? (hipStream_t)stream : g.stream;
+	void *mem = nullptr;
+	TIE_TRY(aux_scratch(st, work, work_bytes, attention_work_bytes(l, s, a), &mem));
+	prof_begin("attention", st);
+	const hipError_t e = launch_attention(l, s, a, mem, st);
+	prof_end(st);
+	HIP_TRY(e);
+	return TIE_HIP_OK;
+}
+
+static int check_verify(int vocab, int n_tokens, int max_children)
+{
+	if (vocab < 1 || vocab > (1 << 24) || n_tokens < 0 || n_tokens > 65535)
+		return set_error(TIE_HIP_EINVAL, "vocab=%d outside [1, 2^24] or n_tokens=%d outside [0, 65535]", vocab, n_tokens);
+	if (max_children < 1 || max_children > VERIFY_KIDS)
+		return set_error(TIE_HIP_EINVAL, "max_children=%d outside [1, %d]", max_children, VERIFY_KIDS);
+	return TIE_HIP_OK;
+}
+
+extern "C" size_t tie_hip_verify_tree_work_bytes(int vocab, int n_tokens, int max_children, int with_draft)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	if (check_verify(vocab, n_tokens, max_children))
+		return 0;
+	VerifyArgs a = {};
+	a.vocab = vocab;
+	a.n_tokens = n_tokens;
+	a.max_children = max_children;
+	return verify_work_bytes(a, with_draft != 0);
+}
+
+extern "C" int tie_hip_verify_tree(const float *logits, size_t logits_stride, const float *draft, size_t draft_stride,
+				   int vocab, int n_seqs, int n_tokens, const int32_t *first, const int32_t *tokens,
+				   const int32_t *parent, const float *u_accept, const float *u_sample, float temperature,
+				   int max_children, int max_path, int32_t *path, int32_t *n_keep, int32_t *next, void *work,
+				   size_t work_bytes, void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	TIE_TRY(check_verify(vocab, n_tokens, max_children));
+	if (n_seqs < 0 || n_seqs > 65535 || max_path < 1)
+		return set_error(TIE_HIP_EINVAL, "n_seqs=%d outside [0, 65535] or max_path=%d < 1", n_seqs, max_path);
+	if (!first && n_seqs != n_tokens)
+		return set_error(TIE_HIP_EINVAL, "without first, n_tokens=%d must be n_seqs=%d", n_tokens, n_seqs);
+	if (logits_stride < (size_t)vocab || (draft && draft_stride < (size_t)vocab))
+		return set_error(TIE_HIP_EINVAL, "a row stride is below vocab=%d", vocab);
+	if (!(temperature >= 0.0f) || !(temperature <= 3.4e38f))
+		return set_error(TIE_HIP_EINVAL, "temperature=%g must be finite and not negative", temperature);
+	if (n_seqs > 0 && (!path || !n_keep || !next))
+		return set_error(TIE_HIP_EINVAL, "null path/n_keep/next");
+	if (n_seqs > 0 && n_tokens > 0 && (!logits || !tokens || !parent || !u_accept || !u_sample))
+		return set_error(TIE_HIP_EINVAL, "null logits/tokens/parent/u_accept/u_sample");
+	TIE_TRY(ensure_init());
+	if (n_seqs == 0)
+		return TIE_HIP_OK;
+	VerifyArgs a;
+	a.logits = logits;
+	a.draft = draft;
+	a.l_stride = logits_stride;
+	a.d_stride = draft_stride;
+	a.first = first;
+	a.tokens = tokens;
+	a.parent = parent;
+	a.u_accept = u_accept;
+	a.u_sample = u_sample;
+	a.vocab = vocab;
+	a.n_seqs = n_seqs;
+	a.n_tokens = n_tokens;
+	a.max_children = max_children;
+	a.max_path = max_path;
+	a.temperature = temperature;
+	a.path = path;
+	a.n_keep = n_keep;
+	a.next = next;
+	hipStream_t st = stream ? (hipStream_t)stream : g.stream;
+	void *mem = nullptr;
+	TIE_TRY(aux_scratch(st, work, work_bytes, verify_work_bytes(a, draft != nullptr), &mem));
+	prof_begin("verify", st);
+	const hipError_t e = launch_verify(a, mem, st);
+	prof_end(st);
+	HIP_TRY(e);
+	return TIE_HIP_OK;
+}
+
 extern "C" int tie_hip_exact_max_tokens(void)
 {
 	return g.exact_max_t;
@@ -1332,6 +1706,7 @@ extern "C" int tie_hip_stream_release(void *stream)
 	it->second.alloc = nullptr;
 	if (it->second.one_status)
 		HIP_TRY(hipHostFree(it->second.one_status));
+	free_aux(it->second);
 	g.ws.erase(it);
 	return TIE_HIP_OK;
 }

@@ -145,6 +145,13 @@ struct Workspace {
 	                               //     no-allocation scratch; that kernel does not run)
 	size_t cap_pairs = 0, cap_F = 0, cap_d = 0, cap_E = 0;
 	void *alloc = nullptr;
+	// scratch of the attention and verification calls, apart from the above;
+	// outgrown blocks stay (captured graphs may hold them) until the stream's
+	// release, each at least twice the one before
+	void *aux = nullptr;
+	size_t aux_bytes = 0;
+	void *aux_old[48] = {};
+	int n_aux_old = 0;
 };
 
 // ---------------------------------------------------------------- launchers

@@ -1,0 +1,124 @@
+// kv.h -- the paged key/value cache and its sequences, as the kernels of the
+// attention half see them (kv.hip, attention.hip).
+#pragma once
+#include "common.h"
+
+namespace tie {
+
+constexpr int PAGE = TIE_HIP_PAGE_ROWS; // rows of a page: one 64-bit mask word, four 16-row matrix-core tiles
+
+// One layer of a cache.  K [page][kv head][PAGE][hd] and V [page][kv
+// head][hd][PAGE]: a V column's rows are contiguous, so that both products of
+// the attention take their operands from memory in 16-byte pieces as they lie.
+// Scales [page][kv head][PAGE], int8 only.
+struct KvLayer {
+	uint8_t *k = nullptr, *v = nullptr;
+	float *ks = nullptr, *vs = nullptr;
+	int n_pages = 0, kvh = 0, hd = 0, i8 = 0;
+	// bytes (and scales) of a layer: the kernels of several layers step by them
+	size_t layer_bytes = 0, layer_scales = 0;
+};
+
+// The sequences of a call: device arrays, read by the kernels only after the
+// bounds checks below.
+struct KvSeqs {
+	const int32_t *pages = nullptr; // [n_seqs][max_pages]
+	const int32_t *len = nullptr;   // [n_seqs]
+	const int32_t *first = nullptr; // [n_seqs + 1], or null: a token each
+	int n_seqs = 0, max_pages = 0, n_tokens = 0;
+};
+
+struct AppendArgs {
+	const float *q, *k, *v;
+	size_t q_stride, k_stride, v_stride; // floats from a token's row to the next
+	float *q_out;
+	size_t qo_stride;
+	const float *q_norm, *k_norm; // [hd], or null: no norm
+	const int32_t *pos;           // [n_tokens], or null: the cache row
+	int n_heads;
+	double eps, log2_theta;
+};
+
+struct AttnArgs {
+	const float *q;
+	size_t q_stride;
+	float *out;
+	size_t o_stride;
+	const uint64_t *mask; // [n_tokens][mask_words], or null: causal
+	int mask_words, n_heads;
+	float scale;
+};
+
+hipError_t launch_kv_append(const KvLayer &c, const KvSeqs &s, const AppendArgs &a, hipStream_t st);
+hipError_t launch_kv_read(const KvLayer &c, int n_layers, const KvSeqs &s, float *k_out, float *v_out, hipStream_t st);
+hipError_t launch_kv_keep(const KvLayer &c, int n_layers, const KvSeqs &s, const int32_t *path, int max_path,
+			  const int32_t *n_keep, int32_t *len_out, hipStream_t st);
+size_t attention_work_bytes(const KvLayer &c, const KvSeqs &s, const AttnArgs &a);
+hipError_t launch_attention(const KvLayer &c, const KvSeqs &s, const AttnArgs &a, void *work, hipStream_t st);
+
+struct VerifyArgs {
+	const float *logits, *draft; // draft null: proposed without probabilities
+	size_t l_stride, d_stride;
+	const int32_t *first, *tokens, *parent;
+	const float *u_accept, *u_sample;
+	int vocab, n_seqs, n_tokens, max_children, max_path;
+	float temperature;
+	int32_t *path, *n_keep, *next;
+};
+constexpr int VERIFY_KIDS = 16; // children of a node that are tried, at most
+size_t verify_work_bytes(const VerifyArgs &a, bool with_draft);
+hipError_t launch_verify(const VerifyArgs &a, void *work, hipStream_t st);
+
+#if defined(__HIPCC__)
+// The token rows of sequence b: [t0, t0 + n), n = 0 where the arrays say
+// something that lies outside the call's own sizes.
+__device__ __forceinline__ void seq_tokens(const KvSeqs &s, int b, int &t0, int &n)
+{
+	t0 = b;
+	n = 1;
+	if (s.first) {
+		t0 = s.first[b];
+		const int t1 = s.first[b + 1];
+		n = t0 >= 0 && t1 >= t0 && t1 <= s.n_tokens ? t1 - t0 : 0;
+	}
+}
+
+// Whether sequence b's rows, n of them behind the committed ones, lie within
+// its page table.
+__device__ __forceinline__ bool seq_fits(const KvSeqs &s, int len, int n)
+{
+	return len >= 0 && (long long)len + n <= (long long)s.max_pages * PAGE;
+}
+
+// The page of row `row` of sequence b, -1 where the table names none.
+__device__ __forceinline__ int page_of(const KvSeqs &s, int n_pages, int b, int row)
+{
+	const int p = s.pages[(size_t)b * s.max_pages + row / PAGE];
+	return p >= 0 && p < n_pages ? p : -1;
+}
+
+// The sequence of token row t (the last b with first[b] <= t), -1 when none
+// holds it.
+__device__ __forceinline__ int seq_of_token(const KvSeqs &s, int t, int &t0, int &n)
+{
+	if (!s.first) {
+		t0 = t;
+		n = 1;
+		return t < s.n_seqs ? t : -1;
+	}
+	int lo = 0, hi = s.n_seqs;
+	while (lo < hi) {
+		const int mid = (lo + hi) >> 1;
+		if (s.first[mid + 1] <= t)
+			lo = mid + 1;
+		else
+			hi = mid;
+	}
+	if (lo >= s.n_seqs)
+		return -1;
+	seq_tokens(s, lo, t0, n);
+	return t >= t0 && t < t0 + n ? lo : -1;
+}
+#endif
+
+} // namespace tie
