@@ -1,8 +1,26 @@
 """Plain 64-bit forms of the cache, the attention and the verification, and
 small caches to test them on."""
+import contextlib
+import gc
+
 import numpy as np
 
 ROWS = 64
+
+
+@contextlib.contextmanager
+def capture(graph, stream=None):
+    """torch.cuda.graph with the garbage collected before and none during the
+    capture: a collection that meets another test's graph there would destroy
+    it inside the capture, which ends the process."""
+    import torch
+    gc.collect()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            yield
+    finally:
+        gc.enable()
 
 
 class Cache:

@@ -1,6 +1,8 @@
 """Attention of single tokens, causal chunks and drafted trees over the paged
 cache, against a plain 64-bit form.  Every row of the cache that belongs to no
 sequence holds NaN.  Tolerances: kv_ref.tolerance (derived there)."""
+import gc
+
 import numpy as np
 import pytest
 
@@ -287,7 +289,7 @@ def test_in_place_streams_work_and_graphs(kind, lens, counts):
     for i in range(2):
         g = torch.cuda.CUDAGraph()
         mine = torch.empty(need, dtype=torch.uint8, device="cuda")
-        with torch.cuda.graph(g, stream=streams[i]):
+        with kv_ref.capture(g, streams[i]):
             kv.attention(0, seqs, q, outs[2 + i], 0.09, work=mine, stream=torch.cuda.current_stream().cuda_stream)
         graphs.append((g, mine))
     for rep in range(3):
@@ -301,11 +303,20 @@ def test_in_place_streams_work_and_graphs(kind, lens, counts):
         torch.cuda.synchronize()
         for i in (0, 2, 3):
             assert torch.equal(outs[i], want), (rep, i)
-    fresh = torch.cuda.Stream()
+    # a stream whose workspace would have to grow: refused, and the capture goes on
+    fresh, said = torch.cuda.Stream(), ""
     g = torch.cuda.CUDAGraph()
-    with pytest.raises(tie_amd.TieError) as e:
-        with torch.cuda.graph(g, stream=fresh):
+    with kv_ref.capture(g, fresh):
+        outs[3].fill_(5.0)
+        try:
             kv.attention(0, seqs, q, outs[1], 0.09, stream=torch.cuda.current_stream().cuda_stream)
-    assert "capture" in str(e.value)
+        except tie_amd.TieError as e:
+            said = str(e)
+    assert "capture" in said
+    g.replay()
+    torch.cuda.synchronize()
+    assert (outs[3] == 5.0).all()
     for s in streams:
         tie_amd.stream_release(s.cuda_stream)
+    del g, graphs
+    gc.collect()

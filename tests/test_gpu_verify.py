@@ -2,6 +2,8 @@
 64-bit form: whole numbers, so equal.  (The kernels' sums and the form's are
 both in 64 bits; a random number within 1e-12 of a border would fall on either
 side, and none of these does.)"""
+import gc
+
 import numpy as np
 import pytest
 
@@ -180,7 +182,7 @@ def test_repeats_work_streams_and_graphs(draft):
     path, n, nxt = torch.zeros(2, 12, dtype=torch.int32, device="cuda"), *(torch.zeros(2, dtype=torch.int32, device="cuda") for _ in range(2))
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(g):
+    with kv_ref.capture(g):
         tie_amd.verify_tree(*args, path, n, nxt, temperature=0.8, draft=d, max_children=3, work=work,
                             stream=torch.cuda.current_stream().cuda_stream)
     for rep in range(3):
@@ -191,3 +193,5 @@ def test_repeats_work_streams_and_graphs(draft):
         torch.cuda.synchronize()
         for a, w in zip((path, n, nxt), want):
             np.testing.assert_array_equal(a.cpu().numpy(), w, str(rep))
+    del g
+    gc.collect()

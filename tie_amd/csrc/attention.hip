@@ -10,12 +10,16 @@
 // exact in f16, so every product is exact and the sums are F32.
 //
 // Both products are computed transposed, S^T = K Q^T and O^T = V^T P^T, with
-// v_mfma_f32_16x16x32_f16.  A lane (n = lane % 16, g = lane / 16) of S^T's
-// four 16-row tiles holds query n and, since tile t's row 4 g + i is page row
-// 16 g + 4 t + i, the 16 rows 16 g .. 16 g + 15 of a page: just what the second
-// product's operand wants of that lane.  So the weights never leave their
-// registers, the running maximum and sum of a query are one value a lane
-// (joined over g), and K and V^T go from the pages straight into operands.
+// v_mfma_f32_16x16x32_f16, over 32 or 64 cache rows at a time (KT = 2 or 4
+// tiles of 16).  A lane (n = lane % 16, g = lane / 16) of S^T's tiles holds
+// query n, and since tile t's row 4 g + i is cache row 4 KT g + 4 t + i, the 4 KT
+// rows from 4 KT g on: just what the second product's operand wants of that
+// lane.  So the weights never leave their registers, the maximum and sum of a
+// query are one value a lane (joined over g), and K and V^T go from the pages
+// straight into operands.
+//
+// The maximum m is a reference only: it moves when some weight would pass
+// 2^MOVE, so most steps need no exchange between lanes and leave O alone.
 #include "kv.h"
 
 namespace tie {
@@ -25,8 +29,8 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr float P_SCALE = 4096.0f; // weights are at most 1; their second f16 part stays above the subnormals
-constexpr int ATTN_UNITS = 512;    // workgroups that the work is cut for
+constexpr float MOVE = 3.0f;       // log2 of the largest weight
+constexpr float P_SCALE = 4096.0f; // with it the weights stay below the f16 limit, their second parts above the subnormals
 
 // four int8 codes to f16: 1024 + (code + 128) is the f16 0x6400 | byte, from
 // which 1152 is taken exactly
@@ -79,12 +83,20 @@ __device__ __forceinline__ float pow2_below(float x)
 // How the work of a call is cut: sequence b has tiles(b) row tiles for each kv
 // head, each over pages(b) pages, in chunks of `chunk` pages -- one unit of
 // work (a workgroup) for each.  Every workgroup finds the cut by itself from
-// the lengths on the device.
-struct Unit {
-	int b, tile, head, part, parts, chunk, t0, n, len, index;
+// the lengths on the device, so that neither a copy to the host nor a launch
+// for a plan stands before the attention and captured calls follow the lengths.
+struct Cut {
+	int cap;   // units that run at once: at most so many where tiles are cut
+	int least; // pages of a unit, at least
+	int whole; // tiles are not cut at all
+	int rows;  // query rows of a tile
 };
 
-__device__ __forceinline__ long long wave_sum(long long x)
+struct Unit {
+	int b, tile, head, part, parts, chunk, t0, n, len, base; // base: the first unit of the sequence
+};
+
+__device__ __forceinline__ int wave_sum(int x)
 {
 #pragma unroll
 	for (int m = 1; m < 64; m <<= 1)
@@ -92,71 +104,111 @@ __device__ __forceinline__ long long wave_sum(long long x)
 	return x;
 }
 
-__device__ __forceinline__ void seq_work(const KvSeqs &s, int b, int group, int rows, int &tiles, int &pages)
+__device__ __forceinline__ void seq_work(const KvSeqs &s, int b, int group, int rows, int &t0, int &n, int &len, int &tiles,
+					 int &pages)
 {
-	int t0, n;
-	tiles = pages = 0;
+	t0 = n = len = tiles = pages = 0;
 	if (b >= s.n_seqs)
 		return;
+	len = s.len[b];
 	seq_tokens(s, b, t0, n);
 	if (n == 0)
 		return;
-	const int len = s.len[b];
 	tiles = (int)(((long long)n * group + rows - 1) / rows);
 	pages = seq_fits(s, len, n) ? (len + n + PAGE - 1) / PAGE : 1;
 }
 
-// pages of a unit: as many as leave about ATTN_UNITS of them
-__device__ __forceinline__ int unit_chunk(const KvSeqs &s, int kvh, int group, int rows, int least)
+__device__ __forceinline__ int div_up(int a, int b)
 {
-	const int lane = threadIdx.x & 63;
-	long long w = 0;
-	for (int b = lane; b < s.n_seqs; b += 64) {
-		int tiles, pages;
-		seq_work(s, b, group, rows, tiles, pages);
-		w += (long long)tiles * pages;
-	}
-	w = wave_sum(w) * kvh;
-	const long long c = (w + ATTN_UNITS - 1) / ATTN_UNITS;
-	return (int)(c < least ? least : c);
+	return (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b);
 }
 
-// the unit of workgroup `index`; false past the last
-__device__ __forceinline__ bool find_unit(const KvSeqs &s, int kvh, int group, int rows, int least, int index, Unit &u)
+// Pages of a unit: the least that leaves no more than cap units (or, where the
+// tiles alone are as many, whole tiles).  The first block of 64 sequences is in
+// the wave's lanes already.
+__device__ __forceinline__ int unit_chunk(const KvSeqs &s, int kvh, int group, const Cut &cut, int tiles0, int pages0)
+{
+	if (cut.whole)
+		return 0x7fffffff;
+	const int lane = threadIdx.x & 63;
+	auto over = [&](auto f) { // the sum of f(tiles, pages) over all sequences
+		int x = f(tiles0, pages0);
+		for (int b = 64 + lane; b < s.n_seqs; b += 64) {
+			int t0, n, len, tiles, pages;
+			seq_work(s, b, group, cut.rows, t0, n, len, tiles, pages);
+			x += f(tiles, pages);
+		}
+		return s.n_seqs > 1 ? wave_sum(x) : __builtin_amdgcn_readfirstlane(x);
+	};
+	const int cap = cut.cap / kvh > 0 ? cut.cap / kvh : 1; // for one kv head
+	if (over([&](int t, int) { return t; }) >= cap)
+		return 0x7fffffff;
+	// (in sixteenths of a unit's share: tiles * pages can pass 32 bits)
+	const float share = 1.0f / cap;
+	float w = (float)tiles0 * pages0 * share;
+	for (int b = 64 + lane; b < s.n_seqs; b += 64) {
+		int t0, n, len, tiles, pages;
+		seq_work(s, b, group, cut.rows, t0, n, len, tiles, pages);
+		w += (float)tiles * pages * share;
+	}
+	if (s.n_seqs > 1)
+#pragma unroll
+		for (int m = 1; m < 64; m <<= 1)
+			w += __shfl_xor(w, m);
+	w = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, w)));
+	int c = (int)__builtin_ceilf(w);
+	c = c < cut.least ? cut.least : c;
+	for (int i = 0; i < 12; i++) {
+		if (over([&](int t, int p) { return t * div_up(p, c); }) <= cap)
+			break;
+		c += c / 8 + 1;
+	}
+	return c;
+}
+
+// The unit of workgroup `index`; false past the last.  Units of a sequence:
+// kv heads innermost (workgroups go to the dies in turn: a die then has few
+// heads' pages in its L2), then parts, then tiles.
+__device__ __forceinline__ bool find_unit(const KvSeqs &s, int kvh, int group, const Cut &cut, int index, Unit &u)
 {
 	const int lane = threadIdx.x & 63;
-	u.chunk = unit_chunk(s, kvh, group, rows, least);
-	u.index = index;
-	long long before = 0;
-	for (int b0 = 0; b0 < s.n_seqs; b0 += 64) {
-		int tiles, pages;
-		seq_work(s, b0 + lane, group, rows, tiles, pages);
-		const int parts = (pages + u.chunk - 1) / u.chunk;
-		const long long mine = (long long)tiles * parts * kvh;
-		long long incl = mine;
+	int t0, n, len, tiles, pages;
+	seq_work(s, lane, group, cut.rows, t0, n, len, tiles, pages);
+	u.chunk = unit_chunk(s, kvh, group, cut, tiles, pages);
+	int before = 0;
+	for (int b0 = 0;;) {
+		const int parts = tiles ? div_up(pages, u.chunk) : 0, mine = tiles * parts * kvh;
+		int incl = mine;
+		if (s.n_seqs > 1)
 #pragma unroll
-		for (int m = 1; m < 64; m <<= 1) {
-			const long long o = __shfl_up(incl, m);
-			if (lane >= m)
-				incl += o;
-		}
+			for (int m = 1; m < 64; m <<= 1) {
+				const int o = __shfl_up(incl, m);
+				if (lane >= m)
+					incl += o;
+			}
 		const unsigned long long past = __ballot(before + incl > index);
 		if (past) {
 			const int l = __builtin_ctzll(past);
-			const int at = (int)(index - (before + __shfl(incl - mine, l)));
+			auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
 			u.b = b0 + l;
-			u.parts = __shfl(parts, l);
-			// (a kv head's parts of a tile lie side by side)
-			u.part = at % u.parts;
-			u.head = at / u.parts % kvh;
-			u.tile = at / u.parts / kvh;
-			seq_tokens(s, u.b, u.t0, u.n);
-			u.len = s.len[u.b];
+			u.base = before + of(incl - mine);
+			u.parts = of(parts);
+			const int at = index - u.base;
+			u.head = (uint32_t)at % (uint32_t)kvh;
+			u.part = (uint32_t)at / (uint32_t)kvh % (uint32_t)u.parts;
+			// (causal: the last tiles have the most pages; they start first)
+			u.tile = of(tiles) - 1 - (uint32_t)at / (uint32_t)kvh / (uint32_t)u.parts;
+			u.t0 = of(t0);
+			u.n = of(n);
+			u.len = of(len);
 			return true;
 		}
-		before += __shfl(incl, 63);
+		before += __builtin_amdgcn_readlane(incl, 63);
+		b0 += 64;
+		if (b0 >= s.n_seqs)
+			return false;
+		seq_work(s, b0 + lane, group, cut.rows, t0, n, len, tiles, pages);
 	}
-	return false;
 }
 
 // Which of the 64 rows of the page at row `start` a token sees: all committed
@@ -181,315 +233,354 @@ __device__ __forceinline__ uint64_t sees(const AttnArgs &a, const Unit &u, int n
 	return w | below(-(long long)rel);
 }
 
-// Partial results of a unit: its rows' maximum and sum, then O.
-constexpr int part_floats(int rows, int hd)
+// Results of a part, for each row of its tile: O [HD], the maximum, the sum.
+constexpr int part_row(int hd)
 {
-	return rows * (hd + 2);
+	return hd + 4; // (16-byte rows)
 }
 
-// A workgroup: NT tiles of 16 query rows (a row: a token and one query head
-// of the unit's kv head), its WK waves taking the unit's pages in turn.
-template <int HD, bool I8, int NT, int WK>
-__global__ __launch_bounds__(64 * WK) void attn_kernel(KvLayer c, KvSeqs s, AttnArgs a, int least, float *part)
+// A token row's query for one lane of an operand: 8 values of each K step,
+// scaled to below 2^10 and split; qs: what the products are multiplied by (with
+// log2 e: exp2 for exp), not negative (the scale's sign is in the query).
+template <int HD, bool PAIRS>
+__device__ __forceinline__ void load_query(const AttnArgs &a, const Unit &u, int node, int head, int g, h8 (&qh)[HD / 32],
+					   h8 (&ql)[HD / 32], float &qs)
 {
-	constexpr int KS = HD / 32, MT = HD / 16, R = 16 * NT;
+	float x[HD / 32][8], m = 0.0f;
+	const float *q = a.q + (size_t)(u.t0 + (node < 0 ? 0 : node)) * a.q_stride + (size_t)head * HD;
+#pragma unroll
+	for (int k = 0; k < HD / 32; k++)
+#pragma unroll
+		for (int j = 0; j < 8; j++) {
+			// (PAIRS: int8 rows straight from memory come 16 codes to a lane)
+			const int at = PAIRS ? (k >> 1) * 64 + g * 16 + (k & 1) * 8 + j : k * 32 + g * 8 + j;
+			x[k][j] = node < 0 ? 0.0f : q[at];
+		}
+#pragma unroll
+	for (int k = 0; k < HD / 32; k++)
+#pragma unroll
+		for (int j = 0; j < 8; j++)
+			m = __builtin_fmaxf(m, __builtin_fabsf(x[k][j]));
+	m = max_g(m);
+	const float p2 = m >= 1e-30f && m < 1e30f ? pow2_below(m) : 1.0f;
+	const float up = __builtin_copysignf(512.0f / p2, a.scale);
+	qs = __builtin_fabsf(a.scale) * 1.44269504088896f * (p2 * (1.0f / 512.0f));
+#pragma unroll
+	for (int k = 0; k < HD / 32; k++)
+#pragma unroll
+		for (int j = 0; j < 8; j += 2) {
+			h2 hi, lo;
+			split2(x[k][j] * up, x[k][j + 1] * up, hi, lo);
+			qh[k][j] = hi.x, qh[k][j + 1] = hi.y;
+			ql[k][j] = lo.x, ql[k][j + 1] = lo.y;
+		}
+}
+
+// The running state of 16 query rows: a lane's query's maximum, the lane's
+// share of its sum, and O^T.
+template <int HD>
+struct Rows {
+	float mx = -__builtin_inff(), sum = 0.0f;
+	f4 o[HD / 16];
+};
+
+// From the products sc of 16 KT cache rows to the weights' two f16 parts for
+// the second product; the state's reference and sum, and O where the reference
+// moved.  bits: which of the lane's 4 KT rows its query sees (whole: all of them
+// for every query of the wave).  int8: ks are the rows' K scales, vs their V
+// scales over the running power of two.
+template <int HD, bool I8, int KT>
+__device__ __forceinline__ void weigh(Rows<HD> &r, f4 (&sc)[KT], const f4 (&ks)[KT], const f4 (&vs)[KT], float qs, uint32_t bits,
+				      bool whole, h8 (&ph)[KT / 2], h8 (&pl)[KT / 2])
+{
+	if (I8)
+#pragma unroll
+		for (int kt = 0; kt < KT; kt++)
+			sc[kt] *= ks[kt];
+	if (!whole)
+#pragma unroll
+		for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+			for (int i = 0; i < 4; i++)
+				if (!(bits >> (4 * kt + i) & 1))
+					sc[kt][i] = -__builtin_inff();
+	float top = -__builtin_inff();
+#pragma unroll
+	for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+			top = __builtin_fmaxf(top, sc[kt][i]);
+	// (qs may be 0: 0 * -inf would be NaN)
+	top = top == -__builtin_inff() ? top : top * qs;
+	if (__any(top > r.mx + MOVE)) {
+		top = __builtin_fmaxf(r.mx, max_g(top));
+		const float f = r.mx == top ? 1.0f : __builtin_amdgcn_exp2f(r.mx - top);
+		r.mx = top;
+		r.sum *= f;
+#pragma unroll
+		for (int m = 0; m < HD / 16; m++)
+			r.o[m] *= f;
+	}
+	const float base = r.mx == -__builtin_inff() ? 0.0f : r.mx;
+#pragma unroll
+	for (int kt = 0; kt < KT; kt++) {
+		float w[4];
+#pragma unroll
+		for (int i = 0; i < 4; i++) {
+			const bool on = whole || (bits >> (4 * kt + i) & 1);
+			w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], qs, -base));
+			w[i] = on ? w[i] : 0.0f;
+			r.sum += w[i];
+			w[i] *= I8 ? vs[kt][i] : P_SCALE;
+			if (I8)
+				w[i] = on ? w[i] : 0.0f; // (the scale of a row that is not seen may be anything)
+		}
+#pragma unroll
+		for (int i = 0; i < 4; i += 2) {
+			h2 hi, lo;
+			split2(w[i], w[i + 1], hi, lo);
+			const int e = (kt & 1) * 4 + i;
+			ph[kt >> 1][e] = hi.x, ph[kt >> 1][e + 1] = hi.y;
+			pl[kt >> 1][e] = lo.x, pl[kt >> 1][e + 1] = lo.y;
+		}
+	}
+}
+
+// int8: the largest power of two among the V scales of the rows so far (vtop;
+// it grows seldom, and O shrinks with it).  top: the largest of the lane's rows
+// that hold anything.
+template <int HD, int NT>
+__device__ __forceinline__ void move_vtop(float top, float &vtop, Rows<HD> (&r)[NT])
+{
+	if (__any(top > vtop)) {
+		const float to = pow2_below(__builtin_fmaxf(max_g(top), vtop)) * 2.0f, f = vtop / to;
+		vtop = to;
+#pragma unroll
+		for (int t = 0; t < NT; t++)
+#pragma unroll
+			for (int m = 0; m < HD / 16; m++)
+				r[t].o[m] *= f;
+	}
+}
+
+// f16 values w of 32 rows that not every query sees, an operand of column tile
+// m: a value that is not finite would reach queries that do not see its row as 0
+// * inf.  Such values are taken out and come back for those that see them.  v:
+// the page's values of this head, the rows from `row0` on, `end` of which hold
+// anything; vis: the rows of these 32 that the lane's query sees.
+template <int HD, int NT>
+__device__ __forceinline__ void guard_values(u4 &w, const uint8_t *v, int row0, int m, int g, int end,
+					     const uint32_t (&vis)[NT], Rows<HD> (&r)[NT])
+{
+	uint32_t odd = 0;
+#pragma unroll
+	for (int e = 0; e < 4; e++) {
+		uint32_t x = w[e];
+		if ((x & 0x7c00u) == 0x7c00u) {
+			x &= 0xffff0000u;
+			odd |= 1u << (2 * e);
+		}
+		if ((x & 0x7c000000u) == 0x7c000000u) {
+			x &= 0xffffu;
+			odd |= 2u << (2 * e);
+		}
+		w[e] = x;
+	}
+	if (!__any(odd != 0))
+		return;
+	for (int row = 0; row < min(end, 32); row++) {
+		const int src = (row >> 3) * 16; // the lane group that has the row
+#pragma unroll
+		for (int i = 0; i < 4; i++) {
+			// (column 4 g + i of the tile: this lane's in O^T)
+			if (!(__shfl(odd, src + 4 * g + i) >> (row & 7) & 1))
+				continue;
+			const float x = (float)reinterpret_cast<const _Float16 *>(v)[(m * 16 + 4 * g + i) * PAGE + row0 + row];
+#pragma unroll
+			for (int t = 0; t < NT; t++)
+				if (vis[t] >> row & 1)
+					r[t].o[m][i] = x != x ? x : r[t].o[m][i] + x;
+		}
+	}
+}
+
+// ---------------------------------------------------------------- few rows
+// A workgroup: 16 query rows (a row: a token and one query head of the unit's
+// kv head), its 8 waves taking the unit's pages in turn.  Bound by the stream of
+// pages: a wave requests a page's K as soon as the products with the last one's
+// are done and its V as soon as O has taken the last one's, so that one of the
+// two is always under way, at 2 waves on a SIMD.
+constexpr int FEW_ROWS = 16, FEW_WAVES = 8;
+
+template <int HD, bool I8>
+__global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, float *part)
+{
+	constexpr int KS = HD / 32, MT = HD / 16, R = FEW_ROWS, WK = FEW_WAVES;
+	constexpr int KT = I8 ? 4 : 2;       // a step: a page of int8, half a page of f16 (16 KB of K and V at HD = 128)
+	constexpr int SP = 4 / KT;           // steps of a page
+	constexpr int KL = I8 ? KS / 2 : KS; // 16-byte loads of a lane for one of a step's K tiles
 	extern __shared__ __attribute__((aligned(16))) float lds[];
 	const int group = a.n_heads / c.kvh;
 	Unit u;
-	if (!find_unit(s, c.kvh, group, R, least, blockIdx.x, u))
+	if (!find_unit(s, c.kvh, group, cut, blockIdx.x, u))
 		return;
-	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
+	const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	bool bad = !seq_fits(s, u.len, u.n); // the rows cannot be read: the result is NaN
 
-	// the queries, scaled to below 2^10 and split
-	h8 qh[NT][KS], ql[NT][KS];
-	float qs[NT]; // what a score is multiplied by: exp2 instead of exp
-	int node[NT];
-#pragma unroll
-	for (int t = 0; t < NT; t++) {
-		const int r = u.tile * R + 16 * t + n16;
-		node[t] = r / group < u.n ? r / group : -1;
-		float x[KS][8], m = 0.0f;
-		const float *q = a.q + (size_t)(u.t0 + (node[t] < 0 ? 0 : node[t])) * a.q_stride +
-				 (size_t)(u.head * group + r % group) * HD;
-#pragma unroll
-		for (int k = 0; k < KS; k++)
-#pragma unroll
-			for (int j = 0; j < 8; j++) {
-				// int8 rows come 16 codes to a lane and load, f16 rows 8
-				const int at = I8 ? (k >> 1) * 64 + g * 16 + (k & 1) * 8 + j : k * 32 + g * 8 + j;
-				x[k][j] = node[t] < 0 ? 0.0f : q[at];
-				m = __builtin_fmaxf(m, __builtin_fabsf(x[k][j]));
-			}
-		m = max_g(m);
-		const float p2 = m >= 1e-30f && m < 1e30f ? pow2_below(m) : 1.0f;
-		const float up = 512.0f / p2;
-		qs[t] = a.scale * 1.44269504088896f * (p2 * (1.0f / 512.0f));
-#pragma unroll
-		for (int k = 0; k < KS; k++)
-#pragma unroll
-			for (int j = 0; j < 8; j += 2) {
-				h2 hi, lo;
-				split2(x[k][j] * up, x[k][j + 1] * up, hi, lo);
-				qh[t][k][j] = hi.x, qh[t][k][j + 1] = hi.y;
-				ql[t][k][j] = lo.x, ql[t][k][j + 1] = lo.y;
-			}
-	}
-
-	f4 o[NT][MT];
-	float mx[NT], sum[NT];
-#pragma unroll
-	for (int t = 0; t < NT; t++) {
-		mx[t] = -__builtin_inff();
-		sum[t] = 0.0f;
-#pragma unroll
-		for (int m = 0; m < MT; m++)
-			o[t][m] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-	}
-	// int8: the weights carry their row's V scale, over the largest power of
-	// two among the scales so far
-	float vtop = 1e-30f;
-
+	const int row = u.tile * R + n16;
+	const int node = row / group < u.n ? row / group : -1;
 	// (causal: nothing behind the tile's last token is seen)
 	const int last = a.mask ? u.n : min(u.n, (u.tile * R + R - 1) / group + 1);
 	const int pages = bad ? 0 : (u.len + last + PAGE - 1) / PAGE;
-	const int p1 = min(pages, (u.part + 1) * u.chunk);
-	for (int p = u.part * u.chunk + wave; p < p1; p += WK) {
-		const int start = p * PAGE, id = page_of(s, c.n_pages, u.b, start);
-		if (id < 0) {
-			bad = true;
-			continue;
-		}
-		const size_t at = (size_t)id * c.kvh + u.head;
-		uint64_t vis[NT];
-		bool whole = true;
-#pragma unroll
-		for (int t = 0; t < NT; t++) {
-			vis[t] = sees(a, u, node[t], start);
-			whole = whole && (vis[t] == ~0ull || node[t] < 0);
-		}
-		whole = __all(whole);
-		const int end = u.len + u.n - start; // rows of the page that hold anything
+	const int p0 = u.part * u.chunk, steps = (min(pages, p0 + min(u.chunk, pages)) - p0) * SP;
 
-		// S^T
-		f4 sc[NT][4];
+	u4 kr[KT][KL], vr[MT];
+	f4 ks[KT], vs[KT];
+	size_t at = 0; // of the page whose V is in (or on its way to) vr
+	auto page = [&](int step) {
+		const int id = page_of(s, c.n_pages, u.b, (p0 + step / SP) * PAGE);
+		bad = bad || id < 0;
+		return (size_t)(id < 0 ? 0 : id) * c.kvh + u.head;
+	};
+	auto get_k = [&](size_t pg, int step) {
+		const int row0 = step % SP * 32;
 #pragma unroll
-		for (int kt = 0; kt < 4; kt++) {
-			const int row = (n16 >> 2) * 16 + kt * 4 + (n16 & 3);
-			h8 kf[KS];
-			if constexpr (I8) {
-				const u4 *kr = reinterpret_cast<const u4 *>(c.k + (at * PAGE + row) * HD) + g;
+		for (int kt = 0; kt < KT; kt++) {
+			const int q = row0 + (n16 >> 2) * 4 * KT + kt * 4 + (n16 & 3);
+			const u4 *p = reinterpret_cast<const u4 *>(c.k + (pg * PAGE + q) * HD * (I8 ? 1 : 2)) + g;
 #pragma unroll
-				for (int q = 0; q < KS / 2; q++) {
-					const u4 w = kr[q * 4];
-					kf[2 * q] = codes8(w.x, w.y);
-					kf[2 * q + 1] = codes8(w.z, w.w);
+			for (int e = 0; e < KL; e++)
+				kr[kt][e] = p[e * 4];
+			if (I8)
+				ks[kt] = reinterpret_cast<const f4 *>(c.ks + pg * PAGE + g * 16)[kt];
+		}
+	};
+	auto get_v = [&](size_t pg, int step) {
+#pragma unroll
+		for (int m = 0; m < MT; m++)
+			vr[m] = reinterpret_cast<const u4 *>(c.v + (pg * HD + m * 16 + n16) * PAGE * (I8 ? 1 : 2))[step % SP * 4 + g];
+		if (I8)
+#pragma unroll
+			for (int kt = 0; kt < KT; kt++)
+				vs[kt] = reinterpret_cast<const f4 *>(c.vs + pg * PAGE + g * 16)[kt];
+	};
+	if (wave < steps) {
+		at = page(wave);
+		get_k(at, wave);
+		get_v(at, wave);
+	}
+	h8 qh[KS], ql[KS];
+	float qs;
+	load_query<HD, I8>(a, u, node, u.head * group + row % group, g, qh, ql, qs);
+	Rows<HD> r[1];
+#pragma unroll
+	for (int m = 0; m < MT; m++)
+		r[0].o[m] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+	float vtop = 1e-30f;
+
+	for (int step = wave; step < steps; step += WK) {
+		const int start = (p0 + step / SP) * PAGE, row0 = step % SP * 32, end = u.len + u.n - start - row0;
+		const uint64_t vis = sees(a, u, node, start) >> row0;
+		constexpr uint64_t all = KT == 4 ? ~0ull : 0xffffffffull;
+		const bool whole = __all((vis & all) == all || node < 0);
+		const bool more = step + WK < steps;
+		const size_t next = more ? page(step + WK) : at;
+		f4 sc[KT], kk[KT];
+#pragma unroll
+		for (int kt = 0; kt < KT; kt++) {
+			f4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+#pragma unroll
+			for (int k = 0; k < KS; k++) {
+				h8 kf;
+				if constexpr (I8) {
+					const u4 w = kr[kt][k >> 1];
+					kf = k & 1 ? codes8(w.z, w.w) : codes8(w.x, w.y);
+				} else {
+					kf = __builtin_bit_cast(h8, kr[kt][k]);
 				}
-			} else {
-				const u4 *kr = reinterpret_cast<const u4 *>(c.k + (at * PAGE + row) * HD * 2) + g;
-#pragma unroll
-				for (int q = 0; q < KS; q++)
-					kf[q] = __builtin_bit_cast(h8, kr[q * 4]);
+				lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[k], lo, 0, 0, 0);
+				hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[k], hi, 0, 0, 0);
 			}
-#pragma unroll
-			for (int t = 0; t < NT; t++) {
-				f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-				for (int k = 0; k < KS; k++)
-					acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], ql[t][k], acc, 0, 0, 0);
-#pragma unroll
-				for (int k = 0; k < KS; k++)
-					acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[k], qh[t][k], acc, 0, 0, 0);
-				sc[t][kt] = acc;
-			}
+			sc[kt] = lo + hi;
+			kk[kt] = ks[kt];
 		}
-
-		// the scales of this lane's 16 rows
-		f4 vsc[4];
-		float vinv = P_SCALE;
+		if (more)
+			get_k(next, step + WK);
+		f4 vv[KT];
 		if constexpr (I8) {
-			const f4 *ks = reinterpret_cast<const f4 *>(c.ks + at * PAGE + g * 16);
-			const f4 *vs = reinterpret_cast<const f4 *>(c.vs + at * PAGE + g * 16);
 			float top = 0.0f;
 #pragma unroll
-			for (int kt = 0; kt < 4; kt++) {
-				const f4 k4 = ks[kt];
-				vsc[kt] = vs[kt];
+			for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-				for (int i = 0; i < 4; i++) {
-					const bool there = g * 16 + kt * 4 + i < end;
-					top = __builtin_fmaxf(top, there ? vsc[kt][i] : 0.0f);
+				for (int i = 0; i < 4; i++)
+					top = __builtin_fmaxf(top, whole || g * 16 + kt * 4 + i < end ? vs[kt][i] : 0.0f);
+			move_vtop<HD, 1>(top, vtop, r);
+			const float inv = P_SCALE / vtop;
 #pragma unroll
-					for (int t = 0; t < NT; t++)
-						sc[t][kt][i] *= k4[i];
-				}
-			}
-			top = max_g(top);
-			if (top > vtop) { // (the same in every lane)
-				const float to = pow2_below(top) * 2.0f, f = vtop / to;
-				vtop = to;
-#pragma unroll
-				for (int t = 0; t < NT; t++)
-#pragma unroll
-					for (int m = 0; m < MT; m++)
-						o[t][m] *= f;
-			}
-			vinv = P_SCALE / vtop;
+			for (int kt = 0; kt < KT; kt++)
+				vv[kt] = vs[kt] * inv;
 		}
-
-		// weights, in two f16 parts
-		h8 ph[NT][2], pl[NT][2];
-#pragma unroll
-		for (int t = 0; t < NT; t++) {
-			float top = -__builtin_inff();
-			const uint32_t bits = (uint32_t)(vis[t] >> (16 * g)) & 0xffffu;
-#pragma unroll
-			for (int kt = 0; kt < 4; kt++)
-#pragma unroll
-				for (int i = 0; i < 4; i++) {
-					float z = sc[t][kt][i] * qs[t];
-					if (!whole && !(bits >> (4 * kt + i) & 1))
-						z = -__builtin_inff();
-					sc[t][kt][i] = z;
-					top = __builtin_fmaxf(top, z);
-				}
-			top = __builtin_fmaxf(mx[t], max_g(top));
-			const float base = top == -__builtin_inff() ? 0.0f : top;
-			const float f = __builtin_amdgcn_exp2f(mx[t] - base);
-			mx[t] = top;
-			float add = 0.0f;
-#pragma unroll
-			for (int kt = 0; kt < 4; kt++) {
-				float w[4];
-#pragma unroll
-				for (int i = 0; i < 4; i++) {
-					w[i] = __builtin_amdgcn_exp2f(sc[t][kt][i] - base);
-					add += w[i];
-					if constexpr (I8) {
-						w[i] *= vsc[kt][i] * vinv;
-						if (!whole && !(bits >> (4 * kt + i) & 1))
-							w[i] = 0.0f;
-					} else {
-						w[i] *= P_SCALE;
-					}
-				}
-#pragma unroll
-				for (int i = 0; i < 4; i += 2) {
-					h2 hi, lo;
-					split2(w[i], w[i + 1], hi, lo);
-					const int e = (kt & 1) * 4 + i;
-					ph[t][kt >> 1][e] = hi.x, ph[t][kt >> 1][e + 1] = hi.y;
-					pl[t][kt >> 1][e] = lo.x, pl[t][kt >> 1][e + 1] = lo.y;
-				}
-			}
-			sum[t] = sum[t] * f + add;
-			if (!__all(f == 1.0f))
-#pragma unroll
-				for (int m = 0; m < MT; m++)
-					o[t][m] *= f;
-		}
-
-		// O^T
+		h8 ph[KT / 2], pl[KT / 2];
+		weigh<HD, I8, KT>(r[0], sc, kk, vv, qs, (uint32_t)(vis >> (4 * KT * g)), whole, ph, pl);
 #pragma unroll
 		for (int m = 0; m < MT; m++) {
-			const size_t col = at * HD + m * 16 + n16;
-			h8 vf[2];
 			if constexpr (I8) {
-				const u4 w = *(reinterpret_cast<const u4 *>(c.v + col * PAGE) + g);
-				vf[0] = codes8(w.x, w.y);
-				vf[1] = codes8(w.z, w.w);
+				const h8 v0 = codes8(vr[m].x, vr[m].y), v1 = codes8(vr[m].z, vr[m].w);
+				r[0].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], r[0].o[m], 0, 0, 0);
+				r[0].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[KT / 2 - 1], r[0].o[m], 0, 0, 0);
+				r[0].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], r[0].o[m], 0, 0, 0);
+				r[0].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[KT / 2 - 1], r[0].o[m], 0, 0, 0);
 			} else {
-				const u4 *vr = reinterpret_cast<const u4 *>(c.v + col * PAGE * 2) + 2 * g;
-				u4 w[2] = {vr[0], vr[1]};
+				u4 w = vr[m];
 				if (!whole) {
-					// a value that is not finite in a row that a token does
-					// not see would reach it as 0 * inf: such values are
-					// taken out here and come back for those that see them
-					uint32_t odd = 0;
-#pragma unroll
-					for (int q = 0; q < 2; q++)
-#pragma unroll
-						for (int e = 0; e < 4; e++) {
-							uint32_t x = w[q][e];
-							if ((x & 0x7c00u) == 0x7c00u) {
-								x &= 0xffff0000u;
-								odd |= 1u << (8 * q + 2 * e);
-							}
-							if ((x & 0x7c000000u) == 0x7c000000u) {
-								x &= 0xffffu;
-								odd |= 2u << (8 * q + 2 * e);
-							}
-							w[q][e] = x;
-						}
-					if (__any(odd != 0)) {
-						for (int r = 0; r < min(end, PAGE); r++) {
-							const int src = (r >> 4) * 16; // the lane group that has row r
-#pragma unroll
-							for (int i = 0; i < 4; i++) {
-								// (column 4 g + i of the tile: a lane of the O^T layout)
-								if (!(__shfl(odd, src + 4 * g + i) >> (r & 15) & 1))
-									continue;
-								const float v = (float)reinterpret_cast<const _Float16 *>(
-									c.v)[(at * HD + m * 16 + 4 * g + i) * PAGE + r];
-#pragma unroll
-								for (int t = 0; t < NT; t++)
-									if (vis[t] >> r & 1)
-										o[t][m][i] = v != v ? v : o[t][m][i] + v;
-							}
-						}
-					}
+					const uint32_t seen[1] = {(uint32_t)vis};
+					guard_values<HD, 1>(w, c.v + at * HD * PAGE * 2, row0, m, g, end, seen, r);
 				}
-				vf[0] = __builtin_bit_cast(h8, w[0]);
-				vf[1] = __builtin_bit_cast(h8, w[1]);
+				const h8 v0 = __builtin_bit_cast(h8, w);
+				r[0].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], r[0].o[m], 0, 0, 0);
+				r[0].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], r[0].o[m], 0, 0, 0);
 			}
-#pragma unroll
-			for (int t = 0; t < NT; t++)
-#pragma unroll
-				for (int q = 0; q < 2; q++) {
-					o[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[q], pl[t][q], o[t][m], 0, 0, 0);
-					o[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[q], ph[t][q], o[t][m], 0, 0, 0);
-				}
 		}
+		if (more)
+			get_v(next, step + WK);
+		at = next;
 	}
 	const float back = I8 ? vtop / P_SCALE : 1.0f / P_SCALE;
 
-	// join the waves: each puts its rows into LDS ([wave][row][HD + 2])
-	constexpr int LR = HD + 4;
-	float *mine = lds + (size_t)wave * R * LR;
+	// join the waves: each puts its rows into LDS ([wave][row][HD + 4])
+	constexpr int LR = part_row(HD);
+	float *mine = lds + ((size_t)wave * R + n16) * LR;
+	const float total = sum_g(r[0].sum);
 #pragma unroll
-	for (int t = 0; t < NT; t++) {
-		const float total = sum_g(sum[t]);
-		float *row = mine + (16 * t + n16) * LR;
-#pragma unroll
-		for (int m = 0; m < MT; m++)
-			*reinterpret_cast<f4 *>(row + m * 16 + 4 * g) = o[t][m] * back;
-		if (g == 0) {
-			row[HD] = bad ? __builtin_nanf("") : mx[t];
-			row[HD + 1] = bad ? __builtin_nanf("") : total;
-		}
+	for (int m = 0; m < MT; m++)
+		*reinterpret_cast<f4 *>(mine + m * 16 + 4 * g) = r[0].o[m] * back;
+	if (g == 0) {
+		mine[HD] = bad ? __builtin_nanf("") : r[0].mx;
+		mine[HD + 1] = bad ? __builtin_nanf("") : total;
 	}
 	__syncthreads();
 	for (int e = threadIdx.x; e < R * HD; e += 64 * WK) {
-		const int r = e / HD, i = e % HD, at = u.tile * R + r;
-		if (at / group >= u.n)
+		const int q = e / HD, i = e % HD, to = u.tile * R + q;
+		if (to / group >= u.n)
 			continue;
 		float m = -__builtin_inff(), l = 0.0f, x = 0.0f;
 #pragma unroll
 		for (int w = 0; w < WK; w++)
-			m = __builtin_fmaxf(m, lds[((size_t)w * R + r) * LR + HD]);
+			m = __builtin_fmaxf(m, lds[((size_t)w * R + q) * LR + HD]);
 		const float base = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
 		for (int w = 0; w < WK; w++) {
-			const float *row = lds + ((size_t)w * R + r) * LR;
-			const float f = __builtin_amdgcn_exp2f(row[HD] - base);
-			l += row[HD + 1] * f;
-			x += row[i] * f;
+			const float *from = lds + ((size_t)w * R + q) * LR;
+			const float f = __builtin_amdgcn_exp2f(from[HD] - base);
+			l += from[HD + 1] * f;
+			x += from[i] * f;
 		}
 		if (u.parts == 1) {
-			a.out[(size_t)(u.t0 + at / group) * a.o_stride + (size_t)(u.head * group + at % group) * HD + i] =
+			a.out[(size_t)(u.t0 + to / group) * a.o_stride + (size_t)(u.head * group + to % group) * HD + i] =
 				l == 0.0f ? 0.0f : x / l;
 		} else {
-			float *pr = part + (size_t)u.index * part_floats(R, HD) + (size_t)r * (HD + 2);
+			float *pr = part + ((size_t)blockIdx.x * R + q) * LR;
 			pr[i] = x;
 			if (i == 0) {
 				pr[HD] = m;
@@ -499,40 +590,294 @@ __global__ __launch_bounds__(64 * WK) void attn_kernel(KvLayer c, KvSeqs s, Attn
 	}
 }
 
-// Join the parts of a tile: one workgroup for each unit that is a tile's
-// first part (a token row and head: HD threads at a time).
-template <int HD>
-__global__ __launch_bounds__(256) void attn_join_kernel(KvLayer c, KvSeqs s, AttnArgs a, int least, int R, const float *part)
+// ---------------------------------------------------------------- many rows
+// A workgroup: 128 query rows of one kv head, 32 to a wave, all over the same
+// pages: a page comes into LDS once (int8 codes as f16), while the one before
+// is worked on.  Bound by the matrix cores and the weights' arithmetic side by
+// side: two waves on a SIMD.
+//
+// LDS rows are swizzled in 16-byte pieces so that the 8 lanes that read
+// together touch all banks: K row r's piece q lies at q ^ f(r), f the lane of
+// the operand that reads the row; V column i's at q ^ (i % 8).
+constexpr int MANY_ROWS = 128, MANY_WAVES = 4;
+
+template <int HD, bool I8>
+__global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, float *part)
 {
+	constexpr int KS = HD / 32, MT = HD / 16, R = MANY_ROWS, NT = 2, KT = 2, E = I8 ? 1 : 2;
+	constexpr int NL = PAGE * HD * E / 16 / 256; // 16-byte pieces of a page's K (and V) for a thread
+	constexpr int KMASK = HD / 8 - 1;            // pieces of a K row in LDS, less one
+	__shared__ __attribute__((aligned(16))) _Float16 lk[2][PAGE * HD], lv[2][PAGE * HD];
+	__shared__ __attribute__((aligned(16))) float lsc[2][2][PAGE];
 	const int group = a.n_heads / c.kvh;
 	Unit u;
-	if (!find_unit(s, c.kvh, group, R, least, blockIdx.x, u) || u.part != 0 || u.parts == 1)
+	// (whole tiles in causal order, two to a CU: the longest with the shortest)
+	int index = blockIdx.x;
+	if (cut.whole && (int)gridDim.x <= cut.cap && index >= cut.cap / 2)
+		index = (int)gridDim.x - 1 - (index - cut.cap / 2);
+	if (!find_unit(s, c.kvh, group, cut, index, u))
 		return;
-	if ((size_t)u.index + u.parts > gridDim.x)
-		return; // (sequences that overlap: more units than the rows can have)
-	for (int e = threadIdx.x; e < R * HD; e += 256) {
-		const int r = e / HD, i = e % HD, at = u.tile * R + r;
-		if (at / group >= u.n)
-			break;
-		const float *row = part + (size_t)u.index * part_floats(R, HD) + (size_t)r * (HD + 2);
-		const size_t step = part_floats(R, HD);
-		float m = -__builtin_inff(), l = 0.0f, x = 0.0f;
-		for (int q = 0; q < u.parts; q++)
-			m = __builtin_fmaxf(m, row[q * step + HD]);
-		const float base = m == -__builtin_inff() ? 0.0f : m;
-		for (int q = 0; q < u.parts; q++) {
-			const float f = __builtin_amdgcn_exp2f(row[q * step + HD] - base);
-			l += row[q * step + HD + 1] * f;
-			x += row[q * step + i] * f;
-		}
-		a.out[(size_t)(u.t0 + at / group) * a.o_stride + (size_t)(u.head * group + at % group) * HD + i] =
-			l == 0.0f ? 0.0f : x / l;
+	const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g = lane >> 4;
+	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	bool bad = !seq_fits(s, u.len, u.n);
+
+	int node[NT];
+	h8 qh[NT][KS], ql[NT][KS];
+	float qs[NT];
+	Rows<HD> r[NT];
+#pragma unroll
+	for (int t = 0; t < NT; t++) {
+		const int row = u.tile * R + wave * 32 + 16 * t + n16;
+		node[t] = row / group < u.n ? row / group : -1;
+		load_query<HD, false>(a, u, node[t], u.head * group + row % group, g, qh[t], ql[t], qs[t]);
+#pragma unroll
+		for (int m = 0; m < MT; m++)
+			r[t].o[m] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 	}
+	float vtop = 1e-30f;
+
+	const int last = a.mask ? u.n : min(u.n, (u.tile * R + R - 1) / group + 1);
+	const int pages = bad ? 0 : (u.len + last + PAGE - 1) / PAGE;
+	const int p0 = u.part * u.chunk, p1 = min(pages, p0 + min(u.chunk, pages));
+	u4 kr[NL], vr[NL];
+	float sr = 0.0f;
+	auto page = [&](int p) {
+		const int id = page_of(s, c.n_pages, u.b, p * PAGE);
+		bad = bad || id < 0;
+		return (size_t)(id < 0 ? 0 : id) * c.kvh + u.head;
+	};
+	auto get = [&](size_t pg) {
+		const u4 *k = reinterpret_cast<const u4 *>(c.k + pg * PAGE * HD * E) + tid;
+		const u4 *v = reinterpret_cast<const u4 *>(c.v + pg * PAGE * HD * E) + tid;
+#pragma unroll
+		for (int q = 0; q < NL; q++) {
+			kr[q] = k[q * 256];
+			vr[q] = v[q * 256];
+		}
+		if (I8 && tid < 2 * PAGE)
+			sr = tid < PAGE ? c.ks[pg * PAGE + tid] : c.vs[pg * PAGE + tid - PAGE];
+	};
+	auto put = [&](int b) {
+#pragma unroll
+		for (int q = 0; q < NL; q++) {
+			const int e = tid + q * 256;
+			const int kw = HD * E / 16, krow = e / kw, kp = e % kw; // pieces of a row in memory
+			const int vw = PAGE * E / 16, vcol = e / vw, vp = e % vw;
+			const int kx = (krow & 3) | (krow >> 3 & 3) << 2, vx = vcol & 7;
+			h8 *ko = reinterpret_cast<h8 *>(lk[b] + krow * HD), *vo = reinterpret_cast<h8 *>(lv[b] + vcol * PAGE);
+			if constexpr (I8) {
+				ko[(2 * kp ^ kx) & KMASK] = codes8(kr[q].x, kr[q].y);
+				ko[((2 * kp + 1) ^ kx) & KMASK] = codes8(kr[q].z, kr[q].w);
+				vo[2 * vp ^ vx] = codes8(vr[q].x, vr[q].y);
+				vo[(2 * vp + 1) ^ vx] = codes8(vr[q].z, vr[q].w);
+			} else {
+				ko[(kp ^ kx) & KMASK] = __builtin_bit_cast(h8, kr[q]);
+				vo[vp ^ vx] = __builtin_bit_cast(h8, vr[q]);
+			}
+		}
+		if (I8 && tid < 2 * PAGE)
+			lsc[b][tid >> 6][tid & 63] = sr;
+	};
+	size_t at = 0;
+	if (p0 < p1) {
+		at = page(p0);
+		get(at);
+		put(0);
+	}
+	__syncthreads();
+	for (int p = p0; p < p1; p++) {
+		const int b = (p - p0) & 1, start = p * PAGE, end = u.len + u.n - start;
+		const bool more = p + 1 < p1;
+		const size_t next = more ? page(p + 1) : at;
+		if (more)
+			get(next);
+		uint64_t vis[NT];
+#pragma unroll
+		for (int t = 0; t < NT; t++)
+			vis[t] = sees(a, u, node[t], start);
+#pragma unroll 1
+		for (int row0 = 0; row0 < PAGE; row0 += 32) {
+			uint32_t seen[NT];
+			bool whole = true, any = false;
+#pragma unroll
+			for (int t = 0; t < NT; t++) {
+				seen[t] = (uint32_t)(vis[t] >> row0);
+				whole = whole && (seen[t] == ~0u || node[t] < 0);
+				any = any || seen[t] != 0;
+			}
+			if (!__any(any))
+				continue;
+			whole = __all(whole);
+			f4 sc[NT][KT];
+#pragma unroll
+			for (int kt = 0; kt < KT; kt++) {
+				const _Float16 *kl = lk[b] + (row0 + (n16 >> 2) * 8 + kt * 4 + (n16 & 3)) * HD;
+#pragma unroll
+				for (int t = 0; t < NT; t++)
+					sc[t][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+				for (int k = 0; k < KS; k++) {
+					const h8 kf = reinterpret_cast<const h8 *>(kl)[((k * 4 + g) ^ n16) & KMASK];
+#pragma unroll
+					for (int t = 0; t < NT; t++)
+						sc[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[t][k], sc[t][kt], 0, 0, 0);
+#pragma unroll
+					for (int t = 0; t < NT; t++)
+						sc[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[t][k], sc[t][kt], 0, 0, 0);
+				}
+			}
+			f4 ks[KT], vs[KT];
+			if constexpr (I8) {
+				float top = 0.0f;
+#pragma unroll
+				for (int kt = 0; kt < KT; kt++) {
+					ks[kt] = reinterpret_cast<const f4 *>(lsc[b][0] + row0 + g * 8)[kt];
+					vs[kt] = reinterpret_cast<const f4 *>(lsc[b][1] + row0 + g * 8)[kt];
+#pragma unroll
+					for (int i = 0; i < 4; i++)
+						top = __builtin_fmaxf(top, whole || row0 + g * 8 + kt * 4 + i < end ? vs[kt][i] : 0.0f);
+				}
+				move_vtop<HD, NT>(top, vtop, r);
+				const float inv = P_SCALE / vtop;
+#pragma unroll
+				for (int kt = 0; kt < KT; kt++)
+					vs[kt] *= inv;
+			}
+			h8 ph[NT][1], pl[NT][1];
+#pragma unroll
+			for (int t = 0; t < NT; t++)
+				weigh<HD, I8, KT>(r[t], sc[t], ks, vs, qs[t], seen[t] >> (8 * g), whole, ph[t], pl[t]);
+#pragma unroll
+			for (int m = 0; m < MT; m++) {
+				const u4 *vl = reinterpret_cast<const u4 *>(lv[b] + (m * 16 + n16) * PAGE);
+				u4 w = vl[(row0 / 8 + g) ^ (n16 & 7)];
+				if constexpr (!I8)
+					if (!whole)
+						guard_values<HD, NT>(w, c.v + at * HD * PAGE * 2, row0, m, g, end - row0, seen, r);
+				const h8 vf = __builtin_bit_cast(h8, w);
+#pragma unroll
+				for (int t = 0; t < NT; t++)
+					r[t].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t][0], r[t].o[m], 0, 0, 0);
+#pragma unroll
+				for (int t = 0; t < NT; t++)
+					r[t].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t][0], r[t].o[m], 0, 0, 0);
+			}
+		}
+		if (more)
+			put(b ^ 1); // (all waves left that buffer at the last barrier)
+		__syncthreads();
+		at = next;
+	}
+	const float back = I8 ? vtop / P_SCALE : 1.0f / P_SCALE;
+#pragma unroll
+	for (int t = 0; t < NT; t++) {
+		const float total = sum_g(r[t].sum);
+		const int q = wave * 32 + 16 * t + n16, to = u.tile * R + q;
+		if (node[t] < 0)
+			continue;
+		float *o = part + ((size_t)index * R + q) * part_row(HD);
+		float f = back;
+		if (u.parts == 1) {
+			o = a.out + (size_t)(u.t0 + to / group) * a.o_stride + (size_t)(u.head * group + to % group) * HD;
+			f = bad ? __builtin_nanf("") : total == 0.0f ? 0.0f : back / total;
+		} else if (g == 0) {
+			o[HD] = bad ? __builtin_nanf("") : r[t].mx;
+			o[HD + 1] = bad ? __builtin_nanf("") : total;
+		}
+		const bool vec = ((uintptr_t)o & 15) == 0;
+#pragma unroll
+		for (int m = 0; m < MT; m++) {
+			const f4 x = total == 0.0f && u.parts == 1 && !bad ? (f4){0.0f, 0.0f, 0.0f, 0.0f} : r[t].o[m] * f;
+			if (vec) {
+				*reinterpret_cast<f4 *>(o + m * 16 + 4 * g) = x;
+			} else {
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					o[m * 16 + 4 * g + i] = x[i];
+			}
+		}
+	}
+}
+
+// ---------------------------------------------------------------- join
+// The parts of one token row and query head: a workgroup, HD / 4 lanes to a
+// part, 1024 / HD parts at a time.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_join_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, int units, const float *part)
+{
+	constexpr int L = HD / 4, G = 256 / L, PR = part_row(HD);
+	__shared__ float lm[G], ll[G];
+	__shared__ f4 lo[G][L];
+	const int group = a.n_heads / c.kvh, t = blockIdx.x, h = blockIdx.y, head = h / group;
+	int st0, sn;
+	const int b = seq_of_token(s, t, st0, sn);
+	if (b < 0)
+		return;
+	// the sequence's units: those of the sequences before it come first
+	const int lane = threadIdx.x & 63;
+	int t0, n, len, tiles, pages;
+	seq_work(s, lane, group, cut.rows, t0, n, len, tiles, pages);
+	const int chunk = unit_chunk(s, c.kvh, group, cut, tiles, pages);
+	int before = 0;
+	for (int b0 = 0; b0 <= b; b0 += 64) {
+		if (b0)
+			seq_work(s, b0 + lane, group, cut.rows, t0, n, len, tiles, pages);
+		before += s.n_seqs > 1 ? wave_sum(b0 + lane < b && tiles ? tiles * div_up(pages, chunk) * c.kvh : 0) : 0;
+	}
+	seq_work(s, b, group, cut.rows, t0, n, len, tiles, pages);
+	const int parts = div_up(pages, chunk);
+	if (parts == 1)
+		return;
+	const int row = (t - t0) * group + h % group, tile = row / cut.rows;
+	const int u0 = before + ((tiles - 1 - tile) * parts) * c.kvh + head; // unit of part q: u0 + q kvh
+	if (u0 < 0 || (long long)u0 + (long long)(parts - 1) * c.kvh >= units)
+		return; // (sequences that overlap: more units than the rows can have)
+	const float *from = part + ((size_t)u0 * cut.rows + row % cut.rows) * PR;
+	const size_t step = (size_t)c.kvh * cut.rows * PR;
+	const int pg = threadIdx.x / L, i = threadIdx.x % L;
+	float m = -__builtin_inff(), l = 0.0f;
+	f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+	for (int q = pg; q < parts; q += G) {
+		const float *pr = from + q * step;
+		const f4 o = reinterpret_cast<const f4 *>(pr)[i];
+		const float pm = pr[HD], pl = pr[HD + 1];
+		const float top = __builtin_fmaxf(m, pm), base = top == -__builtin_inff() ? 0.0f : top;
+		const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(pm - base);
+		m = top;
+		l = l * f0 + pl * f1;
+		x = x * f0 + o * f1;
+	}
+	lo[pg][i] = x;
+	if (i == 0) {
+		lm[pg] = m;
+		ll[pg] = l;
+	}
+	__syncthreads();
+	if (pg)
+		return;
+	float top = -__builtin_inff();
+#pragma unroll
+	for (int q = 0; q < G; q++)
+		top = __builtin_fmaxf(top, lm[q]);
+	const float base = top == -__builtin_inff() ? 0.0f : top;
+	l = 0.0f;
+	x = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+	for (int q = 0; q < G; q++) {
+		const float f = __builtin_amdgcn_exp2f(lm[q] - base);
+		l += ll[q] * f;
+		x += lo[q][i] * f;
+	}
+	float *out = a.out + (size_t)t * a.o_stride + (size_t)h * HD + 4 * i;
+#pragma unroll
+	for (int q = 0; q < 4; q++)
+		out[q] = l == 0.0f ? 0.0f : x[q] / l;
 }
 
 // ---------------------------------------------------------------- launch
 struct Shape {
-	int nt, wk, least;
+	bool few;
+	Cut cut;
 	size_t units; // at most
 };
 
@@ -540,29 +885,39 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 {
 	const size_t group = a.n_heads / c.kvh, rows = (size_t)s.n_tokens * group;
 	Shape h;
-	const size_t avg = rows / s.n_seqs;
-	h.nt = avg <= 16 ? 1 : avg <= 32 ? 2 : 4;
-	h.wk = h.nt == 1 ? 8 : 4;
-	h.least = h.wk;
-	h.units = ATTN_UNITS + (rows / (16 * h.nt) + s.n_seqs) * c.kvh;
+	h.few = rows <= (size_t)FEW_ROWS * s.n_seqs;
+	h.cut.rows = h.few ? FEW_ROWS : MANY_ROWS;
+	// one workgroup of 8 waves on a CU, or two of 4
+	h.cut.cap = h.few ? 256 : 512;
+	h.cut.least = h.few ? FEW_WAVES : 2;
+	const size_t tiles = (rows + (size_t)s.n_seqs * (h.cut.rows - 1)) / h.cut.rows;
+	// as many tiles as fill the card are not cut: no parts, no join
+	h.cut.whole = rows / h.cut.rows * c.kvh >= (size_t)h.cut.cap;
+	h.units = (h.cut.whole ? 0 : h.cut.cap) + tiles * c.kvh;
 	return h;
 }
 
 size_t attention_work_bytes(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 {
 	const Shape h = attn_shape(c, s, a);
-	return h.units * part_floats(16 * h.nt, c.hd) * sizeof(float);
+	return h.cut.whole ? 256 : h.units * h.cut.rows * part_row(c.hd) * sizeof(float);
 }
 
-template <int HD, bool I8, int NT, int WK>
+template <int HD, bool I8>
 static hipError_t go(const Shape &h, const KvLayer &c, const KvSeqs &s, const AttnArgs &a, float *part, hipStream_t st)
 {
-	const size_t lds = (size_t)WK * 16 * NT * (HD + 4) * sizeof(float);
-	const hipError_t e = ensure_lds_limit((const void *)attn_kernel<HD, I8, NT, WK>, lds);
-	if (e != hipSuccess)
-		return e;
-	tie_launch(attn_kernel<HD, I8, NT, WK>, dim3(h.units), dim3(64 * WK), lds, st, c, s, a, h.least, part);
-	tie_launch(attn_join_kernel<HD>, dim3(h.units), dim3(256), 0, st, c, s, a, h.least, 16 * NT, (const float *)part);
+	if (h.few) {
+		const size_t lds = (size_t)FEW_WAVES * FEW_ROWS * part_row(HD) * sizeof(float);
+		const hipError_t e = ensure_lds_limit((const void *)attn_few_kernel<HD, I8>, lds);
+		if (e != hipSuccess)
+			return e;
+		tie_launch(attn_few_kernel<HD, I8>, dim3(h.units), dim3(64 * FEW_WAVES), lds, st, c, s, a, h.cut, part);
+	} else {
+		tie_launch(attn_many_kernel<HD, I8>, dim3(h.units), dim3(64 * MANY_WAVES), 0, st, c, s, a, h.cut, part);
+	}
+	if (!h.cut.whole)
+		tie_launch(attn_join_kernel<HD>, dim3(s.n_tokens, a.n_heads), dim3(256), 0, st, c, s, a, h.cut, (int)h.units,
+			   (const float *)part);
 	return hipGetLastError();
 }
 
@@ -570,13 +925,9 @@ hipError_t launch_attention(const KvLayer &c, const KvSeqs &s, const AttnArgs &a
 {
 	const Shape h = attn_shape(c, s, a);
 	float *part = reinterpret_cast<float *>(work);
-#define TIE_ATTN(HD, I8)                                                             \
-	(h.nt == 1 ? go<HD, I8, 1, 8>(h, c, s, a, part, st)                         \
-	 : h.nt == 2 ? go<HD, I8, 2, 4>(h, c, s, a, part, st) : go<HD, I8, 4, 4>(h, c, s, a, part, st))
 	if (c.hd == 128)
-		return c.i8 ? TIE_ATTN(128, true) : TIE_ATTN(128, false);
-	return c.i8 ? TIE_ATTN(64, true) : TIE_ATTN(64, false);
-#undef TIE_ATTN
+		return c.i8 ? go<128, true>(h, c, s, a, part, st) : go<128, false>(h, c, s, a, part, st);
+	return c.i8 ? go<64, true>(h, c, s, a, part, st) : go<64, false>(h, c, s, a, part, st);
 }
 
 } // namespace tie
