@@ -20,6 +20,8 @@
 //
 // The maximum m is a reference only: it moves when some weight would pass
 // 2^MOVE, so most steps need no exchange between lanes and leave O alone.
+#include <type_traits>
+
 #include "kv.h"
 
 namespace tie {
@@ -30,7 +32,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float MOVE = 3.0f;       // log2 of the largest weight
-constexpr float P_SCALE = 4096.0f; // with it the weights stay below the f16 limit, their second parts above the subnormals
+constexpr float P_LOG2 = 12.0f;    // weights times 2^12 stay below the f16 limit, their second parts above the subnormals
 
 // four int8 codes to f16: 1024 + (code + 128) is the f16 0x6400 | byte, from
 // which 1152 is taken exactly
@@ -58,7 +60,43 @@ __device__ __forceinline__ void split2(float x0, float x1, h2 &hi, h2 &lo)
 {
 	typedef float f2 __attribute__((ext_vector_type(2)));
 	hi = __builtin_convertvector((f2){x0, x1}, h2);
-	lo = __builtin_convertvector((f2){x0 - (float)hi.x, x1 - (float)hi.y}, h2);
+	lo = __builtin_convertvector((f2){__builtin_fmaf((float)hi.x, -1.0f, x0), __builtin_fmaf((float)hi.y, -1.0f, x1)}, h2);
+}
+
+// 16 bytes for each lane from base (the same in all lanes) + off to lds + 16 *
+// lane (lds: the same in all lanes).  In assembly, so that the compiler does not
+// hold back reads of the other buffer for it; the caller waits (s_waitcnt)
+// before the barrier that hands the buffer over.
+__device__ __forceinline__ void load_lds16(const void *base, uint32_t off, const void *lds)
+{
+	const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds); // (the low half of a shared address is its offset)
+	asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to) : "memory", "m0");
+}
+
+// x of lane N of the lane's group of 16
+template <int N> __device__ __forceinline__ float lane16(float x)
+{
+	return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x150 + N, 0xf, 0xf, true));
+}
+
+// v[t][i] *= the s of lane 4 t + i of the group of 16: a lane's 4 KT rows times
+// their scales, of which each lane holds one
+template <int KT> __device__ __forceinline__ void times_rows(float (&v)[4 * KT], float s)
+{
+	v[0] *= lane16<0>(s), v[1] *= lane16<1>(s), v[2] *= lane16<2>(s), v[3] *= lane16<3>(s);
+	v[4] *= lane16<4>(s), v[5] *= lane16<5>(s), v[6] *= lane16<6>(s), v[7] *= lane16<7>(s);
+	if constexpr (KT == 4) {
+		v[8] *= lane16<8>(s), v[9] *= lane16<9>(s), v[10] *= lane16<10>(s), v[11] *= lane16<11>(s);
+		v[12] *= lane16<12>(s), v[13] *= lane16<13>(s), v[14] *= lane16<14>(s), v[15] *= lane16<15>(s);
+	}
+}
+
+// a pointer that is the same in all lanes, in scalar registers
+__device__ __forceinline__ const uint8_t *uniform(const uint8_t *p)
+{
+	const uint64_t x = (uint64_t)p;
+	const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+	return (const uint8_t *)((uint64_t)hi << 32 | lo);
 }
 
 // max over the four lanes of a query (lane, +16, +32, +48)
@@ -264,7 +302,8 @@ __device__ __forceinline__ void load_query(const AttnArgs &a, const Unit &u, int
 	m = max_g(m);
 	const float p2 = m >= 1e-30f && m < 1e30f ? pow2_below(m) : 1.0f;
 	const float up = __builtin_copysignf(512.0f / p2, a.scale);
-	qs = __builtin_fabsf(a.scale) * 1.44269504088896f * (p2 * (1.0f / 512.0f));
+	// (not 0: the score of a row that is not seen, -inf, stays that)
+	qs = __builtin_fmaxf(__builtin_fabsf(a.scale) * 1.44269504088896f * (p2 * (1.0f / 512.0f)), 1.2e-38f);
 #pragma unroll
 	for (int k = 0; k < HD / 32; k++)
 #pragma unroll
@@ -286,32 +325,32 @@ struct Rows {
 
 // From the products sc of 16 KT cache rows to the weights' two f16 parts for
 // the second product; the state's reference and sum, and O where the reference
-// moved.  bits: which of the lane's 4 KT rows its query sees (whole: all of them
-// for every query of the wave).  int8: ks are the rows' K scales, vs their V
-// scales over the running power of two.
+// moved.  whole: every query of the wave sees all the rows; else bits: which of
+// the lane's 4 KT rows its query sees (the weights of the others are 0).  int8:
+// ks and vs are the K and V scale of the lane's row (lane 4 t + i of 16: row 4 t
+// + i of the group's), vs finite unless whole, and none above 2^vlog, which
+// the weights are divided by.  Weights and sum carry 2^(P_LOG2 - vlog), by way
+// of the exponent.
 template <int HD, bool I8, int KT>
-__device__ __forceinline__ void weigh(Rows<HD> &r, f4 (&sc)[KT], const f4 (&ks)[KT], const f4 (&vs)[KT], float qs, uint32_t bits,
-				      bool whole, h8 (&ph)[KT / 2], h8 (&pl)[KT / 2])
+__device__ __forceinline__ void weigh(Rows<HD> &r, const f4 (&sc)[KT], float ks, float vs, float vlog, float qs, bool whole,
+				      uint32_t bits, h8 (&ph)[KT / 2], h8 (&pl)[KT / 2])
 {
-	if (I8)
+	float w[4 * KT];
 #pragma unroll
-		for (int kt = 0; kt < KT; kt++)
-			sc[kt] *= ks[kt];
+	for (int e = 0; e < 4 * KT; e++)
+		w[e] = sc[e / 4][e % 4];
+	if (I8)
+		times_rows<KT>(w, ks);
 	if (!whole)
 #pragma unroll
-		for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-			for (int i = 0; i < 4; i++)
-				if (!(bits >> (4 * kt + i) & 1))
-					sc[kt][i] = -__builtin_inff();
+		for (int e = 0; e < 4 * KT; e++)
+			if (!(bits >> e & 1))
+				w[e] = -__builtin_inff();
 	float top = -__builtin_inff();
 #pragma unroll
-	for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-		for (int i = 0; i < 4; i++)
-			top = __builtin_fmaxf(top, sc[kt][i]);
-	// (qs may be 0: 0 * -inf would be NaN)
-	top = top == -__builtin_inff() ? top : top * qs;
+	for (int e = 0; e < 4 * KT; e++)
+		top = __builtin_fmaxf(top, w[e]);
+	top *= qs;
 	if (__any(top > r.mx + MOVE)) {
 		top = __builtin_fmaxf(r.mx, max_g(top));
 		const float f = r.mx == top ? 1.0f : __builtin_amdgcn_exp2f(r.mx - top);
@@ -321,45 +360,55 @@ __device__ __forceinline__ void weigh(Rows<HD> &r, f4 (&sc)[KT], const f4 (&ks)[
 		for (int m = 0; m < HD / 16; m++)
 			r.o[m] *= f;
 	}
-	const float base = r.mx == -__builtin_inff() ? 0.0f : r.mx;
+	const float base = (r.mx == -__builtin_inff() ? 0.0f : r.mx) + (I8 ? vlog - P_LOG2 : -P_LOG2);
 #pragma unroll
-	for (int kt = 0; kt < KT; kt++) {
-		float w[4];
+	for (int e = 0; e < 4 * KT; e++) {
+		w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[e], qs, -base));
+		r.sum += w[e];
+	}
+	if (I8)
+		times_rows<KT>(w, vs);
 #pragma unroll
-		for (int i = 0; i < 4; i++) {
-			const bool on = whole || (bits >> (4 * kt + i) & 1);
-			w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], qs, -base));
-			w[i] = on ? w[i] : 0.0f;
-			r.sum += w[i];
-			w[i] *= I8 ? vs[kt][i] : P_SCALE;
-			if (I8)
-				w[i] = on ? w[i] : 0.0f; // (the scale of a row that is not seen may be anything)
-		}
-#pragma unroll
-		for (int i = 0; i < 4; i += 2) {
-			h2 hi, lo;
-			split2(w[i], w[i + 1], hi, lo);
-			const int e = (kt & 1) * 4 + i;
-			ph[kt >> 1][e] = hi.x, ph[kt >> 1][e + 1] = hi.y;
-			pl[kt >> 1][e] = lo.x, pl[kt >> 1][e + 1] = lo.y;
-		}
+	for (int e = 0; e < 4 * KT; e += 2) {
+		h2 hi, lo;
+		split2(w[e], w[e + 1], hi, lo);
+		ph[e / 8][e % 8] = hi.x, ph[e / 8][e % 8 + 1] = hi.y;
+		pl[e / 8][e % 8] = lo.x, pl[e / 8][e % 8 + 1] = lo.y;
 	}
 }
 
-// int8: the largest power of two among the V scales of the rows so far (vtop;
-// it grows seldom, and O shrinks with it).  top: the largest of the lane's rows
-// that hold anything.
-template <int HD, int NT>
-__device__ __forceinline__ void move_vtop(float top, float &vtop, Rows<HD> (&r)[NT])
+// int8 rows of which some queries do not see some, or that hold nothing (!
+// there): a V scale that is not finite would reach queries that do not see its
+// row as 0 * inf.  The K scale takes its place, so that those that see the row
+// get NaN.
+__device__ __forceinline__ void guard_scales(float &ks, float &vs, bool there)
 {
-	if (__any(top > vtop)) {
-		const float to = pow2_below(__builtin_fmaxf(max_g(top), vtop)) * 2.0f, f = vtop / to;
-		vtop = to;
+	if (!(__builtin_fabsf(vs) < __builtin_inff()) || !there) {
+		vs = 0.0f;
+		ks = __builtin_nanf("");
+	}
+}
+
+// int8: 2^vlog is a power of two above all V scales so far; it grows seldom, and
+// O and the sum shrink with it.  vs: the scale of the lane's row.
+template <int HD, int NT> __device__ __forceinline__ void move_vlog(float vs, float &vlog, Rows<HD> (&r)[NT])
+{
+	if (__any(vs > __builtin_amdgcn_exp2f(vlog))) {
+		float top = vs;
 #pragma unroll
-		for (int t = 0; t < NT; t++)
+		for (int m = 1; m < 64; m <<= 1)
+			top = __builtin_fmaxf(top, __shfl_xor(top, m));
+		// (the exponent of a finite value, one above)
+		const float to = (float)((int)(__float_as_uint(top) >> 23 & 0xff) - 126);
+		const float f = __builtin_amdgcn_exp2f(vlog - to);
+		vlog = to;
+#pragma unroll
+		for (int t = 0; t < NT; t++) {
+			r[t].sum *= f;
 #pragma unroll
 			for (int m = 0; m < HD / 16; m++)
 				r[t].o[m] *= f;
+		}
 	}
 }
 
@@ -404,6 +453,26 @@ __device__ __forceinline__ void guard_values(u4 &w, const uint8_t *v, int row0, 
 	}
 }
 
+// The values of a page that are not finite, to the queries that see their
+// rows (inf and NaN stay what they are whatever a weight).
+template <int HD, int NT>
+__device__ __forceinline__ void give_back(const uint8_t *v, int g, int end, const uint64_t (&vis)[NT], Rows<HD> (&r)[NT])
+{
+	for (int row = 0; row < min(end, PAGE); row++)
+#pragma unroll
+		for (int m = 0; m < HD / 16; m++)
+#pragma unroll
+			for (int i = 0; i < 4; i++) {
+				const float x = (float)reinterpret_cast<const _Float16 *>(v)[(m * 16 + 4 * g + i) * PAGE + row];
+				if (__builtin_fabsf(x) < __builtin_inff())
+					continue;
+#pragma unroll
+				for (int t = 0; t < NT; t++)
+					if (vis[t] >> row & 1)
+						r[t].o[m][i] += x;
+			}
+}
+
 // ---------------------------------------------------------------- few rows
 // A workgroup: 16 query rows (a row: a token and one query head of the unit's
 // kv head), its 8 waves taking the unit's pages in turn.  Bound by the stream of
@@ -436,10 +505,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 	const int p0 = u.part * u.chunk, steps = (min(pages, p0 + min(u.chunk, pages)) - p0) * SP;
 
 	u4 kr[KT][KL], vr[MT];
-	f4 ks[KT], vs[KT];
+	float ks = 0.0f, vs = 0.0f; // int8: the scales of the lane's row
 	size_t at = 0; // of the page whose V is in (or on its way to) vr
 	auto page = [&](int step) {
-		const int id = page_of(s, c.n_pages, u.b, (p0 + step / SP) * PAGE);
+		const int id = __builtin_amdgcn_readfirstlane(page_of(s, c.n_pages, u.b, (p0 + step / SP) * PAGE));
 		bad = bad || id < 0;
 		return (size_t)(id < 0 ? 0 : id) * c.kvh + u.head;
 	};
@@ -452,18 +521,16 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 #pragma unroll
 			for (int e = 0; e < KL; e++)
 				kr[kt][e] = p[e * 4];
-			if (I8)
-				ks[kt] = reinterpret_cast<const f4 *>(c.ks + pg * PAGE + g * 16)[kt];
 		}
+		if (I8)
+			ks = c.ks[pg * PAGE + lane];
 	};
 	auto get_v = [&](size_t pg, int step) {
 #pragma unroll
 		for (int m = 0; m < MT; m++)
 			vr[m] = reinterpret_cast<const u4 *>(c.v + (pg * HD + m * 16 + n16) * PAGE * (I8 ? 1 : 2))[step % SP * 4 + g];
 		if (I8)
-#pragma unroll
-			for (int kt = 0; kt < KT; kt++)
-				vs[kt] = reinterpret_cast<const f4 *>(c.vs + pg * PAGE + g * 16)[kt];
+			vs = c.vs[pg * PAGE + lane];
 	};
 	if (wave < steps) {
 		at = page(wave);
@@ -477,7 +544,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 #pragma unroll
 	for (int m = 0; m < MT; m++)
 		r[0].o[m] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-	float vtop = 1e-30f;
+	float vlog = -100.0f;
 
 	for (int step = wave; step < steps; step += WK) {
 		const int start = (p0 + step / SP) * PAGE, row0 = step % SP * 32, end = u.len + u.n - start - row0;
@@ -486,7 +553,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 		const bool whole = __all((vis & all) == all || node < 0);
 		const bool more = step + WK < steps;
 		const size_t next = more ? page(step + WK) : at;
-		f4 sc[KT], kk[KT];
+		f4 sc[KT];
 #pragma unroll
 		for (int kt = 0; kt < KT; kt++) {
 			f4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
@@ -503,26 +570,17 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 				hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[k], hi, 0, 0, 0);
 			}
 			sc[kt] = lo + hi;
-			kk[kt] = ks[kt];
 		}
+		float kk = ks;
 		if (more)
 			get_k(next, step + WK);
-		f4 vv[KT];
-		if constexpr (I8) {
-			float top = 0.0f;
-#pragma unroll
-			for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-				for (int i = 0; i < 4; i++)
-					top = __builtin_fmaxf(top, whole || g * 16 + kt * 4 + i < end ? vs[kt][i] : 0.0f);
-			move_vtop<HD, 1>(top, vtop, r);
-			const float inv = P_SCALE / vtop;
-#pragma unroll
-			for (int kt = 0; kt < KT; kt++)
-				vv[kt] = vs[kt] * inv;
+		if (I8) {
+			if (!whole)
+				guard_scales(kk, vs, lane < end);
+			move_vlog<HD, 1>(vs, vlog, r);
 		}
 		h8 ph[KT / 2], pl[KT / 2];
-		weigh<HD, I8, KT>(r[0], sc, kk, vv, qs, (uint32_t)(vis >> (4 * KT * g)), whole, ph, pl);
+		weigh<HD, I8, KT>(r[0], sc, kk, vs, vlog, qs, whole, (uint32_t)(vis >> (4 * KT * g)), ph, pl);
 #pragma unroll
 		for (int m = 0; m < MT; m++) {
 			if constexpr (I8) {
@@ -546,12 +604,12 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 			get_v(next, step + WK);
 		at = next;
 	}
-	const float back = I8 ? vtop / P_SCALE : 1.0f / P_SCALE;
+	const float back = __builtin_amdgcn_exp2f(I8 ? vlog - P_LOG2 : -P_LOG2);
 
 	// join the waves: each puts its rows into LDS ([wave][row][HD + 4])
 	constexpr int LR = part_row(HD);
 	float *mine = lds + ((size_t)wave * R + n16) * LR;
-	const float total = sum_g(r[0].sum);
+	const float total = sum_g(r[0].sum) * back;
 #pragma unroll
 	for (int m = 0; m < MT; m++)
 		*reinterpret_cast<f4 *>(mine + m * 16 + 4 * g) = r[0].o[m] * back;
@@ -606,8 +664,8 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 {
 	constexpr int KS = HD / 32, MT = HD / 16, R = MANY_ROWS, NT = 2, KT = 2, E = I8 ? 1 : 2;
 	constexpr int NL = PAGE * HD * E / 16 / 256; // 16-byte pieces of a page's K (and V) for a thread
-	constexpr int KMASK = HD / 8 - 1;            // pieces of a K row in LDS, less one
-	__shared__ __attribute__((aligned(16))) _Float16 lk[2][PAGE * HD], lv[2][PAGE * HD];
+	constexpr int KP = HD / 8, VP = PAGE / 8;    // pieces of a K row and of a V column in LDS
+	__shared__ __attribute__((aligned(1024))) _Float16 lk[2][PAGE * HD], lv[2][PAGE * HD];
 	__shared__ __attribute__((aligned(16))) float lsc[2][2][PAGE];
 	const int group = a.n_heads / c.kvh;
 	Unit u;
@@ -620,6 +678,69 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 	const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g = lane >> 4;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	bool bad = !seq_fits(s, u.len, u.n);
+
+	const int last = a.mask ? u.n : min(u.n, (u.tile * R + R - 1) / group + 1);
+	const int pages = bad ? 0 : (u.len + last + PAGE - 1) / PAGE;
+	const int p0 = u.part * u.chunk, p1 = min(pages, p0 + min(u.chunk, pages));
+	u4 kr[I8 ? NL : 1], vr[I8 ? NL : 1];
+	float sr = 0.0f;
+	auto page = [&](int p) {
+		const int id = __builtin_amdgcn_readfirstlane(page_of(s, c.n_pages, u.b, p * PAGE));
+		bad = bad || id < 0;
+		return (size_t)(id < 0 ? 0 : id) * c.kvh + u.head;
+	};
+	// where a K row's and a V column's pieces lie
+	auto kx = [](int row) { return ((row & 3) | (row >> 3 & 3) << 2) & (KP - 1); };
+	auto vx = [](int col) { return col & (VP - 1); };
+	// f16: a page's pieces straight to LDS (a thread's piece e there comes from
+	// the place that the swizzle names)
+	uint32_t ko[NL], vo[NL];
+	if (!I8)
+#pragma unroll
+		for (int q = 0; q < NL; q++) {
+			const int e = tid + q * 256;
+			ko[q] = 16 * (e / KP * KP + (e % KP ^ kx(e / KP)));
+			vo[q] = 16 * (e / VP * VP + (e % VP ^ vx(e / VP)));
+		}
+	// request a page: int8 codes to registers, f16 to buffer b
+	auto get = [&](size_t pg, int b) {
+		const uint8_t *k = uniform(c.k + pg * PAGE * HD * E), *v = uniform(c.v + pg * PAGE * HD * E);
+#pragma unroll
+		for (int q = 0; q < NL; q++) {
+			if constexpr (I8) {
+				kr[q] = reinterpret_cast<const u4 *>(k)[tid + q * 256];
+				vr[q] = reinterpret_cast<const u4 *>(v)[tid + q * 256];
+			} else {
+				load_lds16(k, ko[q], lk[b] + (q * 256 + wave * 64) * 8);
+				load_lds16(v, vo[q], lv[b] + (q * 256 + wave * 64) * 8);
+			}
+		}
+		if (I8 && tid < 2 * PAGE)
+			sr = tid < PAGE ? c.ks[pg * PAGE + tid] : c.vs[pg * PAGE + tid - PAGE];
+	};
+	auto put = [&](int b) {
+		if constexpr (I8) {
+#pragma unroll
+			for (int q = 0; q < NL; q++) {
+				const int e = tid + q * 256; // piece of 16 codes: two of f16
+				const int row = e / (KP / 2), kp = e % (KP / 2) * 2, col = e / (VP / 2), vp = e % (VP / 2) * 2;
+				h8 *kl = reinterpret_cast<h8 *>(lk[b] + row * HD), *vl = reinterpret_cast<h8 *>(lv[b] + col * PAGE);
+				kl[kp ^ kx(row)] = codes8(kr[q].x, kr[q].y);
+				kl[(kp + 1) ^ kx(row)] = codes8(kr[q].z, kr[q].w);
+				vl[vp ^ vx(col)] = codes8(vr[q].x, vr[q].y);
+				vl[(vp + 1) ^ vx(col)] = codes8(vr[q].z, vr[q].w);
+			}
+			if (tid < 2 * PAGE)
+				lsc[b][tid >> 6][tid & 63] = sr;
+		} else {
+			__builtin_amdgcn_s_waitcnt(0); // the pieces under way to LDS
+		}
+	};
+	size_t at = 0;
+	if (p0 < p1) {
+		at = page(p0);
+		get(at, 0);
+	}
 
 	int node[NT];
 	h8 qh[NT][KS], ql[NT][KS];
@@ -634,67 +755,42 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 		for (int m = 0; m < MT; m++)
 			r[t].o[m] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 	}
-	float vtop = 1e-30f;
-
-	const int last = a.mask ? u.n : min(u.n, (u.tile * R + R - 1) / group + 1);
-	const int pages = bad ? 0 : (u.len + last + PAGE - 1) / PAGE;
-	const int p0 = u.part * u.chunk, p1 = min(pages, p0 + min(u.chunk, pages));
-	u4 kr[NL], vr[NL];
-	float sr = 0.0f;
-	auto page = [&](int p) {
-		const int id = page_of(s, c.n_pages, u.b, p * PAGE);
-		bad = bad || id < 0;
-		return (size_t)(id < 0 ? 0 : id) * c.kvh + u.head;
-	};
-	auto get = [&](size_t pg) {
-		const u4 *k = reinterpret_cast<const u4 *>(c.k + pg * PAGE * HD * E) + tid;
-		const u4 *v = reinterpret_cast<const u4 *>(c.v + pg * PAGE * HD * E) + tid;
-#pragma unroll
-		for (int q = 0; q < NL; q++) {
-			kr[q] = k[q * 256];
-			vr[q] = v[q * 256];
-		}
-		if (I8 && tid < 2 * PAGE)
-			sr = tid < PAGE ? c.ks[pg * PAGE + tid] : c.vs[pg * PAGE + tid - PAGE];
-	};
-	auto put = [&](int b) {
-#pragma unroll
-		for (int q = 0; q < NL; q++) {
-			const int e = tid + q * 256;
-			const int kw = HD * E / 16, krow = e / kw, kp = e % kw; // pieces of a row in memory
-			const int vw = PAGE * E / 16, vcol = e / vw, vp = e % vw;
-			const int kx = (krow & 3) | (krow >> 3 & 3) << 2, vx = vcol & 7;
-			h8 *ko = reinterpret_cast<h8 *>(lk[b] + krow * HD), *vo = reinterpret_cast<h8 *>(lv[b] + vcol * PAGE);
-			if constexpr (I8) {
-				ko[(2 * kp ^ kx) & KMASK] = codes8(kr[q].x, kr[q].y);
-				ko[((2 * kp + 1) ^ kx) & KMASK] = codes8(kr[q].z, kr[q].w);
-				vo[2 * vp ^ vx] = codes8(vr[q].x, vr[q].y);
-				vo[(2 * vp + 1) ^ vx] = codes8(vr[q].z, vr[q].w);
-			} else {
-				ko[(kp ^ kx) & KMASK] = __builtin_bit_cast(h8, kr[q]);
-				vo[vp ^ vx] = __builtin_bit_cast(h8, vr[q]);
-			}
-		}
-		if (I8 && tid < 2 * PAGE)
-			lsc[b][tid >> 6][tid & 63] = sr;
-	};
-	size_t at = 0;
-	if (p0 < p1) {
-		at = page(p0);
-		get(at);
-		put(0);
-	}
+	float vlog = -100.0f;
+	put(0);
 	__syncthreads();
+
 	for (int p = p0; p < p1; p++) {
 		const int b = (p - p0) & 1, start = p * PAGE, end = u.len + u.n - start;
 		const bool more = p + 1 < p1;
 		const size_t next = more ? page(p + 1) : at;
 		if (more)
-			get(next);
+			get(next, b ^ 1); // (all waves left that buffer at the last barrier)
 		uint64_t vis[NT];
 #pragma unroll
 		for (int t = 0; t < NT; t++)
 			vis[t] = sees(a, u, node[t], start);
+		// a page that not all of the tile sees: f16 values that are not finite
+		// are taken out first (see guard_values), and come back below
+		if (!I8 && (a.mask ? start + PAGE > u.len : start + PAGE > u.len + u.tile * R / group + 1)) {
+			uint32_t odd = 0;
+#pragma unroll
+			for (int q = 0; q < NL; q++) {
+				u4 *x = reinterpret_cast<u4 *>(lv[b]) + tid + q * 256;
+				u4 y = *x;
+				uint32_t here = 0;
+#pragma unroll
+				for (int e = 0; e < 4; e++) {
+					here |= ((y[e] & 0x7c00u) == 0x7c00u) | ((y[e] & 0x7c000000u) == 0x7c000000u);
+					y[e] = ((y[e] & 0x7c00u) == 0x7c00u ? 0u : y[e] & 0xffffu) |
+					       ((y[e] & 0x7c000000u) == 0x7c000000u ? 0u : y[e] & 0xffff0000u);
+				}
+				if (here)
+					*x = y;
+				odd |= here;
+			}
+			if (__syncthreads_or(odd))
+				give_back<HD, NT>(c.v + at * HD * PAGE * 2, g, end, vis, r);
+		}
 #pragma unroll 1
 		for (int row0 = 0; row0 < PAGE; row0 += 32) {
 			uint32_t seen[NT];
@@ -708,53 +804,46 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 			if (!__any(any))
 				continue;
 			whole = __all(whole);
-			f4 sc[NT][KT];
+			h8 kf[KT][KS];
 #pragma unroll
 			for (int kt = 0; kt < KT; kt++) {
-				const _Float16 *kl = lk[b] + (row0 + (n16 >> 2) * 8 + kt * 4 + (n16 & 3)) * HD;
+				const h8 *kl = reinterpret_cast<const h8 *>(lk[b] + (row0 + (n16 >> 2) * 8 + kt * 4 + (n16 & 3)) * HD);
+#pragma unroll
+				for (int k = 0; k < KS; k++)
+					kf[kt][k] = kl[(k * 4 + g) ^ (n16 & (KP - 1))];
+			}
+			f4 sc[NT][KT];
+#pragma unroll
+			for (int kt = 0; kt < KT; kt++)
 #pragma unroll
 				for (int t = 0; t < NT; t++)
 					sc[t][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-				for (int k = 0; k < KS; k++) {
-					const h8 kf = reinterpret_cast<const h8 *>(kl)[((k * 4 + g) ^ n16) & KMASK];
+			for (int k = 0; k < KS; k++)
 #pragma unroll
-					for (int t = 0; t < NT; t++)
-						sc[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[t][k], sc[t][kt], 0, 0, 0);
+				for (int e = 0; e < 2; e++)
 #pragma unroll
-					for (int t = 0; t < NT; t++)
-						sc[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[t][k], sc[t][kt], 0, 0, 0);
-				}
-			}
-			f4 ks[KT], vs[KT];
+					for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+						for (int t = 0; t < NT; t++)
+							sc[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][k], e ? qh[t][k] : ql[t][k],
+													   sc[t][kt], 0, 0, 0);
+			float ks = 0.0f, vs = 0.0f;
 			if constexpr (I8) {
-				float top = 0.0f;
-#pragma unroll
-				for (int kt = 0; kt < KT; kt++) {
-					ks[kt] = reinterpret_cast<const f4 *>(lsc[b][0] + row0 + g * 8)[kt];
-					vs[kt] = reinterpret_cast<const f4 *>(lsc[b][1] + row0 + g * 8)[kt];
-#pragma unroll
-					for (int i = 0; i < 4; i++)
-						top = __builtin_fmaxf(top, whole || row0 + g * 8 + kt * 4 + i < end ? vs[kt][i] : 0.0f);
-				}
-				move_vtop<HD, NT>(top, vtop, r);
-				const float inv = P_SCALE / vtop;
-#pragma unroll
-				for (int kt = 0; kt < KT; kt++)
-					vs[kt] *= inv;
+				const int row = row0 + g * 8 + (n16 & 7);
+				ks = lsc[b][0][row];
+				vs = lsc[b][1][row];
+				if (!whole)
+					guard_scales(ks, vs, row < end);
+				move_vlog<HD, NT>(vs, vlog, r);
 			}
 			h8 ph[NT][1], pl[NT][1];
 #pragma unroll
 			for (int t = 0; t < NT; t++)
-				weigh<HD, I8, KT>(r[t], sc[t], ks, vs, qs[t], seen[t] >> (8 * g), whole, ph[t], pl[t]);
+				weigh<HD, I8, KT>(r[t], sc[t], ks, vs, vlog, qs[t], whole, seen[t] >> (8 * g), ph[t], pl[t]);
 #pragma unroll
 			for (int m = 0; m < MT; m++) {
-				const u4 *vl = reinterpret_cast<const u4 *>(lv[b] + (m * 16 + n16) * PAGE);
-				u4 w = vl[(row0 / 8 + g) ^ (n16 & 7)];
-				if constexpr (!I8)
-					if (!whole)
-						guard_values<HD, NT>(w, c.v + at * HD * PAGE * 2, row0, m, g, end - row0, seen, r);
-				const h8 vf = __builtin_bit_cast(h8, w);
+				const h8 vf = reinterpret_cast<const h8 *>(lv[b] + (m * 16 + n16) * PAGE)[(row0 / 8 + g) ^ (n16 & (VP - 1))];
 #pragma unroll
 				for (int t = 0; t < NT; t++)
 					r[t].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[t][0], r[t].o[m], 0, 0, 0);
@@ -764,14 +853,14 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 			}
 		}
 		if (more)
-			put(b ^ 1); // (all waves left that buffer at the last barrier)
+			put(b ^ 1);
 		__syncthreads();
 		at = next;
 	}
-	const float back = I8 ? vtop / P_SCALE : 1.0f / P_SCALE;
+	const float back = __builtin_amdgcn_exp2f(I8 ? vlog - P_LOG2 : -P_LOG2);
 #pragma unroll
 	for (int t = 0; t < NT; t++) {
-		const float total = sum_g(r[t].sum);
+		const float total = sum_g(r[t].sum) * back;
 		const int q = wave * 32 + 16 * t + n16, to = u.tile * R + q;
 		if (node[t] < 0)
 			continue;
