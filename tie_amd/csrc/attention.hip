@@ -257,6 +257,8 @@ __device__ __forceinline__ uint64_t sees(const AttnArgs &a, const Unit &u, int n
 	if (node < 0)
 		return 0;
 	const int rel = start - u.len; // the page's first row as a node
+	if (rel <= -PAGE)
+		return ~0ull;
 	auto below = [](long long n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
 	if (!a.mask)
 		return below((long long)node + 1 - rel);
@@ -286,19 +288,31 @@ __device__ __forceinline__ void load_query(const AttnArgs &a, const Unit &u, int
 {
 	float x[HD / 32][8], m = 0.0f;
 	const float *q = a.q + (size_t)(u.t0 + (node < 0 ? 0 : node)) * a.q_stride + (size_t)head * HD;
+	const bool vec = (((uintptr_t)a.q | a.q_stride * 4) & 15) == 0;
+#pragma unroll
+	for (int k = 0; k < HD / 32; k++) {
+		// (PAIRS: int8 rows straight from memory come 16 codes to a lane)
+		const float *from = q + (PAIRS ? (k >> 1) * 64 + g * 16 + (k & 1) * 8 : k * 32 + g * 8);
+		if (vec) {
+			const f4 x0 = reinterpret_cast<const f4 *>(from)[0], x1 = reinterpret_cast<const f4 *>(from)[1];
+#pragma unroll
+			for (int j = 0; j < 4; j++) {
+				x[k][j] = x0[j];
+				x[k][4 + j] = x1[j];
+			}
+		} else {
+#pragma unroll
+			for (int j = 0; j < 8; j++)
+				x[k][j] = from[j];
+		}
+	}
 #pragma unroll
 	for (int k = 0; k < HD / 32; k++)
 #pragma unroll
 		for (int j = 0; j < 8; j++) {
-			// (PAIRS: int8 rows straight from memory come 16 codes to a lane)
-			const int at = PAIRS ? (k >> 1) * 64 + g * 16 + (k & 1) * 8 + j : k * 32 + g * 8 + j;
-			x[k][j] = node < 0 ? 0.0f : q[at];
-		}
-#pragma unroll
-	for (int k = 0; k < HD / 32; k++)
-#pragma unroll
-		for (int j = 0; j < 8; j++)
+			x[k][j] = node < 0 ? 0.0f : x[k][j];
 			m = __builtin_fmaxf(m, __builtin_fabsf(x[k][j]));
+		}
 	m = max_g(m);
 	const float p2 = m >= 1e-30f && m < 1e30f ? pow2_below(m) : 1.0f;
 	const float up = __builtin_copysignf(512.0f / p2, a.scale);
