@@ -310,7 +310,9 @@ int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_layers, cons
  *   q    [n_tokens] rows of n_heads heads (as tie_hip_kv_append leaves them)
  *   out  the same shape (may be q, with the same stride)
  *   work work_bytes of device memory, 16-byte aligned, at least
- *        tie_hip_tree_attention_work_bytes; NULL: the stream's workspace, which
+ *        tie_hip_tree_attention_work_bytes, filled with zeros before the first
+ *        call that gets it and after anything else has written to it (calls
+ *        here leave it fit for the next); NULL: the stream's workspace, which
  *        all calls on the stream share and which grows as needed, but not
  *        during HIP graph capture (run the largest call once before, or pass
  *        memory).  Graphs that may run at the same time need memory of their own.

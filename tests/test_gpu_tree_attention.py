@@ -272,7 +272,7 @@ def test_in_place_streams_work_and_graphs(kind, lens, counts):
     want = outs[0].clone()
     both = q.clone()
     need = kv.attention_work_bytes(seqs, H)
-    work = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    work = torch.zeros(need, dtype=torch.uint8, device="cuda")
     torch.cuda.synchronize()
     kv.attention(0, seqs, both, both, 0.09)
     kv.attention(0, seqs, q, outs[1], 0.09, work=work)
@@ -288,7 +288,8 @@ def test_in_place_streams_work_and_graphs(kind, lens, counts):
     graphs = []
     for i in range(2):
         g = torch.cuda.CUDAGraph()
-        mine = torch.empty(need, dtype=torch.uint8, device="cuda")
+        mine = torch.zeros(need, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
         with kv_ref.capture(g, streams[i]):
             kv.attention(0, seqs, q, outs[2 + i], 0.09, work=mine, stream=torch.cuda.current_stream().cuda_stream)
         graphs.append((g, mine))

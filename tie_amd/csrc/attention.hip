@@ -131,7 +131,8 @@ struct Cut {
 };
 
 struct Unit {
-	int b, tile, head, part, parts, chunk, t0, n, len, base; // base: the first unit of the sequence
+	int b, tile, head, part, parts, chunk, t0, n, len;
+	int base, tile_at; // the first unit of the sequence, and the tile's place among its tiles
 };
 
 __device__ __forceinline__ int wave_sum(int x)
@@ -235,7 +236,8 @@ __device__ __forceinline__ bool find_unit(const KvSeqs &s, int kvh, int group, c
 			u.head = (uint32_t)at % (uint32_t)kvh;
 			u.part = (uint32_t)at / (uint32_t)kvh % (uint32_t)u.parts;
 			// (causal: the last tiles have the most pages; they start first)
-			u.tile = of(tiles) - 1 - (uint32_t)at / (uint32_t)kvh / (uint32_t)u.parts;
+			u.tile_at = (uint32_t)at / (uint32_t)kvh / (uint32_t)u.parts;
+			u.tile = of(tiles) - 1 - u.tile_at;
 			u.t0 = of(t0);
 			u.n = of(n);
 			u.len = of(len);
@@ -279,19 +281,15 @@ constexpr int part_row(int hd)
 	return hd + 4; // (16-byte rows)
 }
 
-// A token row's query for one lane of an operand: 8 values of each K step,
-// scaled to below 2^10 and split; qs: what the products are multiplied by (with
-// log2 e: exp2 for exp), not negative (the scale's sign is in the query).
+// A token row's query for one lane of an operand: 8 values of each K step.
+// PAIRS: int8 rows straight from memory come 16 codes to a lane.
 template <int HD, bool PAIRS>
-__device__ __forceinline__ void load_query(const AttnArgs &a, const Unit &u, int node, int head, int g, h8 (&qh)[HD / 32],
-					   h8 (&ql)[HD / 32], float &qs)
+__device__ __forceinline__ void fetch_query(const AttnArgs &a, const Unit &u, int node, int head, int g, float (&x)[HD / 32][8])
 {
-	float x[HD / 32][8], m = 0.0f;
 	const float *q = a.q + (size_t)(u.t0 + (node < 0 ? 0 : node)) * a.q_stride + (size_t)head * HD;
 	const bool vec = (((uintptr_t)a.q | a.q_stride * 4) & 15) == 0;
 #pragma unroll
 	for (int k = 0; k < HD / 32; k++) {
-		// (PAIRS: int8 rows straight from memory come 16 codes to a lane)
 		const float *from = q + (PAIRS ? (k >> 1) * 64 + g * 16 + (k & 1) * 8 : k * 32 + g * 8);
 		if (vec) {
 			const f4 x0 = reinterpret_cast<const f4 *>(from)[0], x1 = reinterpret_cast<const f4 *>(from)[1];
@@ -306,6 +304,16 @@ __device__ __forceinline__ void load_query(const AttnArgs &a, const Unit &u, int
 				x[k][j] = from[j];
 		}
 	}
+}
+
+// The operand's two parts, of the query scaled to below 2^10; qs: what the
+// products are multiplied by (with log2 e: exp2 for exp), positive (the scale's
+// sign is in the query).
+template <int HD>
+__device__ __forceinline__ void split_query(const AttnArgs &a, int node, float (&x)[HD / 32][8], h8 (&qh)[HD / 32],
+					    h8 (&ql)[HD / 32], float &qs)
+{
+	float m = 0.0f;
 #pragma unroll
 	for (int k = 0; k < HD / 32; k++)
 #pragma unroll
@@ -493,10 +501,26 @@ __device__ __forceinline__ void give_back(const uint8_t *v, int g, int end, cons
 // pages: a wave requests a page's K as soon as the products with the last one's
 // are done and its V as soon as O has taken the last one's, so that one of the
 // two is always under way, at 2 waves on a SIMD.
-constexpr int FEW_ROWS = 16, FEW_WAVES = 8;
+constexpr int FEW_ROWS = 16, FEW_WAVES = 8, FEW_CAP = 256;
+constexpr int FEW_PARTS = FEW_CAP + 32; // parts of a tile, at most (a share rounded down can make one more than FEW_CAP)
+
+// two floats past the dies' caches
+__device__ __forceinline__ void put_pair(uint64_t *p, float x, float y)
+{
+	__hip_atomic_store(p, (uint64_t)__float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32, __ATOMIC_RELAXED,
+			   __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ void get_pair(const uint64_t *p, float &x, float &y)
+{
+	const uint64_t v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+	x = __uint_as_float((uint32_t)v);
+	y = __uint_as_float((uint32_t)(v >> 32));
+}
 
 template <int HD, bool I8>
-__global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, float *part)
+__global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, float *part,
+								       int *count)
 {
 	constexpr int KS = HD / 32, MT = HD / 16, R = FEW_ROWS, WK = FEW_WAVES;
 	constexpr int KT = I8 ? 4 : 2;       // a step: a page of int8, half a page of f16 (16 KB of K and V at HD = 128)
@@ -546,6 +570,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 		if (I8)
 			vs = c.vs[pg * PAGE + lane];
 	};
+	float x[KS][8];
+	fetch_query<HD, I8>(a, u, node, u.head * group + row % group, g, x);
 	if (wave < steps) {
 		at = page(wave);
 		get_k(at, wave);
@@ -553,7 +579,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 	}
 	h8 qh[KS], ql[KS];
 	float qs;
-	load_query<HD, I8>(a, u, node, u.head * group + row % group, g, qh, ql, qs);
+	split_query<HD>(a, node, x, qh, ql, qs);
 	Rows<HD> r[1];
 #pragma unroll
 	for (int m = 0; m < MT; m++)
@@ -632,11 +658,16 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 		mine[HD + 1] = bad ? __builtin_nanf("") : total;
 	}
 	__syncthreads();
-	for (int e = threadIdx.x; e < R * HD; e += 64 * WK) {
-		const int q = e / HD, i = e % HD, to = u.tile * R + q;
-		if (to / group >= u.n)
-			continue;
-		float m = -__builtin_inff(), l = 0.0f, x = 0.0f;
+	// (pairs of columns: a part's values go by 8 bytes)
+	auto out_at = [&](int q) {
+		const int to = u.tile * R + q;
+		return a.out + (size_t)(u.t0 + to / group) * a.o_stride + (size_t)(u.head * group + to % group) * HD;
+	};
+	const int live = min(R, u.n * group - u.tile * R); // rows of the tile
+	uint64_t *mine64 = reinterpret_cast<uint64_t *>(part + (size_t)blockIdx.x * R * LR);
+	for (int e = threadIdx.x; e < live * HD / 2; e += 64 * WK) {
+		const int q = e / (HD / 2), i = e % (HD / 2);
+		float m = -__builtin_inff(), l = 0.0f, x0 = 0.0f, x1 = 0.0f;
 #pragma unroll
 		for (int w = 0; w < WK; w++)
 			m = __builtin_fmaxf(m, lds[((size_t)w * R + q) * LR + HD]);
@@ -646,19 +677,96 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 			const float *from = lds + ((size_t)w * R + q) * LR;
 			const float f = __builtin_amdgcn_exp2f(from[HD] - base);
 			l += from[HD + 1] * f;
-			x += from[i] * f;
+			x0 += from[2 * i] * f;
+			x1 += from[2 * i + 1] * f;
 		}
 		if (u.parts == 1) {
-			a.out[(size_t)(u.t0 + to / group) * a.o_stride + (size_t)(u.head * group + to % group) * HD + i] =
-				l == 0.0f ? 0.0f : x / l;
+			float *o = out_at(q) + 2 * i;
+			o[0] = l == 0.0f ? 0.0f : x0 / l;
+			o[1] = l == 0.0f ? 0.0f : x1 / l;
 		} else {
-			float *pr = part + ((size_t)blockIdx.x * R + q) * LR;
-			pr[i] = x;
-			if (i == 0) {
-				pr[HD] = m;
-				pr[HD + 1] = l;
+			put_pair(mine64 + q * (LR / 2) + i, x0, x1);
+			if (i == 0)
+				put_pair(mine64 + q * (LR / 2) + HD / 2, m, l);
+		}
+	}
+	if (u.parts == 1)
+		return;
+	// The last of the tile's parts joins them.  What the parts wrote went past
+	// the dies' caches (agent-scope accesses) and is there once the writer's
+	// loads and stores are done, which each wave waits for before its
+	// workgroup counts; the last one to count leaves the counter as it was, 0.
+	asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+	__syncthreads();
+	const int u0 = u.base + u.tile_at * u.parts * c.kvh + u.head; // unit of part q: u0 + q kvh
+	if ((long long)u0 + (long long)(u.parts - 1) * c.kvh >= gridDim.x || u0 >= WORK_COUNTERS || u.parts > FEW_PARTS)
+		return; // (sequences that overlap: more units than the rows can have)
+	int *last_one = reinterpret_cast<int *>(lds);
+	if (threadIdx.x == 0)
+		*last_one = __hip_atomic_fetch_add(count + u0, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == u.parts - 1;
+	__syncthreads();
+	if (!*last_one)
+		return;
+	if (threadIdx.x == 0)
+		__hip_atomic_store(count + u0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+	__syncthreads();
+	const uint64_t *from64 = reinterpret_cast<const uint64_t *>(part + (size_t)u0 * R * LR);
+	const size_t step64 = (size_t)c.kvh * R * LR / 2;
+	// first the rows' maxima and sums: a row's 32 lanes take parts in turn
+	float *fac = lds; // [live][parts up to FEW_PARTS] the parts' factors
+	{
+		const int q = threadIdx.x / 32, l32 = threadIdx.x % 32;
+		if (q < live) {
+			float pm[FEW_PARTS / 32], pl[FEW_PARTS / 32], m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+			for (int e = 0; e < FEW_PARTS / 32; e++) {
+				const int k = e * 32 + l32;
+				pm[e] = -__builtin_inff();
+				pl[e] = 0.0f;
+				if (k < u.parts)
+					get_pair(from64 + k * step64 + q * (LR / 2) + HD / 2, pm[e], pl[e]);
+			}
+#pragma unroll
+			for (int e = 0; e < FEW_PARTS / 32; e++)
+				m = __builtin_fmaxf(m, pm[e]);
+#pragma unroll
+			for (int k = 1; k < 32; k <<= 1)
+				m = __builtin_fmaxf(m, __shfl_xor(m, k));
+			const float base = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+			for (int e = 0; e < FEW_PARTS / 32; e++) {
+				pm[e] = __builtin_amdgcn_exp2f(pm[e] - base);
+				l += pl[e] * pm[e];
+			}
+#pragma unroll
+			for (int k = 1; k < 32; k <<= 1)
+				l += __shfl_xor(l, k);
+			const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+			for (int e = 0; e < FEW_PARTS / 32; e++)
+				if (e * 32 + l32 < u.parts)
+					fac[q * FEW_PARTS + e * 32 + l32] = l == 0.0f ? 0.0f : pm[e] * inv;
+		}
+	}
+	__syncthreads();
+	for (int e = threadIdx.x; e < live * HD / 2; e += 64 * WK) {
+		const int q = e / (HD / 2), i = e % (HD / 2);
+		float x0 = 0.0f, x1 = 0.0f;
+		for (int k0 = 0; k0 < u.parts; k0 += 16) {
+			float y0[16], y1[16];
+#pragma unroll
+			for (int k = 0; k < 16; k++)
+				get_pair(from64 + min(k0 + k, u.parts - 1) * step64 + q * (LR / 2) + i, y0[k], y1[k]);
+#pragma unroll
+			for (int k = 0; k < 16; k++) {
+				const float f = k0 + k < u.parts ? fac[q * FEW_PARTS + k0 + k] : 0.0f;
+				x0 += k0 + k < u.parts ? y0[k] * f : 0.0f;
+				x1 += k0 + k < u.parts ? y1[k] * f : 0.0f;
 			}
 		}
+		float *o = out_at(q) + 2 * i;
+		o[0] = x0;
+		o[1] = x1;
 	}
 }
 
@@ -764,7 +872,9 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 	for (int t = 0; t < NT; t++) {
 		const int row = u.tile * R + wave * 32 + 16 * t + n16;
 		node[t] = row / group < u.n ? row / group : -1;
-		load_query<HD, false>(a, u, node[t], u.head * group + row % group, g, qh[t], ql[t], qs[t]);
+		float x[KS][8];
+		fetch_query<HD, false>(a, u, node[t], u.head * group + row % group, g, x);
+		split_query<HD>(a, node[t], x, qh[t], ql[t], qs[t]);
 #pragma unroll
 		for (int m = 0; m < MT; m++)
 			r[t].o[m] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -991,33 +1101,40 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 	h.few = rows <= (size_t)FEW_ROWS * s.n_seqs;
 	h.cut.rows = h.few ? FEW_ROWS : MANY_ROWS;
 	// one workgroup of 8 waves on a CU, or two of 4
-	h.cut.cap = h.few ? 256 : 512;
+	h.cut.cap = h.few ? FEW_CAP : 512;
 	h.cut.least = h.few ? FEW_WAVES : 2;
-	const size_t tiles = (rows + (size_t)s.n_seqs * (h.cut.rows - 1)) / h.cut.rows;
+	const size_t seqs = s.n_seqs < s.n_tokens ? s.n_seqs : s.n_tokens; // that have tokens, at most
+	const size_t tiles = (rows + seqs * (h.cut.rows - 1)) / h.cut.rows;
 	// as many tiles as fill the card are not cut: no parts, no join
 	h.cut.whole = rows / h.cut.rows * c.kvh >= (size_t)h.cut.cap;
-	h.units = (h.cut.whole ? 0 : h.cut.cap) + tiles * c.kvh;
+	// (a share that is rounded down can make one more part)
+	h.units = (h.cut.whole ? 0 : h.cut.cap + c.kvh) + tiles * c.kvh;
+	// (not with a kv head for every 8 rows or more, and then: whole tiles)
+	if (h.few && h.units > WORK_COUNTERS)
+		h.cut.whole = 1;
 	return h;
 }
 
 size_t attention_work_bytes(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 {
 	const Shape h = attn_shape(c, s, a);
-	return h.cut.whole ? 256 : h.units * h.cut.rows * part_row(c.hd) * sizeof(float);
+	return WORK_COUNTERS * sizeof(int) + (h.cut.whole ? 0 : h.units * h.cut.rows * part_row(c.hd) * sizeof(float));
 }
 
 template <int HD, bool I8>
-static hipError_t go(const Shape &h, const KvLayer &c, const KvSeqs &s, const AttnArgs &a, float *part, hipStream_t st)
+static hipError_t go(const Shape &h, const KvLayer &c, const KvSeqs &s, const AttnArgs &a, int *count, hipStream_t st)
 {
+	float *part = reinterpret_cast<float *>(count + WORK_COUNTERS);
 	if (h.few) {
 		const size_t lds = (size_t)FEW_WAVES * FEW_ROWS * part_row(HD) * sizeof(float);
 		const hipError_t e = ensure_lds_limit((const void *)attn_few_kernel<HD, I8>, lds);
 		if (e != hipSuccess)
 			return e;
-		tie_launch(attn_few_kernel<HD, I8>, dim3(h.units), dim3(64 * FEW_WAVES), lds, st, c, s, a, h.cut, part);
-	} else {
-		tie_launch(attn_many_kernel<HD, I8>, dim3(h.units), dim3(64 * MANY_WAVES), 0, st, c, s, a, h.cut, part);
+		tie_launch(attn_few_kernel<HD, I8>, dim3(h.units), dim3(64 * FEW_WAVES), lds, st, c, s, a, h.cut,
+			   part, count);
+		return hipGetLastError();
 	}
+	tie_launch(attn_many_kernel<HD, I8>, dim3(h.units), dim3(64 * MANY_WAVES), 0, st, c, s, a, h.cut, part);
 	if (!h.cut.whole)
 		tie_launch(attn_join_kernel<HD>, dim3(s.n_tokens, a.n_heads), dim3(256), 0, st, c, s, a, h.cut, (int)h.units,
 			   (const float *)part);
@@ -1027,10 +1144,10 @@ static hipError_t go(const Shape &h, const KvLayer &c, const KvSeqs &s, const At
 hipError_t launch_attention(const KvLayer &c, const KvSeqs &s, const AttnArgs &a, void *work, hipStream_t st)
 {
 	const Shape h = attn_shape(c, s, a);
-	float *part = reinterpret_cast<float *>(work);
+	int *count = reinterpret_cast<int *>(work);
 	if (c.hd == 128)
-		return c.i8 ? go<128, true>(h, c, s, a, part, st) : go<128, false>(h, c, s, a, part, st);
-	return c.i8 ? go<64, true>(h, c, s, a, part, st) : go<64, false>(h, c, s, a, part, st);
+		return c.i8 ? go<128, true>(h, c, s, a, count, st) : go<128, false>(h, c, s, a, count, st);
+	return c.i8 ? go<64, true>(h, c, s, a, count, st) : go<64, false>(h, c, s, a, count, st);
 }
 
 } // namespace tie

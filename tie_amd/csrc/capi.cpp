@@ -1354,6 +1354,11 @@ static int aux_scratch(hipStream_t s, void *work, size_t work_bytes, size_t need
 		int rc = dev_malloc(&mem, bytes, "attention workspace");
 		if (rc)
 			return rc;
+		const hipError_t e = hipMemsetAsync(mem, 0, WORK_COUNTERS * sizeof(int), s);
+		if (e != hipSuccess) {
+			(void)hipFree(mem);
+			HIP_TRY(e);
+		}
 		if (w.aux)
 			w.aux_old[w.n_aux_old++] = w.aux;
 		w.aux = mem;

@@ -28,6 +28,11 @@ struct KvSeqs {
 	int n_seqs = 0, max_pages = 0, n_tokens = 0;
 };
 
+// The scratch memory of the attention and verification calls begins with this
+// many counters, which every call finds at 0 and leaves at 0 (the rest of it a
+// call may find as it likes).
+constexpr int WORK_COUNTERS = 8192;
+
 struct AppendArgs {
 	const float *q, *k, *v;
 	size_t q_stride, k_stride, v_stride; // floats from a token's row to the next

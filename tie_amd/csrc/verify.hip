@@ -35,7 +35,7 @@ struct VerifyWork {
 
 static size_t carve_verify(const VerifyArgs &a, bool with_draft, uint8_t *base, VerifyWork *w)
 {
-	size_t off = 0;
+	size_t off = WORK_COUNTERS * sizeof(int);
 	auto take = [&](size_t bytes) {
 		const size_t o = off;
 		off += (bytes + 255) & ~(size_t)255;
