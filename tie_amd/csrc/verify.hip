@@ -25,7 +25,7 @@ namespace tie {
 constexpr int V_CHUNK = 4096; // logits of a workgroup
 constexpr int V_THREADS = 256, V_E = V_CHUNK / V_THREADS;
 constexpr int V_KIDS = VERIFY_KIDS;
-constexpr int V_PATH_LDS = 1024; // nodes of a sequence whose outcomes the path's reader keeps in LDS
+constexpr int V_PATH_LDS = 512; // nodes of a sequence whose outcomes the path's reader keeps in LDS
 
 // A row between its passes.
 struct VRow {
@@ -103,12 +103,35 @@ __device__ __forceinline__ double exp_below(double x)
 	return x > -745.0 ? __builtin_amdgcn_ldexp(y, (int)k) : x != x ? x : 0.0;
 }
 
-template <typename T> __device__ __forceinline__ T wave_total(T x)
+// x moved across lanes by a DPP control; lanes that get nothing: `none`
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp(float none, float x)
 {
-#pragma unroll
-	for (int m = 1; m < 64; m <<= 1)
-		x += __shfl_xor(x, m);
-	return x;
+	return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, x), CTRL,
+								     ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp(double none, double x)
+{
+	const uint64_t n = (uint64_t)__double_as_longlong(none), v = (uint64_t)__double_as_longlong(x);
+	const uint32_t lo = __builtin_amdgcn_update_dpp((int)(uint32_t)n, (int)(uint32_t)v, CTRL, ROWS, 0xf, false),
+		       hi = __builtin_amdgcn_update_dpp((int)(n >> 32), (int)(v >> 32), CTRL, ROWS, 0xf, false);
+	return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+
+// The running op(x) over the wave's lanes, in registers: within rows of 16 (row
+// shifts), then the rows' ends into the rows behind (broadcasts).
+template <typename T, typename OP> __device__ __forceinline__ T wave_scan(T x, T none, OP op)
+{
+	x = op(x, dpp<0x111, 0xf>(none, x));
+	x = op(x, dpp<0x112, 0xf>(none, x));
+	x = op(x, dpp<0x114, 0xf>(none, x));
+	x = op(x, dpp<0x118, 0xf>(none, x));
+	x = op(x, dpp<0x142, 0xa>(none, x));
+	return op(x, dpp<0x143, 0xc>(none, x));
+}
+
+__device__ __forceinline__ double running(double x)
+{
+	return wave_scan(x, 0.0, [](double a, double b) { return a + b; });
 }
 
 // x of a lane (the same in all lanes), whether it is active here or not
@@ -117,6 +140,17 @@ __device__ __forceinline__ double of_lane(double x, int lane)
 	const uint64_t v = (uint64_t)__double_as_longlong(x);
 	const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
 	return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+
+__device__ __forceinline__ double wave_total(double x)
+{
+	return of_lane(running(x), 63);
+}
+
+__device__ __forceinline__ float wave_max(float x)
+{
+	x = wave_scan(x, -__builtin_inff(), [](float a, float b) { return __builtin_fmaxf(a, b); });
+	return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
 // what one workgroup writes for another of the same launch goes past the
@@ -159,9 +193,9 @@ __device__ __forceinline__ bool last_of(int *count, int n, int *lds)
 struct Shared {
 	double d[4];
 	float f[4];
-	int i[4];
+	int i[4], j[4];
 	int flag;
-	int32_t path[V_PATH_LDS];
+	int32_t path[V_PATH_LDS], own[V_PATH_LDS], leaf[V_PATH_LDS];
 };
 
 // the sum over the workgroup, in every thread
@@ -176,6 +210,7 @@ __device__ __forceinline__ double block_total(double x, Shared &sh)
 }
 
 // The token rows [t0, t1) of row t's sequence; its number, or -1: none holds it.
+// A wave: the sequences' ends a lane each, after bisection down to 64 of them.
 __device__ __forceinline__ int seq_of_row(const VerifyArgs &a, int t, int &t0, int &t1)
 {
 	t0 = t;
@@ -183,18 +218,23 @@ __device__ __forceinline__ int seq_of_row(const VerifyArgs &a, int t, int &t0, i
 	if (!a.first)
 		return t;
 	int lo = 0, hi = a.n_seqs;
-	while (lo < hi) {
+	while (hi - lo > 64) {
 		const int mid = (lo + hi) >> 1;
-		if (a.first[mid + 1] <= t)
-			lo = mid + 1;
+		if (a.first[mid] <= t)
+			lo = mid;
 		else
 			hi = mid;
 	}
-	if (lo >= a.n_seqs)
+	// the last b in [lo, hi) with first[b] <= t (of equal ones the last: the others hold nothing)
+	const int lane = threadIdx.x & 63, b = lo + lane;
+	const int from = b < hi ? a.first[b] : 0x7fffffff, to = b < hi ? a.first[b + 1] : 0;
+	const unsigned long long below = __ballot(from <= t);
+	if (!below)
 		return -1;
-	t0 = a.first[lo];
-	t1 = a.first[lo + 1];
-	return t0 >= 0 && t0 <= t && t < t1 && t1 <= a.n_tokens ? lo : -1;
+	const int l = 63 - __builtin_clzll(below);
+	t0 = __builtin_amdgcn_readlane(from, l);
+	t1 = __builtin_amdgcn_readlane(to, l);
+	return t0 >= 0 && t < t1 && t1 <= a.n_tokens ? lo + l : -1;
 }
 
 // Whether the sequences' ranges ascend within the rows (the whole workgroup).
@@ -212,20 +252,25 @@ __device__ void write_path(const VerifyArgs &a, const VerifyWork &w, int b, int 
 {
 	int32_t *path = a.path + (size_t)b * a.max_path;
 	const int n = t1 - t0;
-	for (int i = threadIdx.x; i < n && i < V_PATH_LDS; i += blockDim.x)
+	for (int i = threadIdx.x; i < n && i < V_PATH_LDS; i += blockDim.x) {
 		sh.path[i] = have(w.take + t0 + i);
+		sh.own[i] = have(w.own + t0 + i);
+		sh.leaf[i] = have(w.leaf + t0 + i);
+	}
 	__syncthreads();
 	if (threadIdx.x == 0) {
 		int t = t0, k = 0, next = -1;
 		while (n > 0) {
-			path[k++] = t - t0;
+			const int i = t - t0;
+			path[k++] = i;
 			if (k >= a.max_path) {
-				next = have(w.leaf + t); // (its children were never to be tried)
+				// (its children were never to be tried)
+				next = i < V_PATH_LDS ? sh.leaf[i] : have(w.leaf + t);
 				break;
 			}
-			const int kid = t - t0 < V_PATH_LDS ? sh.path[t - t0] : have(w.take + t);
+			const int kid = i < V_PATH_LDS ? sh.path[i] : have(w.take + t);
 			if (kid < 0) {
-				next = have(w.own + t);
+				next = i < V_PATH_LDS ? sh.own[i] : have(w.own + t);
 				break;
 			}
 			t = kid; // (a later row of the same sequence)
@@ -240,15 +285,17 @@ __device__ void write_path(const VerifyArgs &a, const VerifyWork &w, int b, int 
 }
 
 // The first index whose running weight exceeds u times the whole: over the
-// chunks' sums (sum(c): of chunk c), then inside the chunk (weight(i) >= 0).
+// chunks' sums (lane_sum: of the first 64, a lane each; sum(c) of the others),
+// then inside the chunk: weights(i0, w) gives the V_E weights from i0 on (>= 0).
+// A workgroup, once for a row: what bounds it is the chain of its steps.
 template <typename W, typename S>
-__device__ __forceinline__ int locate(const VerifyArgs &a, int chunks, double u, W weight, S sum, Shared &sh)
+__device__ __forceinline__ int locate(const VerifyArgs &a, int chunks, double u, double lane_sum, W weights, S sum, Shared &sh)
 {
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-	// (every wave for itself: a lane a chunk)
-	double all = 0.0;
-	int last = 0;
-	for (int c0 = 0; c0 < chunks; c0 += 64) {
+	double all = wave_total(lane_sum);
+	const unsigned long long some0 = __ballot(lane_sum > 0.0);
+	int last = some0 ? 63 - __builtin_clzll(some0) : 0;
+	for (int c0 = 64; c0 < chunks; c0 += 64) {
 		const double x = c0 + lane < chunks ? sum(c0 + lane) : 0.0;
 		const unsigned long long some = __ballot(x > 0.0);
 		if (some)
@@ -259,67 +306,80 @@ __device__ __forceinline__ int locate(const VerifyArgs &a, int chunks, double u,
 	double before = 0.0, upto = 0.0;
 	int at = -1;
 	for (int c0 = 0; c0 < chunks && at < 0; c0 += 64) {
-		const double x = c0 + lane < chunks ? sum(c0 + lane) : 0.0;
-		double incl = x;
-#pragma unroll
-		for (int m = 1; m < 64; m <<= 1) {
-			const double o = __shfl_up(incl, m);
-			if (lane >= m)
-				incl += o;
-		}
+		const double x = c0 == 0 ? lane_sum : c0 + lane < chunks ? sum(c0 + lane) : 0.0;
+		const double incl = running(x);
 		const unsigned long long over = __ballot(upto + incl > want && c0 + lane < chunks);
 		const int l = over ? __builtin_ctzll(over) : last - c0; // (for the fallback: the last chunk of any weight)
 		if (over || (last >= c0 && last < c0 + 64)) {
-			before = upto + __shfl(incl - x, l & 63);
+			before = upto + of_lane(incl - x, l & 63);
 			if (over)
 				at = c0 + l;
 		}
-		upto += __shfl(incl, 63);
+		upto += of_lane(incl, 63);
 	}
 	if (at < 0)
 		at = last; // (u of one, or a rounding at the end)
-	// thread i has V_E weights in a row
-	const int base = at * V_CHUNK + threadIdx.x * V_E;
-	double x[V_E], mine = 0.0;
+	const int i0 = at * V_CHUNK + threadIdx.x * V_E;
+	double w[V_E], mine = 0.0;
+	weights(i0, w);
+	int some = 0; // the last of the thread's indexes with a weight, + 1
 #pragma unroll
 	for (int e = 0; e < V_E; e++) {
-		x[e] = base + e < a.vocab ? weight(base + e) : 0.0;
-		mine += x[e];
+		mine += w[e];
+		some = w[e] > 0.0 ? e + 1 : some;
 	}
-	double incl = mine;
-#pragma unroll
-	for (int m = 1; m < 64; m <<= 1) {
-		const double o = __shfl_up(incl, m);
-		if (lane >= m)
-			incl += o;
-	}
+	const double incl = running(mine);
 	__syncthreads();
 	if (lane == 63)
 		sh.d[wave] = incl;
-	if (threadIdx.x == 0)
-		sh.i[0] = 0x7fffffff, sh.i[1] = 0;
 	__syncthreads();
-	double run = before + incl - mine;
 	for (int q = 0; q < wave; q++)
-		run += sh.d[q];
-	int first = 0x7fffffff, some = -1;
-#pragma unroll
-	for (int e = 0; e < V_E; e++) {
-		run += x[e];
-		if (x[e] > 0.0) {
-			some = base + e;
-			if (run > want && first == 0x7fffffff)
-				first = base + e;
-		}
+		before += sh.d[q];
+	// the first thread whose weights pass `want`; where none does, the last
+	// that has any
+	const unsigned long long over = __ballot(before + incl > want), any = __ballot(some > 0);
+	if (lane == 0) {
+		sh.i[wave] = over ? wave * 64 + __builtin_ctzll(over) : V_THREADS;
+		sh.j[wave] = any ? wave * 64 + 63 - __builtin_clzll(any) : 0;
 	}
-	if (first != 0x7fffffff)
-		atomicMin(&sh.i[0], first);
-	if (some >= 0)
-		atomicMax(&sh.i[1], some);
 	__syncthreads();
-	const int got = sh.i[0] < a.vocab ? sh.i[0] : sh.i[1];
+	int owner = V_THREADS, end = 0;
+#pragma unroll
+	for (int q = 0; q < V_THREADS / 64; q++) {
+		owner = min(owner, sh.i[q]);
+		end = max(end, sh.j[q]);
+	}
+	owner = owner < V_THREADS ? owner : end;
+	if ((int)threadIdx.x == owner) {
+		double run = before + incl - mine;
+		int e0 = some > 0 ? some - 1 : 0; // (a rounding between the two sums: its last weight)
+#pragma unroll
+		for (int e = 0; e < V_E; e++) {
+			run += w[e];
+			e0 = run > want && w[e] > 0.0 && e < e0 ? e : e0;
+		}
+		sh.flag = i0 + e0;
+	}
 	__syncthreads();
-	return got;
+	const int got = sh.flag;
+	__syncthreads();
+	return got < a.vocab ? got : 0;
+}
+
+// V_E values of a row from i0 on, `none` behind its end
+__device__ __forceinline__ void get_run(const float *row, int i0, int n, float none, float (&x)[V_E])
+{
+	if (i0 + V_E <= n && ((uintptr_t)row & 15) == 0) {
+#pragma unroll
+		for (int e = 0; e < V_E; e += 4) {
+			const float4 v = reinterpret_cast<const float4 *>(row + i0)[e / 4];
+			x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
+		}
+	} else {
+#pragma unroll
+		for (int e = 0; e < V_E; e++)
+			x[e] = i0 + e < n ? row[i0 + e] : none;
+	}
 }
 
 // Row t's outcome as far as the sums so far carry it: the largest logit and the
@@ -335,78 +395,99 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 	const double inv = a.temperature > 0.0f ? 1.0 / (double)a.temperature : 0.0;
 	const double *s = w.s + (size_t)t * w.chunks, *res = w.res + (size_t)t * w.chunks;
 	const uint64_t *top = w.top + (size_t)t * w.chunks;
-	VRow r;
-	if (pass == 0) {
-		r.m = -__builtin_inff();
-		r.best = 0x7fffffff;
-		for (int c0 = 0; c0 < w.chunks; c0 += 64) {
-			if (c0 + lane < w.chunks) {
-				const uint64_t v = have(top + c0 + lane);
-				const float m = __uint_as_float((uint32_t)v);
-				if (m > r.m) {
-					r.m = m;
-					r.best = (int)(v >> 32);
-				}
-			}
-		}
-#pragma unroll
-		for (int q = 1; q < 64; q <<= 1) {
-			const float om = __shfl_xor(r.m, q);
-			const int oi = __shfl_xor(r.best, q);
-			if (om > r.m || (om == r.m && oi < r.best)) {
-				r.m = om;
-				r.best = oi;
-			}
-		}
-		if (r.best >= a.vocab)
-			r.best = 0;
-		double z = 0.0;
-		if (a.temperature > 0.0f)
-			for (int c = lane; c < w.chunks; c += 64) {
-				const float m = __uint_as_float((uint32_t)have(top + c));
-				if (m > -__builtin_inff())
-					z += have(s + c) * exp_below(((double)m - (double)r.m) * inv);
-			}
-		r.scale = 1.0 / wave_total(z);
-		r.c = 0.0;
-		r.M = 1.0;
-		r.kid = 0;
-		r.waits = -1;
-	} else {
-		r = w.row[t];
-		double M = 0.0;
-		for (int c = lane; c < w.chunks; c += 64)
-			M += have(res + c);
-		r.M = wave_total(M);
-		r.waits = -1;
-	}
 	const float *l = a.logits + (size_t)t * a.l_stride, *q = a.draft ? a.draft + (size_t)t * a.d_stride : nullptr;
-	auto p_of = [&](float x) { return exp_below(((double)x - (double)r.m) * inv) * r.scale; };
+	// all that the first steps need is requested at once: the first 64 chunks'
+	// sums, the 64 rows behind this one (its children are among them, mostly)
+	const float us = a.u_sample[t];
+	uint64_t top0 = 0;
+	double s0 = 0.0, r0 = 0.0;
+	if (lane < w.chunks) {
+		top0 = have(top + lane);
+		s0 = have(s + lane);
+		if (pass)
+			r0 = have(res + lane);
+	}
+	const int j1 = min(t + 1 + lane, a.n_tokens - 1);
+	const int parent1 = a.parent[j1], token1 = a.tokens[j1];
+	const float u1 = a.u_accept[j1];
 
 	// the children: later rows of the sequence whose parent this is; lane i has
 	// the i-th
-	int n = 0, kid = -1;
+	int n = 0, kid = -1, x = -1;
+	float uf = 0.0f;
 	for (int j0 = t + 1; j0 < t1 && n < a.max_children; j0 += 64) {
 		const int j = j0 + lane;
-		unsigned long long set = __ballot(j < t1 && a.parent[j < t1 ? j : t] == t - t0);
+		const bool near = j0 == t + 1;
+		unsigned long long set = __ballot(j < t1 && (near ? parent1 : a.parent[j < t1 ? j : t]) == t - t0);
 		while (set && n < a.max_children) {
-			if (lane == n)
-				kid = j0 + __builtin_ctzll(set);
+			const int from = __builtin_ctzll(set);
+			const int xi = near ? __builtin_amdgcn_readlane(token1, from) : a.tokens[j0 + from];
+			const float ui = near ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, u1), from)) : a.u_accept[j0 + from];
+			if (lane == n) {
+				kid = j0 + from;
+				x = xi;
+				uf = ui;
+			}
 			set &= set - 1;
 			n++;
 		}
 	}
-	int x = -1;
-	double px = 0.0, qx = 1.0, u = 0.0;
-	if (kid >= 0) {
-		x = a.tokens[kid];
-		u = (double)a.u_accept[kid];
-		if (x >= 0 && x < a.vocab && a.temperature > 0.0f) {
-			px = p_of(l[x]);
-			if (q)
-				qx = (double)q[x];
+	// (their logits and draft probabilities, on the way while the sums are joined)
+	const bool is_token = kid >= 0 && x >= 0 && x < a.vocab;
+	const float lx = is_token ? l[x] : 0.0f;
+	const double qx = is_token && q ? (double)q[x] : 1.0, u = (double)uf;
+
+	VRow r;
+	double z0 = 0.0; // lane c: the whole of chunk c, times exp(largest of all)
+	if (pass == 0) {
+		r.m = lane < w.chunks ? __uint_as_float((uint32_t)top0) : -__builtin_inff();
+		r.best = lane < w.chunks ? (int)(top0 >> 32) : 0x7fffffff;
+		for (int c = 64 + lane; c < w.chunks; c += 64) {
+			const uint64_t v = have(top + c);
+			const float m = __uint_as_float((uint32_t)v);
+			if (m > r.m) {
+				r.m = m;
+				r.best = (int)(v >> 32);
+			}
 		}
+		const float most = wave_max(r.m);
+		if (a.temperature == 0.0f) {
+			r.best = r.m == most ? r.best : 0x7fffffff;
+#pragma unroll
+			for (int k = 1; k < 64; k <<= 1)
+				r.best = min(r.best, __shfl_xor(r.best, k));
+		}
+		r.m = most;
+		if (r.best < 0 || r.best >= a.vocab)
+			r.best = 0;
+	} else {
+		r = w.row[t];
 	}
+	auto whole_of = [&](uint64_t v, double sum) {
+		const float m = __uint_as_float((uint32_t)v);
+		return m > -__builtin_inff() ? sum * exp_below(((double)m - (double)r.m) * inv) : 0.0;
+	};
+	if (a.temperature > 0.0f && lane < w.chunks)
+		z0 = whole_of(top0, s0);
+	if (pass == 0) {
+		double z = z0;
+		if (a.temperature > 0.0f)
+			for (int c = 64 + lane; c < w.chunks; c += 64)
+				z += whole_of(have(top + c), have(s + c));
+		r.scale = 1.0 / wave_total(z);
+		r.c = 0.0;
+		r.M = 1.0;
+		r.kid = 0;
+	} else {
+		double M = r0;
+		for (int c = 64 + lane; c < w.chunks; c += 64)
+			M += have(res + c);
+		r.M = wave_total(M);
+	}
+	r.waits = -1;
+	auto p_of = [&](float y) { return exp_below(((double)y - (double)r.m) * inv) * r.scale; };
+	const double px = is_token && a.temperature > 0.0f ? p_of(lx) : 0.0;
+
 	int taken = -1;
 	unsigned long long gone = 0; // no draft rows: refused children
 	for (int i = r.kid; i < n; i++) {
@@ -451,44 +532,54 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 
 	int own = r.best, leaf = r.best;
 	if (a.temperature > 0.0f) {
-		auto p_sum = [&](int c) {
-			const float m = __uint_as_float((uint32_t)have(top + c));
-			return m > -__builtin_inff() ? have(s + c) * exp_below(((double)m - (double)r.m) * inv) * r.scale : 0.0;
-		};
-		auto p_at = [&](int i) { return p_of(l[i]); };
-		const double us = (double)a.u_sample[t];
+		auto p_sum = [&](int c) { return whole_of(have(top + c), have(s + c)) * r.scale; };
 		const bool cut = a.max_path < t1 - t0; // a path may end at any node
 		const bool plain = (r.c == 0.0 && !gone) || !(r.M > 0.0);
-		if ((taken < 0 && plain) || (cut && n > 0))
-			own = leaf = locate(a, w.chunks, us, p_at, p_sum, sh);
-		if (taken < 0 && !plain && q)
-			own = locate(
-				a, w.chunks, us,
-				[&](int i) {
-					const double y = p_of(l[i]) - r.c * (double)q[i];
-					return y > 0.0 ? y : 0.0;
-				},
-				[&](int c) { return have(res + c); }, sh);
-		else if (taken < 0 && !plain)
-			own = locate(
-				a, w.chunks, us,
-				[&](int i) {
-					double y = p_of(l[i]);
-					for (unsigned long long g = gone; g; g &= g - 1)
-						if (__builtin_amdgcn_readlane(x, __builtin_ctzll(g)) == i)
-							y = 0.0;
-					return y;
-				},
-				[&](int c) {
-					double y = c < w.chunks ? p_sum(c) : 0.0;
-					for (unsigned long long g = gone; g; g &= g - 1) {
-						const int k = __builtin_ctzll(g);
-						if (__builtin_amdgcn_readlane(x, k) / V_CHUNK == c)
-							y -= of_lane(px, k);
+		auto without = [&](int c, double y) { // of chunk c: less what left p
+			for (unsigned long long g = gone; g; g &= g - 1) {
+				const int k = __builtin_ctzll(g);
+				if (__builtin_amdgcn_readlane(x, k) / V_CHUNK == c)
+					y -= of_lane(px, k);
+			}
+			return y > 0.0 ? y : 0.0;
+		};
+#pragma unroll 1
+		for (int what = 0; what < 2; what++) {
+			if (what == 0 ? taken >= 0 : !(cut && n > 0))
+				continue;
+			const bool of_p = what == 1 || plain;
+			const double c_q = of_p || !q ? 0.0 : r.c;
+			const unsigned long long out = of_p ? 0 : gone;
+			const int got = locate(
+				a, w.chunks, (double)us, c_q > 0.0 ? r0 : out ? without(lane, z0 * r.scale) : z0 * r.scale,
+				[&](int i0, double (&y)[V_E]) {
+					float li[V_E], qi[V_E];
+					get_run(l, i0, a.vocab, -__builtin_inff(), li);
+					if (c_q > 0.0)
+						get_run(q, i0, a.vocab, 0.0f, qi);
+#pragma unroll
+					for (int e = 0; e < V_E; e++)
+						y[e] = p_of(li[e]);
+					if (c_q > 0.0)
+#pragma unroll
+						for (int e = 0; e < V_E; e++)
+							y[e] -= c_q * (double)qi[e];
+					for (unsigned long long g = out; g; g &= g - 1) {
+						const int away = __builtin_amdgcn_readlane(x, __builtin_ctzll(g)) - i0;
+#pragma unroll
+						for (int e = 0; e < V_E; e++)
+							y[e] = away == e ? 0.0 : y[e];
 					}
-					return y > 0.0 ? y : 0.0;
+#pragma unroll
+					for (int e = 0; e < V_E; e++)
+						y[e] = y[e] > 0.0 ? y[e] : 0.0;
 				},
-				sh);
+				[&](int c) { return c_q > 0.0 ? have(res + c) : out ? without(c, p_sum(c)) : p_sum(c); }, sh);
+			if (what == 0)
+				own = got;
+			else
+				leaf = got;
+		}
 		if (n == 0)
 			leaf = own;
 	}
@@ -523,34 +614,29 @@ __global__ __launch_bounds__(V_THREADS) void verify_stats_kernel(VerifyArgs a, V
 			x[e] = i < a.vocab ? l[i] : -__builtin_inff();
 		}
 	}
-	float m = -__builtin_inff();
-	int at = 0x7fffffff;
+	float m = x[0];
 #pragma unroll
-	for (int e = 0; e < V_E; e++)
-		if (x[e] > m) {
-			m = x[e];
-			at = base + (e / 4 * V_THREADS + threadIdx.x) * 4 + e % 4;
-		}
-#pragma unroll
-	for (int q = 1; q < 64; q <<= 1) {
-		const float om = __shfl_xor(m, q);
-		const int oi = __shfl_xor(at, q);
-		if (om > m || (om == m && oi < at)) {
-			m = om;
-			at = oi;
-		}
-	}
-	if ((threadIdx.x & 63) == 0) {
+	for (int e = 1; e < V_E; e++)
+		m = __builtin_fmaxf(m, x[e]);
+	m = wave_max(m);
+	if ((threadIdx.x & 63) == 0)
 		sh.f[threadIdx.x >> 6] = m;
-		sh.i[threadIdx.x >> 6] = at;
-	}
 	__syncthreads();
+	m = __builtin_fmaxf(__builtin_fmaxf(sh.f[0], sh.f[1]), __builtin_fmaxf(sh.f[2], sh.f[3]));
+	int at = 0;
+	if (a.temperature == 0.0f) { // its lowest index
+		at = 0x7fffffff;
 #pragma unroll
-	for (int q = 0; q < 4; q++)
-		if (sh.f[q] > m || (sh.f[q] == m && sh.i[q] < at)) {
-			m = sh.f[q];
-			at = sh.i[q];
-		}
+		for (int e = V_E - 1; e >= 0; e--)
+			at = x[e] == m ? base + (e / 4 * V_THREADS + (int)threadIdx.x) * 4 + e % 4 : at;
+#pragma unroll
+		for (int k = 1; k < 64; k <<= 1)
+			at = min(at, __shfl_xor(at, k));
+		if ((threadIdx.x & 63) == 0)
+			sh.i[threadIdx.x >> 6] = at;
+		__syncthreads();
+		at = min(min(sh.i[0], sh.i[1]), min(sh.i[2], sh.i[3]));
+	}
 	double s = 0.0;
 	if (a.temperature > 0.0f && m > -__builtin_inff()) {
 		const double inv = 1.0 / (double)a.temperature;
