@@ -75,6 +75,61 @@ size_t verify_work_bytes(const VerifyArgs &a, bool with_draft);
 hipError_t launch_verify(const VerifyArgs &a, void *work, hipStream_t st);
 
 #if defined(__HIPCC__)
+// x moved across lanes by a DPP control; lanes that get nothing: `none`
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp(float none, float x)
+{
+	return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, x), CTRL,
+								     ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp(double none, double x)
+{
+	const uint64_t n = (uint64_t)__double_as_longlong(none), v = (uint64_t)__double_as_longlong(x);
+	const uint32_t lo = __builtin_amdgcn_update_dpp((int)(uint32_t)n, (int)(uint32_t)v, CTRL, ROWS, 0xf, false),
+		       hi = __builtin_amdgcn_update_dpp((int)(n >> 32), (int)(v >> 32), CTRL, ROWS, 0xf, false);
+	return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+
+// x of a lane (the same in all lanes), whether it is active here or not
+__device__ __forceinline__ double of_lane(double x, int lane)
+{
+	const uint64_t v = (uint64_t)__double_as_longlong(x);
+	const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+	return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+
+// The running sum, or maximum, over groups of L = 64 or 32 lanes (a group's last
+// lane has the whole), in registers: within rows of 16 by shifts, then the rows'
+// ends into the rows behind.
+template <int L> __device__ __forceinline__ double running_of(double x)
+{
+	x = x + dpp<0x111, 0xf>(0.0, x);
+	x = x + dpp<0x112, 0xf>(0.0, x);
+	x = x + dpp<0x114, 0xf>(0.0, x);
+	x = x + dpp<0x118, 0xf>(0.0, x);
+	x = x + dpp<0x142, 0xa>(0.0, x);
+	return L == 64 ? x + dpp<0x143, 0xc>(0.0, x) : x;
+}
+template <int L> __device__ __forceinline__ float running_max_of(float x)
+{
+	const float none = -__builtin_inff();
+	x = __builtin_fmaxf(x, dpp<0x111, 0xf>(none, x));
+	x = __builtin_fmaxf(x, dpp<0x112, 0xf>(none, x));
+	x = __builtin_fmaxf(x, dpp<0x114, 0xf>(none, x));
+	x = __builtin_fmaxf(x, dpp<0x118, 0xf>(none, x));
+	x = __builtin_fmaxf(x, dpp<0x142, 0xa>(none, x));
+	return L == 64 ? __builtin_fmaxf(x, dpp<0x143, 0xc>(none, x)) : x;
+}
+
+__device__ __forceinline__ double wave_total(double x)
+{
+	return of_lane(running_of<64>(x), 63);
+}
+
+__device__ __forceinline__ float wave_max(float x)
+{
+	return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, running_max_of<64>(x)), 63));
+}
+
 // The token rows of sequence b: [t0, t0 + n), n = 0 where the arrays say
 // something that lies outside the call's own sizes.
 __device__ __forceinline__ void seq_tokens(const KvSeqs &s, int b, int &t0, int &n)

@@ -25,75 +25,93 @@ __device__ __forceinline__ _Float16 half_of(float x)
 	return (_Float16)x;
 }
 
-// A wave takes heads of one token, HD / 2 lanes each: a lane holds the pair
-// (x[i], x[i + HD / 2]) that the rotation turns.  All of it in 64 bits up to
-// the one rounding to F32: positions reach where a 32-bit angle is off by a
-// thousandth, and a key's code must not depend on the order of a 32-bit sum.
+// A workgroup has one token; its waves take heads in turn, HD / 2 lanes each: a
+// lane holds the pair (x[i], x[i + HD / 2]) that the rotation turns, and its
+// cosine and sine stay with it.  All of it in 64 bits up to the one rounding to
+// F32: positions reach where a 32-bit angle is off by a thousandth, and a key's
+// code must not depend on the order of a 32-bit sum.  One token: bound by its
+// chain of steps (position, angle, sincos; row, norm, code).  Many: by the 64-bit
+// arithmetic, about 60 instructions for 64 pairs, and the V columns' pieces (a
+// row's values lie PAGE apart).
 template <int HD, bool I8>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, AppendArgs a, int per_wave)
 {
 	constexpr int L = HD / 2, G = 64 / L; // lanes of a head, heads of a wave at a time
-	const int t = blockIdx.x, lane = threadIdx.x & 63, i = lane % L;
-	const int wave = blockIdx.y * 4 + (threadIdx.x >> 6);
+	const int t = blockIdx.x, lane = threadIdx.x & 63, i = lane % L, part = lane / L;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	int t0, n;
 	const int b = seq_of_token(s, t, t0, n);
 	if (b < 0)
 		return;
+	const int n_all = a.n_heads + 2 * c.kvh;
+	const int u0 = blockIdx.y * per_wave * 4 + wave; // this wave's units: u0, u0 + 4, ...
+	auto source = [&](int h, int &kv) {
+		kv = h - a.n_heads;
+		return kv < 0 ? a.q + (size_t)t * a.q_stride + (size_t)h * HD
+		       : kv < c.kvh ? a.k + (size_t)t * a.k_stride + (size_t)kv * HD
+				    : a.v + (size_t)t * a.v_stride + (size_t)(kv - c.kvh) * HD;
+	};
+	// the first head's row and the norms' weights are requested before the
+	// position is known
+	float n0 = 0.0f, n1 = 0.0f;
+	auto fetch = [&](int u) {
+		int kv;
+		const int h = u * G + part;
+		if (h < n_all) {
+			const float *p = source(h, kv);
+			n0 = p[i];
+			n1 = p[i + L];
+		}
+	};
+	fetch(u0);
+	const double wq0 = a.q_norm ? (double)a.q_norm[i] : 1.0, wq1 = a.q_norm ? (double)a.q_norm[i + L] : 1.0;
+	const double wk0 = a.k_norm ? (double)a.k_norm[i] : 1.0, wk1 = a.k_norm ? (double)a.k_norm[i + L] : 1.0;
 	const int len = s.len[b], row = len + (t - t0);
 	const bool fits = seq_fits(s, len, n);
 	const int page = fits ? page_of(s, c.n_pages, b, row) : -1, r = fits ? row % PAGE : 0;
-	const int n_all = a.n_heads + 2 * c.kvh;
-	double cs = 0.0, sn = 0.0;
-	{
-		const int pos = a.pos ? a.pos[t] : row;
-		const double angle = (double)pos * exp2((double)i * (-2.0 / HD) * a.log2_theta);
-		sincos(angle, &sn, &cs);
-	}
+	double cs, sn;
+	sincos((double)(a.pos ? a.pos[t] : row) * exp2((double)i * (-2.0 / HD) * a.log2_theta), &sn, &cs);
 	for (int u = 0; u < per_wave; u++) {
-		const int h = (wave * per_wave + u) * G + lane / L;
+		const int h = (u0 + 4 * u) * G + part;
+		if ((u0 + 4 * u) * G >= n_all)
+			break;
 		const bool on = h < n_all;
 		const int kv = h - a.n_heads, head = kv < 0 ? h : kv < c.kvh ? kv : kv - c.kvh;
 		const bool is_q = kv < 0, is_v = kv >= c.kvh;
-		float x0 = 0.0f, x1 = 0.0f;
-		if (on) {
-			const float *p = (is_q ? a.q + (size_t)t * a.q_stride
-				       : is_v  ? a.v + (size_t)t * a.v_stride
-					       : a.k + (size_t)t * a.k_stride) +
-					 (size_t)head * HD;
-			x0 = p[i];
-			x1 = p[i + L];
-		}
-		const float *w = is_q ? a.q_norm : a.k_norm;
-		if (!is_v) {
+		float x0 = n0, x1 = n1;
+		if (u + 1 < per_wave)
+			fetch(u0 + 4 * (u + 1));
+		if (!__all(is_v)) {
 			double y0 = x0, y1 = x1;
-			double ss = y0 * y0 + y1 * y1;
-#pragma unroll
-			for (int m = 1; m < L; m <<= 1)
-				ss += __shfl_xor(ss, m);
-			if (w) {
-				const double f = 1.0 / sqrt(ss / HD + a.eps);
-				y0 = y0 * f * (double)w[i];
-				y1 = y1 * f * (double)w[i + L];
+			if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
+				// (a head's sum lies in its last lane)
+				const double ss = running_of<L>(__builtin_fma(y0, y0, y1 * y1));
+				const double total = G == 1 ? of_lane(ss, 63) : part ? of_lane(ss, 63) : of_lane(ss, 31);
+				const double f = rsqrt(__builtin_fma(total, 1.0 / HD, a.eps));
+				y0 *= f * (is_q ? wq0 : wk0);
+				y1 *= f * (is_q ? wq1 : wk1);
 			}
-			x0 = (float)(y0 * cs - y1 * sn);
-			x1 = (float)(y1 * cs + y0 * sn);
+			const float z0 = (float)__builtin_fma(y0, cs, -(y1 * sn)), z1 = (float)__builtin_fma(y1, cs, y0 * sn);
+			x0 = is_v ? x0 : z0;
+			x1 = is_v ? x1 : z1;
 		}
 		if (on && is_q) {
 			float *o = a.q_out + (size_t)t * a.qo_stride + (size_t)head * HD;
 			o[i] = x0;
 			o[i + L] = x1;
 		}
+		if (__all(is_q))
+			continue;
 		// (every lane of a head takes part in its row's largest magnitude)
 		float scale = 0.0f;
 		if (I8) {
-			float m = __builtin_fmaxf(__builtin_fabsf(x0), __builtin_fabsf(x1));
-			bool bad = !(__builtin_fabsf(x0) < __builtin_inff()) || !(__builtin_fabsf(x1) < __builtin_inff());
-#pragma unroll
-			for (int q = 1; q < L; q <<= 1) {
-				m = __builtin_fmaxf(m, __shfl_xor(m, q));
-				bad |= __shfl_xor((int)bad, q) != 0;
-			}
-			scale = bad ? __builtin_nanf("") : m / 127.0f;
+			const float big = __builtin_fmaxf(__builtin_fabsf(x0), __builtin_fabsf(x1));
+			const unsigned long long mine = G == 1 ? ~0ull : part ? 0xffffffff00000000ull : 0xffffffffull;
+			const bool bad = (__ballot(!(__builtin_fabsf(x0) < __builtin_inff()) || !(__builtin_fabsf(x1) < __builtin_inff())) & mine) != 0;
+			const float m = running_max_of<L>(big);
+			const int top = G == 1 || part ? 63 : 31;
+			const float most = __shfl(m, top);
+			scale = bad ? __builtin_nanf("") : most / 127.0f;
 		}
 		if (!on || is_q || page < 0)
 			continue;
@@ -116,12 +134,12 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 
 hipError_t launch_kv_append(const KvLayer &c, const KvSeqs &s, const AppendArgs &a, hipStream_t st)
 {
-	const int units = (a.n_heads + 2 * c.kvh + 128 / c.hd - 1) / (128 / c.hd); // waves with a head (pair) each
-	// a wave takes one unit where there are few tokens, else several: the
-	// angles' cosines are the same for all of them
-	int per = 1;
-	while (per < 16 && (size_t)s.n_tokens * units > (size_t)4096 * per)
-		per *= 2;
+	const int units = (a.n_heads + 2 * c.kvh + 128 / c.hd - 1) / (128 / c.hd); // a wave's share at a time: a head of 128, two of 64
+	// a wave takes one unit where there are few tokens, else as many as leave
+	// 4096 waves: the angles' cosines are the same for all of them
+	const size_t all = (size_t)s.n_tokens * units;
+	int per = all > 4096 ? (int)(all / 4096) : 1;
+	per = per > (units + 3) / 4 ? (units + 3) / 4 : per;
 	const dim3 grid(s.n_tokens, (units + 4 * per - 1) / (4 * per));
 	auto go = [&](auto kern) { tie_launch(kern, grid, dim3(256), 0, st, c, s, a, per); };
 	if (c.hd == 128)
@@ -132,141 +150,239 @@ hipError_t launch_kv_append(const KvLayer &c, const KvSeqs &s, const AppendArgs 
 }
 
 // ---------------------------------------------------------------- read
-// One workgroup a token row and layer.  A row that the table does not reach
-// reads as NaN.
-template <bool I8>
+// A workgroup has the rows of one sequence in one page, of one kv head and layer.
+// K rows go through as they lie; V columns come into LDS in 16-byte pieces and
+// leave it as rows (columns 4 bytes further apart than they are long: the lanes
+// of a row read different banks).  Bound by the F32 rows written.  Rows that the
+// table does not reach read as NaN.
+template <int HD, bool I8>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvLayer c, KvSeqs s, float *k_out, float *v_out)
 {
-	const int t = blockIdx.x, layer = blockIdx.y, w = c.kvh * c.hd;
-	int t0, n;
-	const int b = seq_of_token(s, t, t0, n);
+	constexpr int E = I8 ? 1 : 2, CS = PAGE * E + 4; // bytes of a column in LDS
+	__shared__ __attribute__((aligned(16))) uint8_t tile[HD * CS];
+	__shared__ float scale[PAGE];
+	const int lane = threadIdx.x & 63, h = blockIdx.y, layer = blockIdx.z;
+	// the sequence and page of this workgroup
+	int b = -1, t0 = 0, n = 0, len = 0, p = 0;
+	for (int b0 = 0, before = 0; b0 < s.n_seqs; b0 += 64) {
+		int st0 = 0, sn = 0, sl = 0, pages = 0;
+		if (b0 + lane < s.n_seqs) {
+			sl = s.len[b0 + lane];
+			seq_tokens(s, b0 + lane, st0, sn);
+			if (sn > 0) {
+				// (rows that do not fit: one workgroup for each 64 of them)
+				const int from = seq_fits(s, sl, sn) ? sl % PAGE : 0;
+				pages = (from + sn + PAGE - 1) / PAGE;
+			}
+		}
+		int incl = pages;
+		if (s.n_seqs > 1)
+#pragma unroll
+			for (int m = 1; m < 64; m <<= 1) {
+				const int o = __shfl_up(incl, m);
+				if (lane >= m)
+					incl += o;
+			}
+		const unsigned long long past = __ballot(before + incl > (int)blockIdx.x);
+		if (past) {
+			const int l = __builtin_ctzll(past);
+			b = b0 + l;
+			t0 = __builtin_amdgcn_readlane(st0, l);
+			n = __builtin_amdgcn_readlane(sn, l);
+			len = __builtin_amdgcn_readlane(sl, l);
+			p = (int)blockIdx.x - before - __builtin_amdgcn_readlane(incl - pages, l);
+			break;
+		}
+		before += __builtin_amdgcn_readlane(incl, 63);
+	}
 	if (b < 0)
 		return;
-	const int len = s.len[b], row = len + (t - t0);
-	const int page = seq_fits(s, len, n) ? page_of(s, c.n_pages, b, row) : -1, r = page < 0 ? 0 : row % PAGE;
-	const size_t o = ((size_t)layer * s.n_tokens + t) * w;
-	for (int e = threadIdx.x; e < w; e += 256) {
-		if (page < 0) {
-			k_out[o + e] = v_out[o + e] = __builtin_nanf("");
+	const bool fits = seq_fits(s, len, n);
+	// rows [r0, r1) of the page are token rows t0 + first ...
+	const int from = fits ? len % PAGE : 0;
+	const int r0 = p == 0 ? from : 0, r1 = min(PAGE, from + n - p * PAGE), first = t0 + p * PAGE + r0 - from;
+	const int page = fits ? page_of(s, c.n_pages, b, len - from + p * PAGE) : -1;
+	const size_t width = (size_t)c.kvh * HD;
+	const size_t o = ((size_t)layer * s.n_tokens + first) * width + (size_t)h * HD;
+	if (page < 0) {
+		for (int e = threadIdx.x; e < (r1 - r0) * HD; e += 256)
+			k_out[o + e / HD * width + e % HD] = v_out[o + e / HD * width + e % HD] = __builtin_nanf("");
+		return;
+	}
+	const size_t at = (size_t)page * c.kvh + h;
+	const uint8_t *k = c.k + layer * c.layer_bytes + at * PAGE * HD * E, *v = c.v + layer * c.layer_bytes + at * PAGE * HD * E;
+	const float *ks = I8 ? c.ks + layer * c.layer_scales + at * PAGE : nullptr;
+	constexpr int VP = PAGE * E / 16; // pieces of a column
+	for (int e = threadIdx.x; e < HD * VP; e += 256) {
+		const int col = e / VP, q = e % VP;
+		if ((q + 1) * 16 / E <= r0 || q * 16 / E >= r1)
 			continue;
-		}
-		const int h = e / c.hd, i = e % c.hd;
-		const size_t at = (size_t)page * c.kvh + h;
-		const size_t ek = (size_t)layer * c.layer_bytes + (at * PAGE + r) * c.hd + i,
-			     ev = (size_t)layer * c.layer_bytes + (at * c.hd + i) * PAGE + r;
+		const uint4 x = reinterpret_cast<const uint4 *>(v)[e];
+		uint32_t *to = reinterpret_cast<uint32_t *>(tile + col * CS + q * 16);
+		to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+	}
+	if (I8 && threadIdx.x < PAGE)
+		scale[threadIdx.x] = c.vs[layer * c.layer_scales + at * PAGE + threadIdx.x];
+	// K: 4 values of a row to a thread
+	for (int e = threadIdx.x; e < (r1 - r0) * (HD / 4); e += 256) {
+		const int r = r0 + e / (HD / 4), i = e % (HD / 4) * 4;
+		float x[4];
 		if (I8) {
-			const size_t sc = (size_t)layer * c.layer_scales + at * PAGE + r;
-			k_out[o + e] = (float)reinterpret_cast<const int8_t *>(c.k)[ek] * c.ks[sc];
-			v_out[o + e] = (float)reinterpret_cast<const int8_t *>(c.v)[ev] * c.vs[sc];
+			const uint32_t w = *reinterpret_cast<const uint32_t *>(k + r * HD + i);
+			const float f = ks[r];
+#pragma unroll
+			for (int q = 0; q < 4; q++)
+				x[q] = sbyte_f(w, q) * f;
 		} else {
-			// (layer_bytes counts two for an element)
-			const size_t half = (size_t)layer * (c.layer_bytes / 2);
-			k_out[o + e] = (float)reinterpret_cast<const _Float16 *>(c.k)[half + (at * PAGE + r) * c.hd + i];
-			v_out[o + e] = (float)reinterpret_cast<const _Float16 *>(c.v)[half + (at * c.hd + i) * PAGE + r];
+			typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+			const h4 w = *reinterpret_cast<const h4 *>(k + (r * HD + i) * 2);
+#pragma unroll
+			for (int q = 0; q < 4; q++)
+				x[q] = (float)w[q];
 		}
+		float *to = k_out + o + (size_t)(r - r0) * width + i;
+		if (((uintptr_t)to & 15) == 0) {
+			*reinterpret_cast<float4 *>(to) = make_float4(x[0], x[1], x[2], x[3]);
+		} else {
+#pragma unroll
+			for (int q = 0; q < 4; q++)
+				to[q] = x[q];
+		}
+	}
+	__syncthreads();
+	// V: a column to a thread, a word's rows at a time
+	constexpr int W = 4 / E;
+	for (int e = threadIdx.x; e < (PAGE / W) * HD; e += 256) {
+		const int i = e % HD, r = e / HD * W;
+		if (r + W <= r0 || r >= r1)
+			continue;
+		const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + i * CS + r * E);
+#pragma unroll
+		for (int q = 0; q < W; q++)
+			if (r + q >= r0 && r + q < r1)
+				v_out[o + (size_t)(r + q - r0) * width + i] =
+					I8 ? sbyte_f(w, q) * scale[r + q] : (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> (16 * q)));
 	}
 }
 
 hipError_t launch_kv_read(const KvLayer &c, int n_layers, const KvSeqs &s, float *k_out, float *v_out, hipStream_t st)
 {
-	const dim3 grid(s.n_tokens, n_layers);
-	if (c.i8)
-		tie_launch(kv_read_kernel<true>, grid, dim3(256), 0, st, c, s, k_out, v_out);
+	// pages: a sequence's rows fill n / 64 of them, less what is left at both ends
+	const size_t seqs = s.n_seqs < s.n_tokens ? s.n_seqs : s.n_tokens;
+	const dim3 grid((uint32_t)((s.n_tokens + seqs * 2 * (PAGE - 1)) / PAGE), c.kvh, n_layers);
+	auto go = [&](auto kern) { tie_launch(kern, grid, dim3(256), 0, st, c, s, k_out, v_out); };
+	if (c.hd == 128)
+		c.i8 ? go(kv_read_kernel<128, true>) : go(kv_read_kernel<128, false>);
 	else
-		tie_launch(kv_read_kernel<false>, grid, dim3(256), 0, st, c, s, k_out, v_out);
+		c.i8 ? go(kv_read_kernel<64, true>) : go(kv_read_kernel<64, false>);
 	return hipGetLastError();
 }
 
 // ---------------------------------------------------------------- keep
-// Row len + path[j] to row len + j for j < n_keep, in every layer.  A thread
-// has one column (or the two scales) of one kv head and layer and moves its
-// rows in order, KEEP_BATCH loads before their stores: a path ascends, so
-// path[j] >= j and no store reaches a row that a later load wants.
+// Row len + path[j] to row len + j for j < n_keep, in every layer.  A workgroup
+// has one kv head and layer of a sequence, a thread one column of K or V: it
+// moves its rows in order, KEEP_BATCH loads before their stores.  A path ascends,
+// so path[j] >= j and no store reaches a row that a later load wants.  Where the
+// rows lie is worked out once, by the first wave.
 constexpr int KEEP_BATCH = 8;
+constexpr int KEEP_TABLE = 64; // path entries at a time
 
 // How many entries of sequence b's path can be moved: up to the first that
-// does not ascend or is none of its n nodes.
+// does not ascend or is none of its n nodes.  A wave.
 __device__ __forceinline__ int keep_count(const int32_t *path, int want, int n)
 {
-	int prev = -1, j = 0;
-	for (; j < want; j++) {
-		const int p = path[j];
-		if (p <= prev || p >= n)
-			break;
-		prev = p;
+	const int lane = threadIdx.x & 63;
+	for (int j0 = 0; j0 < want; j0 += 64) {
+		const int j = j0 + lane;
+		const bool in = j < want;
+		const int p = in ? path[j] : 0, prev = in && j > 0 ? path[j - 1] : -1;
+		const unsigned long long bad = __ballot(in && (p <= prev || p >= n));
+		if (bad)
+			return j0 + __builtin_ctzll(bad);
 	}
-	return j;
-}
-
-template <typename T>
-__device__ __forceinline__ void keep_rows(T *base, size_t page_stride, int row_stride, const KvLayer &c, const KvSeqs &s,
-					  int b, int len, const int32_t *path, int count)
-{
-	for (int j0 = 0; j0 < count; j0 += KEEP_BATCH) {
-		T v[KEEP_BATCH];
-		int to[KEEP_BATCH];
-#pragma unroll
-		for (int q = 0; q < KEEP_BATCH; q++) {
-			const int j = j0 + q;
-			to[q] = -1;
-			if (j < count && path[j] != j) {
-				const int from = page_of(s, c.n_pages, b, len + path[j]);
-				to[q] = page_of(s, c.n_pages, b, len + j);
-				if (from < 0)
-					to[q] = -1;
-				else
-					v[q] = base[from * page_stride + (size_t)((len + path[j]) % PAGE) * row_stride];
-			}
-		}
-#pragma unroll
-		for (int q = 0; q < KEEP_BATCH; q++)
-			if (to[q] >= 0)
-				base[to[q] * page_stride + (size_t)((len + j0 + q) % PAGE) * row_stride] = v[q];
-	}
+	return want > 0 ? want : 0;
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void kv_keep_kernel(KvLayer c, KvSeqs s, const int32_t *path, int max_path,
 						      const int32_t *n_keep, int32_t *len_out)
 {
+	// source and target, as page * PAGE + row; target -1: nothing to move
+	__shared__ int from[KEEP_TABLE], to[KEEP_TABLE];
 	const int h = blockIdx.x % c.kvh, layer = blockIdx.x / c.kvh, b = blockIdx.y, i = threadIdx.x % c.hd;
 	const bool is_v = (int)threadIdx.x >= c.hd;
 	int t0, n;
-	seq_tokens(s, b, t0, n);
 	const int len = s.len[b];
+	const int want = min(n_keep[b], max_path);
+	seq_tokens(s, b, t0, n);
 	const int32_t *pb = path + (size_t)b * max_path;
-	const int count = seq_fits(s, len, n) ? keep_count(pb, min(n_keep[b], max_path), n) : 0;
+	const int count = seq_fits(s, len, n) ? keep_count(pb, want, n) : 0;
+	if (len_out && blockIdx.x == 0 && threadIdx.x == 0)
+		len_out[b] = len + count;
 	T *base = reinterpret_cast<T *>((is_v ? c.v : c.k) + (size_t)layer * c.layer_bytes) + (size_t)h * PAGE * c.hd;
-	keep_rows(base + (is_v ? i * PAGE : i), (size_t)c.kvh * PAGE * c.hd, is_v ? 1 : c.hd, c, s, b, len, pb, count);
-	if (c.i8 && i == 0)
-		keep_rows((is_v ? c.vs : c.ks) + (size_t)layer * c.layer_scales + (size_t)h * PAGE, (size_t)c.kvh * PAGE, 1, c, s,
-			  b, len, pb, count);
-	// (written last by a workgroup of its own that moves nothing: len_out may
-	// be len itself, which the others read)
+	float *scales = (is_v ? c.vs : c.ks) + (size_t)layer * c.layer_scales + (size_t)h * PAGE;
+	const size_t page = (size_t)c.kvh * PAGE * c.hd;
+	for (int j1 = 0; j1 < count; j1 += KEEP_TABLE) {
+		const int m = min(KEEP_TABLE, count - j1);
+		__syncthreads();
+		if ((int)threadIdx.x < m) {
+			const int j = j1 + threadIdx.x, p = pb[j];
+			const int fp = page_of(s, c.n_pages, b, len + p), tp = page_of(s, c.n_pages, b, len + j);
+			from[threadIdx.x] = fp * PAGE + (len + p) % PAGE;
+			to[threadIdx.x] = p == j || fp < 0 || tp < 0 ? -1 : tp;
+		}
+		__syncthreads();
+		for (int j0 = 0; j0 < m; j0 += KEEP_BATCH) {
+			T x[KEEP_BATCH];
+			float f[KEEP_BATCH];
+#pragma unroll
+			for (int q = 0; q < KEEP_BATCH; q++) {
+				const int j = j0 + q;
+				if (j >= m || to[j] < 0)
+					continue;
+				const int fp = from[j] / PAGE, fr = from[j] % PAGE;
+				x[q] = base[fp * page + (is_v ? i * PAGE + fr : fr * c.hd + i)];
+				if (sizeof(T) == 1 && i == 0)
+					f[q] = scales[(size_t)fp * c.kvh * PAGE + fr];
+			}
+#pragma unroll
+			for (int q = 0; q < KEEP_BATCH; q++) {
+				const int j = j0 + q;
+				if (j >= m || to[j] < 0)
+					continue;
+				const int tr = (len + j1 + j) % PAGE;
+				base[to[j] * page + (is_v ? i * PAGE + tr : tr * c.hd + i)] = x[q];
+				if (sizeof(T) == 1 && i == 0)
+					scales[(size_t)to[j] * c.kvh * PAGE + tr] = f[q];
+			}
+		}
+	}
 }
 
 __global__ __launch_bounds__(64) void kv_keep_len_kernel(KvSeqs s, const int32_t *path, int max_path,
 							 const int32_t *n_keep, int32_t *len_out)
 {
-	const int b = blockIdx.x * 64 + threadIdx.x;
-	if (b >= s.n_seqs)
-		return;
+	const int b = blockIdx.x;
 	int t0, n;
 	seq_tokens(s, b, t0, n);
 	const int len = s.len[b];
-	len_out[b] = len + (seq_fits(s, len, n) ? keep_count(path + (size_t)b * max_path, min(n_keep[b], max_path), n) : 0);
+	const int count = seq_fits(s, len, n) ? keep_count(path + (size_t)b * max_path, min(n_keep[b], max_path), n) : 0;
+	if (threadIdx.x == 0)
+		len_out[b] = len + count;
 }
 
 hipError_t launch_kv_keep(const KvLayer &c, int n_layers, const KvSeqs &s, const int32_t *path, int max_path,
 			  const int32_t *n_keep, int32_t *len_out, hipStream_t st)
 {
 	const dim3 grid(n_layers * c.kvh, s.n_seqs), block(2 * c.hd);
+	// (lengths updated in place: by a launch behind the one that reads them)
+	int32_t *now = len_out == s.len ? nullptr : len_out;
 	if (c.i8)
-		tie_launch(kv_keep_kernel<uint8_t>, grid, block, 0, st, c, s, path, max_path, n_keep, len_out);
+		tie_launch(kv_keep_kernel<uint8_t>, grid, block, 0, st, c, s, path, max_path, n_keep, now);
 	else
-		tie_launch(kv_keep_kernel<uint16_t>, grid, block, 0, st, c, s, path, max_path, n_keep, len_out);
-	if (len_out)
-		tie_launch(kv_keep_len_kernel, dim3((s.n_seqs + 63) / 64), dim3(64), 0, st, s, path, max_path, n_keep, len_out);
+		tie_launch(kv_keep_kernel<uint16_t>, grid, block, 0, st, c, s, path, max_path, n_keep, now);
+	if (len_out && !now)
+		tie_launch(kv_keep_len_kernel, dim3(s.n_seqs), dim3(64), 0, st, s, path, max_path, n_keep, len_out);
 	return hipGetLastError();
 }
 

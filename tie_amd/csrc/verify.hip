@@ -103,56 +103,6 @@ __device__ __forceinline__ double exp_below(double x)
 	return x > -745.0 ? __builtin_amdgcn_ldexp(y, (int)k) : x != x ? x : 0.0;
 }
 
-// x moved across lanes by a DPP control; lanes that get nothing: `none`
-template <int CTRL, int ROWS> __device__ __forceinline__ float dpp(float none, float x)
-{
-	return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, x), CTRL,
-								     ROWS, 0xf, false));
-}
-template <int CTRL, int ROWS> __device__ __forceinline__ double dpp(double none, double x)
-{
-	const uint64_t n = (uint64_t)__double_as_longlong(none), v = (uint64_t)__double_as_longlong(x);
-	const uint32_t lo = __builtin_amdgcn_update_dpp((int)(uint32_t)n, (int)(uint32_t)v, CTRL, ROWS, 0xf, false),
-		       hi = __builtin_amdgcn_update_dpp((int)(n >> 32), (int)(v >> 32), CTRL, ROWS, 0xf, false);
-	return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
-}
-
-// The running op(x) over the wave's lanes, in registers: within rows of 16 (row
-// shifts), then the rows' ends into the rows behind (broadcasts).
-template <typename T, typename OP> __device__ __forceinline__ T wave_scan(T x, T none, OP op)
-{
-	x = op(x, dpp<0x111, 0xf>(none, x));
-	x = op(x, dpp<0x112, 0xf>(none, x));
-	x = op(x, dpp<0x114, 0xf>(none, x));
-	x = op(x, dpp<0x118, 0xf>(none, x));
-	x = op(x, dpp<0x142, 0xa>(none, x));
-	return op(x, dpp<0x143, 0xc>(none, x));
-}
-
-__device__ __forceinline__ double running(double x)
-{
-	return wave_scan(x, 0.0, [](double a, double b) { return a + b; });
-}
-
-// x of a lane (the same in all lanes), whether it is active here or not
-__device__ __forceinline__ double of_lane(double x, int lane)
-{
-	const uint64_t v = (uint64_t)__double_as_longlong(x);
-	const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
-	return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
-}
-
-__device__ __forceinline__ double wave_total(double x)
-{
-	return of_lane(running(x), 63);
-}
-
-__device__ __forceinline__ float wave_max(float x)
-{
-	x = wave_scan(x, -__builtin_inff(), [](float a, float b) { return __builtin_fmaxf(a, b); });
-	return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
-}
-
 // what one workgroup writes for another of the same launch goes past the
 // dies' caches
 template <typename T> __device__ __forceinline__ void give(T *p, T x)
@@ -307,7 +257,7 @@ __device__ __forceinline__ int locate(const VerifyArgs &a, int chunks, double u,
 	int at = -1;
 	for (int c0 = 0; c0 < chunks && at < 0; c0 += 64) {
 		const double x = c0 == 0 ? lane_sum : c0 + lane < chunks ? sum(c0 + lane) : 0.0;
-		const double incl = running(x);
+		const double incl = running_of<64>(x);
 		const unsigned long long over = __ballot(upto + incl > want && c0 + lane < chunks);
 		const int l = over ? __builtin_ctzll(over) : last - c0; // (for the fallback: the last chunk of any weight)
 		if (over || (last >= c0 && last < c0 + 64)) {
@@ -328,7 +278,7 @@ __device__ __forceinline__ int locate(const VerifyArgs &a, int chunks, double u,
 		mine += w[e];
 		some = w[e] > 0.0 ? e + 1 : some;
 	}
-	const double incl = running(mine);
+	const double incl = running_of<64>(mine);
 	__syncthreads();
 	if (lane == 63)
 		sh.d[wave] = incl;
@@ -595,7 +545,7 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 }
 
 // The first launch: largest logit and sum of each chunk.
-__global__ __launch_bounds__(V_THREADS) void verify_stats_kernel(VerifyArgs a, VerifyWork w)
+__global__ __launch_bounds__(V_THREADS, 4) void verify_stats_kernel(VerifyArgs a, VerifyWork w)
 {
 	__shared__ Shared sh;
 	const int t = blockIdx.y, chunk = blockIdx.x, base = chunk * V_CHUNK;
@@ -669,7 +619,7 @@ __global__ __launch_bounds__(V_THREADS) void verify_stats_kernel(VerifyArgs a, V
 }
 
 // One more residual sum for the rows that wait for it.
-__global__ __launch_bounds__(V_THREADS) void verify_residual_kernel(VerifyArgs a, VerifyWork w, int pass)
+__global__ __launch_bounds__(V_THREADS, 4) void verify_residual_kernel(VerifyArgs a, VerifyWork w, int pass)
 {
 	__shared__ Shared sh;
 	const int t = blockIdx.y, base = blockIdx.x * V_CHUNK;
