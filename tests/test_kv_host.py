@@ -137,7 +137,7 @@ def test_the_binding_checks_tensors():
             bad()
     q, kk = torch.zeros(5, 4, 64), torch.zeros(5, 2, 64)
     for bad in (dict(q=q[:4]), dict(q=q[:, :, :32]), dict(q=q.double()), dict(q_out=q.transpose(0, 1)), dict(k=q), dict(v=kk[:3]),
-                dict(q_norm=torch.zeros(32)), dict(pos=torch.zeros(4, **i32))):
+                dict(q_norm=torch.zeros(32)), dict(k=kk[:1].expand(5, 2, 64)), dict(pos=torch.zeros(4, **i32))):
         with pytest.raises(ValueError):
             c.append(0, s, **dict(dict(q=q, k=kk, v=kk, q_out=q.clone()), **bad))
     for bad in (dict(mask=torch.zeros(4, 1, dtype=torch.int64)), dict(mask=torch.zeros(5, 1, **i32)), dict(out=q[:, :3])):

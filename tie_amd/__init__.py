@@ -457,24 +457,41 @@ class Layer:
             pass
 
 
-def _rows(a, what, width=None):
-    """(pointer, row stride, values of a row) of F32 rows: a 2-D tensor, or one
-    of [rows][heads][head_dim] whose rows are contiguous."""
+def _dtype(name):
+    """torch's type of this name (torch is the caller's: the library needs none)."""
+    t = _dtypes.get(name)
+    if t is None:
+        import torch
+        t = _dtypes[name] = getattr(torch, name)
+    return t
+
+
+_dtypes = {}
+
+
+def _rows(a, what, width=None, n_rows=0):
+    """(pointer, row stride, values of a row) of n_rows or more F32 rows: a 2-D
+    tensor, or one of [rows][heads][head_dim] whose rows are contiguous."""
     st, sh = a.stride(), a.shape
-    if str(a.dtype) != "torch.float32" or len(sh) not in (2, 3):
-        raise ValueError("%s: rows of float32 values are wanted (got %s, %d dimensions)" % (what, a.dtype, len(sh)))
-    n = sh[1] if len(sh) == 2 else sh[1] * sh[2]
-    inner = (st[-1] == 1 or sh[-1] == 1) and (len(sh) == 2 or st[1] == sh[2] or sh[1] == 1)
-    if not inner or (width is not None and n != width):
-        raise ValueError("%s: rows of %s contiguous values are wanted (got shape %s, strides %s)" % (what, width or "", tuple(sh), st))
-    return a.data_ptr(), (st[0] if sh[0] > 1 else max(n, st[0])), n
+    if len(st) == 2:
+        n, inner = sh[1], st[1] == 1 or sh[1] == 1
+    elif len(st) == 3:
+        n = sh[1] * sh[2]
+        inner = (st[2] == 1 or sh[2] == 1) and (st[1] == sh[2] or sh[1] == 1)
+    else:
+        n, inner = -1, False
+    if a.dtype is not _dtype("float32") or not inner or (width is not None and n != width) or sh[0] < n_rows or \
+            (st[0] < n and sh[0] > 1):
+        raise ValueError("%s: %d rows of %s contiguous float32 values are wanted (got %s, shape %s, strides %s)"
+                         % (what, n_rows, width or "", a.dtype, tuple(sh), st))
+    return a.data_ptr(), (st[0] if st[0] > n else n), n
 
 
 def _array(a, dtype, shape, what):
     """The pointer of a contiguous device array of this type and shape (None for None)."""
     if a is None:
         return None
-    if str(a.dtype) != "torch." + dtype or tuple(a.shape) != tuple(shape) or not a.is_contiguous():
+    if a.dtype is not _dtype(dtype) or a.shape != shape or not a.is_contiguous():
         raise ValueError("%s: a contiguous %s array of shape %s is wanted (got %s, %s)" % (what, dtype, tuple(shape), a.dtype,
                                                                                            tuple(a.shape)))
     return a.data_ptr()
@@ -511,6 +528,7 @@ class KVCache:
         if kind == I8 and (k_scale is None or v_scale is None):
             raise ValueError("an int8 cache needs k_scale and v_scale")
         self.kv_heads, self.head_dim, self.n_layers, self.keep_alive = kvh, hd, nl, (k, v, k_scale, v_scale)
+        self.width, self.head_shape = kvh * hd, (hd,)
         self.desc = KVCacheDesc(kind, nl, npg, kvh, hd, _array(k, name, k.shape, "k"),
                                 _array(v, name, (nl, npg, kvh, hd, PAGE_ROWS), "v"),
                                 _array(k_scale, "float32", k.shape[:4], "k_scale"),
@@ -523,24 +541,23 @@ class KVCache:
         return width // self.head_dim
 
     def _q(self, q, out, seqs, what):
-        pq, sq, w = _rows(q, "q")
-        po, so, _ = _rows(out, what, w)
-        if q.shape[0] < seqs.n_tokens or out.shape[0] < seqs.n_tokens:
-            raise ValueError("q/%s: %d rows are wanted (got %d, %d)" % (what, seqs.n_tokens, q.shape[0], out.shape[0]))
+        pq, sq, w = _rows(q, "q", None, seqs.n_tokens)
+        if out is q:
+            po, so = pq, sq
+        else:
+            po, so, _ = _rows(out, what, w, seqs.n_tokens)
         return pq, sq, po, so, self._heads(w, "q")
 
     def append(self, layer, seqs, q, k, v, q_out, pos=None, q_norm=None, k_norm=None, eps=1e-6, theta=1e6, stream=None):
         """tie_hip_kv_append: norm and rotation of q and k, cache write of k and v."""
+        n = seqs.n_tokens
         pq, sq, po, so, heads = self._q(q, q_out, seqs, "q_out")
-        w = self.kv_heads * self.head_dim
-        pk, sk, _ = _rows(k, "k", w)
-        pv, sv, _ = _rows(v, "v", w)
-        if min(k.shape[0], v.shape[0]) < seqs.n_tokens:
-            raise ValueError("k/v: %d rows are wanted" % seqs.n_tokens)
+        pk, sk, _ = _rows(k, "k", self.width, n)
+        pv, sv, _ = _rows(v, "v", self.width, n)
         check(lib().tie_hip_kv_append(self.ref, layer, seqs.ref, pq, sq, pk, sk, pv, sv, heads,
-                                      _array(q_norm, "float32", (self.head_dim,), "q_norm"),
-                                      _array(k_norm, "float32", (self.head_dim,), "k_norm"), eps, theta,
-                                      _array(pos, "int32", (seqs.n_tokens,), "pos"), po, so, stream))
+                                      _array(q_norm, "float32", self.head_shape, "q_norm"),
+                                      _array(k_norm, "float32", self.head_shape, "k_norm"), eps, theta,
+                                      _array(pos, "int32", (n,), "pos"), po, so, stream))
 
     def read(self, seqs, k_out, v_out, layer=0, n_layers=1, stream=None):
         """tie_hip_kv_read: rows of the cache as float32 [n_layers][n_tokens][kv_heads][head_dim]."""
@@ -574,10 +591,8 @@ def verify_tree(logits, first, tokens, parent, u_accept, u_sample, path, n_keep,
                 max_children=1, work=None, stream=None):
     """tie_hip_verify_tree: the accepted path [n_seqs][max_path], its length and the next token of each sequence."""
     n, n_seqs = tokens.shape[0], n_keep.shape[0]
-    pl, sl, vocab = _rows(logits, "logits")
-    pd, sd, _ = (None, 0, 0) if draft is None else _rows(draft, "draft", vocab)
-    if logits.shape[0] < n or (draft is not None and draft.shape[0] < n):
-        raise ValueError("logits/draft: %d rows are wanted" % n)
+    pl, sl, vocab = _rows(logits, "logits", None, n)
+    pd, sd, _ = (None, 0, 0) if draft is None else _rows(draft, "draft", vocab, n)
     check(lib().tie_hip_verify_tree(pl, sl, pd, sd, vocab, n_seqs, n, _array(first, "int32", (n_seqs + 1,), "first"),
                                     _array(tokens, "int32", (n,), "tokens"), _array(parent, "int32", (n,), "parent"),
                                     _array(u_accept, "float32", (n,), "u_accept"),

@@ -937,6 +937,8 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 					kf[kt][k] = kl[(k * 4 + g) ^ (n16 & (KP - 1))];
 			}
 			f4 sc[NT][KT];
+			// (the wave that feeds the matrix cores goes before the other: 2%)
+			__builtin_amdgcn_s_setprio(1);
 #pragma unroll
 			for (int kt = 0; kt < KT; kt++)
 #pragma unroll
@@ -952,6 +954,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 						for (int t = 0; t < NT; t++)
 							sc[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][k], e ? qh[t][k] : ql[t][k],
 													   sc[t][kt], 0, 0, 0);
+			__builtin_amdgcn_s_setprio(0);
 			float ks = 0.0f, vs = 0.0f;
 			if constexpr (I8) {
 				const int row = row0 + g * 8 + (n16 & 7);
@@ -965,6 +968,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 #pragma unroll
 			for (int t = 0; t < NT; t++)
 				weigh<HD, I8, KT>(r[t], sc[t], ks, vs, vlog, qs[t], whole, seen[t] >> (8 * g), ph[t], pl[t]);
+			__builtin_amdgcn_s_setprio(1);
 #pragma unroll
 			for (int m = 0; m < MT; m++) {
 				const h8 vf = reinterpret_cast<const h8 *>(lv[b] + (m * 16 + n16) * PAGE)[(row0 / 8 + g) ^ (n16 & (VP - 1))];
@@ -975,6 +979,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 				for (int t = 0; t < NT; t++)
 					r[t].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t][0], r[t].o[m], 0, 0, 0);
 			}
+			__builtin_amdgcn_s_setprio(0);
 		}
 		if (more)
 			put(b ^ 1);
