@@ -119,19 +119,21 @@ __device__ __forceinline__ float pow2_below(float x)
 }
 
 // How the work of a call is cut: sequence b has tiles(b) row tiles for each kv
-// head, each over pages(b) pages, in chunks of `chunk` pages -- one unit of
-// work (a workgroup) for each.  Every workgroup finds the cut by itself from
+// head, each over pages(b) pages, in parts of as many pages -- one unit of work
+// (a workgroup) for each.  Every workgroup finds the cut by itself from
 // the lengths on the device, so that neither a copy to the host nor a launch
 // for a plan stands before the attention and captured calls follow the lengths.
 struct Cut {
 	int cap;   // units that run at once: at most so many where tiles are cut
-	int least; // pages of a unit, at least
+	int full;  // so many tiles are not cut
+	int grain; // pages that are not cut
+	int least; // grains of a unit, at least
 	int whole; // tiles are not cut at all
 	int rows;  // query rows of a tile
 };
 
 struct Unit {
-	int b, tile, head, part, parts, chunk, t0, n, len;
+	int b, tile, head, part, parts, t0, n, len;
 	int base, tile_at; // the first unit of the sequence, and the tile's place among its tiles
 };
 
@@ -162,47 +164,44 @@ __device__ __forceinline__ int div_up(int a, int b)
 	return (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b);
 }
 
-// Pages of a unit: the least that leaves no more than cap units (or, where the
-// tiles alone are as many, whole tiles).  The first block of 64 sequences is in
-// the wave's lanes already.
-__device__ __forceinline__ int unit_chunk(const KvSeqs &s, int kvh, int group, const Cut &cut, int tiles0, int pages0)
+// Parts of a tile for a grain of its pages, so that no more than cap units come
+// (0: whole tiles; so where the tiles alone fill the card).  The first block of
+// 64 sequences is in the wave's lanes already.
+__device__ __forceinline__ int tile_parts(const Cut &cut, int pages, float rate)
+{
+	const int grains = div_up(pages, cut.grain), most = grains / cut.least, p = (int)((float)grains * rate + 0.5f);
+	return p < 2 || most < 2 ? 1 : p < most ? p : most;
+}
+
+__device__ __forceinline__ float part_rate(const KvSeqs &s, int kvh, int group, const Cut &cut, int tiles0, int pages0)
 {
 	if (cut.whole)
-		return 0x7fffffff;
+		return 0.0f;
 	const int lane = threadIdx.x & 63;
 	auto over = [&](auto f) { // the sum of f(tiles, pages) over all sequences
-		int x = f(tiles0, pages0);
+		auto x = f(tiles0, pages0);
 		for (int b = 64 + lane; b < s.n_seqs; b += 64) {
 			int t0, n, len, tiles, pages;
 			seq_work(s, b, group, cut.rows, t0, n, len, tiles, pages);
 			x += f(tiles, pages);
 		}
-		return s.n_seqs > 1 ? wave_sum(x) : __builtin_amdgcn_readfirstlane(x);
+		if (s.n_seqs > 1)
+#pragma unroll
+			for (int m = 1; m < 64; m <<= 1)
+				x += __shfl_xor(x, m);
+		return of_lane(x, 0);
 	};
 	const int cap = cut.cap / kvh > 0 ? cut.cap / kvh : 1; // for one kv head
-	if (over([&](int t, int) { return t; }) >= cap)
-		return 0x7fffffff;
-	// (in sixteenths of a unit's share: tiles * pages can pass 32 bits)
-	const float share = 1.0f / cap;
-	float w = (float)tiles0 * pages0 * share;
-	for (int b = 64 + lane; b < s.n_seqs; b += 64) {
-		int t0, n, len, tiles, pages;
-		seq_work(s, b, group, cut.rows, t0, n, len, tiles, pages);
-		w += (float)tiles * pages * share;
+	if ((long long)over([](int t, int) { return t; }) * kvh >= cut.full)
+		return 0.0f;
+	// the nearest number to each tile's share; a little less where those are too many
+	float rate = (float)cap / over([&](int t, int p) { return (float)t * div_up(p, cut.grain); });
+	for (int i = 0; i < 16; i++) {
+		if (over([&](int t, int p) { return t * tile_parts(cut, p, rate); }) <= cap)
+			return rate;
+		rate *= 0.92f;
 	}
-	if (s.n_seqs > 1)
-#pragma unroll
-		for (int m = 1; m < 64; m <<= 1)
-			w += __shfl_xor(w, m);
-	w = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, w)));
-	int c = (int)__builtin_ceilf(w);
-	c = c < cut.least ? cut.least : c;
-	for (int i = 0; i < 12; i++) {
-		if (over([&](int t, int p) { return t * div_up(p, c); }) <= cap)
-			break;
-		c += c / 8 + 1;
-	}
-	return c;
+	return 0.0f;
 }
 
 // The unit of workgroup `index`; false past the last.  Units of a sequence:
@@ -213,10 +212,10 @@ __device__ __forceinline__ bool find_unit(const KvSeqs &s, int kvh, int group, c
 	const int lane = threadIdx.x & 63;
 	int t0, n, len, tiles, pages;
 	seq_work(s, lane, group, cut.rows, t0, n, len, tiles, pages);
-	u.chunk = unit_chunk(s, kvh, group, cut, tiles, pages);
+	const float rate = part_rate(s, kvh, group, cut, tiles, pages);
 	int before = 0;
 	for (int b0 = 0;;) {
-		const int parts = tiles ? div_up(pages, u.chunk) : 0, mine = tiles * parts * kvh;
+		const int parts = tiles ? tile_parts(cut, pages, rate) : 0, mine = tiles * parts * kvh;
 		int incl = mine;
 		if (s.n_seqs > 1)
 #pragma unroll
@@ -241,6 +240,12 @@ __device__ __forceinline__ bool find_unit(const KvSeqs &s, int kvh, int group, c
 			u.t0 = of(t0);
 			u.n = of(n);
 			u.len = of(len);
+			u.base = __builtin_amdgcn_readfirstlane(u.base);
+			u.b = __builtin_amdgcn_readfirstlane(u.b);
+			u.head = __builtin_amdgcn_readfirstlane(u.head);
+			u.part = __builtin_amdgcn_readfirstlane(u.part);
+			u.tile = __builtin_amdgcn_readfirstlane(u.tile);
+			u.tile_at = __builtin_amdgcn_readfirstlane(u.tile_at);
 			return true;
 		}
 		before += __builtin_amdgcn_readlane(incl, 63);
@@ -249,6 +254,14 @@ __device__ __forceinline__ bool find_unit(const KvSeqs &s, int kvh, int group, c
 			return false;
 		seq_work(s, b0 + lane, group, cut.rows, t0, n, len, tiles, pages);
 	}
+}
+
+// The first page of the unit's part, and behind its last.
+__device__ __forceinline__ void part_pages(const Cut &cut, const Unit &u, int pages, int &p0, int &p1)
+{
+	const int grains = div_up((u.len + u.n + PAGE - 1) / PAGE, cut.grain), q = grains / u.parts, r = grains % u.parts;
+	p0 = (u.part * q + min(u.part, r)) * cut.grain;
+	p1 = min(pages, p0 + (q + (u.part < r)) * cut.grain);
 }
 
 // Which of the 64 rows of the page at row `start` a token sees: all committed
@@ -274,6 +287,29 @@ __device__ __forceinline__ uint64_t sees(const AttnArgs &a, const Unit &u, int n
 	w &= below((long long)u.n - rel); // no bit names a node that is not there
 	return w | below(-(long long)rel);
 }
+
+// The page table's entries of a unit, a lane each, 64 pages at a time: a page's
+// number is then a register away (a load of it stands before the page's own loads
+// otherwise: 800 cycles a page).
+struct PageIds {
+	int first, ids; // pages first .. first + 63
+	__device__ __forceinline__ void get(const KvSeqs &s, const Unit &u, int p)
+	{
+		first = p;
+		const int at = p + (int)(threadIdx.x & 63);
+		ids = at < s.max_pages ? s.pages[(size_t)u.b * s.max_pages + at] : -1;
+	}
+	// the number of page p, p not below the last one asked for; bad: it is none
+	__device__ __forceinline__ int of(const KvSeqs &s, const Unit &u, int n_pages, int p, bool &bad)
+	{
+		if (p - first >= 64)
+			get(s, u, p);
+		const int id = __builtin_amdgcn_readlane(ids, p - first);
+		const bool ok = id >= 0 && id < n_pages;
+		bad = bad || !ok;
+		return ok ? id : 0;
+	}
+};
 
 // Results of a part, for each row of its tile: O [HD], the maximum, the sum.
 constexpr int part_row(int hd)
@@ -540,15 +576,17 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 	// (causal: nothing behind the tile's last token is seen)
 	const int last = a.mask ? u.n : min(u.n, (u.tile * R + R - 1) / group + 1);
 	const int pages = bad ? 0 : (u.len + last + PAGE - 1) / PAGE;
-	const int p0 = u.part * u.chunk, steps = (min(pages, p0 + min(u.chunk, pages)) - p0) * SP;
+	int p0, p1;
+	part_pages(cut, u, pages, p0, p1);
+	const int steps = (p1 - p0) * SP;
 
+	PageIds ids;
+	ids.get(s, u, p0);
 	u4 kr[KT][KL], vr[MT];
 	float ks = 0.0f, vs = 0.0f; // int8: the scales of the lane's row
 	size_t at = 0; // of the page whose V is in (or on its way to) vr
 	auto page = [&](int step) {
-		const int id = __builtin_amdgcn_readfirstlane(page_of(s, c.n_pages, u.b, (p0 + step / SP) * PAGE));
-		bad = bad || id < 0;
-		return (size_t)(id < 0 ? 0 : id) * c.kvh + u.head;
+		return (size_t)ids.of(s, u, c.n_pages, p0 + step / SP, bad) * c.kvh + u.head;
 	};
 	auto get_k = [&](size_t pg, int step) {
 		const int row0 = step % SP * 32;
@@ -771,20 +809,23 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 }
 
 // ---------------------------------------------------------------- many rows
-// A workgroup: 128 query rows of one kv head, 32 to a wave, all over the same
+// A workgroup: 32 RG query rows of one kv head, 32 to a wave, all over the same
 // pages: a page comes into LDS once (int8 codes as f16), while the one before
-// is worked on.  Bound by the matrix cores and the weights' arithmetic side by
-// side: two waves on a SIMD.
+// is worked on.  RG = 2: a wave takes half of a page for its rows, and two waves'
+// rows are joined at the end.  Bound by the matrix cores and the weights'
+// arithmetic: two workgroups on a CU hide less of each other's waits than their
+// waves' turns suggest (2.05 us a page of 128 rows for a CU with two, 2.26 alone;
+// the matrix instructions are 0.86 of them).
 //
 // LDS rows are swizzled in 16-byte pieces so that the 8 lanes that read
 // together touch all banks: K row r's piece q lies at q ^ f(r), f the lane of
 // the operand that reads the row; V column i's at q ^ (i % 8).
-constexpr int MANY_ROWS = 128, MANY_WAVES = 4;
+constexpr int MANY_WAVES = 4;
 
-template <int HD, bool I8>
+template <int HD, bool I8, int RG>
 __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, float *part)
 {
-	constexpr int KS = HD / 32, MT = HD / 16, R = MANY_ROWS, NT = 2, KT = 2, E = I8 ? 1 : 2;
+	constexpr int KS = HD / 32, MT = HD / 16, R = 32 * RG, NT = 2, KT = 2, E = I8 ? 1 : 2;
 	constexpr int NL = PAGE * HD * E / 16 / 256; // 16-byte pieces of a page's K (and V) for a thread
 	constexpr int KP = HD / 8, VP = PAGE / 8;    // pieces of a K row and of a V column in LDS
 	__shared__ __attribute__((aligned(1024))) _Float16 lk[2][PAGE * HD], lv[2][PAGE * HD];
@@ -803,13 +844,15 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 
 	const int last = a.mask ? u.n : min(u.n, (u.tile * R + R - 1) / group + 1);
 	const int pages = bad ? 0 : (u.len + last + PAGE - 1) / PAGE;
-	const int p0 = u.part * u.chunk, p1 = min(pages, p0 + min(u.chunk, pages));
-	u4 kr[I8 ? NL : 1], vr[I8 ? NL : 1];
+	int p0, p1;
+	part_pages(cut, u, pages, p0, p1);
+	const int all_below = u.len + (a.mask ? 0 : u.tile * R / group + 1); // rows below it every query of the tile sees
+	PageIds ids;
+	ids.get(s, u, p0);
+	u4 codes[I8 ? NL : 1];
 	float sr = 0.0f;
 	auto page = [&](int p) {
-		const int id = __builtin_amdgcn_readfirstlane(page_of(s, c.n_pages, u.b, p * PAGE));
-		bad = bad || id < 0;
-		return (size_t)(id < 0 ? 0 : id) * c.kvh + u.head;
+		return (size_t)ids.of(s, u, c.n_pages, p, bad) * c.kvh + u.head;
 	};
 	// where a K row's and a V column's pieces lie
 	auto kx = [](int row) { return ((row & 3) | (row >> 3 & 3) << 2) & (KP - 1); };
@@ -824,78 +867,111 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 			ko[q] = 16 * (e / KP * KP + (e % KP ^ kx(e / KP)));
 			vo[q] = 16 * (e / VP * VP + (e % VP ^ vx(e / VP)));
 		}
-	// request a page: int8 codes to registers, f16 to buffer b
+	// f16: request a page, to buffer b
 	auto get = [&](size_t pg, int b) {
 		const uint8_t *k = uniform(c.k + pg * PAGE * HD * E), *v = uniform(c.v + pg * PAGE * HD * E);
 #pragma unroll
 		for (int q = 0; q < NL; q++) {
-			if constexpr (I8) {
-				kr[q] = reinterpret_cast<const u4 *>(k)[tid + q * 256];
-				vr[q] = reinterpret_cast<const u4 *>(v)[tid + q * 256];
-			} else {
-				load_lds16(k, ko[q], lk[b] + (q * 256 + wave * 64) * 8);
-				load_lds16(v, vo[q], lv[b] + (q * 256 + wave * 64) * 8);
-			}
+			load_lds16(k, ko[q], lk[b] + (q * 256 + wave * 64) * 8);
+			load_lds16(v, vo[q], lv[b] + (q * 256 + wave * 64) * 8);
 		}
-		if (I8 && tid < 2 * PAGE)
+	};
+	// int8: a page's codes by way of registers, K and the scales (half 0) and then
+	// V (both at once are 32 registers, and some of them went to scratch memory:
+	// 1000 tokens over 2000 rows 156 us)
+	auto get8 = [&](size_t pg, int half) {
+		const uint8_t *from = uniform((half ? c.v : c.k) + pg * PAGE * HD);
+#pragma unroll
+		for (int q = 0; q < NL; q++)
+			codes[q] = reinterpret_cast<const u4 *>(from)[tid + q * 256];
+		if (!half && tid < 2 * PAGE)
 			sr = tid < PAGE ? c.ks[pg * PAGE + tid] : c.vs[pg * PAGE + tid - PAGE];
 	};
-	auto put = [&](int b) {
-		if constexpr (I8) {
+	auto put8 = [&](int b, int half) {
+		if (!half) {
 #pragma unroll
 			for (int q = 0; q < NL; q++) {
 				const int e = tid + q * 256; // piece of 16 codes: two of f16
-				const int row = e / (KP / 2), kp = e % (KP / 2) * 2, col = e / (VP / 2), vp = e % (VP / 2) * 2;
-				h8 *kl = reinterpret_cast<h8 *>(lk[b] + row * HD), *vl = reinterpret_cast<h8 *>(lv[b] + col * PAGE);
-				kl[kp ^ kx(row)] = codes8(kr[q].x, kr[q].y);
-				kl[(kp + 1) ^ kx(row)] = codes8(kr[q].z, kr[q].w);
-				vl[vp ^ vx(col)] = codes8(vr[q].x, vr[q].y);
-				vl[(vp + 1) ^ vx(col)] = codes8(vr[q].z, vr[q].w);
+				const int row = e / (KP / 2), kp = e % (KP / 2) * 2;
+				h8 *kl = reinterpret_cast<h8 *>(lk[b] + row * HD);
+				kl[kp ^ kx(row)] = codes8(codes[q].x, codes[q].y);
+				kl[(kp + 1) ^ kx(row)] = codes8(codes[q].z, codes[q].w);
 			}
 			if (tid < 2 * PAGE)
 				lsc[b][tid >> 6][tid & 63] = sr;
 		} else {
-			__builtin_amdgcn_s_waitcnt(0); // the pieces under way to LDS
+#pragma unroll
+			for (int q = 0; q < NL; q++) {
+				const int e = tid + q * 256;
+				const int col = e / (VP / 2), vp = e % (VP / 2) * 2;
+				h8 *vl = reinterpret_cast<h8 *>(lv[b] + col * PAGE);
+				vl[vp ^ vx(col)] = codes8(codes[q].x, codes[q].y);
+				vl[(vp + 1) ^ vx(col)] = codes8(codes[q].z, codes[q].w);
+			}
 		}
 	};
 	size_t at = 0;
+	u4 first[I8 ? NL : 1]; // of K: all that a unit begins with is under way at once
 	if (p0 < p1) {
 		at = page(p0);
-		get(at, 0);
+		if (I8) {
+			get8(at, 0);
+#pragma unroll
+			for (int q = 0; q < NL; q++)
+				first[q] = codes[q];
+			get8(at, 1);
+		} else {
+			get(at, 0);
+		}
 	}
 
 	int node[NT];
 	h8 qh[NT][KS], ql[NT][KS];
-	float qs[NT];
+	float qs[NT], x[NT][KS][8];
 	Rows<HD> r[NT];
 #pragma unroll
 	for (int t = 0; t < NT; t++) {
-		const int row = u.tile * R + wave * 32 + 16 * t + n16;
+		const int row = u.tile * R + wave % RG * 32 + 16 * t + n16;
 		node[t] = row / group < u.n ? row / group : -1;
-		float x[KS][8];
-		fetch_query<HD, false>(a, u, node[t], u.head * group + row % group, g, x);
-		split_query<HD>(a, node[t], x, qh[t], ql[t], qs[t]);
+		fetch_query<HD, false>(a, u, node[t], u.head * group + row % group, g, x[t]);
+	}
+#pragma unroll
+	for (int t = 0; t < NT; t++) {
+		split_query<HD>(a, node[t], x[t], qh[t], ql[t], qs[t]);
 #pragma unroll
 		for (int m = 0; m < MT; m++)
 			r[t].o[m] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 	}
 	float vlog = -100.0f;
-	put(0);
+	if (I8) {
+		put8(0, 1);
+#pragma unroll
+		for (int q = 0; q < NL; q++)
+			codes[q] = first[q];
+		put8(0, 0);
+	} else {
+		__builtin_amdgcn_s_waitcnt(0); // the pieces under way to LDS
+	}
 	__syncthreads();
 
 	for (int p = p0; p < p1; p++) {
 		const int b = (p - p0) & 1, start = p * PAGE, end = u.len + u.n - start;
 		const bool more = p + 1 < p1;
 		const size_t next = more ? page(p + 1) : at;
-		if (more)
+		if (!I8 && more)
 			get(next, b ^ 1); // (all waves left that buffer at the last barrier)
+		const bool seen_all = start + PAGE <= all_below;
 		uint64_t vis[NT];
 #pragma unroll
 		for (int t = 0; t < NT; t++)
-			vis[t] = sees(a, u, node[t], start);
+			vis[t] = ~0ull;
+		if (!seen_all)
+#pragma unroll
+			for (int t = 0; t < NT; t++)
+				vis[t] = sees(a, u, node[t], start);
 		// a page that not all of the tile sees: f16 values that are not finite
 		// are taken out first (see guard_values), and come back below
-		if (!I8 && (a.mask ? start + PAGE > u.len : start + PAGE > u.len + u.tile * R / group + 1)) {
+		if (!I8 && !seen_all) {
 			uint32_t odd = 0;
 #pragma unroll
 			for (int q = 0; q < NL; q++) {
@@ -912,22 +988,31 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 					*x = y;
 				odd |= here;
 			}
-			if (__syncthreads_or(odd))
-				give_back<HD, NT>(c.v + at * HD * PAGE * 2, g, end, vis, r);
-		}
-#pragma unroll 1
-		for (int row0 = 0; row0 < PAGE; row0 += 32) {
-			uint32_t seen[NT];
-			bool whole = true, any = false;
+			if (__syncthreads_or(odd)) {
+				uint64_t mine[NT];
 #pragma unroll
-			for (int t = 0; t < NT; t++) {
-				seen[t] = (uint32_t)(vis[t] >> row0);
-				whole = whole && (seen[t] == ~0u || node[t] < 0);
-				any = any || seen[t] != 0;
+				for (int t = 0; t < NT; t++)
+					mine[t] = RG == MANY_WAVES ? vis[t] : vis[t] & 0xffffffffull << wave / RG * 32;
+				give_back<HD, NT>(c.v + at * HD * PAGE * 2, g, end, mine, r);
 			}
-			if (!__any(any))
-				continue;
-			whole = __all(whole);
+		}
+		auto weigh_half = [&](int row0, h8 (&ph)[NT][1], h8 (&pl)[NT][1]) {
+			uint32_t seen[NT];
+			bool whole = seen_all;
+#pragma unroll
+			for (int t = 0; t < NT; t++)
+				seen[t] = (uint32_t)(vis[t] >> row0);
+			if (!seen_all) {
+				bool all = true, any = false;
+#pragma unroll
+				for (int t = 0; t < NT; t++) {
+					all = all && (seen[t] == ~0u || node[t] < 0);
+					any = any || seen[t] != 0;
+				}
+				if (!__any(any))
+					return false;
+				whole = __all(all);
+			}
 			h8 kf[KT][KS];
 #pragma unroll
 			for (int kt = 0; kt < KT; kt++) {
@@ -964,10 +1049,12 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 					guard_scales(ks, vs, row < end);
 				move_vlog<HD, NT>(vs, vlog, r);
 			}
-			h8 ph[NT][1], pl[NT][1];
 #pragma unroll
 			for (int t = 0; t < NT; t++)
 				weigh<HD, I8, KT>(r[t], sc[t], ks, vs, vlog, qs[t], whole, seen[t] >> (8 * g), ph[t], pl[t]);
+			return true;
+		};
+		auto add_half = [&](int row0, const h8 (&ph)[NT][1], const h8 (&pl)[NT][1]) {
 			__builtin_amdgcn_s_setprio(1);
 #pragma unroll
 			for (int m = 0; m < MT; m++) {
@@ -980,16 +1067,75 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 					r[t].o[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[t][0], r[t].o[m], 0, 0, 0);
 			}
 			__builtin_amdgcn_s_setprio(0);
+		};
+		h8 ph[NT][1], pl[NT][1];
+		if constexpr (RG == MANY_WAVES) {
+#pragma unroll 1
+			for (int row0 = 0; row0 < PAGE; row0 += 32) {
+				if (I8 && more)
+					get8(next, row0 >> 5);
+				if (weigh_half(row0, ph, pl))
+					add_half(row0, ph, pl);
+				if (I8 && more)
+					put8(b ^ 1, row0 >> 5);
+			}
+		} else {
+			const int row0 = wave / RG * 32;
+			if (I8 && more)
+				get8(next, 0);
+			const bool any = weigh_half(row0, ph, pl);
+			if (I8 && more) {
+				put8(b ^ 1, 0);
+				get8(next, 1);
+			}
+			if (any)
+				add_half(row0, ph, pl);
+			if (I8 && more)
+				put8(b ^ 1, 1);
 		}
-		if (more)
-			put(b ^ 1);
+		if (!I8)
+			__builtin_amdgcn_s_waitcnt(0);
 		__syncthreads();
 		at = next;
 	}
-	const float back = __builtin_amdgcn_exp2f(I8 ? vlog - P_LOG2 : -P_LOG2);
+	float back = __builtin_amdgcn_exp2f(I8 ? vlog - P_LOG2 : -P_LOG2), total[NT];
+#pragma unroll
+	for (int t = 0; t < NT; t++)
+		total[t] = sum_g(r[t].sum) * back;
+	if constexpr (RG < MANY_WAVES) {
+		// the waves of the pages' second halves hand their rows to the others:
+		// O ([wave][t][m][lane], in K's buffers) and the maxima and sums
+		static_assert(RG == MANY_WAVES / 2, "a row group: two waves");
+		f4 *lo = reinterpret_cast<f4 *>(&lk[0][0]) + (size_t)wave % RG * NT * MT * 64 + lane;
+		float *lm = &lsc[0][0][0] + wave % RG * 64 + n16;
+		if (wave >= RG)
+#pragma unroll
+			for (int t = 0; t < NT; t++) {
+#pragma unroll
+				for (int m = 0; m < MT; m++)
+					lo[(t * MT + m) * 64] = r[t].o[m] * back;
+				if (g == 0) {
+					lm[t * 32] = r[t].mx;
+					lm[t * 32 + 16] = total[t];
+				}
+			}
+		__syncthreads();
+		if (wave >= RG)
+			return;
+#pragma unroll
+		for (int t = 0; t < NT; t++) {
+			const float om = lm[t * 32], top = __builtin_fmaxf(r[t].mx, om), base = top == -__builtin_inff() ? 0.0f : top;
+			const float f0 = __builtin_amdgcn_exp2f(r[t].mx - base), f1 = __builtin_amdgcn_exp2f(om - base);
+			r[t].mx = top;
+			total[t] = total[t] * f0 + lm[t * 32 + 16] * f1;
+#pragma unroll
+			for (int m = 0; m < MT; m++)
+				r[t].o[m] = r[t].o[m] * (back * f0) + lo[(t * MT + m) * 64] * f1;
+		}
+		back = 1.0f;
+	}
 #pragma unroll
 	for (int t = 0; t < NT; t++) {
-		const float total = sum_g(r[t].sum) * back;
 		const int q = wave * 32 + 16 * t + n16, to = u.tile * R + q;
 		if (node[t] < 0)
 			continue;
@@ -997,15 +1143,15 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 		float f = back;
 		if (u.parts == 1) {
 			o = a.out + (size_t)(u.t0 + to / group) * a.o_stride + (size_t)(u.head * group + to % group) * HD;
-			f = bad ? __builtin_nanf("") : total == 0.0f ? 0.0f : back / total;
+			f = bad ? __builtin_nanf("") : total[t] == 0.0f ? 0.0f : back / total[t];
 		} else if (g == 0) {
 			o[HD] = bad ? __builtin_nanf("") : r[t].mx;
-			o[HD + 1] = bad ? __builtin_nanf("") : total;
+			o[HD + 1] = bad ? __builtin_nanf("") : total[t];
 		}
 		const bool vec = ((uintptr_t)o & 15) == 0;
 #pragma unroll
 		for (int m = 0; m < MT; m++) {
-			const f4 x = total == 0.0f && u.parts == 1 && !bad ? (f4){0.0f, 0.0f, 0.0f, 0.0f} : r[t].o[m] * f;
+			const f4 x = total[t] == 0.0f && u.parts == 1 && !bad ? (f4){0.0f, 0.0f, 0.0f, 0.0f} : r[t].o[m] * f;
 			if (vec) {
 				*reinterpret_cast<f4 *>(o + m * 16 + 4 * g) = x;
 			} else {
@@ -1018,15 +1164,17 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 }
 
 // ---------------------------------------------------------------- join
-// The parts of one token row and query head: a workgroup, HD / 4 lanes to a
-// part, 1024 / HD parts at a time.
+// A workgroup: JOIN_HEADS query heads of one token, HD / 4 lanes to a head: first
+// the parts' maxima and sums, a lane to a part, then their rows, 16 under way
+// at once.  Bound by the parts' bytes.
+constexpr int JOIN_HEADS = 8;
 template <int HD>
-__global__ __launch_bounds__(256) void attn_join_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, int units, const float *part)
+__global__ __launch_bounds__(JOIN_HEADS *HD / 4) void attn_join_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, int units,
+								       const float *part)
 {
-	constexpr int L = HD / 4, G = 256 / L, PR = part_row(HD);
-	__shared__ float lm[G], ll[G];
-	__shared__ f4 lo[G][L];
-	const int group = a.n_heads / c.kvh, t = blockIdx.x, h = blockIdx.y, head = h / group;
+	constexpr int L = HD / 4, PR = part_row(HD);
+	const int group = a.n_heads / c.kvh, blocks = div_up(a.n_heads, JOIN_HEADS);
+	const int t = blockIdx.x / blocks, h = blockIdx.x % blocks * JOIN_HEADS + threadIdx.x / L, head = min(h, a.n_heads - 1) / group;
 	int st0, sn;
 	const int b = seq_of_token(s, t, st0, sn);
 	if (b < 0)
@@ -1035,56 +1183,59 @@ __global__ __launch_bounds__(256) void attn_join_kernel(KvLayer c, KvSeqs s, Att
 	const int lane = threadIdx.x & 63;
 	int t0, n, len, tiles, pages;
 	seq_work(s, lane, group, cut.rows, t0, n, len, tiles, pages);
-	const int chunk = unit_chunk(s, c.kvh, group, cut, tiles, pages);
+	const float rate = part_rate(s, c.kvh, group, cut, tiles, pages);
 	int before = 0;
 	for (int b0 = 0; b0 <= b; b0 += 64) {
 		if (b0)
 			seq_work(s, b0 + lane, group, cut.rows, t0, n, len, tiles, pages);
-		before += s.n_seqs > 1 ? wave_sum(b0 + lane < b && tiles ? tiles * div_up(pages, chunk) * c.kvh : 0) : 0;
+		before += s.n_seqs > 1 ? wave_sum(b0 + lane < b && tiles ? tiles * tile_parts(cut, pages, rate) * c.kvh : 0) : 0;
 	}
 	seq_work(s, b, group, cut.rows, t0, n, len, tiles, pages);
-	const int parts = div_up(pages, chunk);
+	const int parts = tile_parts(cut, pages, rate);
 	if (parts == 1)
 		return;
 	const int row = (t - t0) * group + h % group, tile = row / cut.rows;
 	const int u0 = before + ((tiles - 1 - tile) * parts) * c.kvh + head; // unit of part q: u0 + q kvh
-	if (u0 < 0 || (long long)u0 + (long long)(parts - 1) * c.kvh >= units)
+	if (h >= a.n_heads || u0 < 0 || (long long)u0 + (long long)(parts - 1) * c.kvh >= units)
 		return; // (sequences that overlap: more units than the rows can have)
 	const float *from = part + ((size_t)u0 * cut.rows + row % cut.rows) * PR;
 	const size_t step = (size_t)c.kvh * cut.rows * PR;
-	const int pg = threadIdx.x / L, i = threadIdx.x % L;
+	const int i = threadIdx.x % L;
 	float m = -__builtin_inff(), l = 0.0f;
 	f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-	for (int q = pg; q < parts; q += G) {
-		const float *pr = from + q * step;
-		const f4 o = reinterpret_cast<const f4 *>(pr)[i];
-		const float pm = pr[HD], pl = pr[HD + 1];
-		const float top = __builtin_fmaxf(m, pm), base = top == -__builtin_inff() ? 0.0f : top;
-		const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(pm - base);
+	for (int q0 = 0; q0 < parts; q0 += L) {
+		float pm = -__builtin_inff(), pl = 0.0f;
+		if (q0 + i < parts) {
+			const float *pr = from + (q0 + i) * step;
+			pm = pr[HD];
+			pl = pr[HD + 1];
+		}
+		float top = __builtin_fmaxf(m, pm);
+#pragma unroll
+		for (int k = 1; k < L; k <<= 1)
+			top = __builtin_fmaxf(top, __shfl_xor(top, k, L));
+		const float base = top == -__builtin_inff() ? 0.0f : top;
+		const float back = __builtin_amdgcn_exp2f(m - base);
+		const float f = __builtin_amdgcn_exp2f(pm - base);
 		m = top;
-		l = l * f0 + pl * f1;
-		x = x * f0 + o * f1;
-	}
-	lo[pg][i] = x;
-	if (i == 0) {
-		lm[pg] = m;
-		ll[pg] = l;
-	}
-	__syncthreads();
-	if (pg)
-		return;
-	float top = -__builtin_inff();
+		float sum = pl * f;
 #pragma unroll
-	for (int q = 0; q < G; q++)
-		top = __builtin_fmaxf(top, lm[q]);
-	const float base = top == -__builtin_inff() ? 0.0f : top;
-	l = 0.0f;
-	x = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+		for (int k = 1; k < L; k <<= 1)
+			sum += __shfl_xor(sum, k, L);
+		l = l * back + sum;
+		x *= back;
+		const int n8 = min(L, parts - q0);
+		for (int q = 0; q < n8; q += 16) {
+			f4 o[16];
 #pragma unroll
-	for (int q = 0; q < G; q++) {
-		const float f = __builtin_amdgcn_exp2f(lm[q] - base);
-		l += ll[q] * f;
-		x += lo[q][i] * f;
+			for (int k = 0; k < 16; k++)
+				o[k] = reinterpret_cast<const f4 *>(from + (q0 + min(q + k, n8 - 1)) * step)[i];
+#pragma unroll
+			for (int k = 0; k < 16; k++) {
+				const float fk = __shfl(f, min(q + k, n8 - 1), L);
+				x += q + k < n8 ? o[k] * fk : (f4){0.0f, 0.0f, 0.0f, 0.0f};
+			}
+		}
 	}
 	float *out = a.out + (size_t)t * a.o_stride + (size_t)h * HD + 4 * i;
 #pragma unroll
@@ -1093,6 +1244,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(KvLayer c, KvSeqs s, Att
 }
 
 // ---------------------------------------------------------------- launch
+// a tile for every CU, and none is cut (600 tokens over 1100 rows, 300 tiles, 54 us; cut in two 68)
+constexpr int MANY_FULL = 256;
+
 struct Shape {
 	bool few;
 	Cut cut;
@@ -1104,14 +1258,21 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 	const size_t group = a.n_heads / c.kvh, rows = (size_t)s.n_tokens * group;
 	Shape h;
 	h.few = rows <= (size_t)FEW_ROWS * s.n_seqs;
-	h.cut.rows = h.few ? FEW_ROWS : MANY_ROWS;
+	// many: 128 rows where such tiles fill the card (4096 tokens of 32 heads 240
+	// us, by 64 rows 257), or 64: as many units and half the parts' bytes, less
+	// left of tiles that a mask or a sequence's end cuts (1000 tokens over 2000
+	// rows 55 us, by 128 rows 89)
+	h.cut.rows = h.few ? FEW_ROWS : rows * c.kvh < (size_t)MANY_FULL * 128 ? 64 : 128;
 	// one workgroup of 8 waves on a CU, or two of 4
 	h.cut.cap = h.few ? FEW_CAP : 512;
-	h.cut.least = h.few ? FEW_WAVES : 2;
+	h.cut.full = h.few ? FEW_CAP : MANY_FULL;
+	// (few: a grain is a round of the waves)
+	h.cut.grain = !h.few ? 1 : c.i8 ? FEW_WAVES : FEW_WAVES / 2;
+	h.cut.least = !h.few ? 2 : c.i8 ? 1 : 2;
 	const size_t seqs = s.n_seqs < s.n_tokens ? s.n_seqs : s.n_tokens; // that have tokens, at most
 	const size_t tiles = (rows + seqs * (h.cut.rows - 1)) / h.cut.rows;
 	// as many tiles as fill the card are not cut: no parts, no join
-	h.cut.whole = rows / h.cut.rows * c.kvh >= (size_t)h.cut.cap;
+	h.cut.whole = rows / h.cut.rows * c.kvh >= (size_t)h.cut.full;
 	// (a share that is rounded down can make one more part)
 	h.units = (h.cut.whole ? 0 : h.cut.cap + c.kvh) + tiles * c.kvh;
 	// (not with a kv head for every 8 rows or more, and then: whole tiles)
@@ -1139,10 +1300,11 @@ static hipError_t go(const Shape &h, const KvLayer &c, const KvSeqs &s, const At
 			   part, count);
 		return hipGetLastError();
 	}
-	tie_launch(attn_many_kernel<HD, I8>, dim3(h.units), dim3(64 * MANY_WAVES), 0, st, c, s, a, h.cut, part);
+	tie_launch(h.cut.rows == 64 ? attn_many_kernel<HD, I8, 2> : attn_many_kernel<HD, I8, 4>, dim3(h.units), dim3(64 * MANY_WAVES),
+		   0, st, c, s, a, h.cut, part);
 	if (!h.cut.whole)
-		tie_launch(attn_join_kernel<HD>, dim3(s.n_tokens, a.n_heads), dim3(256), 0, st, c, s, a, h.cut, (int)h.units,
-			   (const float *)part);
+		tie_launch(attn_join_kernel<HD>, dim3((size_t)s.n_tokens * ((a.n_heads + JOIN_HEADS - 1) / JOIN_HEADS)),
+			   dim3(JOIN_HEADS * HD / 4), 0, st, c, s, a, h.cut, (int)h.units, (const float *)part);
 	return hipGetLastError();
 }
 
