@@ -45,6 +45,7 @@ struct VerifyWork {
 	int32_t *take; // [n_tokens] the child taken (a token row), -1: none
 	int32_t *own;  // [n_tokens] the next token where none is taken
 	int32_t *leaf; // [n_tokens] the next token where the children do not count
+	int32_t *act;  // [n_tokens] draft rows: the residual sum that the row takes part in
 	double *res;   // [n_tokens][chunks] the residual's sums
 	int *count;    // [n_tokens] rows, [n_seqs] sequences
 };
@@ -69,6 +70,7 @@ static size_t carve_verify(const VerifyArgs &a, bool with_draft, uint8_t *base, 
 	v.take = (int32_t *)take(N * 4);
 	v.own = (int32_t *)take(N * 4);
 	v.leaf = (int32_t *)take(N * 4);
+	v.act = (int32_t *)take(with_draft ? N * 4 : 0);
 	if (w)
 		*w = v;
 	return off;
@@ -79,28 +81,33 @@ size_t verify_work_bytes(const VerifyArgs &a, bool with_draft)
 	return carve_verify(a, with_draft, nullptr, nullptr);
 }
 
-// exp(x) for x <= 0, to about 1e-15: 2^k times the series of exp(r), |r| <= ln 2
-// / 2 (0.3466^13 / 13! < 1e-15)
-__device__ __forceinline__ double exp_below(double x)
+// 2^(j / 16), which every workgroup copies to LDS (16 entries: a wave's lanes
+// read them without bank conflicts)
+__constant__ const double POW16[16] = {
+	1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
+	1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
+	1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
+	1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+
+// exp(x inv) = 2^(t / 16) with t = x EXP16 inv, x <= 0: 2^k of the table's
+// entry and the series of 2^(r / 16), |r| <= 1 / 2 (0.0217^7 / 7! = 5e-16).  A
+// series alone takes twice the steps.
+constexpr double EXP16 = 16.0 * 1.4426950408889634;
+__device__ __forceinline__ double pow16(double t, const double *tab)
 {
-	const double k = __builtin_rint(x * 1.4426950408889634);
-	// ln 2 in two parts: its first 32 bits, and the rest
-	double r = __builtin_fma(k, -2977044471.0 / 4294967296.0, x);
-	r = __builtin_fma(k, -1.90821492927058770e-10, r);
-	double y = 1.0 / 479001600.0;
-	y = __builtin_fma(y, r, 1.0 / 39916800.0);
-	y = __builtin_fma(y, r, 1.0 / 3628800.0);
-	y = __builtin_fma(y, r, 1.0 / 362880.0);
-	y = __builtin_fma(y, r, 1.0 / 40320.0);
-	y = __builtin_fma(y, r, 1.0 / 5040.0);
-	y = __builtin_fma(y, r, 1.0 / 720.0);
-	y = __builtin_fma(y, r, 1.0 / 120.0);
-	y = __builtin_fma(y, r, 1.0 / 24.0);
-	y = __builtin_fma(y, r, 1.0 / 6.0);
-	y = __builtin_fma(y, r, 0.5);
+	constexpr double L = 0.69314718055994531 / 16.0;
+	const double s = t + 6755399441055744.0; // 1.5 2^52: the nearest integer, in the low bits
+	const int n = (int)(uint32_t)(uint64_t)__double_as_longlong(s);
+	const double r = t - (s - 6755399441055744.0);
+	double y = L * L * L * L * L * L / 720.0;
+	y = __builtin_fma(y, r, L * L * L * L * L / 120.0);
+	y = __builtin_fma(y, r, L * L * L * L / 24.0);
+	y = __builtin_fma(y, r, L * L * L / 6.0);
+	y = __builtin_fma(y, r, L * L / 2.0);
+	y = __builtin_fma(y, r, L);
 	y = __builtin_fma(y, r, 1.0);
-	y = __builtin_fma(y, r, 1.0);
-	return x > -745.0 ? __builtin_amdgcn_ldexp(y, (int)k) : x != x ? x : 0.0;
+	y = __builtin_amdgcn_ldexp(y * tab[n & 15], n >> 4);
+	return t < -17400.0 ? 0.0 : y; // (NaN stays NaN)
 }
 
 // what one workgroup writes for another of the same launch goes past the
@@ -145,7 +152,14 @@ struct Shared {
 	float f[4];
 	int i[4], j[4];
 	int flag;
-	int32_t path[V_PATH_LDS], own[V_PATH_LDS], leaf[V_PATH_LDS];
+	double pow[16];
+	int32_t path[V_PATH_LDS], own[V_PATH_LDS], leaf[V_PATH_LDS], parent[V_PATH_LDS];
+
+	__device__ __forceinline__ void fill() // (a barrier before its use)
+	{
+		if (threadIdx.x < 16)
+			pow[threadIdx.x] = POW16[threadIdx.x];
+	}
 };
 
 // the sum over the workgroup, in every thread
@@ -197,17 +211,23 @@ __device__ __forceinline__ bool ranges_good(const VerifyArgs &a)
 	return !__syncthreads_or(bad);
 }
 
-// The path of sequence b, rows [t0, t1): a workgroup; the outcomes through LDS.
+// The outcomes of rows [t0, t1) into LDS, as many as it holds (a workgroup).
+__device__ void get_outcomes(const VerifyArgs &a, const VerifyWork &w, int t0, int t1, Shared &sh)
+{
+	for (int i = threadIdx.x; i < t1 - t0 && i < V_PATH_LDS; i += blockDim.x) {
+		sh.path[i] = have(w.take + t0 + i);
+		sh.own[i] = have(w.own + t0 + i);
+		sh.leaf[i] = have(w.leaf + t0 + i);
+		sh.parent[i] = a.parent[t0 + i];
+	}
+	__syncthreads();
+}
+
+// The path of sequence b, rows [t0, t1): a workgroup.
 __device__ void write_path(const VerifyArgs &a, const VerifyWork &w, int b, int t0, int t1, Shared &sh)
 {
 	int32_t *path = a.path + (size_t)b * a.max_path;
 	const int n = t1 - t0;
-	for (int i = threadIdx.x; i < n && i < V_PATH_LDS; i += blockDim.x) {
-		sh.path[i] = have(w.take + t0 + i);
-		sh.own[i] = have(w.own + t0 + i);
-		sh.leaf[i] = have(w.leaf + t0 + i);
-	}
-	__syncthreads();
 	if (threadIdx.x == 0) {
 		int t = t0, k = 0, next = -1;
 		while (n > 0) {
@@ -232,6 +252,40 @@ __device__ void write_path(const VerifyArgs &a, const VerifyWork &w, int b, int 
 	__syncthreads();
 	for (int i = sh.flag + threadIdx.x; i < a.max_path; i += blockDim.x)
 		path[i] = -1;
+}
+
+// All rows of sequence b have arrived with an outcome, or with the child they
+// refused last (take = -2 - its row) and a residual sum to wait for: the path, or
+// which of the waiting rows the next launch works on.  A row that the path
+// cannot reach any more is left: an ancestor took another child, none, or
+// refused the one on the way here.
+__device__ void settle(const VerifyArgs &a, const VerifyWork &w, int b, int t0, int t1, int pass, Shared &sh)
+{
+	const int n = t1 - t0;
+	get_outcomes(a, w, t0, t1, sh);
+	int waiting = 0;
+	for (int i0 = 0; i0 < n; i0 += V_THREADS) {
+		const int i = i0 + threadIdx.x;
+		const int take = i >= n ? -1 : i < V_PATH_LDS ? sh.path[i] : have(w.take + t0 + i);
+		bool act = take <= -2;
+		if (n <= V_PATH_LDS)
+			for (int j = i; act && j > 0;) {
+				const int up = sh.parent[j];
+				act = up >= 0 && up < j;
+				if (act) {
+					const int of_up = sh.path[up];
+					act = of_up >= -1 ? of_up == t0 + j : t0 + j > -2 - of_up;
+					j = up;
+				}
+			}
+		if (a.draft && i < n)
+			give(w.act + t0 + i, act ? pass : -1);
+		waiting += __syncthreads_count(act);
+	}
+	if (waiting == 0)
+		write_path(a, w, b, t0, t1, sh);
+	else if (threadIdx.x == 0)
+		give(w.count + a.n_tokens + b, n - waiting); // (the others are there already)
 }
 
 // The first index whose running weight exceeds u times the whole: over the
@@ -342,7 +396,7 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 	const int b = seq_of_row(a, t, t0, t1);
 	if (b < 0)
 		return;
-	const double inv = a.temperature > 0.0f ? 1.0 / (double)a.temperature : 0.0;
+	const double rate = a.temperature > 0.0f ? EXP16 / (double)a.temperature : 0.0;
 	const double *s = w.s + (size_t)t * w.chunks, *res = w.res + (size_t)t * w.chunks;
 	const uint64_t *top = w.top + (size_t)t * w.chunks;
 	const float *l = a.logits + (size_t)t * a.l_stride, *q = a.draft ? a.draft + (size_t)t * a.d_stride : nullptr;
@@ -415,7 +469,7 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 	}
 	auto whole_of = [&](uint64_t v, double sum) {
 		const float m = __uint_as_float((uint32_t)v);
-		return m > -__builtin_inff() ? sum * exp_below(((double)m - (double)r.m) * inv) : 0.0;
+		return m > -__builtin_inff() ? sum * pow16(((double)m - (double)r.m) * rate, sh.pow) : 0.0;
 	};
 	if (a.temperature > 0.0f && lane < w.chunks)
 		z0 = whole_of(top0, s0);
@@ -435,10 +489,10 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 		r.M = wave_total(M);
 	}
 	r.waits = -1;
-	auto p_of = [&](float y) { return exp_below(((double)y - (double)r.m) * inv) * r.scale; };
+	auto p_of = [&](float y) { return pow16(((double)y - (double)r.m) * rate, sh.pow) * r.scale; };
 	const double px = is_token && a.temperature > 0.0f ? p_of(lx) : 0.0;
 
-	int taken = -1;
+	int taken = -1, refused = 0;
 	unsigned long long gone = 0; // no draft rows: refused children
 	for (int i = r.kid; i < n; i++) {
 		const int xi = __builtin_amdgcn_readlane(x, i);
@@ -461,6 +515,7 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 			r.c += r.M;
 			r.kid = i + 1;
 			r.waits = pass;
+			refused = __builtin_amdgcn_readlane(kid, i);
 			break;
 		}
 		if (__ballot(x == xi) & gone)
@@ -472,16 +527,15 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 		gone |= 1ull << i;
 		r.M -= pi;
 	}
-	if (r.waits >= 0) {
-		if (threadIdx.x == 0)
+	if (threadIdx.x == 0) {
+		if (r.waits >= 0)
 			w.row[t] = r; // (for the next launch)
-		return;
+		else if (!w.join)
+			w.row[t].waits = -1;
 	}
-	if (pass == 0 && threadIdx.x == 0)
-		w.row[t].waits = -1;
 
 	int own = r.best, leaf = r.best;
-	if (a.temperature > 0.0f) {
+	if (a.temperature > 0.0f && r.waits < 0) {
 		auto p_sum = [&](int c) { return whole_of(have(top + c), have(s + c)) * r.scale; };
 		const bool cut = a.max_path < t1 - t0; // a path may end at any node
 		const bool plain = (r.c == 0.0 && !gone) || !(r.M > 0.0);
@@ -534,14 +588,32 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 			leaf = own;
 	}
 	if (threadIdx.x == 0) {
-		give(w.take + t, taken);
+		give(w.take + t, r.waits >= 0 ? -2 - refused : taken);
 		give(w.own + t, own);
 		give(w.leaf + t, leaf);
 	}
 	if (!w.join || !ranges_good(a))
 		return;
 	if (last_of(w.count + a.n_tokens + b, t1 - t0, &sh.flag))
-		write_path(a, w, b, t0, t1, sh);
+		settle(a, w, b, t0, t1, pass, sh);
+}
+
+// A workgroup's logits (or draft probabilities): four at a time to a thread
+__device__ __forceinline__ void get_chunk(const float *row, int base, int n, float none, float (&x)[V_E])
+{
+	if (base + V_CHUNK <= n && ((uintptr_t)(row + base) & 15) == 0) {
+#pragma unroll
+		for (int e = 0; e < V_E; e += 4) {
+			const float4 v = reinterpret_cast<const float4 *>(row + base)[e / 4 * V_THREADS + threadIdx.x];
+			x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
+		}
+	} else {
+#pragma unroll
+		for (int e = 0; e < V_E; e++) {
+			const int i = base + (e / 4 * V_THREADS + threadIdx.x) * 4 + e % 4;
+			x[e] = i < n ? row[i] : none;
+		}
+	}
 }
 
 // The first launch: largest logit and sum of each chunk.
@@ -551,19 +623,8 @@ __global__ __launch_bounds__(V_THREADS, 4) void verify_stats_kernel(VerifyArgs a
 	const int t = blockIdx.y, chunk = blockIdx.x, base = chunk * V_CHUNK;
 	const float *l = a.logits + (size_t)t * a.l_stride;
 	float x[V_E];
-	if (base + V_CHUNK <= a.vocab && ((uintptr_t)(l + base) & 15) == 0) {
-#pragma unroll
-		for (int e = 0; e < V_E; e += 4) {
-			const float4 v = reinterpret_cast<const float4 *>(l + base)[e / 4 * V_THREADS + threadIdx.x];
-			x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
-		}
-	} else {
-#pragma unroll
-		for (int e = 0; e < V_E; e++) {
-			const int i = base + (e / 4 * V_THREADS + threadIdx.x) * 4 + e % 4;
-			x[e] = i < a.vocab ? l[i] : -__builtin_inff();
-		}
-	}
+	sh.fill();
+	get_chunk(l, base, a.vocab, -__builtin_inff(), x);
 	float m = x[0];
 #pragma unroll
 	for (int e = 1; e < V_E; e++)
@@ -589,10 +650,10 @@ __global__ __launch_bounds__(V_THREADS, 4) void verify_stats_kernel(VerifyArgs a
 	}
 	double s = 0.0;
 	if (a.temperature > 0.0f && m > -__builtin_inff()) {
-		const double inv = 1.0 / (double)a.temperature;
+		const double rate = EXP16 / (double)a.temperature;
 #pragma unroll
 		for (int e = 0; e < V_E; e++)
-			s += exp_below(((double)x[e] - (double)m) * inv);
+			s += pow16(((double)x[e] - (double)m) * rate, sh.pow);
 		s = block_total(s, sh);
 	}
 	if (threadIdx.x == 0) {
@@ -623,18 +684,19 @@ __global__ __launch_bounds__(V_THREADS, 4) void verify_residual_kernel(VerifyArg
 {
 	__shared__ Shared sh;
 	const int t = blockIdx.y, base = blockIdx.x * V_CHUNK;
-	if (w.row[t].waits != pass)
-		return;
 	const VRow r = w.row[t];
-	const double inv = 1.0 / (double)a.temperature;
-	const float *l = a.logits + (size_t)t * a.l_stride, *q = a.draft + (size_t)t * a.d_stride;
+	if ((w.join ? w.act[t] : r.waits) != pass)
+		return;
+	sh.fill();
+	float li[V_E], qi[V_E];
+	get_chunk(a.logits + (size_t)t * a.l_stride, base, a.vocab, -__builtin_inff(), li);
+	get_chunk(a.draft + (size_t)t * a.d_stride, base, a.vocab, 0.0f, qi);
+	const double rate = EXP16 / (double)a.temperature;
 	double s = 0.0;
+	__syncthreads();
 #pragma unroll
 	for (int e = 0; e < V_E; e++) {
-		const int i = base + e * V_THREADS + threadIdx.x;
-		const bool in = i < a.vocab;
-		const float li = in ? l[i] : -__builtin_inff(), qi = in ? q[i] : 0.0f;
-		const double y = exp_below(((double)li - (double)r.m) * inv) * r.scale - r.c * (double)qi;
+		const double y = pow16(((double)li[e] - (double)r.m) * rate, sh.pow) * r.scale - r.c * (double)qi[e];
 		s += y > 0.0 ? y : 0.0;
 	}
 	s = block_total(s, sh);
@@ -650,6 +712,8 @@ __global__ __launch_bounds__(V_THREADS) void verify_row_kernel(VerifyArgs a, Ver
 	__shared__ Shared sh;
 	if (pass && w.row[blockIdx.x].waits != pass - 1)
 		return;
+	sh.fill();
+	__syncthreads();
 	row_step(a, w, blockIdx.x, pass, sh);
 }
 
@@ -658,6 +722,7 @@ __global__ __launch_bounds__(V_THREADS) void verify_path_kernel(VerifyArgs a, Ve
 	__shared__ Shared sh;
 	const bool good = ranges_good(a);
 	const int b = blockIdx.x, t0 = a.first ? a.first[b] : b, t1 = a.first ? a.first[b + 1] : b + 1;
+	get_outcomes(a, w, good ? t0 : 0, good ? t1 : 0, sh);
 	write_path(a, w, b, good ? t0 : 0, good ? t1 : 0, sh);
 }
 
