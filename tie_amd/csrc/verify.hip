@@ -24,6 +24,7 @@ namespace tie {
 
 constexpr int V_CHUNK = 4096; // logits of a workgroup
 constexpr int V_THREADS = 256, V_E = V_CHUNK / V_THREADS;
+constexpr size_t V_AT_ONCE = 1024; // workgroups that run together: 4 on a CU
 constexpr int V_KIDS = VERIFY_KIDS;
 constexpr int V_PATH_LDS = 512; // nodes of a sequence whose outcomes the path's reader keeps in LDS
 
@@ -616,50 +617,72 @@ __device__ __forceinline__ void get_chunk(const float *row, int base, int n, flo
 	}
 }
 
-// The first launch: largest logit and sum of each chunk.
+// The first launch: largest logit and sum of each chunk; a workgroup PER chunks,
+// whose logits are under way together.
+template <int PER>
 __global__ __launch_bounds__(V_THREADS, 4) void verify_stats_kernel(VerifyArgs a, VerifyWork w)
 {
 	__shared__ Shared sh;
-	const int t = blockIdx.y, chunk = blockIdx.x, base = chunk * V_CHUNK;
+	__shared__ float fs[PER][4];
+	__shared__ double ds[PER][4];
+	__shared__ int is[PER][4];
+	const int t = blockIdx.y, chunk = blockIdx.x * PER, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
 	const float *l = a.logits + (size_t)t * a.l_stride;
-	float x[V_E];
+	float x[PER][V_E], m[PER];
 	sh.fill();
-	get_chunk(l, base, a.vocab, -__builtin_inff(), x);
-	float m = x[0];
 #pragma unroll
-	for (int e = 1; e < V_E; e++)
-		m = __builtin_fmaxf(m, x[e]);
-	m = wave_max(m);
-	if ((threadIdx.x & 63) == 0)
-		sh.f[threadIdx.x >> 6] = m;
-	__syncthreads();
-	m = __builtin_fmaxf(__builtin_fmaxf(sh.f[0], sh.f[1]), __builtin_fmaxf(sh.f[2], sh.f[3]));
-	int at = 0;
-	if (a.temperature == 0.0f) { // its lowest index
-		at = 0x7fffffff;
+	for (int q = 0; q < PER; q++)
+		get_chunk(l, (chunk + q) * V_CHUNK, a.vocab, -__builtin_inff(), x[q]);
 #pragma unroll
-		for (int e = V_E - 1; e >= 0; e--)
-			at = x[e] == m ? base + (e / 4 * V_THREADS + (int)threadIdx.x) * 4 + e % 4 : at;
+	for (int q = 0; q < PER; q++) {
+		m[q] = x[q][0];
 #pragma unroll
-		for (int k = 1; k < 64; k <<= 1)
-			at = min(at, __shfl_xor(at, k));
-		if ((threadIdx.x & 63) == 0)
-			sh.i[threadIdx.x >> 6] = at;
-		__syncthreads();
-		at = min(min(sh.i[0], sh.i[1]), min(sh.i[2], sh.i[3]));
+		for (int e = 1; e < V_E; e++)
+			m[q] = __builtin_fmaxf(m[q], x[q][e]);
+		m[q] = wave_max(m[q]);
+		if (lane == 0)
+			fs[q][wave] = m[q];
 	}
-	double s = 0.0;
-	if (a.temperature > 0.0f && m > -__builtin_inff()) {
+	__syncthreads();
+#pragma unroll
+	for (int q = 0; q < PER; q++)
+		m[q] = __builtin_fmaxf(__builtin_fmaxf(fs[q][0], fs[q][1]), __builtin_fmaxf(fs[q][2], fs[q][3]));
+	if (a.temperature == 0.0f) { // its lowest index
+#pragma unroll
+		for (int q = 0; q < PER; q++) {
+			int at = 0x7fffffff;
+#pragma unroll
+			for (int e = V_E - 1; e >= 0; e--)
+				at = x[q][e] == m[q] ? (chunk + q) * V_CHUNK + (e / 4 * V_THREADS + (int)threadIdx.x) * 4 + e % 4 : at;
+#pragma unroll
+			for (int k = 1; k < 64; k <<= 1)
+				at = min(at, __shfl_xor(at, k));
+			if (lane == 0)
+				is[q][wave] = at;
+		}
+	} else {
 		const double rate = EXP16 / (double)a.temperature;
 #pragma unroll
-		for (int e = 0; e < V_E; e++)
-			s += pow16(((double)x[e] - (double)m) * rate, sh.pow);
-		s = block_total(s, sh);
+		for (int q = 0; q < PER; q++) {
+			double s = 0.0;
+			if (m[q] > -__builtin_inff())
+#pragma unroll
+				for (int e = 0; e < V_E; e++)
+					s += pow16(((double)x[q][e] - (double)m[q]) * rate, sh.pow);
+			s = wave_total(s);
+			if (lane == 0)
+				ds[q][wave] = s;
+		}
 	}
-	if (threadIdx.x == 0) {
-		const size_t o = (size_t)t * w.chunks + chunk;
-		give(w.top + o, (uint64_t)__float_as_uint(m) | (uint64_t)(uint32_t)at << 32);
-		give(w.s + o, s);
+	__syncthreads();
+	if (threadIdx.x < PER && chunk + (int)threadIdx.x < w.chunks) {
+		const int q = threadIdx.x;
+		const size_t o = (size_t)t * w.chunks + chunk + q;
+		const bool greedy = a.temperature == 0.0f;
+		const int at = greedy ? min(min(is[q][0], is[q][1]), min(is[q][2], is[q][3])) : 0;
+		const float most = __builtin_fmaxf(__builtin_fmaxf(fs[q][0], fs[q][1]), __builtin_fmaxf(fs[q][2], fs[q][3]));
+		give(w.top + o, (uint64_t)__float_as_uint(most) | (uint64_t)(uint32_t)at << 32);
+		give(w.s + o, greedy ? 0.0 : (ds[q][0] + ds[q][1]) + (ds[q][2] + ds[q][3]));
 	}
 	if (w.join) {
 		// sequences of no rows have nobody to arrive; ranges that do not ascend
@@ -674,7 +697,7 @@ __global__ __launch_bounds__(V_THREADS, 4) void verify_stats_kernel(VerifyArgs a
 					a.next[b] = -1;
 				}
 		}
-		if (last_of(w.count + t, w.chunks, &sh.flag))
+		if (last_of(w.count + t, gridDim.x, &sh.flag))
 			row_step(a, w, t, 0, sh);
 	}
 }
@@ -733,7 +756,11 @@ hipError_t launch_verify(const VerifyArgs &a, void *work, hipStream_t st)
 	const dim3 grid(w.chunks, a.n_tokens), block(V_THREADS);
 	const int passes = a.draft && a.temperature > 0.0f ? a.max_children : 0;
 	if (a.n_tokens > 0) {
-		tie_launch(verify_stats_kernel, grid, block, 0, st, a, w);
+		// (as many workgroups as run at once: two chunks each where there are more)
+		if ((size_t)w.chunks * a.n_tokens <= V_AT_ONCE)
+			tie_launch(verify_stats_kernel<1>, grid, block, 0, st, a, w);
+		else
+			tie_launch(verify_stats_kernel<2>, dim3((w.chunks + 1) / 2, a.n_tokens), block, 0, st, a, w);
 		if (!w.join)
 			tie_launch(verify_row_kernel, dim3(a.n_tokens), block, 0, st, a, w, 0);
 		for (int p = 0; p < passes; p++) {
