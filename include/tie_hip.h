@@ -316,6 +316,8 @@ int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_layers, cons
  *        all calls on the stream share and which grows as needed, but not
  *        during HIP graph capture (run the largest call once before, or pass
  *        memory).  Graphs that may run at the same time need memory of their own.
+ * Scores are held in F32; past 2^24 in magnitude their rounding is larger than
+ * what a softmax tells apart, and a row's result means nothing.
  * A row's result is the same whatever else the call holds only up to F32
  * rounding: how the rows are cut follows the lengths.  Two equal calls give
  * equal bits. */

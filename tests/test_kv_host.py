@@ -146,3 +146,28 @@ def test_the_binding_checks_tensors():
     with pytest.raises(tie_amd.TieError) as e:
         c.attention(0, s, q, q.clone(), 1.0)
     assert e.value.code == tie_amd.ENOINIT
+
+
+def test_the_binding_refuses_other_devices(monkeypatch):
+    """(get_device of a tensor on the CPU is -1: the library is made to say that it has another GPU)"""
+    import torch
+    i32 = dict(dtype=torch.int32)
+    k = torch.zeros(1, 2, 2, 64, 64, dtype=torch.float16)
+    c, s = tie_amd.KVCache(k, k.clone()), tie_amd.KVSeqs(torch.zeros(2, 3, **i32), torch.zeros(2, **i32))
+    q, kv, two = torch.zeros(2, 256), torch.zeros(2, 128), torch.zeros(2, **i32)
+    calls = (lambda: c.append(0, s, q, kv, kv, q), lambda: c.read(s, kv.view(1, 2, 2, 64), kv.view(1, 2, 2, 64).clone()),
+             lambda: c.attention(0, s, q, q, 1.0), lambda: c.keep(s, torch.zeros(2, 3, **i32), two),
+             lambda: tie_amd.verify_tree(torch.zeros(2, 50), None, two, two, torch.zeros(2), torch.zeros(2), torch.zeros(2, 3, **i32),
+                                         two, two))
+    for call in calls:
+        with pytest.raises(tie_amd.TieError):  # (not initialised)
+            call()
+    monkeypatch.setattr(tie_amd, "_device", 0)
+    for call in calls:
+        with pytest.raises(ValueError, match="device"):
+            call()
+    monkeypatch.setattr(tie_amd, "_device", None)
+    monkeypatch.setattr(c, "device", 1)
+    for call in calls[:4]:
+        with pytest.raises(ValueError, match="device"):
+            call()

@@ -201,12 +201,19 @@ def _p(a):
     return a.ctypes.data
 
 
+_device = None  # the library's GPU
+
+
 def init(device=0):
+    global _device
     check(lib().tie_hip_init(device))
+    _device = device
 
 
 def shutdown():
+    global _device
     lib().tie_hip_shutdown()
+    _device = None
 
 
 def silu_table_host():
@@ -469,7 +476,13 @@ def _dtype(name):
 _dtypes = {}
 
 
-def _rows(a, what, width=None, n_rows=0):
+def _on_device(device, other, what):
+    """Tensors of another GPU than the library's, or of the CPU, would be read as addresses of it."""
+    if other != device or (_device is not None and device != _device):
+        raise ValueError("%s on device %s: device %s is wanted" % (what, other, device if _device is None else _device))
+
+
+def _rows(a, what, device, width=None, n_rows=0):
     """(pointer, row stride, values of a row) of n_rows or more F32 rows: a 2-D
     tensor, or one of [rows][heads][head_dim] whose rows are contiguous."""
     st, sh = a.stride(), a.shape
@@ -484,17 +497,31 @@ def _rows(a, what, width=None, n_rows=0):
             (st[0] < n and sh[0] > 1):
         raise ValueError("%s: %d rows of %s contiguous float32 values are wanted (got %s, shape %s, strides %s)"
                          % (what, n_rows, width or "", a.dtype, tuple(sh), st))
+    if a.get_device() != device:
+        _on_device(device, a.get_device(), what)
     return a.data_ptr(), (st[0] if st[0] > n else n), n
 
 
-def _array(a, dtype, shape, what):
-    """The pointer of a contiguous device array of this type and shape (None for None)."""
+def _array(a, dtype, shape, what, device):
+    """The pointer of a contiguous array on `device` of this type and shape (None for None)."""
     if a is None:
         return None
     if a.dtype is not _dtype(dtype) or a.shape != shape or not a.is_contiguous():
         raise ValueError("%s: a contiguous %s array of shape %s is wanted (got %s, %s)" % (what, dtype, tuple(shape), a.dtype,
                                                                                            tuple(a.shape)))
+    if a.get_device() != device:
+        _on_device(device, a.get_device(), what)
     return a.data_ptr()
+
+
+def _work(work, device):
+    """Pointer and bytes of a call's scratch memory (None: the stream's own)."""
+    if work is None:
+        return None, 0
+    if not work.is_contiguous() or work.get_device() != device:
+        _on_device(device, work.get_device(), "work")
+        raise ValueError("work: contiguous memory is wanted")
+    return work.data_ptr(), work.numel() * work.element_size()
 
 
 class KVSeqs:
@@ -506,9 +533,11 @@ class KVSeqs:
         n_seqs, max_pages = pages.shape
         if n_tokens is None:
             n_tokens = n_seqs if first is None else int(first[-1])
-        self.n_seqs, self.n_tokens, self.keep = n_seqs, n_tokens, (pages, lens, first)
-        self.desc = KVSeqsDesc(n_seqs, max_pages, n_tokens, _array(pages, "int32", pages.shape, "pages"),
-                               _array(lens, "int32", (n_seqs,), "lens"), _array(first, "int32", (n_seqs + 1,), "first"))
+        dev = pages.get_device()
+        self.n_seqs, self.n_tokens, self.device, self.keep = n_seqs, n_tokens, dev, (pages, lens, first)
+        self.desc = KVSeqsDesc(n_seqs, max_pages, n_tokens, _array(pages, "int32", pages.shape, "pages", dev),
+                               _array(lens, "int32", (n_seqs,), "lens", dev),
+                               _array(first, "int32", (n_seqs + 1,), "first", dev))
         self.ref = ctypes.byref(self.desc)
 
 
@@ -528,11 +557,12 @@ class KVCache:
         if kind == I8 and (k_scale is None or v_scale is None):
             raise ValueError("an int8 cache needs k_scale and v_scale")
         self.kv_heads, self.head_dim, self.n_layers, self.keep_alive = kvh, hd, nl, (k, v, k_scale, v_scale)
-        self.width, self.head_shape = kvh * hd, (hd,)
-        self.desc = KVCacheDesc(kind, nl, npg, kvh, hd, _array(k, name, k.shape, "k"),
-                                _array(v, name, (nl, npg, kvh, hd, PAGE_ROWS), "v"),
-                                _array(k_scale, "float32", k.shape[:4], "k_scale"),
-                                _array(v_scale, "float32", k.shape[:4], "v_scale"))
+        self.width, self.head_shape, self.device = kvh * hd, (hd,), k.get_device()
+        dev = self.device
+        self.desc = KVCacheDesc(kind, nl, npg, kvh, hd, _array(k, name, k.shape, "k", dev),
+                                _array(v, name, (nl, npg, kvh, hd, PAGE_ROWS), "v", dev),
+                                _array(k_scale, "float32", k.shape[:4], "k_scale", dev),
+                                _array(v_scale, "float32", k.shape[:4], "v_scale", dev))
         self.ref = ctypes.byref(self.desc)
 
     def _heads(self, width, what):
@@ -540,47 +570,55 @@ class KVCache:
             raise ValueError("%s: rows of %d values are no whole heads of %d" % (what, width, self.head_dim))
         return width // self.head_dim
 
+    def _seqs(self, seqs):
+        if seqs.device != self.device or self.device != _device:
+            _on_device(self.device, seqs.device, "seqs")
+
     def _q(self, q, out, seqs, what):
-        pq, sq, w = _rows(q, "q", None, seqs.n_tokens)
+        self._seqs(seqs)
+        pq, sq, w = _rows(q, "q", self.device, None, seqs.n_tokens)
         if out is q:
             po, so = pq, sq
         else:
-            po, so, _ = _rows(out, what, w, seqs.n_tokens)
+            po, so, _ = _rows(out, what, self.device, w, seqs.n_tokens)
         return pq, sq, po, so, self._heads(w, "q")
 
     def append(self, layer, seqs, q, k, v, q_out, pos=None, q_norm=None, k_norm=None, eps=1e-6, theta=1e6, stream=None):
         """tie_hip_kv_append: norm and rotation of q and k, cache write of k and v."""
-        n = seqs.n_tokens
+        n, dev = seqs.n_tokens, self.device
         pq, sq, po, so, heads = self._q(q, q_out, seqs, "q_out")
-        pk, sk, _ = _rows(k, "k", self.width, n)
-        pv, sv, _ = _rows(v, "v", self.width, n)
+        pk, sk, _ = _rows(k, "k", dev, self.width, n)
+        pv, sv, _ = _rows(v, "v", dev, self.width, n)
         check(lib().tie_hip_kv_append(self.ref, layer, seqs.ref, pq, sq, pk, sk, pv, sv, heads,
-                                      _array(q_norm, "float32", self.head_shape, "q_norm"),
-                                      _array(k_norm, "float32", self.head_shape, "k_norm"), eps, theta,
-                                      _array(pos, "int32", (n,), "pos"), po, so, stream))
+                                      _array(q_norm, "float32", self.head_shape, "q_norm", dev),
+                                      _array(k_norm, "float32", self.head_shape, "k_norm", dev), eps, theta,
+                                      _array(pos, "int32", (n,), "pos", dev), po, so, stream))
 
     def read(self, seqs, k_out, v_out, layer=0, n_layers=1, stream=None):
         """tie_hip_kv_read: rows of the cache as float32 [n_layers][n_tokens][kv_heads][head_dim]."""
-        shape = (n_layers, seqs.n_tokens, self.kv_heads, self.head_dim)
-        check(lib().tie_hip_kv_read(self.ref, layer, n_layers, seqs.ref, _array(k_out, "float32", shape, "k_out"),
-                                    _array(v_out, "float32", shape, "v_out"), stream))
+        self._seqs(seqs)
+        shape, dev = (n_layers, seqs.n_tokens, self.kv_heads, self.head_dim), self.device
+        check(lib().tie_hip_kv_read(self.ref, layer, n_layers, seqs.ref, _array(k_out, "float32", shape, "k_out", dev),
+                                    _array(v_out, "float32", shape, "v_out", dev), stream))
 
     def attention(self, layer, seqs, q, out, scale, mask=None, work=None, stream=None):
         """tie_hip_tree_attention; mask: int64 [n_tokens][words] (bit patterns), None: causal; work: a uint8 tensor."""
         pq, sq, po, so, heads = self._q(q, out, seqs, "out")
-        words = 0 if mask is None else mask.shape[1]
+        words, (pw, nw) = 0 if mask is None else mask.shape[1], _work(work, self.device)
         check(lib().tie_hip_tree_attention(self.ref, layer, seqs.ref, pq, sq, heads, scale,
-                                           _array(mask, "int64", (seqs.n_tokens, words), "mask"), words, po, so, _p(work),
-                                           0 if work is None else work.numel() * work.element_size(), stream))
+                                           _array(mask, "int64", (seqs.n_tokens, words), "mask", self.device), words, po, so, pw,
+                                           nw, stream))
 
     def attention_work_bytes(self, seqs, n_heads):
         return lib().tie_hip_tree_attention_work_bytes(self.ref, seqs.ref, n_heads)
 
     def keep(self, seqs, path, n_keep, len_out=None, stream=None):
         """tie_hip_kv_keep: the accepted paths' rows moved down in every layer."""
-        check(lib().tie_hip_kv_keep(self.ref, seqs.ref, _array(path, "int32", (seqs.n_seqs, path.shape[1]), "path"),
-                                    path.shape[1], _array(n_keep, "int32", (seqs.n_seqs,), "n_keep"),
-                                    _array(len_out, "int32", (seqs.n_seqs,), "len_out"), stream))
+        self._seqs(seqs)
+        dev = self.device
+        check(lib().tie_hip_kv_keep(self.ref, seqs.ref, _array(path, "int32", (seqs.n_seqs, path.shape[1]), "path", dev),
+                                    path.shape[1], _array(n_keep, "int32", (seqs.n_seqs,), "n_keep", dev),
+                                    _array(len_out, "int32", (seqs.n_seqs,), "len_out", dev), stream))
 
 
 def verify_tree_work_bytes(vocab, n_tokens, max_children, with_draft):
@@ -590,14 +628,16 @@ def verify_tree_work_bytes(vocab, n_tokens, max_children, with_draft):
 def verify_tree(logits, first, tokens, parent, u_accept, u_sample, path, n_keep, next_token, temperature=1.0, draft=None,
                 max_children=1, work=None, stream=None):
     """tie_hip_verify_tree: the accepted path [n_seqs][max_path], its length and the next token of each sequence."""
-    n, n_seqs = tokens.shape[0], n_keep.shape[0]
-    pl, sl, vocab = _rows(logits, "logits", None, n)
-    pd, sd, _ = (None, 0, 0) if draft is None else _rows(draft, "draft", vocab, n)
-    check(lib().tie_hip_verify_tree(pl, sl, pd, sd, vocab, n_seqs, n, _array(first, "int32", (n_seqs + 1,), "first"),
-                                    _array(tokens, "int32", (n,), "tokens"), _array(parent, "int32", (n,), "parent"),
-                                    _array(u_accept, "float32", (n,), "u_accept"),
-                                    _array(u_sample, "float32", (n,), "u_sample"), temperature, max_children, path.shape[1],
-                                    _array(path, "int32", (n_seqs, path.shape[1]), "path"),
-                                    _array(n_keep, "int32", (n_seqs,), "n_keep"),
-                                    _array(next_token, "int32", (n_seqs,), "next_token"), _p(work),
-                                    0 if work is None else work.numel() * work.element_size(), stream))
+    n, n_seqs, dev = tokens.shape[0], n_keep.shape[0], logits.get_device()
+    if dev != _device:
+        _on_device(dev, dev, "logits")
+    pl, sl, vocab = _rows(logits, "logits", dev, None, n)
+    pd, sd, _ = (None, 0, 0) if draft is None else _rows(draft, "draft", dev, vocab, n)
+    pw, nw = _work(work, dev)
+    check(lib().tie_hip_verify_tree(pl, sl, pd, sd, vocab, n_seqs, n, _array(first, "int32", (n_seqs + 1,), "first", dev),
+                                    _array(tokens, "int32", (n,), "tokens", dev), _array(parent, "int32", (n,), "parent", dev),
+                                    _array(u_accept, "float32", (n,), "u_accept", dev),
+                                    _array(u_sample, "float32", (n,), "u_sample", dev), temperature, max_children, path.shape[1],
+                                    _array(path, "int32", (n_seqs, path.shape[1]), "path", dev),
+                                    _array(n_keep, "int32", (n_seqs,), "n_keep", dev),
+                                    _array(next_token, "int32", (n_seqs,), "next_token", dev), pw, nw, stream))

@@ -358,7 +358,7 @@ __device__ __forceinline__ void split_query(const AttnArgs &a, int node, float (
 			m = __builtin_fmaxf(m, __builtin_fabsf(x[k][j]));
 		}
 	m = max_g(m);
-	const float p2 = m >= 1e-30f && m < 1e30f ? pow2_below(m) : 1.0f;
+	const float p2 = m >= 1e-30f && m < __builtin_inff() ? pow2_below(m) : 1.0f;
 	const float up = __builtin_copysignf(512.0f / p2, a.scale);
 	// (not 0: the score of a row that is not seen, -inf, stays that)
 	qs = __builtin_fmaxf(__builtin_fabsf(a.scale) * 1.44269504088896f * (p2 * (1.0f / 512.0f)), 1.2e-38f);
