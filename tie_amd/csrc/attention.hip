@@ -1153,7 +1153,9 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 		for (int m = 0; m < MT; m++) {
 			const f4 x = total[t] == 0.0f && u.parts == 1 && !bad ? (f4){0.0f, 0.0f, 0.0f, 0.0f} : r[t].o[m] * f;
 			if (vec) {
-				*reinterpret_cast<f4 *>(o + m * 16 + 4 * g) = x;
+				// (past the caches: what lies there at a launch's end is written back first,
+				// 3 us of a tree's parts)
+				__builtin_nontemporal_store(x, reinterpret_cast<f4 *>(o + m * 16 + 4 * g));
 			} else {
 #pragma unroll
 				for (int i = 0; i < 4; i++)
