@@ -259,9 +259,11 @@ __device__ __forceinline__ bool find_unit(const KvSeqs &s, int kvh, int group, c
 // The first page of the unit's part, and behind its last.
 __device__ __forceinline__ void part_pages(const Cut &cut, const Unit &u, int pages, int &p0, int &p1)
 {
-	const int grains = div_up((u.len + u.n + PAGE - 1) / PAGE, cut.grain), q = grains / u.parts, r = grains % u.parts;
-	p0 = (u.part * q + min(u.part, r)) * cut.grain;
-	p1 = min(pages, p0 + (q + (u.part < r)) * cut.grain);
+	// (in grains where a part has few of them, else to the page)
+	const int all = (u.len + u.n + PAGE - 1) / PAGE, grain = all / u.parts < 4 * cut.grain ? cut.grain : 1;
+	const int grains = div_up(all, grain), q = grains / u.parts, r = grains % u.parts;
+	p0 = (u.part * q + min(u.part, r)) * grain;
+	p1 = min(pages, p0 + (q + (u.part < r)) * grain);
 }
 
 // Which of the 64 rows of the page at row `start` a token sees: all committed
@@ -287,29 +289,6 @@ __device__ __forceinline__ uint64_t sees(const AttnArgs &a, const Unit &u, int n
 	w &= below((long long)u.n - rel); // no bit names a node that is not there
 	return w | below(-(long long)rel);
 }
-
-// The page table's entries of a unit, a lane each, 64 pages at a time: a page's
-// number is then a register away (a load of it stands before the page's own loads
-// otherwise: 800 cycles a page).
-struct PageIds {
-	int first, ids; // pages first .. first + 63
-	__device__ __forceinline__ void get(const KvSeqs &s, const Unit &u, int p)
-	{
-		first = p;
-		const int at = p + (int)(threadIdx.x & 63);
-		ids = at < s.max_pages ? s.pages[(size_t)u.b * s.max_pages + at] : -1;
-	}
-	// the number of page p, p not below the last one asked for; bad: it is none
-	__device__ __forceinline__ int of(const KvSeqs &s, const Unit &u, int n_pages, int p, bool &bad)
-	{
-		if (p - first >= 64)
-			get(s, u, p);
-		const int id = __builtin_amdgcn_readlane(ids, p - first);
-		const bool ok = id >= 0 && id < n_pages;
-		bad = bad || !ok;
-		return ok ? id : 0;
-	}
-};
 
 // Results of a part, for each row of its tile: O [HD], the maximum, the sum.
 constexpr int part_row(int hd)
@@ -580,13 +559,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 	part_pages(cut, u, pages, p0, p1);
 	const int steps = (p1 - p0) * SP;
 
-	PageIds ids;
-	ids.get(s, u, p0);
 	u4 kr[KT][KL], vr[MT];
 	float ks = 0.0f, vs = 0.0f; // int8: the scales of the lane's row
 	size_t at = 0; // of the page whose V is in (or on its way to) vr
 	auto page = [&](int step) {
-		return (size_t)ids.of(s, u, c.n_pages, p0 + step / SP, bad) * c.kvh + u.head;
+		const int id = __builtin_amdgcn_readfirstlane(page_of(s, c.n_pages, u.b, (p0 + step / SP) * PAGE));
+		bad = bad || id < 0;
+		return (size_t)(id < 0 ? 0 : id) * c.kvh + u.head;
 	};
 	auto get_k = [&](size_t pg, int step) {
 		const int row0 = step % SP * 32;
@@ -821,6 +800,30 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 // together touch all banks: K row r's piece q lies at q ^ f(r), f the lane of
 // the operand that reads the row; V column i's at q ^ (i % 8).
 constexpr int MANY_WAVES = 4;
+
+// The page table's entries of a unit, a lane each, 64 pages at a time: a page's
+// number is then a register away (a load of it stands before the page's own loads
+// otherwise: 800 cycles a page; the kernel of few rows has eight waves to hide
+// that, and is 0.6 us slower this way).
+struct PageIds {
+	int first, ids; // pages first .. first + 63
+	__device__ __forceinline__ void get(const KvSeqs &s, const Unit &u, int p)
+	{
+		first = p;
+		const int at = p + (int)(threadIdx.x & 63);
+		ids = at < s.max_pages ? s.pages[(size_t)u.b * s.max_pages + at] : -1;
+	}
+	// the number of page p, p not below the last one asked for; bad: it is none
+	__device__ __forceinline__ int of(const KvSeqs &s, const Unit &u, int n_pages, int p, bool &bad)
+	{
+		if (p - first >= 64)
+			get(s, u, p);
+		const int id = __builtin_amdgcn_readlane(ids, p - first);
+		const bool ok = id >= 0 && id < n_pages;
+		bad = bad || !ok;
+		return ok ? id : 0;
+	}
+};
 
 template <int HD, bool I8, int RG>
 __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, float *part)
