@@ -1262,7 +1262,15 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 {
 	const size_t group = a.n_heads / c.kvh, rows = (size_t)s.n_tokens * group;
 	Shape h;
-	h.few = rows <= (size_t)FEW_ROWS * s.n_seqs;
+	// The kernel of few rows reads a page again for each 16 of them, but its parts
+	// are joined in the same launch and a wave waits for none: small trees take it
+	// too, int8 ones (half the bytes; codes are converted for every 16 rows) up to
+	// larger sizes.  int8: 5 tokens of 32 heads over 8000 rows 17 us (by the other
+	// kernel 26), 26 over 8000 26.5 (31), over 32000 61 (59), 16 sequences of 16
+	// over 8000 70 (64).  f16: 4 tokens over 8000 rows 19.6 (25.6), 8 over 1000 19.9
+	// (18.2), 8 sequences of 8 over 8000 39 (32).
+	const size_t most = c.i8 ? 256 : 64, units = c.i8 ? 448 : 64;
+	h.few = rows <= (size_t)FEW_ROWS * s.n_seqs || (rows <= most * s.n_seqs && rows * c.kvh <= units * FEW_ROWS);
 	// many: 128 rows where such tiles fill the card (4096 tokens of 32 heads 240
 	// us, by 64 rows 257), or 64: as many units and half the parts' bytes, less
 	// left of tiles that a mask or a sequence's end cuts (1000 tokens over 2000
