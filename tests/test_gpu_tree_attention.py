@@ -190,6 +190,55 @@ def test_masked_values_that_are_not_finite(kind):
     assert (np.abs(o - want)[ok] <= tol[ok]).all()
 
 
+# sizes that take each kernel: tiles of 16 rows, of 64 (cut into parts or
+# whole) and of 128
+@pytest.mark.parametrize("kind", ["f16", "i8"])
+@pytest.mark.parametrize("H,kvh,hd,length,n", [(8, 1, 128, 900, 30), (16, 1, 128, 900, 41), (8, 2, 64, 700, 90), (64, 8, 64, 70, 300),
+                                               (64, 4, 128, 45, 515), (64, 2, 64, 100, 515)])
+def test_any_mask_at_every_size(kind, H, kvh, hd, length, n):
+    """Random masks, rows that see nothing, and rows of the cache with values
+    that are not finite, which one token sees and the others do not."""
+    rng = np.random.default_rng(n)
+    lens, counts = [length, 0], [n, 6]
+    c = kv_ref.Cache(rng, kind, kvh, hd, lens, counts)
+    q = rng.standard_normal((n + 6, H, hd)).astype(np.float32)
+    sees = [rng.random((m, m)) < 0.3 for m in counts]
+    sees[0][::3] = sees[1][::2] = False
+    sees[0][:, [5, 20, 29]] = False
+    want, tol = kv_ref.attention(c, 0, q, hd ** -0.5, lambda b, i, j: sees[b][i, j])
+    sees[0][[7, 9, 11], [5, 20, 29]] = True
+    (p5, r5), (p20, r20), (p29, r29) = (c.place(0, length + j) for j in (5, 20, 29))
+    bad, half = np.zeros((n + 6, H, hd), bool), H // kvh
+    if kind == "f16":
+        c.v[0, p5, 0, 3, r5] = np.nan
+        c.v[0, p20, kvh - 1, hd - 4, r20] = np.inf
+        c.k[0, p29, 0, r29, 9] = np.nan
+        bad[7, :half, 3] = bad[9, -half:, hd - 4] = bad[11, :half] = True
+    else:
+        c.vs[0, p5, 0, r5] = np.nan
+        c.vs[0, p20, kvh - 1, r20] = np.nan
+        c.ks[0, p29, 0, r29] = np.nan
+        bad[7, :half] = bad[9, -half:] = bad[11, :half] = True
+    o = run(c, q, hd ** -0.5, words(sees))
+    assert not np.isfinite(o[bad]).any()
+    # (tokens 7, 9 and 11 see a row more than `want` knows in their other heads)
+    ok = ~bad
+    ok[[7, 9, 11]] = False
+    assert np.isfinite(o[ok]).all() and (np.abs(o - want)[ok] <= tol[ok]).all()
+    assert (o[n:n + 6:2] == 0).all() and (o[:n] != 0).any(-1).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "i8"])
+@pytest.mark.parametrize("H,kvh,hd,lens,counts", [(64, 4, 128, [70, 3], [300, 230]), (64, 2, 64, [10], [520]), (8, 1, 128, [2500], [33]),
+                                                  (8, 1, 128, [2500], [7]), (16, 4, 64, [700, 0, 65], [20, 64, 130])])
+def test_causal_at_every_size(kind, H, kvh, hd, lens, counts):
+    rng = np.random.default_rng(sum(counts) + H)
+    c = kv_ref.Cache(rng, kind, kvh, hd, lens, counts)
+    q = rng.standard_normal((sum(counts), H, hd)).astype(np.float32)
+    want, tol = kv_ref.attention(c, 0, q, hd ** -0.5, lambda b, i, j: j <= i)
+    check(run(c, q, hd ** -0.5), want, tol)
+
+
 @pytest.mark.parametrize("kind", ["f16", "i8"])
 @pytest.mark.parametrize("size", [1e-4, 1.0, 3e3])
 def test_sizes_of_queries_and_values(kind, size):

@@ -101,6 +101,56 @@ def test_large_vocabulary(draft):
 
 
 @pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+def test_more_logits_than_run_at_once(draft, temperature):
+    """(two blocks of 4096 logits to a workgroup; the last has one logit)"""
+    Case(21, [13] * 14 + [1, 7], 5 * 4096 + 1, draft, branch=2).check(temperature, 2, 13)
+    Case(22, [13] * 20, 4 * 4096, draft, branch=3).check(temperature, 3, 13, stride=1)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_more_rows_than_counters(draft):
+    """(past 8192 rows and sequences the steps are launches of their own)"""
+    c = Case(23, [9, 0, 8] * 520, 40, draft, branch=2, peaked=1.0)
+    c.check(1.0, 2, 9)
+    c.check(0.0, 2, 4)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_large_trees(draft):
+    """(more nodes than the path's reader keeps in LDS)"""
+    c = Case(24, [700, 511, 513], 64, draft, branch=3, peaked=1.0)
+    for seed in range(3):
+        c.ua[:] = np.random.default_rng(seed).random(len(c.ua)).astype(np.float32) ** 3
+        c.check(1.0, 3, 12)
+
+
+@pytest.mark.parametrize("kids", [1, 3])
+def test_parents_that_are_no_nodes(kids):
+    """A parent at or past its child, or below none, makes a node nobody's child."""
+    c = Case(25, [6, 6], 50, True, branch=2, peaked=1.0)
+    c.parent[3], c.parent[4], c.parent[8], c.parent[9] = 3, 5, -1, 100
+    c.ua[:] = 0.0
+    c.check(1.0, kids, 6)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_rows_that_are_no_distribution(draft, temperature, value):
+    """Logits of NaN or infinity alone: the sequence's outputs are tokens and
+    nodes of it, and the other sequences' are what they were."""
+    c = Case(26, [7, 7, 7], 9000, draft, branch=2)
+    want = c.want(temperature, 2, 7)
+    c.logits[7:14] = value
+    path, n, nxt = c.run(temperature, 2, 7)
+    for g, w in zip((path, n, nxt), want):
+        np.testing.assert_array_equal(g[[0, 2]], w[[0, 2]])
+    assert 1 <= n[1] <= 7 and 0 <= nxt[1] < 9000
+    assert path[1, 0] == 0 and (np.diff(path[1, :n[1]]) > 0).all() and (path[1, n[1]:] == -1).all() and path[1].max() < 7
+
+
+@pytest.mark.parametrize("draft", [False, True])
 def test_many_children_and_cut_paths(draft):
     """16 children of one node, fewer tried than there are, paths cut at the
     outputs' depth, sequences of one node and of none, siblings of one token."""
