@@ -493,7 +493,7 @@ def _rows(a, what, device, width=None, n_rows=0):
         inner = (st[2] == 1 or sh[2] == 1) and (st[1] == sh[2] or sh[1] == 1)
     else:
         n, inner = -1, False
-    if a.dtype is not _dtype("float32") or not inner or (width is not None and n != width) or sh[0] < n_rows or \
+    if a.dtype is not (_dtypes.get("float32") or _dtype("float32")) or not inner or (width is not None and n != width) or sh[0] < n_rows or \
             (st[0] < n and sh[0] > 1):
         raise ValueError("%s: %d rows of %s contiguous float32 values are wanted (got %s, shape %s, strides %s)"
                          % (what, n_rows, width or "", a.dtype, tuple(sh), st))
@@ -506,7 +506,7 @@ def _array(a, dtype, shape, what, device):
     """The pointer of a contiguous array on `device` of this type and shape (None for None)."""
     if a is None:
         return None
-    if a.dtype is not _dtype(dtype) or a.shape != shape or not a.is_contiguous():
+    if a.dtype is not (_dtypes.get(dtype) or _dtype(dtype)) or a.shape != shape or not a.is_contiguous():
         raise ValueError("%s: a contiguous %s array of shape %s is wanted (got %s, %s)" % (what, dtype, tuple(shape), a.dtype,
                                                                                            tuple(a.shape)))
     if a.get_device() != device:
