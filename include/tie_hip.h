@@ -290,7 +290,8 @@ typedef struct tie_hip_kv_seqs {
  *             head_dim); pos [n_tokens] (a tree's nodes at one depth share a
  *             position), NULL: the token's cache row
  * in 64 bits, rounded once.  The queries go to q_out (which may be q, with the
- * same stride), keys and values to the cache. */
+ * same stride, or other columns of the same matrix), keys and values to the
+ * cache. */
 int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q, size_t q_stride,
 		      const float *k, size_t k_stride, const float *v, size_t v_stride, int n_heads, const float *q_norm,
 		      const float *k_norm, float eps, float theta, const int32_t *pos, float *q_out, size_t q_out_stride,
@@ -315,7 +316,8 @@ int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_layers, cons
  *        here leave it fit for the next); NULL: the stream's workspace, which
  *        all calls on the stream share and which grows as needed, but not
  *        during HIP graph capture (run the largest call once before, or pass
- *        memory).  Graphs that may run at the same time need memory of their own.
+ *        memory).  Calls and graphs that may run at the same time on different
+ *        streams need memory of their own.
  * Scores are held in F32; past 2^24 in magnitude their rounding is larger than
  * what a softmax tells apart, and a row's result means nothing.
  * A row's result is the same whatever else the call holds only up to F32
@@ -355,7 +357,8 @@ int tie_hip_kv_keep(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, 
  * whole.  temperature 0: the largest logit (the lowest of equals) alone counts.
  *   path   [n_seqs][max_path] accepted nodes, the root first; -1 behind them
  *   n_keep [n_seqs] how many; next [n_seqs] (0 and -1 for a sequence of no rows)
- * All sums in 64 bits.  work as for tie_hip_tree_attention. */
+ * All sums in 64 bits.  No output may share memory with an input.  work as for
+ * tie_hip_tree_attention. */
 size_t tie_hip_verify_tree_work_bytes(int vocab, int n_tokens, int max_children, int with_draft);
 int tie_hip_verify_tree(const float *logits, size_t logits_stride, const float *draft, size_t draft_stride, int vocab,
 			int n_seqs, int n_tokens, const int32_t *first, const int32_t *tokens, const int32_t *parent,

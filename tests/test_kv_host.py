@@ -52,7 +52,7 @@ def attention(c=None, s=None, layer=0, heads=4, scale=0.1, mask=None, words=0, q
 
 
 def verify(logits=A, ls=100, draft=None, ds=0, vocab=100, n_seqs=2, n=5, first=A, tokens=A, parent=A, ua=A, us=A, temp=1.0, kids=2,
-           most=3, path=A, nk=A, nxt=A):
+           most=3, path=A + 4096, nk=A + 8192, nxt=A + 8448):
     return tie_amd.lib().tie_hip_verify_tree(logits, ls, draft, ds, vocab, n_seqs, n, first, tokens, parent, ua, us, temp, kids, most,
                                              path, nk, nxt, None, 0, None)
 
@@ -89,7 +89,8 @@ NAN, INF = float("nan"), float("inf")
     (verify, [dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(n=-1), dict(n=65536), dict(n_seqs=-1), dict(ls=99), dict(draft=A, ds=99),
               dict(temp=-1.0), dict(temp=NAN), dict(temp=INF), dict(kids=0), dict(kids=17), dict(most=0), dict(first=None),
               dict(logits=None), dict(tokens=None), dict(parent=None), dict(ua=None), dict(us=None), dict(path=None), dict(nk=None),
-              dict(nxt=None)]),
+              dict(nxt=None), dict(path=A + 16), dict(nk=A + 4096 + 20), dict(nxt=A + 8196), dict(nxt=A),
+              dict(draft=A + 8192, ds=100)]),
 ])
 def test_arguments(call, bad):
     assert call() == tie_amd.ENOINIT
@@ -101,6 +102,15 @@ def test_arguments(call, bad):
 def test_in_place_is_no_overlap():
     assert append(out=A) == tie_amd.ENOINIT
     assert attention(out=A) == tie_amd.ENOINIT
+    # rows side by side in one matrix are none either; rows that share columns are
+    one = dict(sq=1024, sk=1024, sv=1024, so=1024)
+    beside = dict(one, k=A + W * 4, v=A + W * 4 + 512, out=A)
+    assert append(**beside) == tie_amd.ENOINIT
+    assert append(**dict(beside, out=A + W * 4 + 1024)) == tie_amd.ENOINIT
+    for bad in (dict(k=A), dict(v=A + W * 4 - 4), dict(k=A + 4096 + 256), dict(out=A + W * 4 + 1020), dict(out=A + 4096 - 4)):
+        assert append(**dict(beside, **bad)) == tie_amd.EINVAL, bad
+    assert attention(out=A + 4 * W, sq=2 * W, so=2 * W) == tie_amd.ENOINIT
+    assert attention(out=A + 4 * W - 4, sq=2 * W, so=2 * W) == tie_amd.EINVAL
 
 
 def test_null_structures():

@@ -1432,6 +1432,19 @@ static size_t row_span(int T, size_t stride, size_t width)
 	return T > 0 ? ((size_t)(T - 1) * stride + width) * 4 : 0;
 }
 
+// Whether T rows of `wa` and of `wb` floats share memory.  Rows of one stride may
+// lie side by side in one matrix.
+static bool rows_overlap(int T, const float *a, size_t sa, size_t wa, const float *b, size_t sb, size_t wb)
+{
+	if (!overlap(a, row_span(T, sa, wa), b, row_span(T, sb, wb)))
+		return false;
+	const intptr_t d = (intptr_t)b - (intptr_t)a, row = (intptr_t)sa * 4;
+	if (sa != sb || T == 1)
+		return true;
+	const size_t off = (size_t)((d % row + row) % row); // b's row begins so far behind one of a's
+	return off < wa * 4 || off + wb * 4 > (size_t)row;
+}
+
 } // namespace tie
 
 #define TIE_TRY(expr)                     \
@@ -1462,10 +1475,8 @@ extern "C" int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const
 	if (!none && (!q || !k || !v || !q_out))
 		return set_error(TIE_HIP_EINVAL, "null q/k/v/q_out");
 	const int T = s.n_tokens;
-	const size_t no = row_span(T, q_out_stride, wq);
-	if (!(q_out == q && q_out_stride == q_stride) &&
-	    (overlap(q_out, no, q, row_span(T, q_stride, wq)) || overlap(q_out, no, k, row_span(T, k_stride, wk)) ||
-	     overlap(q_out, no, v, row_span(T, v_stride, wk))))
+	if ((!(q_out == q && q_out_stride == q_stride) && rows_overlap(T, q_out, q_out_stride, wq, q, q_stride, wq)) ||
+	    rows_overlap(T, q_out, q_out_stride, wq, k, k_stride, wk) || rows_overlap(T, q_out, q_out_stride, wq, v, v_stride, wk))
 		return set_error(TIE_HIP_EINVAL, "q_out overlaps an input (it may be q itself, with q's stride)");
 	TIE_TRY(ensure_init());
 	if (none)
@@ -1585,7 +1596,7 @@ extern "C" int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, 
 	if (!none && (!q || !out))
 		return set_error(TIE_HIP_EINVAL, "null q/out");
 	if (!(out == q && out_stride == q_stride) &&
-	    overlap(out, row_span(s.n_tokens, out_stride, w), q, row_span(s.n_tokens, q_stride, w)))
+	    rows_overlap(s.n_tokens, out, out_stride, w, q, q_stride, w))
 		return set_error(TIE_HIP_EINVAL, "out overlaps q (it may be q itself, with q's stride)");
 	TIE_TRY(ensure_init());
 	if (none)
@@ -1652,6 +1663,22 @@ extern "C" int tie_hip_verify_tree(const float *logits, size_t logits_stride, co
 		return set_error(TIE_HIP_EINVAL, "null path/n_keep/next");
 	if (n_seqs > 0 && n_tokens > 0 && (!logits || !tokens || !parent || !u_accept || !u_sample))
 		return set_error(TIE_HIP_EINVAL, "null logits/tokens/parent/u_accept/u_sample");
+	{
+		// (rows are read while others' outcomes are written)
+		const size_t nb = (size_t)n_seqs * 4, nt = (size_t)n_tokens * 4;
+		const void *outs[3] = {path, n_keep, next}, *ins[7] = {first, tokens, parent, u_accept, u_sample, logits, draft};
+		const size_t no[3] = {nb * max_path, nb, nb},
+			     ni[7] = {nb + 4, nt, nt, nt, nt, row_span(n_tokens, logits_stride, vocab),
+				      row_span(n_tokens, draft_stride, vocab)};
+		for (int o = 0; o < 3; o++) {
+			for (int i = 0; i < 7; i++)
+				if (overlap(outs[o], no[o], ins[i], ni[i]))
+					return set_error(TIE_HIP_EINVAL, "path/n_keep/next overlap an input");
+			for (int i = 0; i < o; i++)
+				if (overlap(outs[o], no[o], outs[i], no[i]))
+					return set_error(TIE_HIP_EINVAL, "path, n_keep and next overlap");
+		}
+	}
 	TIE_TRY(ensure_init());
 	if (n_seqs == 0)
 		return TIE_HIP_OK;
