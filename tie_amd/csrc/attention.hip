@@ -883,8 +883,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 		}
 	};
 	// int8: a page's codes by way of registers, K and the scales (half 0) and then
-	// V (both at once are 32 registers, and some of them went to scratch memory:
-	// 1000 tokens over 2000 rows 156 us)
+	// V (both at once would be more registers than there are)
 	auto get8 = [&](size_t pg, int half) {
 		const uint8_t *from = uniform((half ? c.v : c.k) + pg * PAGE * HD);
 #pragma unroll

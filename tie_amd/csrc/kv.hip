@@ -293,19 +293,27 @@ constexpr int KEEP_BATCH = 8;
 constexpr int KEEP_TABLE = 64; // path entries at a time
 
 // How many entries of sequence b's path can be moved: up to the first that
-// does not ascend or is none of its n nodes.  A wave.
-__device__ __forceinline__ int keep_count(const int32_t *path, int want, int n)
+// does not ascend or is none of its n nodes.  A wave, whose lanes have the first
+// entries already (they are requested with the lengths).
+__device__ __forceinline__ int keep_count(const int32_t *path, int mine, int want, int n)
 {
 	const int lane = threadIdx.x & 63;
 	for (int j0 = 0; j0 < want; j0 += 64) {
 		const int j = j0 + lane;
 		const bool in = j < want;
-		const int p = in ? path[j] : 0, prev = in && j > 0 ? path[j - 1] : -1;
+		const int p = j0 == 0 ? mine : in ? path[j] : 0, before = __shfl_up(p, 1);
+		const int prev = lane > 0 ? before : j0 > 0 ? path[j0 - 1] : -1;
 		const unsigned long long bad = __ballot(in && (p <= prev || p >= n));
 		if (bad)
 			return j0 + __builtin_ctzll(bad);
 	}
 	return want > 0 ? want : 0;
+}
+
+__device__ __forceinline__ int first_entry(const int32_t *path, int max_path)
+{
+	const int lane = threadIdx.x & 63;
+	return path[lane < max_path ? lane : max_path - 1];
 }
 
 template <typename T>
@@ -317,11 +325,12 @@ __global__ __launch_bounds__(256) void kv_keep_kernel(KvLayer c, KvSeqs s, const
 	const int h = blockIdx.x % c.kvh, layer = blockIdx.x / c.kvh, b = blockIdx.y, i = threadIdx.x % c.hd;
 	const bool is_v = (int)threadIdx.x >= c.hd;
 	int t0, n;
+	const int32_t *pb = path + (size_t)b * max_path;
+	const int entry = first_entry(pb, max_path);
 	const int len = s.len[b];
 	const int want = min(n_keep[b], max_path);
 	seq_tokens(s, b, t0, n);
-	const int32_t *pb = path + (size_t)b * max_path;
-	const int count = seq_fits(s, len, n) ? keep_count(pb, want, n) : 0;
+	const int count = seq_fits(s, len, n) ? keep_count(pb, entry, want, n) : 0;
 	if (len_out && blockIdx.x == 0 && threadIdx.x == 0)
 		len_out[b] = len + count;
 	T *base = reinterpret_cast<T *>((is_v ? c.v : c.k) + (size_t)layer * c.layer_bytes) + (size_t)h * PAGE * c.hd;
@@ -331,7 +340,7 @@ __global__ __launch_bounds__(256) void kv_keep_kernel(KvLayer c, KvSeqs s, const
 		const int m = min(KEEP_TABLE, count - j1);
 		__syncthreads();
 		if ((int)threadIdx.x < m) {
-			const int j = j1 + threadIdx.x, p = pb[j];
+			const int j = j1 + threadIdx.x, p = j1 ? pb[j] : entry;
 			const int fp = page_of(s, c.n_pages, b, len + p), tp = page_of(s, c.n_pages, b, len + j);
 			from[threadIdx.x] = fp * PAGE + (len + p) % PAGE;
 			to[threadIdx.x] = p == j || fp < 0 || tp < 0 ? -1 : tp;
@@ -371,7 +380,8 @@ __global__ __launch_bounds__(64) void kv_keep_len_kernel(KvSeqs s, const int32_t
 	int t0, n;
 	seq_tokens(s, b, t0, n);
 	const int len = s.len[b];
-	const int count = seq_fits(s, len, n) ? keep_count(path + (size_t)b * max_path, min(n_keep[b], max_path), n) : 0;
+	const int32_t *pb = path + (size_t)b * max_path;
+	const int count = seq_fits(s, len, n) ? keep_count(pb, first_entry(pb, max_path), min(n_keep[b], max_path), n) : 0;
 	if (threadIdx.x == 0)
 		len_out[b] = len + count;
 }

@@ -176,10 +176,13 @@ __device__ __forceinline__ double block_total(double x, Shared &sh)
 
 // The token rows [t0, t1) of row t's sequence; its number, or -1: none holds it.
 // A wave: the sequences' ends a lane each, after bisection down to 64 of them.
-__device__ __forceinline__ int seq_of_row(const VerifyArgs &a, int t, int &t0, int &t1)
+// good: whether all ranges ascend within the rows, as far as the wave has seen
+// (all of them up to 64; else ranges_good has to look).
+__device__ __forceinline__ int seq_of_row(const VerifyArgs &a, int t, int &t0, int &t1, bool &good)
 {
 	t0 = t;
 	t1 = t + 1;
+	good = true;
 	if (!a.first)
 		return t;
 	int lo = 0, hi = a.n_seqs;
@@ -193,6 +196,7 @@ __device__ __forceinline__ int seq_of_row(const VerifyArgs &a, int t, int &t0, i
 	// the last b in [lo, hi) with first[b] <= t (of equal ones the last: the others hold nothing)
 	const int lane = threadIdx.x & 63, b = lo + lane;
 	const int from = b < hi ? a.first[b] : 0x7fffffff, to = b < hi ? a.first[b + 1] : 0;
+	good = !__ballot(b < hi && (from < 0 || from > to || to > a.n_tokens));
 	const unsigned long long below = __ballot(from <= t);
 	if (!below)
 		return -1;
@@ -394,7 +398,8 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 {
 	const int lane = threadIdx.x & 63;
 	int t0, t1;
-	const int b = seq_of_row(a, t, t0, t1);
+	bool good;
+	const int b = seq_of_row(a, t, t0, t1, good);
 	if (b < 0)
 		return;
 	const double rate = a.temperature > 0.0f ? EXP16 / (double)a.temperature : 0.0;
@@ -593,7 +598,7 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 		give(w.own + t, own);
 		give(w.leaf + t, leaf);
 	}
-	if (!w.join || !ranges_good(a))
+	if (!w.join || !good || (a.n_seqs > 64 && !ranges_good(a)))
 		return;
 	if (last_of(w.count + a.n_tokens + b, t1 - t0, &sh.flag))
 		settle(a, w, b, t0, t1, pass, sh);
