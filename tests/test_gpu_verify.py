@@ -125,6 +125,31 @@ def test_large_trees(draft):
         c.check(1.0, 3, 12)
 
 
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("first", [[0, 9, 5, 21], [0, 5, 9, 22], [-1, 5, 9, 21], [7, 3, 3, 3]])
+def test_ranges_that_do_not_ascend(draft, first):
+    """No paths, whatever the call before left in the workspace; rows behind
+    the last sequence are nobody's.  Also where more sequences than a wave has
+    lanes are searched."""
+    import torch
+    for more in (0, 70):
+        c = Case(27, [5, 4, 12] + [1] * more, 3000, draft, branch=2, peaked=1.0)
+        work = torch.full((tie_amd.verify_tree_work_bytes(3000, 21 + more, 2, draft),), 7, dtype=torch.uint8, device="cuda")
+        work[:1 << 15] = 0
+        good = c.first.copy()
+        c.first[:4] = first
+        if (np.diff(c.first) >= 0).all() and c.first[0] >= 0 and c.first[-1] <= 21 + more:
+            continue  # (with the sequences behind them these ranges do ascend within the rows)
+        path, n, nxt = c.run(1.0, 2, 6, work=work)
+        assert (path == -1).all() and (n == 0).all() and (nxt == -1).all()
+        c.first[:] = good
+        c.check(1.0, 2, 6, work=work)
+        c.first[3:] = 9
+        if not more:
+            c.counts = [5, 4, 0]
+            c.check(1.0, 2, 6, work=work)
+
+
 @pytest.mark.parametrize("kids", [1, 3])
 def test_parents_that_are_no_nodes(kids):
     """A parent at or past its child, or below none, makes a node nobody's child."""

@@ -402,6 +402,9 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 	const int b = seq_of_row(a, t, t0, t1, good);
 	if (b < 0)
 		return;
+	// (no row of such a call has what a later pass would read)
+	if (w.join && (!good || (a.n_seqs > 64 && !ranges_good(a))))
+		return;
 	const double rate = a.temperature > 0.0f ? EXP16 / (double)a.temperature : 0.0;
 	const double *s = w.s + (size_t)t * w.chunks, *res = w.res + (size_t)t * w.chunks;
 	const uint64_t *top = w.top + (size_t)t * w.chunks;
@@ -598,7 +601,7 @@ __device__ void row_step(const VerifyArgs &a, const VerifyWork &w, int t, int pa
 		give(w.own + t, own);
 		give(w.leaf + t, leaf);
 	}
-	if (!w.join || !good || (a.n_seqs > 64 && !ranges_good(a)))
+	if (!w.join)
 		return;
 	if (last_of(w.count + a.n_tokens + b, t1 - t0, &sh.flag))
 		settle(a, w, b, t0, t1, pass, sh);
