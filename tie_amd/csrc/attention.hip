@@ -137,12 +137,10 @@ struct Unit {
 	int base, tile_at; // the first unit of the sequence, and the tile's place among its tiles
 };
 
+// (in 64-bit floats: exact, and without the LDS instructions of a shuffle)
 __device__ __forceinline__ int wave_sum(int x)
 {
-#pragma unroll
-	for (int m = 1; m < 64; m <<= 1)
-		x += __shfl_xor(x, m);
-	return x;
+	return (int)wave_total((double)x);
 }
 
 __device__ __forceinline__ void seq_work(const KvSeqs &s, int b, int group, int rows, int &t0, int &n, int &len, int &tiles,
@@ -179,23 +177,19 @@ __device__ __forceinline__ float part_rate(const KvSeqs &s, int kvh, int group, 
 		return 0.0f;
 	const int lane = threadIdx.x & 63;
 	auto over = [&](auto f) { // the sum of f(tiles, pages) over all sequences
-		auto x = f(tiles0, pages0);
+		double x = f(tiles0, pages0);
 		for (int b = 64 + lane; b < s.n_seqs; b += 64) {
 			int t0, n, len, tiles, pages;
 			seq_work(s, b, group, cut.rows, t0, n, len, tiles, pages);
 			x += f(tiles, pages);
 		}
-		if (s.n_seqs > 1)
-#pragma unroll
-			for (int m = 1; m < 64; m <<= 1)
-				x += __shfl_xor(x, m);
-		return of_lane(x, 0);
+		return s.n_seqs > 1 ? wave_total(x) : of_lane(x, 0);
 	};
 	const int cap = cut.cap / kvh > 0 ? cut.cap / kvh : 1; // for one kv head
-	if ((long long)over([](int t, int) { return t; }) * kvh >= cut.full)
+	if (over([](int t, int) { return t; }) * kvh >= cut.full)
 		return 0.0f;
 	// the nearest number to each tile's share; a little less where those are too many
-	float rate = (float)cap / over([&](int t, int p) { return (float)t * div_up(p, cut.grain); });
+	float rate = (float)(cap / over([&](int t, int p) { return (double)t * div_up(p, cut.grain); }));
 	for (int i = 0; i < 16; i++) {
 		if (over([&](int t, int p) { return t * tile_parts(cut, p, rate); }) <= cap)
 			return rate;
@@ -216,14 +210,7 @@ __device__ __forceinline__ bool find_unit(const KvSeqs &s, int kvh, int group, c
 	int before = 0;
 	for (int b0 = 0;;) {
 		const int parts = tiles ? tile_parts(cut, pages, rate) : 0, mine = tiles * parts * kvh;
-		int incl = mine;
-		if (s.n_seqs > 1)
-#pragma unroll
-			for (int m = 1; m < 64; m <<= 1) {
-				const int o = __shfl_up(incl, m);
-				if (lane >= m)
-					incl += o;
-			}
+		const int incl = s.n_seqs > 1 ? (int)running_of<64>((double)mine) : mine;
 		const unsigned long long past = __ballot(before + incl > index);
 		if (past) {
 			const int l = __builtin_ctzll(past);

@@ -158,7 +158,7 @@ __device__ __forceinline__ int page_of(const KvSeqs &s, int n_pages, int b, int 
 }
 
 // The sequence of token row t (the last b with first[b] <= t), -1 when none
-// holds it.
+// holds it.  A wave: the ranges a lane each, after bisection down to 64 of them.
 __device__ __forceinline__ int seq_of_token(const KvSeqs &s, int t, int &t0, int &n)
 {
 	if (!s.first) {
@@ -167,17 +167,22 @@ __device__ __forceinline__ int seq_of_token(const KvSeqs &s, int t, int &t0, int
 		return t < s.n_seqs ? t : -1;
 	}
 	int lo = 0, hi = s.n_seqs;
-	while (lo < hi) {
+	while (hi - lo > 64) {
 		const int mid = (lo + hi) >> 1;
-		if (s.first[mid + 1] <= t)
-			lo = mid + 1;
+		if (s.first[mid] <= t)
+			lo = mid;
 		else
 			hi = mid;
 	}
-	if (lo >= s.n_seqs)
+	const int b = lo + (int)(threadIdx.x & 63);
+	const int from = b < hi ? s.first[b] : 0x7fffffff, to = b < hi ? s.first[b + 1] : 0;
+	const unsigned long long below = __ballot(from <= t);
+	if (!below)
 		return -1;
-	seq_tokens(s, lo, t0, n);
-	return t >= t0 && t < t0 + n ? lo : -1;
+	const int l = 63 - __builtin_clzll(below), t1 = __builtin_amdgcn_readlane(to, l);
+	t0 = __builtin_amdgcn_readlane(from, l);
+	n = t1 - t0;
+	return t0 >= 0 && t < t1 && t1 <= s.n_tokens ? lo + l : -1;
 }
 #endif
 

@@ -178,14 +178,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvLayer c, KvSeqs s, float
 				pages = (from + sn + PAGE - 1) / PAGE;
 			}
 		}
-		int incl = pages;
-		if (s.n_seqs > 1)
-#pragma unroll
-			for (int m = 1; m < 64; m <<= 1) {
-				const int o = __shfl_up(incl, m);
-				if (lane >= m)
-					incl += o;
-			}
+		const int incl = s.n_seqs > 1 ? (int)running_of<64>((double)pages) : pages;
 		const unsigned long long past = __ballot(before + incl > (int)blockIdx.x);
 		if (past) {
 			const int l = __builtin_ctzll(past);
