@@ -222,6 +222,46 @@ def test_keep(kind, kvh, hd, in_place):
 
 
 @pytest.mark.parametrize("kind", ["f16", "i8"])
+def test_many_sequences(kind):
+    """More than a wave has lanes, some of no tokens."""
+    rng = np.random.default_rng(22)
+    lens, counts = [int(x) for x in rng.integers(0, 100, 150)], [int(x) for x in rng.integers(0, 4, 150)]
+    counts[63:66] = [0, 0, 0]
+    test_append((kind, 4, 2, 64, lens, counts), 1e6, 0, True)
+    test_read(kind, 4, 2, 64, lens, counts)
+
+
+@pytest.mark.parametrize("kind", ["f16", "i8"])
+def test_keep_long_paths(kind):
+    """Paths of more entries than a wave has lanes, one that stops ascending
+    behind them."""
+    import torch
+    rng = np.random.default_rng(23)
+    kvh, hd, lens, counts = 1, 64, [30, 64, 0], [300, 200, 140]
+    paths = [sorted(rng.choice(300, 150, replace=False).tolist()), list(range(200)), list(range(1, 131)) + [130, 131]]
+    valid = [150, 200, 130]
+    c = kv_ref.Cache(rng, kind, kvh, hd, lens, counts, layers=2)
+    kv, seqs = c.gpu(), c.seqs()
+    pad = np.full((3, 203), -1, np.int32)
+    for b, p in enumerate(paths):
+        pad[b, : len(p)] = p
+    len_out = torch.zeros(3, dtype=torch.int32, device="cuda")
+    kv.keep(seqs, cuda(pad), cuda(np.array([len(p) for p in paths], np.int32)), len_out)
+    got, = done(len_out)
+    same(got, (np.array(lens) + valid).astype(np.int32))
+    for b, (n, p) in enumerate(zip(lens, paths)):
+        for layer in range(2):
+            for j in range(valid[b]):
+                (fp, fr), (tp, tr) = c.place(b, n + p[j]), c.place(b, n + j)
+                c.k[layer, tp, :, tr], c.v[layer, tp, :, :, tr] = c.k[layer, fp, :, fr].copy(), c.v[layer, fp, :, :, fr].copy()
+                if kind == "i8":
+                    c.ks[layer, tp, :, tr], c.vs[layer, tp, :, tr] = c.ks[layer, fp, :, fr].copy(), c.vs[layer, fp, :, fr].copy()
+    for a, w in zip(c.back(), (c.k, c.v, c.ks, c.vs)):
+        if w is not None:
+            same(a, w)
+
+
+@pytest.mark.parametrize("kind", ["f16", "i8"])
 def test_what_the_device_arrays_may_not_say(kind):
     """Lengths, row ranges and pages outside the call's sizes: nothing is
     written to the cache, reads give NaN, and good sequences are served."""

@@ -240,6 +240,53 @@ def test_causal_at_every_size(kind, H, kvh, hd, lens, counts):
 
 
 @pytest.mark.parametrize("kind", ["f16", "i8"])
+@pytest.mark.parametrize("most", [2, 5, 40])
+def test_many_sequences(kind, most):
+    """More than a wave has lanes, of 0 to `most` - 1 tokens, one of them long."""
+    rng = np.random.default_rng(90 + most)
+    lens, counts = [int(x) for x in rng.integers(0, 100, 140)], [int(x) for x in rng.integers(0, most, 140)]
+    lens[100], counts[63:66], counts[100] = 1500, [0, 0, 0], 1
+    c = kv_ref.Cache(rng, kind, 2, 64, lens, counts)
+    q = rng.standard_normal((sum(counts), 8, 64)).astype(np.float32)
+    want, tol = kv_ref.attention(c, 0, q, 0.125, lambda b, i, j: j <= i)
+    check(run(c, q, 0.125), want, tol)
+
+
+@pytest.mark.parametrize("kind", ["f16", "i8"])
+@pytest.mark.parametrize("H,kvh,hd,lens,counts", [(8, 1, 128, [700], [3]), (16, 1, 128, [900, 4], [41, 2]), (64, 4, 128, [45], [515])])
+def test_rows_behind_the_last_sequence(kind, H, kvh, hd, lens, counts):
+    """A batch padded to more token rows than its sequences have, and a replay
+    of it with other ranges: rows of no sequence stay."""
+    import torch
+    rng = np.random.default_rng(95)
+    c = kv_ref.Cache(rng, kind, kvh, hd, lens, counts)
+    kv, T = c.gpu(), sum(counts)
+    q = rng.standard_normal((T + 9, H, hd)).astype(np.float32)
+    first = cuda(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+    seqs = tie_amd.KVSeqs(cuda(c.table), cuda(np.array(lens, np.int32)), first, T + 9)
+    qd, out = cuda(q), torch.full((T + 9, H, hd), -7.0, device="cuda")
+    work = torch.zeros(kv.attention_work_bytes(seqs, H), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    g, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with kv_ref.capture(g, stream):
+        kv.attention(0, seqs, qd, out, hd ** -0.5, work=work, stream=torch.cuda.current_stream().cuda_stream)
+    for last in (counts[-1], 1, counts[-1]):
+        c.counts[-1] = last
+        n = sum(c.counts)
+        first[-1] = n
+        out.fill_(-7.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        want, tol = kv_ref.attention(c, 0, q[:n], hd ** -0.5, lambda b, i, j: j <= i)
+        o = out.cpu().numpy()
+        check(o[:n], want, tol)
+        assert (o[n:] == -7.0).all()
+    del g
+    gc.collect()
+
+
+@pytest.mark.parametrize("kind", ["f16", "i8"])
 @pytest.mark.parametrize("size", [1e-4, 1.0, 3e3])
 def test_sizes_of_queries_and_values(kind, size):
     """Values and queries of other sizes than a trained layer's, and rows a
