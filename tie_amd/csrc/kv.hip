@@ -35,11 +35,17 @@ __device__ __forceinline__ _Float16 half_of(float x)
 // chain of steps (position, angle, sincos; row, norm, code).  Many: by the 64-bit
 // arithmetic, about 60 instructions for 64 pairs, and the V columns' pieces (a
 // row's values lie PAGE apart).
+constexpr int DIES = 8;
+
 template <int HD, bool I8>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, AppendArgs a, int per_wave)
 {
 	constexpr int L = HD / 2, G = 64 / L; // lanes of a head, heads of a wave at a time
-	const int t = blockIdx.x, lane = threadIdx.x & 63, i = lane % L, part = lane / L;
+	// (workgroups go to the dies in turn: each die has neighbouring tokens)
+	const int t = blockIdx.x % DIES * (gridDim.x / DIES) + blockIdx.x / DIES;
+	const int lane = threadIdx.x & 63, i = lane % L, part = lane / L;
+	if (t >= s.n_tokens)
+		return;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	int t0, n;
 	const int b = seq_of_token(s, t, t0, n);
@@ -142,7 +148,7 @@ hipError_t launch_kv_append(const KvLayer &c, const KvSeqs &s, const AppendArgs 
 	const size_t all = (size_t)s.n_tokens * units;
 	int per = all > 4096 ? (int)(all / 4096) : 1;
 	per = per > (units + 3) / 4 ? (units + 3) / 4 : per;
-	const dim3 grid(s.n_tokens, (units + 4 * per - 1) / (4 * per));
+	const dim3 grid((s.n_tokens + DIES - 1) / DIES * DIES, (units + 4 * per - 1) / (4 * per));
 	auto go = [&](auto kern) { tie_launch(kern, grid, dim3(256), 0, st, c, s, a, per); };
 	if (c.hd == 128)
 		c.i8 ? go(kv_append_kernel<128, true>) : go(kv_append_kernel<128, false>);
