@@ -988,7 +988,8 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 				give_back<HD, NT>(c.v + at * HD * PAGE * 2, g, end, mine, r);
 			}
 		}
-		auto weigh_half = [&](int row0, h8 (&ph)[NT][1], h8 (&pl)[NT][1]) {
+		// (between: what is done between the products and the weights)
+		auto weigh_half = [&](int row0, h8 (&ph)[NT][1], h8 (&pl)[NT][1], auto between) {
 			uint32_t seen[NT];
 			bool whole = seen_all;
 #pragma unroll
@@ -1001,8 +1002,10 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 					all = all && (seen[t] == ~0u || node[t] < 0);
 					any = any || seen[t] != 0;
 				}
-				if (!__any(any))
+				if (!__any(any)) {
+					between();
 					return false;
+				}
 				whole = __all(all);
 			}
 			h8 kf[KT][KS];
@@ -1032,6 +1035,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 							sc[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kt][k], e ? qh[t][k] : ql[t][k],
 													   sc[t][kt], 0, 0, 0);
 			__builtin_amdgcn_s_setprio(0);
+			between();
 			float ks = 0.0f, vs = 0.0f;
 			if constexpr (I8) {
 				const int row = row0 + g * 8 + (n16 & 7);
@@ -1066,7 +1070,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 			for (int row0 = 0; row0 < PAGE; row0 += 32) {
 				if (I8 && more)
 					get8(next, row0 >> 5);
-				if (weigh_half(row0, ph, pl))
+				if (weigh_half(row0, ph, pl, [] {}))
 					add_half(row0, ph, pl);
 				if (I8 && more)
 					put8(b ^ 1, row0 >> 5);
@@ -1075,11 +1079,12 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 			const int row0 = wave / RG * 32;
 			if (I8 && more)
 				get8(next, 0);
-			const bool any = weigh_half(row0, ph, pl);
-			if (I8 && more) {
-				put8(b ^ 1, 0);
-				get8(next, 1);
-			}
+			const bool any = weigh_half(row0, ph, pl, [&] {
+				if (I8 && more) {
+					put8(b ^ 1, 0);
+					get8(next, 1);
+				}
+			});
 			if (any)
 				add_half(row0, ph, pl);
 			if (I8 && more)
