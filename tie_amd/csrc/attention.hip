@@ -1165,7 +1165,8 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 // ---------------------------------------------------------------- join
 // A workgroup: JOIN_HEADS query heads of one token, HD / 4 lanes to a head: first
 // the parts' maxima and sums, a lane to a part, then their rows, 16 under way
-// at once.  Bound by the parts' bytes.
+// at once.  Bound by the parts' bytes and the chain of steps: 26 tokens of 64 heads
+// in 18 parts (16 MB) 8.9 us, of which 2 find the parts.
 constexpr int JOIN_HEADS = 8;
 template <int HD>
 __global__ __launch_bounds__(JOIN_HEADS *HD / 4) void attn_join_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, int units,

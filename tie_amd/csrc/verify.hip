@@ -12,10 +12,10 @@
 // draft was.
 //
 // Each node's outcome depends on its own rows and random numbers alone, so all
-// nodes are worked on at once, a workgroup to V_CHUNK logits, and the path is
-// read off at the end.  The last workgroup of a row forms the row's outcome, the
+// nodes are worked on at once, a workgroup to one or two V_CHUNK logits, and the
+// path is read off at the end.  The last workgroup of a row forms the row's outcome, the
 // last row of a sequence its path: one launch, and one more for each residual
-// sum that some row may need (rows that do not leave it at once).  Sums are in 64
+// sum that some row may need, for the rows that the path can still reach.  Sums are in 64
 // bits: the running sum crosses u M at the same token whatever the order of the
 // sum.
 #include "kv.h"
@@ -25,7 +25,6 @@ namespace tie {
 constexpr int V_CHUNK = 4096; // logits of a workgroup
 constexpr int V_THREADS = 256, V_E = V_CHUNK / V_THREADS;
 constexpr size_t V_AT_ONCE = 1024; // workgroups that run together: 4 on a CU
-constexpr int V_KIDS = VERIFY_KIDS;
 constexpr int V_PATH_LDS = 512; // nodes of a sequence whose outcomes the path's reader keeps in LDS
 
 // A row between its passes.
@@ -626,7 +625,11 @@ __device__ __forceinline__ void get_chunk(const float *row, int base, int n, flo
 }
 
 // The first launch: largest logit and sum of each chunk; a workgroup PER chunks,
-// whose logits are under way together.
+// whose logits are under way together.  57 rows of 151936 logits (35 MB): 23 us, of
+// which the sums are 15 (bound by the 64-bit exponentials and the loads in turn)
+// and the last rows' steps 8; one chunk each 30.6.  5 rows of 32000: 12 us, 4.5 to
+// the sums and then the chain of a row's steps (children, the next token's search,
+// the sequence's count, the path).
 template <int PER>
 __global__ __launch_bounds__(V_THREADS, 4) void verify_stats_kernel(VerifyArgs a, VerifyWork w)
 {
@@ -710,7 +713,8 @@ __global__ __launch_bounds__(V_THREADS, 4) void verify_stats_kernel(VerifyArgs a
 	}
 }
 
-// One more residual sum for the rows that wait for it.
+// One more residual sum for the rows that wait for it.  (Eight trees with draft
+// rows of 151936: 11 to 13 us, nearly all of it a row's chain of steps.)
 __global__ __launch_bounds__(V_THREADS, 4) void verify_residual_kernel(VerifyArgs a, VerifyWork w, int pass)
 {
 	__shared__ Shared sh;
