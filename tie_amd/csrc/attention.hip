@@ -128,6 +128,7 @@ struct Cut {
 	int full;  // so many tiles are not cut
 	int grain; // pages that are not cut
 	int least; // grains of a unit, at least
+	int alone; // so few grains of a tile are one unit
 	int whole; // tiles are not cut at all
 	int rows;  // query rows of a tile
 };
@@ -168,7 +169,7 @@ __device__ __forceinline__ int div_up(int a, int b)
 __device__ __forceinline__ int tile_parts(const Cut &cut, int pages, float rate)
 {
 	const int grains = div_up(pages, cut.grain), most = grains / cut.least, p = (int)((float)grains * rate + 0.5f);
-	return p < 2 || most < 2 ? 1 : p < most ? p : most;
+	return p < 2 || grains <= cut.alone ? 1 : p < most ? p : most;
 }
 
 __device__ __forceinline__ float part_rate(const KvSeqs &s, int kvh, int group, const Cut &cut, int tiles0, int pages0)
@@ -1274,9 +1275,12 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 	// one workgroup of 8 waves on a CU, or two of 4
 	h.cut.cap = h.few ? FEW_CAP : 512;
 	h.cut.full = h.few ? FEW_CAP : MANY_FULL;
-	// (few: a grain is a round of the waves)
+	// (few: a grain is a round of the waves; a second one costs as much as joining
+	// two parts: one f16 token over 300 rows of 8 kv heads of 64 7.8 us, in two parts
+	// 10.2, over 1000 10.7, in two parts of two rounds 11.6)
 	h.cut.grain = !h.few ? 1 : c.i8 ? FEW_WAVES : FEW_WAVES / 2;
-	h.cut.least = !h.few ? 2 : c.i8 ? 1 : 2;
+	h.cut.least = h.few ? 1 : 2;
+	h.cut.alone = h.few ? 2 : 3;
 	const size_t seqs = s.n_seqs < s.n_tokens ? s.n_seqs : s.n_tokens; // that have tokens, at most
 	const size_t tiles = (rows + seqs * (h.cut.rows - 1)) / h.cut.rows;
 	// as many tiles as fill the card are not cut: no parts, no join
