@@ -1263,9 +1263,12 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 	// too, int8 ones (half the bytes; codes are converted for every 16 rows) up to
 	// larger sizes.  int8: 5 tokens of 32 heads over 8000 rows 17 us (by the other
 	// kernel 26), 26 over 8000 26.5 (31), over 32000 61 (59), 16 sequences of 16
-	// over 8000 70 (64).  f16: 4 tokens over 8000 rows 19.6 (25.6), 8 over 1000 19.9
-	// (18.2), 8 sequences of 8 over 8000 39 (32).
-	const size_t most = c.i8 ? 256 : 64, units = c.i8 ? 448 : 64;
+	// over 8000 70 (64).  f16: 8 tokens over 1000 rows 16.7 (18.6), over 8000 20 (27),
+	// 16 over 8000 26 (31), 8 sequences of 8 over 8000 38 (31); with 8 kv heads of 64
+	// 26 over 2000 13 (16), over 8000 23.5 (23), but over 30000, which a die's cache
+	// does not hold, 60 (34): more than 64 f16 rows only where the page table, all
+	// that is known here of the lengths, ends at 10000.
+	const size_t most = c.i8 ? 256 : s.max_pages * PAGE <= 10240 ? 128 : 64, units = c.i8 ? 448 : 64;
 	h.few = rows <= (size_t)FEW_ROWS * s.n_seqs || (rows <= most * s.n_seqs && rows * c.kvh <= units * FEW_ROWS);
 	// many: 128 rows where such tiles fill the card (4096 tokens of 32 heads 240
 	// us, by 64 rows 257), or 64: as many units and half the parts' bytes, less
