@@ -134,7 +134,7 @@ def run_dense(torch, tie_amd, cfg, steps, warmup, n_copies, flags):
     # bracket the timed calls (one call is one kernel, or three on the
     # matrix cores: its average duration is the events' interval / steps;
     # events around every call would add their own gaps)
-    cs = torch.cuda.Stream()  # a stream of its own (handle 0 would mean the library's stream)
+    cs = torch.cuda.Stream()  # a stream of its own
 
     def step(s):
         mats[s % n_copies].mat_mat(X[s % n_copies], T, out, flags=flags, stream=cs.cuda_stream)

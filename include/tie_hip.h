@@ -154,6 +154,12 @@ void tie_hip_layer_destroy(tie_hip_layer *layer);
 /* Device bytes held by a layer. */
 size_t tie_hip_layer_bytes(const tie_hip_layer *layer);
 
+/* Every call on device pointers is enqueued on its `stream`: a hipStream_t,
+ * NULL for the library's stream (non-blocking: it is ordered with no other
+ * stream, the default one among them), or this for HIP's default stream,
+ * whose handle is 0. */
+#define TIE_HIP_STREAM_DEFAULT ((void *)1)
+
 /* MoE block on device pointers, enqueued on `stream` (a hipStream_t; NULL =
  * the library stream).  x_dev/out_dev are [T][d] F32; topk outputs are
  * optional [T][k].  Returns once enqueued; the caller synchronises.

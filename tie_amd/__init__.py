@@ -21,6 +21,7 @@ PAGE_ROWS = 64
 OK, EINVAL, EHIP, ENOMEM, ENOINIT = 0, -1, -2, -3, -4
 PATH_AUTO, PATH_EXACT, PATH_MFMA = 0, 1, 2
 ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
+DEFAULT_STREAM = 1  # TIE_HIP_STREAM_DEFAULT: HIP's default stream
 SILU_TABLE_SIZE = 8192
 
 # every symbol include/tie_hip.h declares
@@ -201,6 +202,12 @@ def _p(a):
     return a.ctypes.data
 
 
+def _s(stream):
+    """A stream's handle for the library.  None is the library's own stream;
+    torch's handle of the default stream, 0, would be that one too."""
+    return DEFAULT_STREAM if stream == 0 else stream
+
+
 _device = None  # the library's GPU
 
 
@@ -237,12 +244,12 @@ def host_expf(x):
 def stream_status(stream=None):
     """tie_hip_stream_status: raises TieError when a one-token forward on
     the stream had a wait between workgroups give up since the last check."""
-    check(lib().tie_hip_stream_status(stream))
+    check(lib().tie_hip_stream_status(_s(stream)))
 
 
 def stream_release(stream=None):
     """tie_hip_stream_release: free the workspace kept for the stream."""
-    check(lib().tie_hip_stream_release(stream))
+    check(lib().tie_hip_stream_release(_s(stream)))
 
 
 def debug_decode_give_up(n):
@@ -390,7 +397,7 @@ class Matrix:
         """out[t][r] = W[r] . x[t] on device pointers (dispatch_mat_mat);
         PATH_AUTO takes the matrix cores above the exact threshold where the
         matrix allows them, PATH_EXACT always TIE's row kernels."""
-        check(lib().tie_hip_mat_mat(self.handle, _p(x_dev), T, _p(out_dev), flags, stream))
+        check(lib().tie_hip_mat_mat(self.handle, _p(x_dev), T, _p(out_dev), flags, _s(stream)))
 
     def close(self):
         if self.handle:
@@ -435,14 +442,14 @@ class Layer:
     def forward(self, x_dev, T, k, out_dev, topk_idx_dev=None, topk_w_dev=None, flags=PATH_AUTO, stream=None):
         """Enqueue the block on device pointers (torch tensors or ints)."""
         check(lib().tie_hip_moe_forward(self.handle, _p(x_dev), T, k, _p(out_dev), _p(topk_idx_dev),
-                                        _p(topk_w_dev), flags, stream))
+                                        _p(topk_w_dev), flags, _s(stream)))
 
     def forward_noalloc(self, x_dev, T, k, out_dev, topk_idx_dev=None, topk_w_dev=None, flags=PATH_AUTO,
                         stream=None):
         """tie_hip_moe_forward_noalloc: forward with the library's static
         scratch array (no allocation; small T only)."""
         check(lib().tie_hip_moe_forward_noalloc(self.handle, _p(x_dev), T, k, _p(out_dev), _p(topk_idx_dev),
-                                                _p(topk_w_dev), flags, stream))
+                                                _p(topk_w_dev), flags, _s(stream)))
 
     def forward_residual(self, hidden_dev, ffn_norm_dev, eps, T, k, out_dev=None, topk_idx_dev=None,
                          topk_w_dev=None, flags=PATH_AUTO, stream=None):
@@ -450,7 +457,7 @@ class Layer:
         defaults to hidden: the in-place update)."""
         check(lib().tie_hip_moe_forward_residual(self.handle, _p(hidden_dev), _p(ffn_norm_dev), eps, T, k,
                                                  _p(hidden_dev if out_dev is None else out_dev), _p(topk_idx_dev),
-                                                 _p(topk_w_dev), flags, stream))
+                                                 _p(topk_w_dev), flags, _s(stream)))
 
     def close(self):
         if self.handle:
@@ -514,6 +521,22 @@ def _array(a, dtype, shape, what, device):
     return a.data_ptr()
 
 
+_raw_stream = None
+
+
+def _current(stream, device):
+    """The handle of `stream`; None: the stream that torch works on now, on which the tensors are made and used."""
+    if stream is None:
+        if device < 0:
+            return None  # (tensors of the CPU: the call is refused)
+        global _raw_stream
+        if _raw_stream is None:
+            from torch._C import _cuda_getCurrentRawStream
+            _raw_stream = _cuda_getCurrentRawStream  # (torch.cuda.current_stream makes an object for each call)
+        stream = _raw_stream(device)
+    return stream or DEFAULT_STREAM
+
+
 def _work(work, device):
     """Pointer and bytes of a call's scratch memory (None: the stream's own)."""
     if work is None:
@@ -545,7 +568,12 @@ class KVCache:
     """A paged cache in the caller's tensors (tie_hip_kv_cache): k [n_layers]
     [n_pages][kv_heads][64][head_dim] and v [n_layers][n_pages][kv_heads]
     [head_dim][64], float16, or int8 with float32 scales [n_layers][n_pages]
-    [kv_heads][64]."""
+    [kv_heads][64].
+
+    The calls go to `stream`, or, where that is None, to the stream that torch
+    works on when they are made, in order with the tensors' other uses.  (None
+    is the library's own stream for Layer and Matrix, whose buffers need not be
+    torch's: calls of both kinds in one program get one stream.)"""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         kind = {"torch.float16": F16, "torch.int8": I8}.get(str(k.dtype))
@@ -592,14 +620,14 @@ class KVCache:
         check(lib().tie_hip_kv_append(self.ref, layer, seqs.ref, pq, sq, pk, sk, pv, sv, heads,
                                       _array(q_norm, "float32", self.head_shape, "q_norm", dev),
                                       _array(k_norm, "float32", self.head_shape, "k_norm", dev), eps, theta,
-                                      _array(pos, "int32", (n,), "pos", dev), po, so, stream))
+                                      _array(pos, "int32", (n,), "pos", dev), po, so, _current(stream, dev)))
 
     def read(self, seqs, k_out, v_out, layer=0, n_layers=1, stream=None):
         """tie_hip_kv_read: rows of the cache as float32 [n_layers][n_tokens][kv_heads][head_dim]."""
         self._seqs(seqs)
         shape, dev = (n_layers, seqs.n_tokens, self.kv_heads, self.head_dim), self.device
         check(lib().tie_hip_kv_read(self.ref, layer, n_layers, seqs.ref, _array(k_out, "float32", shape, "k_out", dev),
-                                    _array(v_out, "float32", shape, "v_out", dev), stream))
+                                    _array(v_out, "float32", shape, "v_out", dev), _current(stream, dev)))
 
     def attention(self, layer, seqs, q, out, scale, mask=None, work=None, stream=None):
         """tie_hip_tree_attention; mask: int64 [n_tokens][words] (bit patterns), None: causal; work: a uint8 tensor."""
@@ -607,7 +635,7 @@ class KVCache:
         words, (pw, nw) = 0 if mask is None else mask.shape[1], _work(work, self.device)
         check(lib().tie_hip_tree_attention(self.ref, layer, seqs.ref, pq, sq, heads, scale,
                                            _array(mask, "int64", (seqs.n_tokens, words), "mask", self.device), words, po, so, pw,
-                                           nw, stream))
+                                           nw, _current(stream, self.device)))
 
     def attention_work_bytes(self, seqs, n_heads):
         return lib().tie_hip_tree_attention_work_bytes(self.ref, seqs.ref, n_heads)
@@ -618,7 +646,7 @@ class KVCache:
         dev = self.device
         check(lib().tie_hip_kv_keep(self.ref, seqs.ref, _array(path, "int32", (seqs.n_seqs, path.shape[1]), "path", dev),
                                     path.shape[1], _array(n_keep, "int32", (seqs.n_seqs,), "n_keep", dev),
-                                    _array(len_out, "int32", (seqs.n_seqs,), "len_out", dev), stream))
+                                    _array(len_out, "int32", (seqs.n_seqs,), "len_out", dev), _current(stream, dev)))
 
 
 def verify_tree_work_bytes(vocab, n_tokens, max_children, with_draft):
@@ -627,7 +655,8 @@ def verify_tree_work_bytes(vocab, n_tokens, max_children, with_draft):
 
 def verify_tree(logits, first, tokens, parent, u_accept, u_sample, path, n_keep, next_token, temperature=1.0, draft=None,
                 max_children=1, work=None, stream=None):
-    """tie_hip_verify_tree: the accepted path [n_seqs][max_path], its length and the next token of each sequence."""
+    """tie_hip_verify_tree: the accepted path [n_seqs][max_path], its length and the next token of each sequence; stream
+    as for KVCache."""
     n, n_seqs, dev = tokens.shape[0], n_keep.shape[0], logits.get_device()
     if dev != _device:
         _on_device(dev, dev, "logits")
@@ -640,4 +669,5 @@ def verify_tree(logits, first, tokens, parent, u_accept, u_sample, path, n_keep,
                                     _array(u_sample, "float32", (n,), "u_sample", dev), temperature, max_children, path.shape[1],
                                     _array(path, "int32", (n_seqs, path.shape[1]), "path", dev),
                                     _array(n_keep, "int32", (n_seqs,), "n_keep", dev),
-                                    _array(next_token, "int32", (n_seqs,), "next_token", dev), pw, nw, stream))
+                                    _array(next_token, "int32", (n_seqs,), "next_token", dev), pw, nw,
+                                    _current(stream, dev)))

@@ -238,6 +238,13 @@ static int check_shape(int d, int F, int E)
 	return TIE_HIP_OK;
 }
 
+// The stream that a call names: NULL is the library's own, and HIP's default
+// stream, whose handle is 0 as well, has a name of its own.
+static hipStream_t stream_of(void *stream)
+{
+	return !stream ? g.stream : stream == TIE_HIP_STREAM_DEFAULT ? (hipStream_t) nullptr : (hipStream_t)stream;
+}
+
 static int ensure_init()
 {
 	if (g.device < 0)
@@ -862,7 +869,7 @@ extern "C" int tie_hip_moe_forward(tie_hip_layer *layer, const float *x_dev, int
 	int rc = ensure_init();
 	if (rc)
 		return rc;
-	hipStream_t s = stream ? (hipStream_t)stream : g.stream;
+	hipStream_t s = stream_of(stream);
 	return forward(layer, x_dev, T, k, out_dev, topk_idx_dev, topk_w_dev, flags, s);
 }
 
@@ -890,7 +897,7 @@ extern "C" int tie_hip_moe_forward_noalloc(tie_hip_layer *layer, const float *x_
 				 T, k, need, SCRATCH_BYTES);
 	Workspace ws;
 	carve_workspace(g_scratch, P, L.F, L.d, L.E, &ws, false);
-	hipStream_t s = stream ? (hipStream_t)stream : g.stream;
+	hipStream_t s = stream_of(stream);
 	return forward(layer, x_dev, T, k, out_dev, topk_idx_dev, topk_w_dev, flags, s, nullptr, &ws);
 }
 
@@ -1249,7 +1256,7 @@ extern "C" int tie_hip_mat_mat(tie_hip_matrix *m, const float *x_dev, int T, flo
 		return TIE_HIP_OK;
 	if (!x_dev || !out_dev)
 		return set_error(TIE_HIP_EINVAL, "null x/out");
-	hipStream_t s = stream ? (hipStream_t)stream : g.stream;
+	hipStream_t s = stream_of(stream);
 	// the matrix cores only when asked for (Q4_K / Q6_K, rows a multiple of
 	// 256): TIE_HIP_PATH_AUTO keeps TIE's exact row kernels at every T, so a
 	// caller of dispatch_mat_mat gets TIE's bits unless it opts in
@@ -1289,7 +1296,7 @@ extern "C" int tie_hip_moe_forward_residual(tie_hip_layer *layer, const float *h
 	int rc = ensure_init();
 	if (rc)
 		return rc;
-	hipStream_t s = stream ? (hipStream_t)stream : g.stream;
+	hipStream_t s = stream_of(stream);
 	return forward_residual(layer, hidden_dev, ffn_norm_dev, eps, T, k, out_dev, topk_idx_dev, topk_w_dev, flags,
 				s);
 }
@@ -1496,7 +1503,7 @@ extern "C" int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const
 	a.n_heads = n_heads;
 	a.eps = eps;
 	a.log2_theta = log2((double)theta);
-	hipStream_t st = stream ? (hipStream_t)stream : g.stream;
+	hipStream_t st = stream_of(stream);
 	prof_begin("kv_append", st);
 	const hipError_t e = launch_kv_append(l, s, a, st);
 	prof_end(st);
@@ -1522,7 +1529,7 @@ extern "C" int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_l
 	TIE_TRY(ensure_init());
 	if (none)
 		return TIE_HIP_OK;
-	hipStream_t st = stream ? (hipStream_t)stream : g.stream;
+	hipStream_t st = stream_of(stream);
 	prof_begin("kv_read", st);
 	const hipError_t e = launch_kv_read(l, n_layers, s, k_out, v_out, st);
 	prof_end(st);
@@ -1551,7 +1558,7 @@ extern "C" int tie_hip_kv_keep(const tie_hip_kv_cache *cache, const tie_hip_kv_s
 	TIE_TRY(ensure_init());
 	if (s.n_seqs == 0)
 		return TIE_HIP_OK;
-	hipStream_t st = stream ? (hipStream_t)stream : g.stream;
+	hipStream_t st = stream_of(stream);
 	prof_begin("kv_keep", st);
 	const hipError_t e = launch_kv_keep(l, cache->n_layers, s, path, max_path, n_keep, len_out, st);
 	prof_end(st);
@@ -1610,7 +1617,7 @@ extern "C" int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, 
 	a.mask_words = mask ? mask_words : 0;
 	a.n_heads = n_heads;
 	a.scale = scale;
-	hipStream_t st = stream ? (hipStream_t)stream : g.stream;
+	hipStream_t st = stream_of(stream);
 	void *mem = nullptr;
 	TIE_TRY(aux_scratch(st, work, work_bytes, attention_work_bytes(l, s, a), &mem));
 	prof_begin("attention", st);
@@ -1701,7 +1708,7 @@ extern "C" int tie_hip_verify_tree(const float *logits, size_t logits_stride, co
 	a.path = path;
 	a.n_keep = n_keep;
 	a.next = next;
-	hipStream_t st = stream ? (hipStream_t)stream : g.stream;
+	hipStream_t st = stream_of(stream);
 	void *mem = nullptr;
 	TIE_TRY(aux_scratch(st, work, work_bytes, verify_work_bytes(a, draft != nullptr), &mem));
 	prof_begin("verify", st);
@@ -1729,7 +1736,7 @@ extern "C" int tie_hip_stream_release(void *stream)
 	int rc = ensure_init();
 	if (rc)
 		return rc;
-	auto it = g.ws.find(stream ? (hipStream_t)stream : g.stream);
+	auto it = g.ws.find(stream_of(stream));
 	if (it == g.ws.end())
 		return TIE_HIP_OK;
 	HIP_TRY(hipDeviceSynchronize());
@@ -1750,7 +1757,7 @@ extern "C" int tie_hip_stream_status(void *stream)
 	int rc = ensure_init();
 	if (rc)
 		return rc;
-	return take_stream_status(stream ? (hipStream_t)stream : g.stream);
+	return take_stream_status(stream_of(stream));
 }
 
 extern "C" void tie_hip_debug_decode_give_up(int n)
