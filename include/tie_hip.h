@@ -246,7 +246,9 @@ int tie_hip_mat_mat(tie_hip_matrix *m, const float *x_dev, int T, float *out_dev
  * rows (tie_hip_kv_keep).  Everything is on device pointers, enqueued on
  * `stream` (NULL: the library stream) and captures into HIP graphs.  No call
  * here reproduces TIE's arithmetic bit for bit: they are held to 64-bit
- * results (F32 outputs to about 1e-6 relative).
+ * results (F32 outputs to about 1e-6 relative; an element of the attention's to
+ * that of sum_j p_j max_i |v_ji|, the rows' largest magnitudes by their weights;
+ * over f16 rows, weights below 2^-36 of the largest may be taken for 0).
  *
  * The caller owns the cache's memory, in pages of TIE_HIP_PAGE_ROWS rows (a
  * row: one token) that the layers share the numbering of:

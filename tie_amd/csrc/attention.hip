@@ -19,7 +19,8 @@
 // straight into operands.
 //
 // The maximum m is a reference only: it moves when some weight would pass
-// 2^MOVE, so most steps need no exchange between lanes and leave O alone.
+// 2^MOVE, so most steps need no exchange between lanes and leave O alone.  (int8:
+// when some weight times its row's V scale would pass f16; see weigh8.)
 #include <type_traits>
 
 #include "kv.h"
@@ -33,6 +34,9 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float MOVE = 3.0f;       // log2 of the largest weight
 constexpr float P_LOG2 = 12.0f;    // weights times 2^12 stay below the f16 limit, their second parts above the subnormals
+constexpr float V_UP = 0x1p12f;    // int8: V scales times this (those of a trained layer's values are then about 1)
+constexpr float SCALE_LOW = -90.0f; // log2 of the smallest of them that the weights' reference goes by
+constexpr float SUM_MOST = 0x1p107f; // of a step's weights before their V scales: 16 rows of SCALE_LOW and 2^(P_LOG2 + 1)
 
 // four int8 codes to f16: 1024 + (code + 128) is the f16 0x6400 | byte, from
 // which 1152 is taken exactly
@@ -340,32 +344,40 @@ __device__ __forceinline__ void split_query(const AttnArgs &a, int node, float (
 		}
 }
 
-// The running state of 16 query rows: a lane's query's maximum, the lane's
-// share of its sum, and O^T.
+// The running state of 16 query rows: a lane's query's reference (log2 of what
+// the lane's share of the sum, and O^T, are multiples of).
 template <int HD>
 struct Rows {
 	float mx = -__builtin_inff(), sum = 0.0f;
 	f4 o[HD / 16];
 };
 
-// From the products sc of 16 KT cache rows to the weights' two f16 parts for
-// the second product; the state's reference and sum, and O where the reference
-// moved.  whole: every query of the wave sees all the rows; else bits: which of
-// the lane's 4 KT rows its query sees (the weights of the others are 0).  int8:
-// ks and vs are the K and V scale of the lane's row (lane 4 t + i of 16: row 4 t
-// + i of the group's), vs finite unless whole, and none above 2^vlog, which
-// the weights are divided by.  Weights and sum carry 2^(P_LOG2 - vlog), by way
-// of the exponent.
-template <int HD, bool I8, int KT>
-__device__ __forceinline__ void weigh(Rows<HD> &r, const f4 (&sc)[KT], float ks, float vs, float vlog, float qs, bool whole,
-				      uint32_t bits, h8 (&ph)[KT / 2], h8 (&pl)[KT / 2])
+// The weights w in the two f16 parts of the second product's operand.
+template <int KT> __device__ __forceinline__ void split_weights(const float (&w)[4 * KT], h8 (&ph)[KT / 2], h8 (&pl)[KT / 2])
+{
+#pragma unroll
+	for (int e = 0; e < 4 * KT; e += 2) {
+		h2 hi, lo;
+		split2(w[e], w[e + 1], hi, lo);
+		ph[e / 8][e % 8] = hi.x, ph[e / 8][e % 8 + 1] = hi.y;
+		pl[e / 8][e % 8] = lo.x, pl[e / 8][e % 8 + 1] = lo.y;
+	}
+}
+
+// f16 rows: from the products sc of 16 KT cache rows to the weights' two f16
+// parts for the second product; the state's reference and sum, and O where the
+// reference moved.  whole: every query of the wave sees all the rows; else bits:
+// which of the lane's 4 KT rows its query sees (the weights of the others are
+// 0).  Weights, O and sum carry 2^P_LOG2, by way of the exponent, until
+// finish().
+template <int HD, int KT>
+__device__ __forceinline__ void weigh(Rows<HD> &r, const f4 (&sc)[KT], float qs, bool whole, uint32_t bits, h8 (&ph)[KT / 2],
+				      h8 (&pl)[KT / 2])
 {
 	float w[4 * KT];
 #pragma unroll
 	for (int e = 0; e < 4 * KT; e++)
 		w[e] = sc[e / 4][e % 4];
-	if (I8)
-		times_rows<KT>(w, ks);
 	if (!whole)
 #pragma unroll
 		for (int e = 0; e < 4 * KT; e++)
@@ -385,21 +397,120 @@ __device__ __forceinline__ void weigh(Rows<HD> &r, const f4 (&sc)[KT], float ks,
 		for (int m = 0; m < HD / 16; m++)
 			r.o[m] *= f;
 	}
-	const float base = (r.mx == -__builtin_inff() ? 0.0f : r.mx) + (I8 ? vlog - P_LOG2 : -P_LOG2);
+	const float base = (r.mx == -__builtin_inff() ? 0.0f : r.mx) - P_LOG2;
 #pragma unroll
 	for (int e = 0; e < 4 * KT; e++) {
 		w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[e], qs, -base));
 		r.sum += w[e];
 	}
-	if (I8)
+	split_weights<KT>(w, ph, pl);
+}
+
+// int8 rows: the same.  ks and vs are the K and V scale of the lane's row (lane
+// 4 t + i of 16: row 4 t + i of the group's), vs times `up` and finite unless
+// whole.  The second product's weights are y = 2^(score - mx) vs, and it is y that
+// has to stay in f16's range, though V scales may lie any number of binades apart:
+// so the reference is not the largest score but the largest y of the rows that the
+// query sees (held at 2^P_LOG2 when it moves, and moved past 2^15).  A row that a
+// query does not see, or that weighs nothing, has no part in it, whatever its
+// scale.  Rows of scales below 2^SCALE_LOW count as that for the reference alone,
+// so that the sum stays in F32's range.  The reference is a whole number: what
+// moves with it stays exact.
+//
+// The weights are formed with the reference as it stands, and again where it turns
+// out to have to move (a few times in a pass): no maximum of the scores is
+// needed in the common path.
+template <int HD, int KT>
+__device__ __forceinline__ void weigh8(Rows<HD> &r, const f4 (&sc)[KT], float ks, float vs, float qs, bool whole, uint32_t bits,
+				       h8 (&ph)[KT / 2], h8 (&pl)[KT / 2])
+{
+	float s[4 * KT], w[4 * KT], add, most;
+#pragma unroll
+	for (int e = 0; e < 4 * KT; e++)
+		s[e] = sc[e / 4][e % 4];
+	times_rows<KT>(s, ks);
+	if (!whole)
+#pragma unroll
+		for (int e = 0; e < 4 * KT; e++)
+			if (!(bits >> e & 1))
+				s[e] = -__builtin_inff();
+	auto weights = [&](float base) {
+		add = most = 0.0f;
+#pragma unroll
+		for (int e = 0; e < 4 * KT; e++) {
+			w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], qs, -base));
+			add += w[e];
+		}
 		times_rows<KT>(w, vs);
 #pragma unroll
-	for (int e = 0; e < 4 * KT; e += 2) {
-		h2 hi, lo;
-		split2(w[e], w[e + 1], hi, lo);
-		ph[e / 8][e % 8] = hi.x, ph[e / 8][e % 8 + 1] = hi.y;
-		pl[e / 8][e % 8] = lo.x, pl[e / 8][e % 8 + 1] = lo.y;
+		for (int e = 0; e < 4 * KT; e++)
+			most = __builtin_fmaxf(most, __builtin_fabsf(w[e]));
+	};
+	weights(r.mx); // (before the first row: not a number, or infinite)
+	if (__any(!(add <= SUM_MOST) || most > 32768.0f)) {
+		// log2 of y without the reference
+		float y[4 * KT], top = -__builtin_inff();
+#pragma unroll
+		for (int e = 0; e < 4 * KT; e++)
+			y[e] = 1.0f;
+		times_rows<KT>(y, __builtin_fminf(__builtin_fmaxf(__builtin_amdgcn_logf(__builtin_fabsf(vs)), SCALE_LOW), 100.0f));
+#pragma unroll
+		for (int e = 0; e < 4 * KT; e++)
+			top = __builtin_fmaxf(top, __builtin_fmaf(s[e], qs, y[e]));
+		top = __builtin_fmaxf(r.mx, __builtin_ceilf(max_g(top)) - P_LOG2);
+		const float f = __builtin_ldexpf(1.0f, (int)__builtin_fmaxf(r.mx - top, -200.0f));
+		r.mx = top;
+		r.sum *= f;
+#pragma unroll
+		for (int m = 0; m < HD / 16; m++)
+			r.o[m] *= f;
+		weights(top == -__builtin_inff() ? 0.0f : top);
 	}
+	r.sum += add;
+	split_weights<KT>(w, ph, pl);
+}
+
+// The V scale of a lane's row as weigh8() takes it.  Where one is above 2^60 the
+// factor `up` (the same in all lanes) goes down by 2^64, once, and the references
+// with it (by less where the sum would leave F32's range: then all values so far
+// are below 2^SCALE_LOW of the present one).
+template <int HD, int NT> __device__ __forceinline__ float scale_up(float vs, float &up, Rows<HD> (&r)[NT])
+{
+	if (up == V_UP && __any(__builtin_fabsf(vs) > 0x1p60f / V_UP)) {
+		up = V_UP * 0x1p-64f;
+#pragma unroll
+		for (int t = 0; t < NT; t++) {
+			const int d = min(max(104 + 127 - (int)(__float_as_uint(max_g(r[t].sum)) >> 23 & 0xff), 0), 64);
+			r[t].mx -= (float)d;
+			r[t].sum = __builtin_ldexpf(r[t].sum, d);
+#pragma unroll
+			for (int m = 0; m < HD / 16; m++)
+				r[t].o[m] *= __builtin_ldexpf(1.0f, d - 64);
+		}
+	}
+	return vs * up;
+}
+
+// At the end: the sum over a query's four lanes (returned), and what O is to be
+// multiplied by.  int8: O and the sum as multiples of another 2^mx, so that the
+// sum is about 1.
+template <int HD, bool I8> __device__ __forceinline__ float finish(Rows<HD> &r, float up, float &back)
+{
+	const float total = sum_g(r.sum);
+	if (!I8) {
+		back = 1.0f / (1 << (int)P_LOG2);
+		return total * back;
+	}
+	back = 1.0f;
+	const bool any = total > 0.0f && total < __builtin_inff();
+	const int k = any ? (int)(__float_as_uint(total) >> 23) - 127 : 0, k_up = (int)(__float_as_uint(up) >> 23) - 127;
+	r.mx = any ? r.mx + (float)k : r.mx;
+#pragma unroll
+	for (int m = 0; m < HD / 16; m++)
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+			r.o[m][i] = __builtin_ldexpf(r.o[m][i], -k - k_up);
+	return __builtin_ldexpf(total, -k);
 }
 
 // int8 rows of which some queries do not see some, or that hold nothing (!
@@ -411,29 +522,6 @@ __device__ __forceinline__ void guard_scales(float &ks, float &vs, bool there)
 	if (!(__builtin_fabsf(vs) < __builtin_inff()) || !there) {
 		vs = 0.0f;
 		ks = __builtin_nanf("");
-	}
-}
-
-// int8: 2^vlog is a power of two above all V scales so far; it grows seldom, and
-// O and the sum shrink with it.  vs: the scale of the lane's row.
-template <int HD, int NT> __device__ __forceinline__ void move_vlog(float vs, float &vlog, Rows<HD> (&r)[NT])
-{
-	if (__any(vs > __builtin_amdgcn_exp2f(vlog))) {
-		float top = vs;
-#pragma unroll
-		for (int m = 1; m < 64; m <<= 1)
-			top = __builtin_fmaxf(top, __shfl_xor(top, m));
-		// (the exponent of a finite value, one above)
-		const float to = (float)((int)(__float_as_uint(top) >> 23 & 0xff) - 126);
-		const float f = __builtin_amdgcn_exp2f(vlog - to);
-		vlog = to;
-#pragma unroll
-		for (int t = 0; t < NT; t++) {
-			r[t].sum *= f;
-#pragma unroll
-			for (int m = 0; m < HD / 16; m++)
-				r[t].o[m] *= f;
-		}
 	}
 }
 
@@ -592,7 +680,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 #pragma unroll
 	for (int m = 0; m < MT; m++)
 		r[0].o[m] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-	float vlog = -100.0f;
+	float up = V_UP;
 
 	for (int step = wave; step < steps; step += WK) {
 		const int start = (p0 + step / SP) * PAGE, row0 = step % SP * 32, end = u.len + u.n - start - row0;
@@ -622,13 +710,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 		float kk = ks;
 		if (more)
 			get_k(next, step + WK);
+		h8 ph[KT / 2], pl[KT / 2];
 		if (I8) {
 			if (!whole)
 				guard_scales(kk, vs, lane < end);
-			move_vlog<HD, 1>(vs, vlog, r);
+			weigh8<HD, KT>(r[0], sc, kk, scale_up<HD, 1>(vs, up, r), qs, whole, (uint32_t)(vis >> (4 * KT * g)), ph, pl);
+		} else {
+			weigh<HD, KT>(r[0], sc, qs, whole, (uint32_t)(vis >> (4 * KT * g)), ph, pl);
 		}
-		h8 ph[KT / 2], pl[KT / 2];
-		weigh<HD, I8, KT>(r[0], sc, kk, vs, vlog, qs, whole, (uint32_t)(vis >> (4 * KT * g)), ph, pl);
 #pragma unroll
 		for (int m = 0; m < MT; m++) {
 			if constexpr (I8) {
@@ -652,12 +741,12 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 			get_v(next, step + WK);
 		at = next;
 	}
-	const float back = __builtin_amdgcn_exp2f(I8 ? vlog - P_LOG2 : -P_LOG2);
+	float back;
+	const float total = finish<HD, I8>(r[0], up, back);
 
 	// join the waves: each puts its rows into LDS ([wave][row][HD + 4])
 	constexpr int LR = part_row(HD);
 	float *mine = lds + ((size_t)wave * R + n16) * LR;
-	const float total = sum_g(r[0].sum) * back;
 #pragma unroll
 	for (int m = 0; m < MT; m++)
 		*reinterpret_cast<f4 *>(mine + m * 16 + 4 * g) = r[0].o[m] * back;
@@ -935,7 +1024,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 		for (int m = 0; m < MT; m++)
 			r[t].o[m] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 	}
-	float vlog = -100.0f;
+	float up = V_UP;
 	if (I8) {
 		put8(0, 1);
 #pragma unroll
@@ -1044,11 +1133,14 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 				vs = lsc[b][1][row];
 				if (!whole)
 					guard_scales(ks, vs, row < end);
-				move_vlog<HD, NT>(vs, vlog, r);
+				vs = scale_up<HD, NT>(vs, up, r);
 			}
 #pragma unroll
 			for (int t = 0; t < NT; t++)
-				weigh<HD, I8, KT>(r[t], sc[t], ks, vs, vlog, qs[t], whole, seen[t] >> (8 * g), ph[t], pl[t]);
+				if (I8)
+					weigh8<HD, KT>(r[t], sc[t], ks, vs, qs[t], whole, seen[t] >> (8 * g), ph[t], pl[t]);
+				else
+					weigh<HD, KT>(r[t], sc[t], qs[t], whole, seen[t] >> (8 * g), ph[t], pl[t]);
 			return true;
 		};
 		auto add_half = [&](int row0, const h8 (&ph)[NT][1], const h8 (&pl)[NT][1]) {
@@ -1096,10 +1188,10 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 		__syncthreads();
 		at = next;
 	}
-	float back = __builtin_amdgcn_exp2f(I8 ? vlog - P_LOG2 : -P_LOG2), total[NT];
+	float back, total[NT];
 #pragma unroll
 	for (int t = 0; t < NT; t++)
-		total[t] = sum_g(r[t].sum) * back;
+		total[t] = finish<HD, I8>(r[t], up, back);
 	if constexpr (RG < MANY_WAVES) {
 		// the waves of the pages' second halves hand their rows to the others:
 		// O ([wave][t][m][lane], in K's buffers) and the maxima and sums
