@@ -321,11 +321,14 @@ int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_layers, cons
  *   work work_bytes of device memory, 16-byte aligned, at least
  *        tie_hip_tree_attention_work_bytes, filled with zeros before the first
  *        call that gets it and after anything else has written to it (calls
- *        here leave it fit for the next); NULL: the stream's workspace, which
- *        all calls on the stream share and which grows as needed, but not
- *        during HIP graph capture (run the largest call once before, or pass
- *        memory).  Calls and graphs that may run at the same time on different
- *        streams need memory of their own.
+ *        here leave it fit for the next); what is enough for a call is enough
+ *        for every one of the same heads and cache type with no more tokens,
+ *        sequences and columns of the page table.  NULL: the stream's
+ *        workspace, which all calls on the stream share and which grows as
+ *        needed, but not during HIP graph capture (run the largest call once
+ *        before, on the stream that captures, or pass memory).  Calls and
+ *        graphs that may run at the same time on different streams need memory
+ *        of their own.
  * Scores are held in F32; past 2^24 in magnitude their rounding is larger than
  * what a softmax tells apart, and a row's result means nothing.
  * A row's result is the same whatever else the call holds only up to F32
@@ -366,7 +369,8 @@ int tie_hip_kv_keep(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, 
  *   path   [n_seqs][max_path] accepted nodes, the root first; -1 behind them
  *   n_keep [n_seqs] how many; next [n_seqs] (0 and -1 for a sequence of no rows)
  * All sums in 64 bits.  No output may share memory with an input.  work as for
- * tie_hip_tree_attention. */
+ * tie_hip_tree_attention (the same memory will do for both; what is enough for a
+ * call is enough for every one of no more tokens and logits). */
 size_t tie_hip_verify_tree_work_bytes(int vocab, int n_tokens, int max_children, int with_draft);
 int tie_hip_verify_tree(const float *logits, size_t logits_stride, const float *draft, size_t draft_stride, int vocab,
 			int n_seqs, int n_tokens, const int32_t *first, const int32_t *tokens, const int32_t *parent,

@@ -1338,7 +1338,7 @@ __global__ __launch_bounds__(JOIN_HEADS *HD / 4) void attn_join_kernel(KvLayer c
 
 // ---------------------------------------------------------------- launch
 // a tile for every CU, and none is cut (600 tokens over 1100 rows, 300 tiles, 54 us; cut in two 68)
-constexpr int MANY_FULL = 256;
+constexpr int MANY_FULL = 256, MANY_CAP = 512;
 
 struct Shape {
 	bool few;
@@ -1346,10 +1346,9 @@ struct Shape {
 	size_t units; // at most
 };
 
-static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
+// Whether `rows` query rows (of one kv head) of n_seqs sequences go to the kernel of few rows.
+static bool few_of(const KvLayer &c, int max_pages, size_t rows, size_t n_seqs)
 {
-	const size_t group = a.n_heads / c.kvh, rows = (size_t)s.n_tokens * group;
-	Shape h;
 	// The kernel of few rows reads a page again for each 16 of them, but its parts
 	// are joined in the same launch and a wave waits for none: small trees take it
 	// too, int8 ones (half the bytes; codes are converted for every 16 rows) up to
@@ -1360,15 +1359,22 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 	// 26 over 2000 13 (16), over 8000 23.5 (23), but over 30000, which a die's cache
 	// does not hold, 60 (34): more than 64 f16 rows only where the page table, all
 	// that is known here of the lengths, ends at 10000.
-	const size_t most = c.i8 ? 256 : s.max_pages * PAGE <= 10240 ? 128 : 64, units = c.i8 ? 448 : 64;
-	h.few = rows <= (size_t)FEW_ROWS * s.n_seqs || (rows <= most * s.n_seqs && rows * c.kvh <= units * FEW_ROWS);
+	const size_t most = c.i8 ? 256 : max_pages * PAGE <= 10240 ? 128 : 64, units = c.i8 ? 448 : 64;
+	return rows <= FEW_ROWS * n_seqs || (rows <= most * n_seqs && rows * c.kvh <= units * FEW_ROWS);
+}
+
+static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
+{
+	const size_t group = a.n_heads / c.kvh, rows = (size_t)s.n_tokens * group;
+	Shape h;
+	h.few = few_of(c, s.max_pages, rows, s.n_seqs);
 	// many: 128 rows where such tiles fill the card (4096 tokens of 32 heads 240
 	// us, by 64 rows 257), or 64: as many units and half the parts' bytes, less
 	// left of tiles that a mask or a sequence's end cuts (1000 tokens over 2000
 	// rows 55 us, by 128 rows 89)
 	h.cut.rows = h.few ? FEW_ROWS : rows * c.kvh < (size_t)MANY_FULL * 128 ? 64 : 128;
 	// one workgroup of 8 waves on a CU, or two of 4
-	h.cut.cap = h.few ? FEW_CAP : 512;
+	h.cut.cap = h.few ? FEW_CAP : MANY_CAP;
 	h.cut.full = h.few ? FEW_CAP : MANY_FULL;
 	// (few: a grain is a round of the waves; a second one costs as much as joining
 	// two parts: one f16 token over 300 rows of 8 kv heads of 64 7.8 us, in two parts
@@ -1388,10 +1394,34 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 	return h;
 }
 
+// Enough for this call and for every one of the same heads and type with no more
+// tokens, sequences and columns of the page table.  (Calls whose tiles fill the
+// card have no parts, smaller ones do: memory for a prompt's chunk is memory for
+// the tokens decoded behind it.)
 size_t attention_work_bytes(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 {
-	const Shape h = attn_shape(c, s, a);
-	return WORK_COUNTERS * sizeof(int) + (h.cut.whole ? 0 : h.units * h.cut.rows * part_row(c.hd) * sizeof(float));
+	const size_t group = a.n_heads / c.kvh, rows = (size_t)s.n_tokens * group;
+	const size_t seqs = s.n_seqs < s.n_tokens ? s.n_seqs : s.n_tokens;
+	// rows of the largest such call whose tiles are cut, 0: there is none
+	auto most_rows = [&](size_t tile, size_t full) {
+		const size_t below = tile * ((full + c.kvh - 1) / c.kvh) - 1;
+		return (rows < below ? rows : below) / group * group;
+	};
+	auto values = [&](size_t r, size_t n, size_t tile, size_t cap) {
+		n = n < r / group ? n : r / group;
+		return r == 0 ? 0 : (cap + c.kvh + (r + n * (tile - 1)) / tile * c.kvh) * tile * part_row(c.hd);
+	};
+	size_t most = values(most_rows(FEW_ROWS, FEW_CAP), seqs, FEW_ROWS, FEW_CAP);
+	for (size_t tile = 64; tile <= 128; tile *= 2) {
+		const size_t r = most_rows(tile, MANY_FULL);
+		// (one sequence's rows are the first that this kernel takes, and it takes
+		// more than FEW_ROWS for each sequence)
+		if (few_of(c, s.max_pages, r, 1) || (tile == 128 && r * c.kvh < (size_t)MANY_FULL * 128))
+			continue;
+		const size_t by_rows = (r - 1) / FEW_ROWS, v = values(r, seqs < by_rows ? seqs : by_rows, tile, MANY_CAP);
+		most = most > v ? most : v;
+	}
+	return WORK_COUNTERS * sizeof(int) + most * sizeof(float);
 }
 
 template <int HD, bool I8>
