@@ -296,7 +296,8 @@ typedef struct tie_hip_kv_seqs {
  *             F32 [head_dim] (NULL: none)
  *   rotation  the pair (x[i], x[i + head_dim / 2]) by pos * theta^(-2 i /
  *             head_dim); pos [n_tokens] (a tree's nodes at one depth share a
- *             position), NULL: the token's cache row
+ *             position), NULL: the token's cache row (a query without one, as
+ *             its sequence's length is none, is NaN)
  * in 64 bits, rounded once.  The queries go to q_out (which may be q, with the
  * same stride, or other columns of the same matrix), keys and values to the
  * cache. */

@@ -1,0 +1,85 @@
+"""What the device arrays say wrong (lengths, ranges of rows, pages, paths): the
+cache's every byte, and each row of the outputs."""
+import numpy as np
+import pytest
+
+import kv_ref
+import tie_amd
+from test_gpu_kv import EPS, cuda, device, done, same  # noqa: F401 (device: the module's fixture)
+
+pytestmark = pytest.mark.gpu
+
+H, KVH, HD = 4, 2, 64
+KINDS = pytest.mark.parametrize("kind", ["f16", "i8"])
+
+
+class Call:
+    """Four sequences of two tokens behind ten rows each, and the call's buffers."""
+
+    def __init__(self, kind, seed, lens=(10, 10, 10, 10), counts=(2, 2, 2, 2), rows=8):
+        self.rng = np.random.default_rng(seed)
+        self.c = kv_ref.Cache(self.rng, kind, KVH, HD, lens, counts, layers=2)
+        self.kind, self.rows, self.table, self.lens = kind, rows, self.c.table.copy(), np.array(lens, np.int32)
+        self.first = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        self.x = self.rng.standard_normal((rows, (H + 2 * KVH) * HD)).astype(np.float32)
+        self.kv = self.c.gpu()
+
+    def seqs(self):
+        return tie_amd.KVSeqs(cuda(self.table), cuda(self.lens), cuda(self.first), self.rows)
+
+    def append(self, pos=None):
+        """The queries; layer 1."""
+        import torch
+        xd = cuda(self.x)
+        out = torch.full((self.rows, H, HD), -7.0, device="cuda")
+        self.kv.append(1, self.seqs(), xd[:, :H * HD], xd[:, H * HD:(H + KVH) * HD], xd[:, (H + KVH) * HD:], out,
+                       None if pos is None else cuda(pos))
+        return done(out)[0]
+
+    def read(self):
+        import torch
+        k, v = (torch.full((2, self.rows, KVH, HD), -7.0, device="cuda") for _ in range(2))
+        self.kv.read(self.seqs(), k, v, n_layers=2)
+        return done(k, v)
+
+    def written(self, b, t0, t1, first_row, pos):
+        """Rows t0 .. t1 - 1 go to sequence b's cache rows from `first_row` on."""
+        k = kv_ref.norm_rotate(self.x[t0:t1].reshape(t1 - t0, -1, HD)[:, H:H + KVH], None, pos, EPS, 1e6).astype(np.float32)
+        self.c.set_rows(1, b, first_row, k, self.x[t0:t1, (H + KVH) * HD:].reshape(t1 - t0, KVH, HD))
+
+    def query(self, t0, t1, pos):
+        return kv_ref.norm_rotate(self.x[t0:t1, :H * HD].reshape(t1 - t0, H, HD), None, pos, EPS, 1e6)
+
+    def check_cache(self, what=""):
+        for name, got, want in zip(("k", "v", "k_scale", "v_scale"), self.c.back(), (self.c.k, self.c.v, self.c.ks, self.c.vs)):
+            if want is not None:
+                same(got.view(np.uint8) if got.dtype != np.float32 else got, want.view(np.uint8) if got.dtype != np.float32 else want,
+                     (name, what))
+
+
+def near(got, want):
+    np.testing.assert_allclose(got, want, rtol=2.0 ** -23, atol=1e-8)
+
+
+@KINDS
+@pytest.mark.parametrize("bad", [-5, -2 ** 31, 63, 64, 2 ** 31 - 1])
+def test_append_of_a_length_that_is_none(kind, bad):
+    """Without positions the queries' rotation goes by the length: NaN, for that
+    sequence.  With positions they are what they are.  Nothing is written for
+    it either way, and the other sequences are served."""
+    for pos in (None, np.array([3, 9, 4, 4, 1000, 0, 77, 8], np.int32)):
+        m = Call(kind, 5)
+        m.lens[1] = bad
+        q = m.append(pos)
+        for b in range(4):
+            t = slice(2 * b, 2 * b + 2)
+            if b == 1:
+                if pos is None:
+                    assert np.isnan(q[t]).all()
+                else:
+                    near(q[t], m.query(2, 4, pos[t]))
+                continue
+            at = np.array([10, 11]) if pos is None else pos[t]
+            near(q[t], m.query(2 * b, 2 * b + 2, at))
+            m.written(b, 2 * b, 2 * b + 2, 10, at)
+        m.check_cache((bad, pos is None))

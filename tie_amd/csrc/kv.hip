@@ -75,11 +75,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 	fetch(u0);
 	const double wq0 = a.q_norm ? (double)a.q_norm[i] : 1.0, wq1 = a.q_norm ? (double)a.q_norm[i + L] : 1.0;
 	const double wk0 = a.k_norm ? (double)a.k_norm[i] : 1.0, wk1 = a.k_norm ? (double)a.k_norm[i + L] : 1.0;
-	const int len = s.len[b], row = len + (t - t0);
+	const int len = s.len[b];
 	const bool fits = seq_fits(s, len, n);
-	const int page = fits ? page_of(s, c.n_pages, b, row) : -1, r = fits ? row % PAGE : 0;
+	const int row = fits ? len + (t - t0) : 0;
+	const int page = fits ? page_of(s, c.n_pages, b, row) : -1, r = row % PAGE;
 	double cs, sn;
 	sincos((double)(a.pos ? a.pos[t] : row) * exp2((double)i * (-2.0 / HD) * a.log2_theta), &sn, &cs);
+	if (!fits && !a.pos)
+		cs = sn = __builtin_nan(""); // (no row: no position)
 	for (int u = 0; u < per_wave; u++) {
 		const int h = (u0 + 4 * u) * G + part;
 		if ((u0 + 4 * u) * G >= n_all)
