@@ -79,10 +79,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 	const bool fits = seq_fits(s, len, n);
 	const int row = fits ? len + (t - t0) : 0;
 	const int page = fits ? page_of(s, c.n_pages, b, row) : -1, r = row % PAGE;
+	// (no row: no position)
+	const double at = a.pos ? (double)a.pos[t] : fits ? (double)row : __builtin_nan("");
 	double cs, sn;
-	sincos((double)(a.pos ? a.pos[t] : row) * exp2((double)i * (-2.0 / HD) * a.log2_theta), &sn, &cs);
-	if (!fits && !a.pos)
-		cs = sn = __builtin_nan(""); // (no row: no position)
+	sincos(at * exp2((double)i * (-2.0 / HD) * a.log2_theta), &sn, &cs);
 	for (int u = 0; u < per_wave; u++) {
 		const int h = (u0 + 4 * u) * G + part;
 		if ((u0 + 4 * u) * G >= n_all)
