@@ -343,8 +343,9 @@ int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, const tie_h
 /* Keep the accepted path of each sequence: cache row len + path[b][j] becomes
  * row len + j for j < n_keep[b], in all layers, and len_out[b] = len[b] +
  * n_keep[b] (len_out may be len; NULL: not wanted).  path [n_seqs][max_path]
- * holds tokens of the sequence, ascending; an entry that does not ascend or
- * is no token of it ends the path there. */
+ * holds tokens of the sequence, ascending; an entry that does not ascend, is
+ * no token of it, or whose row lies on no page, before or after, ends the path
+ * there. */
 int tie_hip_kv_keep(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, const int32_t *path, int max_path,
 		    const int32_t *n_keep, int32_t *len_out, void *stream);
 

@@ -83,3 +83,38 @@ def test_append_of_a_length_that_is_none(kind, bad):
             near(q[t], m.query(2 * b, 2 * b + 2, at))
             m.written(b, 2 * b, 2 * b + 2, 10, at)
         m.check_cache((bad, pos is None))
+
+
+@KINDS
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("long", [False, True])
+def test_keep_over_pages_that_are_none(kind, in_place, long):
+    """A path ends at the first entry whose row has no page, or goes to a row
+    that has none: the length counts the rows before it, which are moved, and
+    nothing else is.  (long: entries past the first 64 as well)"""
+    import torch
+    m = Call(kind, 7, lens=(60, 60, 60, 60, 5), counts=(200, 200, 200, 200, 200), rows=1000)
+    c = m.c
+    # sequence 0: rows of page 2 (nodes 68 .. 131) have none; 1: page 0 (the first 4 targets); 2: page 1; 3: a page past the last; 4: all good
+    m.table[0, 2], m.table[1, 0], m.table[2, 1], m.table[3, 3] = -1, -7, c.n_pages, 2 ** 31 - 1
+    step = 1 if long else 9
+    path = list(range(1, 200, step))
+    pad = np.full((5, 220), -1, np.int32)
+    pad[:, :len(path)] = path
+    want = []
+    for b in range(5):
+        def there(node):
+            return 0 <= m.table[b, (m.lens[b] + node) // 64] < c.n_pages
+        kept = next((j for j, p in enumerate(path) if not (there(p) and there(j))), len(path))
+        want.append(m.lens[b] + kept)
+        for j in range(kept):
+            (fp, fr), (tp, tr) = c.place(b, m.lens[b] + path[j]), c.place(b, m.lens[b] + j)
+            c.k[:, tp, :, tr], c.v[:, tp, :, :, tr] = c.k[:, fp, :, fr].copy(), c.v[:, fp, :, :, fr].copy()
+            if kind == "i8":
+                c.ks[:, tp, :, tr], c.vs[:, tp, :, tr] = c.ks[:, fp, :, fr].copy(), c.vs[:, fp, :, fr].copy()
+    assert len(set(want)) == 5 and want[1] == 60 and want[4] == 5 + len(path)
+    seqs = m.seqs()
+    lens = seqs.keep[1] if in_place else torch.full((5,), -7, dtype=torch.int32, device="cuda")
+    m.kv.keep(seqs, cuda(pad), cuda(np.full(5, len(path), np.int32)), lens)
+    same(done(lens)[0], np.array(want, np.int32))
+    m.check_cache()

@@ -298,17 +298,29 @@ constexpr int KEEP_BATCH = 8;
 constexpr int KEEP_TABLE = 64; // path entries at a time
 
 // How many entries of sequence b's path can be moved: up to the first that
-// does not ascend or is none of its n nodes.  A wave, whose lanes have the first
-// entries already (they are requested with the lengths).
-__device__ __forceinline__ int keep_count(const int32_t *path, int mine, int want, int n)
+// does not ascend, is none of its n nodes, or lies on no page or is to.  A wave,
+// whose lanes have the first entries already (they are requested with the
+// lengths), and get those entries' pages, before and after.  len + n lies within
+// the page table.
+__device__ __forceinline__ int keep_count(const KvSeqs &s, int n_pages, int b, int len, const int32_t *path, int mine, int want,
+					  int n, int &from, int &to)
 {
 	const int lane = threadIdx.x & 63;
+	from = to = -1;
 	for (int j0 = 0; j0 < want; j0 += 64) {
 		const int j = j0 + lane;
 		const bool in = j < want;
-		const int p = j0 == 0 ? mine : in ? path[j] : 0, before = __shfl_up(p, 1);
-		const int prev = lane > 0 ? before : j0 > 0 ? path[j0 - 1] : -1;
-		const unsigned long long bad = __ballot(in && (p <= prev || p >= n));
+		const int p = j0 == 0 ? mine : in ? path[j] : 0;
+		// (both pages requested before anything else is known of the entry; the
+		// first row's stand for those of an entry that names no node)
+		const bool node = in && p >= 0 && p < n && j < n;
+		const int f = page_of(s, n_pages, b, node ? len + p : 0), t = page_of(s, n_pages, b, node ? len + j : 0);
+		const int before = __shfl_up(p, 1), prev = lane > 0 ? before : j0 > 0 ? path[j0 - 1] : -1;
+		if (j0 == 0) {
+			from = f;
+			to = t;
+		}
+		const unsigned long long bad = __ballot(in && !(node && p > prev && f >= 0 && t >= 0));
 		if (bad)
 			return j0 + __builtin_ctzll(bad);
 	}
@@ -326,31 +338,44 @@ __global__ __launch_bounds__(256) void kv_keep_kernel(KvLayer c, KvSeqs s, const
 						      const int32_t *n_keep, int32_t *len_out)
 {
 	// source and target, as page * PAGE + row; target -1: nothing to move
-	__shared__ int from[KEEP_TABLE], to[KEEP_TABLE];
+	__shared__ int from[KEEP_TABLE], to[KEEP_TABLE], rows;
 	const int h = blockIdx.x % c.kvh, layer = blockIdx.x / c.kvh, b = blockIdx.y, i = threadIdx.x % c.hd;
 	const bool is_v = (int)threadIdx.x >= c.hd;
-	int t0, n;
 	const int32_t *pb = path + (size_t)b * max_path;
-	const int entry = first_entry(pb, max_path);
 	const int len = s.len[b];
-	const int want = min(n_keep[b], max_path);
-	seq_tokens(s, b, t0, n);
-	const int count = seq_fits(s, len, n) ? keep_count(pb, entry, want, n) : 0;
-	if (len_out && blockIdx.x == 0 && threadIdx.x == 0)
-		len_out[b] = len + count;
+	// entry j of the path, a thread's: its pages are fp and tp
+	auto put = [&](int j, int p, int fp, int tp) {
+		from[threadIdx.x] = fp * PAGE + (len + p) % PAGE;
+		to[threadIdx.x] = p == j ? -1 : tp;
+	};
+	if (threadIdx.x < 64) {
+		int t0, n, fp, tp;
+		const int entry = first_entry(pb, max_path), want = min(n_keep[b], max_path);
+		seq_tokens(s, b, t0, n);
+		const int count = seq_fits(s, len, n) ? keep_count(s, c.n_pages, b, len, pb, entry, want, n, fp, tp) : 0;
+		if ((int)threadIdx.x < count)
+			put(threadIdx.x, entry, fp, tp);
+		if (threadIdx.x == 0) {
+			rows = count;
+			if (len_out && blockIdx.x == 0)
+				len_out[b] = len + count;
+		}
+	}
+	__syncthreads();
+	const int count = rows;
 	T *base = reinterpret_cast<T *>((is_v ? c.v : c.k) + (size_t)layer * c.layer_bytes) + (size_t)h * PAGE * c.hd;
 	float *scales = (is_v ? c.vs : c.ks) + (size_t)layer * c.layer_scales + (size_t)h * PAGE;
 	const size_t page = (size_t)c.kvh * PAGE * c.hd;
 	for (int j1 = 0; j1 < count; j1 += KEEP_TABLE) {
 		const int m = min(KEEP_TABLE, count - j1);
-		__syncthreads();
-		if ((int)threadIdx.x < m) {
-			const int j = j1 + threadIdx.x, p = j1 ? pb[j] : entry;
-			const int fp = page_of(s, c.n_pages, b, len + p), tp = page_of(s, c.n_pages, b, len + j);
-			from[threadIdx.x] = fp * PAGE + (len + p) % PAGE;
-			to[threadIdx.x] = p == j || fp < 0 || tp < 0 ? -1 : tp;
+		if (j1) {
+			__syncthreads();
+			if ((int)threadIdx.x < m) {
+				const int j = j1 + threadIdx.x, p = pb[j];
+				put(j, p, page_of(s, c.n_pages, b, len + p), page_of(s, c.n_pages, b, len + j));
+			}
+			__syncthreads();
 		}
-		__syncthreads();
 		for (int j0 = 0; j0 < m; j0 += KEEP_BATCH) {
 			T x[KEEP_BATCH];
 			float f[KEEP_BATCH];
@@ -378,7 +403,7 @@ __global__ __launch_bounds__(256) void kv_keep_kernel(KvLayer c, KvSeqs s, const
 	}
 }
 
-__global__ __launch_bounds__(64) void kv_keep_len_kernel(KvSeqs s, const int32_t *path, int max_path,
+__global__ __launch_bounds__(64) void kv_keep_len_kernel(KvSeqs s, int n_pages, const int32_t *path, int max_path,
 							 const int32_t *n_keep, int32_t *len_out)
 {
 	const int b = blockIdx.x;
@@ -386,7 +411,9 @@ __global__ __launch_bounds__(64) void kv_keep_len_kernel(KvSeqs s, const int32_t
 	seq_tokens(s, b, t0, n);
 	const int len = s.len[b];
 	const int32_t *pb = path + (size_t)b * max_path;
-	const int count = seq_fits(s, len, n) ? keep_count(pb, first_entry(pb, max_path), min(n_keep[b], max_path), n) : 0;
+	const int entry = first_entry(pb, max_path), want = min(n_keep[b], max_path);
+	int from, to;
+	const int count = seq_fits(s, len, n) ? keep_count(s, n_pages, b, len, pb, entry, want, n, from, to) : 0;
 	if (threadIdx.x == 0)
 		len_out[b] = len + count;
 }
@@ -402,7 +429,8 @@ hipError_t launch_kv_keep(const KvLayer &c, int n_layers, const KvSeqs &s, const
 	else
 		tie_launch(kv_keep_kernel<uint16_t>, grid, block, 0, st, c, s, path, max_path, n_keep, now);
 	if (len_out && !now)
-		tie_launch(kv_keep_len_kernel, dim3(s.n_seqs), dim3(64), 0, st, s, path, max_path, n_keep, len_out);
+		tie_launch(kv_keep_len_kernel, dim3(s.n_seqs), dim3(64), 0, st, s, c.n_pages, path, max_path, n_keep,
+			   len_out);
 	return hipGetLastError();
 }
 
