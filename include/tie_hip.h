@@ -276,9 +276,15 @@ typedef struct tie_hip_kv_cache {
  * first[b] .. first[b + 1] - 1 of the activations; its token j is cache row
  * len[b] + j, on page pages[b][(len[b] + j) / 64].  Rows that belong to no
  * sequence are left as they are.  The arrays are read on the device, so no call
- * can refuse what they say; it is checked there: where a length, a range of
- * rows or a page lies outside the call's sizes, nothing is written to the
- * cache, and the outputs that would need it are NaN. */
+ * can refuse what they say; it is checked there.  Where a sequence's rows do not
+ * lie within its row of the page table (a length below 0 or too large), or one's
+ * page is none, nothing is written to the cache for them, and the outputs that
+ * would need them are NaN (of the attention others of the sequence may be, too).
+ * A sequence whose range of token rows falls, begins below 0 or ends past
+ * n_tokens has no rows in the call.  Where ranges that do not ascend overlap, a row's outputs
+ * are those of one of its sequences, and its cache row is written for one at
+ * most.  (tie_hip_verify_tree: where any range does not ascend within the rows,
+ * no sequence has any.) */
 typedef struct tie_hip_kv_seqs {
 	int n_seqs;           /* at most 65535 */
 	int max_pages;        /* columns of the page table */

@@ -118,3 +118,160 @@ def test_keep_over_pages_that_are_none(kind, in_place, long):
     m.kv.keep(seqs, cuda(pad), cuda(np.full(5, len(path), np.int32)), lens)
     same(done(lens)[0], np.array(want, np.int32))
     m.check_cache()
+
+
+RANGES = pytest.mark.parametrize("first", [[0, 2, 1, 6, 8], [0, 2, 1, 6, 9], [-4, 2, 4, 900, 901], [0, 2, 4, 4, 4], [5, 2, 2, 8, 3],
+                                           [8, 8, 9, 2, 4], [2 ** 31 - 1, -2 ** 31, 0, 3, 8]])
+
+
+def good_rows(m):
+    """For each token row the (sequence, token) that a good range makes of it."""
+    rows = [[] for _ in range(m.rows)]
+    for b in range(4):
+        t0, t1 = int(m.first[b]), int(m.first[b + 1])
+        if 0 <= t0 <= t1 <= m.rows:
+            for t in range(t0, t1):
+                rows[t].append((b, t - t0))
+    return rows
+
+
+@KINDS
+@RANGES
+def test_append_of_ranges_that_do_not_ascend(kind, first):
+    """A row goes to the last sequence that begins at or before it, if that one's
+    range is good and holds it; the others' queries stay, and so does every
+    byte of the cache that is no such row."""
+    m = Call(kind, 9)
+    m.first = np.array(first, np.int32)
+    q = m.append()
+    for t in range(m.rows):
+        begun = [b for b in range(4) if first[b] <= t]
+        b = begun[-1] if begun else -1
+        if b < 0 or not (0 <= first[b] <= t < first[b + 1] <= m.rows):
+            assert (q[t] == -7.0).all(), t
+            continue
+        j = t - first[b]
+        near(q[t:t + 1], m.query(t, t + 1, np.array([10 + j])))
+        m.written(b, t, t + 1, 10 + j, np.array([10 + j]))
+    m.check_cache(first)
+
+
+@KINDS
+@RANGES
+def test_read_of_ranges_that_do_not_ascend(kind, first):
+    """Rows of a good range are read (of either sequence where two have it), the others stay."""
+    m = Call(kind, 10, counts=(8, 8, 8, 8))
+    m.first = np.array(first, np.int32)
+    k, v = m.read()
+    for t, of in enumerate(good_rows(m)):
+        for layer in range(2):
+            want = [[x[0].astype(np.float32) for x in m.c.rows(layer, b, 10 + j, 11 + j)] for b, j in of] or [[np.full((KVH, HD), -7.0)] * 2]
+            assert any((k[layer, t] == w[0]).all() for w in want) and any((v[layer, t] == w[1]).all() for w in want), (t, of)
+    m.check_cache(first)
+
+
+@KINDS
+@RANGES
+def test_attention_of_ranges_that_do_not_ascend(kind, first):
+    import torch
+    m = Call(kind, 11, counts=(8, 8, 8, 8))
+    m.first = np.array(first, np.int32)
+    q = m.rng.standard_normal((m.rows, H, HD)).astype(np.float32)
+    out = torch.full((m.rows, H, HD), -7.0, device="cuda")
+    m.kv.attention(1, m.seqs(), cuda(q), out, 0.125)
+    o, = done(out)
+    for t, of in enumerate(good_rows(m)):
+        if not of:
+            assert (o[t] == -7.0).all(), t
+            continue
+        held = np.zeros((len(of), H), bool)
+        for i, (b, j) in enumerate(of):
+            k, v = m.c.rows(1, b, 0, 11 + j)
+            for h in range(H):
+                qq, kk, vv = q[t, h].astype(np.float64), k[:, h // (H // KVH)], v[:, h // (H // KVH)]
+                w = np.exp(kk @ qq * 0.125 - (kk @ qq * 0.125).max())
+                w /= w.sum()
+                held[i, h] = (np.abs(o[t, h] - w @ vv) <= kv_ref.tolerance(qq, kk, vv, w, 0.125)).all()
+        assert held.any(0).all(), (t, of)
+
+
+@KINDS
+@RANGES
+def test_keep_of_ranges_that_do_not_ascend(kind, first):
+    """A path of nodes 1, 3, 7: those that are nodes of a good range."""
+    import torch
+    m = Call(kind, 12, counts=(8, 8, 8, 8))
+    m.first = np.array(first, np.int32)
+    c, want = m.c, []
+    for b in range(4):
+        n = first[b + 1] - first[b] if 0 <= first[b] <= first[b + 1] <= m.rows else 0
+        kept = [p for p in (1, 3, 7) if p < n]
+        want.append(10 + len(kept))
+        for j, p in enumerate(kept):
+            (fp, fr), (tp, tr) = c.place(b, 10 + p), c.place(b, 10 + j)
+            c.k[:, tp, :, tr], c.v[:, tp, :, :, tr] = c.k[:, fp, :, fr].copy(), c.v[:, fp, :, :, fr].copy()
+            if kind == "i8":
+                c.ks[:, tp, :, tr], c.vs[:, tp, :, tr] = c.ks[:, fp, :, fr].copy(), c.vs[:, fp, :, fr].copy()
+    lens = torch.full((4,), -7, dtype=torch.int32, device="cuda")
+    m.kv.keep(m.seqs(), cuda(np.array([[1, 3, 7]] * 4, np.int32)), cuda(np.array([3, 3, 3, 3], np.int32)), lens)
+    same(done(lens)[0], np.array(want, np.int32))
+    m.check_cache(first)
+
+
+@KINDS
+def test_pages_that_are_none(kind):
+    """Below 0, past the last: nothing is written there, reads give NaN, the
+    attention of that sequence too; queries need no page; the others are served."""
+    import torch
+    m = Call(kind, 13)
+    m.table[0, 0], m.table[2, 0] = -3, m.c.n_pages
+    q = m.append()
+    near(q, m.query(0, 8, np.array([10, 11] * 4)))
+    for b in (1, 3):
+        m.written(b, 2 * b, 2 * b + 2, 10, np.array([10, 11]))
+    m.check_cache("append")
+    k, v = m.read()
+    for b in range(4):
+        t = slice(2 * b, 2 * b + 2)
+        if b in (0, 2):
+            assert np.isnan(k[:, t]).all() and np.isnan(v[:, t]).all()
+            continue
+        for layer in range(2):
+            wk, wv = m.c.rows(layer, b, 10, 12)
+            same(k[layer, t], wk.astype(np.float32))
+            same(v[layer, t], wv.astype(np.float32))
+    out = torch.full((8, H, HD), -7.0, device="cuda")
+    m.kv.attention(1, m.seqs(), cuda(q), out, 0.125)
+    o, = done(out)
+    want, tol = kv_ref.attention(m.c, 1, q, 0.125, lambda b, i, j: j <= i)
+    for b in range(4):
+        t = slice(2 * b, 2 * b + 2)
+        assert np.isnan(o[t]).all() if b in (0, 2) else (np.abs(o[t] - want[t]) <= tol[t]).all(), b
+
+
+@KINDS
+@pytest.mark.parametrize("bad", [-1, -2 ** 31, 63, 2 ** 31 - 1])
+def test_lengths_that_are_none(kind, bad):
+    """Reads and attention give NaN, keep moves nothing and leaves the length."""
+    import torch
+    m = Call(kind, 14)
+    m.lens[2] = bad
+    k, v = m.read()
+    out, q = torch.full((8, H, HD), -7.0, device="cuda"), m.rng.standard_normal((8, H, HD)).astype(np.float32)
+    m.kv.attention(1, m.seqs(), cuda(q), out, 0.125)
+    o, = done(out)
+    want, tol = kv_ref.attention(m.c, 1, q, 0.125, lambda b, i, j: j <= i)
+    for b in range(4):
+        t = slice(2 * b, 2 * b + 2)
+        if b == 2:
+            assert np.isnan(k[:, t]).all() and np.isnan(v[:, t]).all() and np.isnan(o[t]).all()
+            continue
+        for layer in range(2):
+            wk, wv = m.c.rows(layer, b, 10, 12)
+            same(k[layer, t], wk.astype(np.float32))
+            same(v[layer, t], wv.astype(np.float32))
+        assert (np.abs(o[t] - want[t]) <= tol[t]).all()
+    lens = torch.full((4,), -7, dtype=torch.int32, device="cuda")
+    m.kv.keep(m.seqs(), cuda(np.array([[0, 1]] * 4, np.int32)), cuda(np.array([2, 1, 2, -3], np.int32)), lens)
+    same(done(lens)[0], np.array([12, 11, bad, 10], np.int32))
+    m.check_cache(bad)
