@@ -264,7 +264,7 @@ int tie_hip_mat_mat(tie_hip_matrix *m, const float *x_dev, int T, float *out_dev
 typedef struct tie_hip_kv_cache {
 	int type;     /* TIE_GGML_F16 or TIE_GGML_I8 */
 	int n_layers; /* layers in the arrays */
-	int n_pages;  /* pages of a layer */
+	int n_pages;  /* pages of a layer, at most 2^25 */
 	int kv_heads;
 	int head_dim; /* 64 or 128 */
 	void *k, *v;  /* 16-byte aligned */

@@ -118,3 +118,22 @@ def test_small_calls_behind_a_large_one(kind):
         gc.collect()
     tie_amd.stream_release(stream.cuda_stream)
     tie_amd.shutdown()
+
+
+@needs_lib
+def test_pages_whose_rows_pass_32_bits_are_refused():
+    """(keep forms page * 64 + row in 32 bits: the last page of 2^25 is the last that fits)"""
+    assert (2 ** 25 - 1) * 64 + 63 == 2 ** 31 - 1
+    mem = np.zeros(1 << 17, np.uint8)
+    a = (mem.ctypes.data + 255) & ~255
+    s = tie_amd.KVSeqsDesc(n_seqs=2, max_pages=3, n_tokens=5, pages=a, len=a, first=a)
+    L, r = tie_amd.lib(), ctypes.byref
+    for kind in (tie_amd.F16, tie_amd.I8):
+        for n, want in ((2 ** 25, tie_amd.ENOINIT), (2 ** 25 + 1, tie_amd.EINVAL), (2 ** 31 - 1, tie_amd.EINVAL)):
+            c = tie_amd.KVCacheDesc(type=kind, n_layers=1, n_pages=n, kv_heads=1, head_dim=64, k=a, v=a, k_scale=a, v_scale=a)
+            assert L.tie_hip_kv_keep(r(c), r(s), a, 4, a + 4096, None, None) == want
+            assert L.tie_hip_kv_read(r(c), 0, 1, r(s), a, a + 32768, None) == want
+            assert L.tie_hip_tree_attention(r(c), 0, r(s), a, 256, 4, 0.1, None, 0, a + 32768, 256, None, 0, None) == want
+            assert L.tie_hip_kv_append(r(c), 0, r(s), a, 256, a + 8192, 64, a + 16384, 64, 4, a, a, 1e-6, 1e6, None, a + 32768, 256,
+                                       None) == want
+            assert (L.tie_hip_tree_attention_work_bytes(r(c), r(s), 4) > 0) == (want == tie_amd.ENOINIT)

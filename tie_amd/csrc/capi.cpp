@@ -1383,9 +1383,10 @@ static int check_cache(const tie_hip_kv_cache *c, int layer, int n_layers, KvLay
 		return set_error(TIE_HIP_EINVAL, "cache type %d unsupported (F16, I8)", c->type);
 	if (c->head_dim != 64 && c->head_dim != 128)
 		return set_error(TIE_HIP_EINVAL, "head_dim=%d unsupported (64, 128)", c->head_dim);
-	if (c->kv_heads < 1 || c->kv_heads > 1024 || c->n_layers < 1 || c->n_layers > 4096 || c->n_pages < 1)
-		return set_error(TIE_HIP_EINVAL, "bad cache: kv_heads=%d n_layers=%d n_pages=%d", c->kv_heads, c->n_layers,
-				 c->n_pages);
+	if (c->kv_heads < 1 || c->kv_heads > 1024 || c->n_layers < 1 || c->n_layers > 4096 || c->n_pages < 1 ||
+	    c->n_pages > MAX_PAGES)
+		return set_error(TIE_HIP_EINVAL, "bad cache: kv_heads=%d n_layers=%d n_pages=%d (at most %d)", c->kv_heads,
+				 c->n_layers, c->n_pages, MAX_PAGES);
 	if (layer < 0 || n_layers < 1 || layer >= c->n_layers || n_layers > c->n_layers - layer)
 		return set_error(TIE_HIP_EINVAL, "layer %d (%d of them) outside [0, %d)", layer, n_layers, c->n_layers);
 	l.i8 = c->type == TIE_GGML_I8;

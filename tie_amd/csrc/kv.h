@@ -6,6 +6,7 @@
 namespace tie {
 
 constexpr int PAGE = TIE_HIP_PAGE_ROWS; // rows of a page: one 64-bit mask word, four 16-row matrix-core tiles
+constexpr int MAX_PAGES = 1 << 25; // of a layer: page * PAGE + row is an int (256 GiB of one int8 kv head of 64)
 
 // One layer of a cache.  K [page][kv head][PAGE][hd] and V [page][kv
 // head][hd][PAGE]: a V column's rows are contiguous, so that both products of
