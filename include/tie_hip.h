@@ -183,7 +183,8 @@ size_t tie_hip_layer_bytes(const tie_hip_layer *layer);
 /* Frees the scratch workspace the library keeps for `stream` (grown by the
  * forwards enqueued on it; at the 235B shape and large T, hundreds of MiB).
  * Call it before destroying a stream that forwards ran on; otherwise the
- * workspace lives until tie_hip_shutdown.  Drains the device first. */
+ * workspace lives until tie_hip_shutdown.  Drains the device first.  A graph
+ * captured with that workspace is not to be replayed afterwards. */
 int tie_hip_stream_release(void *stream);
 
 int tie_hip_moe_forward(tie_hip_layer *layer, const float *x_dev, int T, int k, float *out_dev,
@@ -339,8 +340,11 @@ int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_layers, cons
  * Scores are held in F32; past 2^24 in magnitude their rounding is larger than
  * what a softmax tells apart, and a row's result means nothing.
  * A row's result is the same whatever else the call holds only up to F32
- * rounding: how the rows are cut follows the lengths.  Two equal calls give
- * equal bits. */
+ * rounding: which kernel takes the rows and how they are cut follows the
+ * lengths and the call's sizes, the page table's columns among them.  Two equal
+ * calls give equal bits.  A value in the cache that is not finite does nothing
+ * to the results that do not see its row; of those that do it spoils its column
+ * (an f16 value of V) or all of the head's (a key or a scale). */
 size_t tie_hip_tree_attention_work_bytes(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, int n_heads);
 int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
 			   size_t q_stride, int n_heads, float scale, const uint64_t *mask, int mask_words, float *out,
