@@ -172,3 +172,23 @@ def test_the_older_calls_take_the_default_stream(device):
     torch.cuda.synchronize()
     assert torch.equal(got, want) and float(want.abs().max()) > 0
     m.close()
+
+
+@pytest.mark.gpu
+def test_the_callers_device_stays(device):
+    """Calls on the library's GPU from a program whose current device is another."""
+    import torch
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    k = torch.zeros(1, 2, 2, 64, 64, dtype=torch.float16, device="cuda:0")
+    i32 = dict(dtype=torch.int32, device="cuda:0")
+    c, s = tie_amd.KVCache(k, k.clone()), tie_amd.KVSeqs(torch.zeros(2, 3, **i32), torch.zeros(2, **i32))
+    q, kv, rows, two = (torch.zeros(n, device="cuda:0") for n in ((2, 256), (2, 128), (1, 2, 2, 64), 2))
+    nodes = torch.zeros(2, **i32)
+    with torch.cuda.device(1):
+        for call in (lambda: c.append(0, s, q, kv, kv, q), lambda: c.read(s, rows, rows.clone()), lambda: c.attention(0, s, q, q, 1.0),
+                     lambda: c.keep(s, torch.zeros(2, 3, **i32), nodes),
+                     lambda: tie_amd.verify_tree(torch.zeros(2, 50, device="cuda:0"), None, nodes, nodes, two, two,
+                                                 torch.zeros(2, 3, **i32), nodes.clone(), nodes.clone())):
+            call()
+            assert torch.cuda.current_device() == 1

@@ -1335,6 +1335,23 @@ extern "C" int tie_hip_qwen3_ffn(float *hidden, int T, int d, int F, int E, int 
 // ---------------------------------------------------- the attention half
 namespace tie {
 
+// The caller's device, set again when a call is done (ensure_init sets the library's).
+struct CallersDevice {
+	int device = -1;
+	CallersDevice()
+	{
+		if (hipGetDevice(&device) != hipSuccess) {
+			(void)hipGetLastError();
+			device = -1;
+		}
+	}
+	~CallersDevice()
+	{
+		if (device >= 0 && device != g.device)
+			(void)hipSetDevice(device);
+	}
+};
+
 // `need` bytes of scratch: the caller's, or the stream's own, grown.
 static int aux_scratch(hipStream_t s, void *work, size_t work_bytes, size_t need, void **out)
 {
@@ -1486,6 +1503,7 @@ extern "C" int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const
 	if ((!(q_out == q && q_out_stride == q_stride) && rows_overlap(T, q_out, q_out_stride, wq, q, q_stride, wq)) ||
 	    rows_overlap(T, q_out, q_out_stride, wq, k, k_stride, wk) || rows_overlap(T, q_out, q_out_stride, wq, v, v_stride, wk))
 		return set_error(TIE_HIP_EINVAL, "q_out overlaps an input (it may be q itself, with q's stride)");
+	CallersDevice back;
 	TIE_TRY(ensure_init());
 	if (none)
 		return TIE_HIP_OK;
@@ -1527,6 +1545,7 @@ extern "C" int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_l
 	const size_t n = (size_t)n_layers * s.n_tokens * l.kvh * l.hd * 4;
 	if (overlap(k_out, n, v_out, n))
 		return set_error(TIE_HIP_EINVAL, "k_out and v_out overlap");
+	CallersDevice back;
 	TIE_TRY(ensure_init());
 	if (none)
 		return TIE_HIP_OK;
@@ -1556,6 +1575,7 @@ extern "C" int tie_hip_kv_keep(const tie_hip_kv_cache *cache, const tie_hip_kv_s
 			overlap(len_out, nb, path, nb * max_path) || overlap(len_out, nb, s.first, nb + 4) ||
 			overlap(len_out, nb, s.pages, nb * s.max_pages)))
 		return set_error(TIE_HIP_EINVAL, "len_out overlaps an input (it may be len itself)");
+	CallersDevice back;
 	TIE_TRY(ensure_init());
 	if (s.n_seqs == 0)
 		return TIE_HIP_OK;
@@ -1606,6 +1626,7 @@ extern "C" int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, 
 	if (!(out == q && out_stride == q_stride) &&
 	    rows_overlap(s.n_tokens, out, out_stride, w, q, q_stride, w))
 		return set_error(TIE_HIP_EINVAL, "out overlaps q (it may be q itself, with q's stride)");
+	CallersDevice back;
 	TIE_TRY(ensure_init());
 	if (none)
 		return TIE_HIP_OK;
@@ -1687,6 +1708,7 @@ extern "C" int tie_hip_verify_tree(const float *logits, size_t logits_stride, co
 					return set_error(TIE_HIP_EINVAL, "path, n_keep and next overlap");
 		}
 	}
+	CallersDevice back;
 	TIE_TRY(ensure_init());
 	if (n_seqs == 0)
 		return TIE_HIP_OK;
