@@ -1378,7 +1378,9 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 	h.cut.full = h.few ? FEW_CAP : MANY_FULL;
 	// (few: a grain is a round of the waves; a second one costs as much as joining
 	// two parts: one f16 token over 300 rows of 8 kv heads of 64 7.8 us, in two parts
-	// 10.2, over 1000 10.7, in two parts of two rounds 11.6)
+	// 10.2, over 1000 10.7, in two parts of two rounds 11.6; one int8 token over 600
+	// rows of 4 kv heads of 128 12.5, in two parts 14.4, over 1000 14.7 either way, of
+	// 8 kv heads of 64 8.6, in two parts 10.7, over 1000 9.9 and 10.8)
 	h.cut.grain = !h.few ? 1 : c.i8 ? FEW_WAVES : FEW_WAVES / 2;
 	h.cut.least = h.few ? 1 : 2;
 	h.cut.alone = h.few ? 2 : 3;

@@ -32,10 +32,10 @@ __device__ __forceinline__ _Float16 half_of(float x)
 // cosine and sine stay with it.  All of it in 64 bits up to the one rounding to
 // F32: positions reach where a 32-bit angle is off by a thousandth, and a key's
 // code must not depend on the order of a 32-bit sum.  One token: bound by its
-// chain of steps (position, angle, sincos; row, norm, code), 3.7 us.  Many: by the
-// bytes, the 64-bit arithmetic (about 60 instructions for 64 pairs) and the V
-// columns' pieces (a row's values lie PAGE apart) together: 2048 tokens of 40 heads
-// 22.5 us, 3.5 TB/s; 20 to 21.5 without any one of them.
+// chain of steps (position, angle, sincos; row, norm, code), 3.6 us (on the default
+// stream 4.1).  Many: by the bytes, the 64-bit arithmetic (about 60 instructions
+// for 64 pairs) and the V columns' pieces (a row's values lie PAGE apart) together:
+// 2048 tokens of 40 heads 22.5 us, 3.5 TB/s; 20 to 21.5 without any one of them.
 constexpr int DIES = 8;
 
 template <int HD, bool I8>
@@ -292,7 +292,7 @@ hipError_t launch_kv_read(const KvLayer &c, int n_layers, const KvSeqs &s, float
 // moves its rows in order, KEEP_BATCH loads before their stores.  A path ascends,
 // so path[j] >= j and no store reaches a row that a later load wants.  Where the
 // rows lie is worked out once, by the first wave.  Bound by V's lines (a row's values
-// lie in one for each column): 16 paths in 48 layers of 4 heads 15 us; one path 4.4,
+// lie in one for each column): 16 paths in 48 layers of 4 heads 16 us; one path 4.3,
 // the chain of its steps.
 constexpr int KEEP_BATCH = 8;
 constexpr int KEEP_TABLE = 64; // path entries at a time
