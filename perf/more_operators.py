@@ -351,7 +351,8 @@ def _plain_plan(case, s):
     row = lens[b] + t - first[b]
     on = t < first[-1]
     row = torch.where(on, row, torch.zeros_like(row))
-    slot = torch.where(on, out[b, row // ROWS] * ROWS + row % ROWS, -1)
+    page = out[b, row // ROWS]
+    slot = torch.where(on & (page >= 0) & (page < P), page * ROWS + row % ROWS, -1)
     pos = torch.where(on, row, torch.full_like(row, -1))
     return out.int(), first.int(), pos.int(), slot.int(), ring[:P].int(), state.int()
 
