@@ -313,6 +313,20 @@ int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv
 		      const float *k_norm, float eps, float theta, const int32_t *pos, float *q_out, size_t q_out_stride,
 		      void *stream);
 
+/* tie_hip_kv_append for tokens whose position has several axes (time, height
+ * and width of an image's patches): pair i is rotated by pos[axis[i]][t] *
+ * theta^(-2 i / head_dim).
+ *   pos   [n_axes][n_tokens] (text has the same position on all axes)
+ *   axis  [head_dim / 2], each below n_axes: host memory, read before the call
+ *         returns (a captured graph keeps what it said)
+ * Positions need not be cache rows: an image's tokens take fewer positions than
+ * rows, and a cache's rows, masks and windows go by rows. */
+#define TIE_HIP_MAX_AXES 4
+int tie_hip_kv_append_axes(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
+			   size_t q_stride, const float *k, size_t k_stride, const float *v, size_t v_stride, int n_heads,
+			   const float *q_norm, const float *k_norm, float eps, float theta, const int32_t *pos, int n_axes,
+			   const uint8_t *axis, float *q_out, size_t q_out_stride, void *stream);
+
 /* The cache rows of the sequences' tokens as F32, of n_layers layers from
  * `layer` on: k_out and v_out [n_layers][n_tokens][kv_heads][head_dim].  (len
  * of zeros and first over whole lengths reads whole sequences.) */
@@ -350,6 +364,25 @@ int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, const tie_h
 			   size_t q_stride, int n_heads, float scale, const uint64_t *mask, int mask_words, float *out,
 			   size_t out_stride, void *work, size_t work_bytes, void *stream);
 
+/* tie_hip_tree_attention through a sliding window, with a few first rows that
+ * stay visible: token t of a sequence, which stands at row at[t] ([n_tokens];
+ * NULL: its own row, len + its index), sees row r of the committed ones where
+ *   r < sinks  or  r > at[t] - window
+ * (at says where a window begins, not where it ends: all committed rows above
+ * are seen).  mask NULL: its own tokens up to itself, by the same rule for their
+ * rows.  With a mask: the own tokens that it names, whatever the window.  A tree
+ * of drafted tokens has at = len + the node's depth, and no bits for ancestors
+ * that lie behind the window.
+ * Pages that hold no row that a token sees are not looked at: their entries in
+ * the page table may be none, as tie_hip_kv_plan leaves them.
+ * window at least 1, sinks 0 or more; everything else, scratch memory included, as
+ * for tie_hip_tree_attention.  The work bytes are enough for any window. */
+size_t tie_hip_window_attention_work_bytes(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, int n_heads);
+int tie_hip_window_attention(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
+			     size_t q_stride, int n_heads, float scale, int window, int sinks, const int32_t *at,
+			     const uint64_t *mask, int mask_words, float *out, size_t out_stride, void *work, size_t work_bytes,
+			     void *stream);
+
 /* Keep the accepted path of each sequence: cache row len + path[b][j] becomes
  * row len + j for j < n_keep[b], in all layers, and len_out[b] = len[b] +
  * n_keep[b] (len_out may be len; NULL: not wanted).  path [n_seqs][max_path]
@@ -358,6 +391,67 @@ int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, const tie_h
  * there. */
 int tie_hip_kv_keep(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, const int32_t *path, int max_path,
 		    const int32_t *n_keep, int32_t *len_out, void *stream);
+
+/* The pages of a step, from the requests' lengths: one row of the page table
+ * for each request, pages taken from a pool of free ones and given back to it, and
+ * where the step's tokens go.  Everything is on the device, so that a captured
+ * graph goes on while requests grow.
+ *
+ * The pool: free pages lie in a ring, free[state[0]], free[state[0] + 1], ...
+ * (after the last place the first), state[1] of them.  Pages are taken from its head;
+ * pages that come free are put behind its tail, and can be had from the next
+ * call on.  A state that is none (a place outside the ring, more than n_pages) has
+ * no pages and takes none.
+ *
+ * Request b has len[b] rows and asks for n_new[b] more; its pages in
+ * ceil(len / 64) .. ceil((len + n_new) / 64) - 1 that the table does not name are
+ * taken from the pool (a page that an earlier call's drafts left there stays).
+ * Requests are served in order: the first whose pages or token rows are not
+ * there any more and all behind it get nothing (first[b + 1] = first[b]).  One whose
+ * rows do not lie within its row of the table (len below 0, or too large) asks for
+ * nothing.  n_new below 0: the request has ended, and all its pages go back.
+ * window > 0: of every other request the pages go back that the next token, at
+ * row len, and those after it do not see through tie_hip_window_attention: those whose
+ * rows all lie below len - window + 1, but for those of the first `sinks` rows.  Entries
+ * of pages that went back are -1.  Where more pages come back than the ring has
+ * places (a page named twice), those left over stay in the table.
+ *   pages      [n_seqs][max_pages]; pages_out the same shape, the new table (may be pages)
+ *   first      [n_seqs + 1] the requests' token rows: tie_hip_kv_seqs.first
+ *   pos, slot  [n_tokens] or NULL: each token row's place in its sequence (its
+ *              cache row), and in the cache (page * 64 + row in it); -1 for rows
+ *              of no request and (slot) rows on no page
+ *   state_out  the pool's state behind the call (may be state)
+ * n_tokens is the most token rows that the step has.  No other output may share
+ * memory with an input or another output.  work as for tie_hip_tree_attention. */
+typedef struct tie_hip_kv_pool {
+	int n_pages;          /* of a layer of the cache */
+	int32_t *free;        /* [n_pages] */
+	const int32_t *state; /* [2] */
+	int32_t *state_out;   /* [2] */
+} tie_hip_kv_pool;
+
+size_t tie_hip_kv_plan_work_bytes(int n_seqs);
+int tie_hip_kv_plan(const tie_hip_kv_pool *pool, int n_seqs, int max_pages, int n_tokens, const int32_t *pages,
+		    const int32_t *len, const int32_t *n_new, int window, int sinks, int32_t *pages_out, int32_t *first,
+		    int32_t *pos, int32_t *slot, void *work, size_t work_bytes, void *stream);
+
+/* Log-probabilities under p = softmax(logits / temperature) of each row:
+ *   logprob  [n_tokens] of tokens[t]; rank [n_tokens] how many tokens come before
+ *            it (a larger logit, or an equal one and a lower index)
+ *   entropy  [n_tokens] -sum p log p
+ *   top_tokens, top_logprobs  [n_tokens][n_top] the n_top (at most 64) likeliest
+ *            tokens in that order, and theirs; -1 and -infinity behind the last
+ *            whose logit is above -infinity
+ * Any output may be NULL (the top ones with n_top 0), tokens NULL with logprob and
+ * rank.  A row with a logit of NaN or +infinity, or with none above -infinity, has no
+ * distribution: NaN, rank and top tokens -1.  A token outside [0, vocab): NaN and
+ * rank -1.  temperature from 1e-6 to 1e6; rows of `vocab` (at most 2^24), logits_stride
+ * floats apart.  Sums in 64 bits of exponentials in 32.  No output may share memory
+ * with an input or another output.  work as for tie_hip_verify_tree. */
+size_t tie_hip_token_logprobs_work_bytes(int vocab, int n_tokens, int n_top);
+int tie_hip_token_logprobs(const float *logits, size_t logits_stride, int vocab, int n_tokens, const int32_t *tokens,
+			   float temperature, int n_top, float *logprob, int32_t *rank, float *entropy, int32_t *top_tokens,
+			   float *top_logprobs, void *work, size_t work_bytes, void *stream);
 
 /* Which drafted tokens the target accepts, and the token after them, so that
  * tokens follow the target's distribution whatever the draft proposed.  Token

@@ -35,8 +35,9 @@ EXPORTS = (
     "tie_hip_debug_fail_alloc", "tie_hip_host_expf", "tie_hip_profile_enable", "tie_hip_profile_read",
     "tie_hip_moe_forward_noalloc", "tie_hip_stream_status", "tie_hip_debug_decode_give_up", "tie_hip_debug_decode_form",
     "tie_hip_stream_release", "tie_hip_debug_layer_shifts",
-    "tie_hip_kv_append", "tie_hip_kv_read", "tie_hip_kv_keep", "tie_hip_tree_attention",
-    "tie_hip_tree_attention_work_bytes", "tie_hip_verify_tree", "tie_hip_verify_tree_work_bytes",
+    "tie_hip_kv_append", "tie_hip_kv_append_axes", "tie_hip_kv_read", "tie_hip_kv_keep", "tie_hip_tree_attention",
+    "tie_hip_tree_attention_work_bytes", "tie_hip_window_attention", "tie_hip_window_attention_work_bytes", "tie_hip_verify_tree", "tie_hip_verify_tree_work_bytes",
+    "tie_hip_kv_plan", "tie_hip_kv_plan_work_bytes", "tie_hip_token_logprobs", "tie_hip_token_logprobs_work_bytes",
 )
 
 
@@ -75,6 +76,12 @@ class KVCacheDesc(ctypes.Structure):
         ("type", ctypes.c_int), ("n_layers", ctypes.c_int), ("n_pages", ctypes.c_int), ("kv_heads", ctypes.c_int),
         ("head_dim", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
         ("v_scale", ctypes.c_void_p),
+    ]
+
+
+class KVPoolDesc(ctypes.Structure):
+    _fields_ = [
+        ("n_pages", ctypes.c_int), ("free", ctypes.c_void_p), ("state", ctypes.c_void_p), ("state_out", ctypes.c_void_p),
     ]
 
 
@@ -166,6 +173,8 @@ def lib():
         Z, F = ctypes.c_size_t, ctypes.c_float
         L.tie_hip_kv_append.argtypes = [P, I, P, P, Z, P, Z, P, Z, I, P, P, F, F, P, P, Z, P]
         L.tie_hip_kv_append.restype = I
+        L.tie_hip_kv_append_axes.argtypes = [P, I, P, P, Z, P, Z, P, Z, I, P, P, F, F, P, I, P, P, Z, P]
+        L.tie_hip_kv_append_axes.restype = I
         L.tie_hip_kv_read.argtypes = [P, I, I, P, P, P, P]
         L.tie_hip_kv_read.restype = I
         L.tie_hip_kv_keep.argtypes = [P, P, P, I, P, P, P]
@@ -174,10 +183,22 @@ def lib():
         L.tie_hip_tree_attention.restype = I
         L.tie_hip_tree_attention_work_bytes.argtypes = [P, P, I]
         L.tie_hip_tree_attention_work_bytes.restype = Z
+        L.tie_hip_window_attention.argtypes = [P, I, P, P, Z, I, F, I, I, P, P, I, P, Z, P, Z, P]
+        L.tie_hip_window_attention.restype = I
+        L.tie_hip_window_attention_work_bytes.argtypes = [P, P, I]
+        L.tie_hip_window_attention_work_bytes.restype = Z
         L.tie_hip_verify_tree.argtypes = [P, Z, P, Z, I, I, I, P, P, P, P, P, F, I, I, P, P, P, P, Z, P]
         L.tie_hip_verify_tree.restype = I
         L.tie_hip_verify_tree_work_bytes.argtypes = [I, I, I, I]
         L.tie_hip_verify_tree_work_bytes.restype = Z
+        L.tie_hip_kv_plan.argtypes = [P, I, I, I, P, P, P, I, I, P, P, P, P, P, Z, P]
+        L.tie_hip_kv_plan.restype = I
+        L.tie_hip_kv_plan_work_bytes.argtypes = [I]
+        L.tie_hip_kv_plan_work_bytes.restype = Z
+        L.tie_hip_token_logprobs.argtypes = [P, Z, I, I, P, F, I, P, P, P, P, P, P, Z, P]
+        L.tie_hip_token_logprobs.restype = I
+        L.tie_hip_token_logprobs_work_bytes.argtypes = [I, I, I]
+        L.tie_hip_token_logprobs_work_bytes.restype = Z
         _lib = L
     return _lib
 
@@ -622,6 +643,22 @@ class KVCache:
                                       _array(k_norm, "float32", self.head_shape, "k_norm", dev), eps, theta,
                                       _array(pos, "int32", (n,), "pos", dev), po, so, _current(stream, dev)))
 
+    def append_axes(self, layer, seqs, q, k, v, q_out, pos, axes, q_norm=None, k_norm=None, eps=1e-6, theta=1e6, stream=None):
+        """tie_hip_kv_append_axes: append with pos [n_axes][n_tokens]; axes: the axis of each of a head's head_dim / 2 pairs
+        (small whole numbers, or bytes)."""
+        n, dev, axes = seqs.n_tokens, self.device, bytes(axes)
+        if len(axes) != self.head_dim // 2:
+            raise ValueError("axes: one for each of %d pairs is wanted (got %d)" % (self.head_dim // 2, len(axes)))
+        pq, sq, po, so, heads = self._q(q, q_out, seqs, "q_out")
+        pk, sk, _ = _rows(k, "k", dev, self.width, n)
+        pv, sv, _ = _rows(v, "v", dev, self.width, n)
+        n_axes = pos.shape[0]
+        check(lib().tie_hip_kv_append_axes(self.ref, layer, seqs.ref, pq, sq, pk, sk, pv, sv, heads,
+                                           _array(q_norm, "float32", self.head_shape, "q_norm", dev),
+                                           _array(k_norm, "float32", self.head_shape, "k_norm", dev), eps, theta,
+                                           _array(pos, "int32", (n_axes, n), "pos", dev), n_axes, axes, po, so,
+                                           _current(stream, dev)))
+
     def read(self, seqs, k_out, v_out, layer=0, n_layers=1, stream=None):
         """tie_hip_kv_read: rows of the cache as float32 [n_layers][n_tokens][kv_heads][head_dim]."""
         self._seqs(seqs)
@@ -637,6 +674,19 @@ class KVCache:
                                            _array(mask, "int64", (seqs.n_tokens, words), "mask", self.device), words, po, so, pw,
                                            nw, _current(stream, self.device)))
 
+    def window_attention(self, layer, seqs, q, out, scale, window, sinks=0, at=None, mask=None, work=None, stream=None):
+        """tie_hip_window_attention: attention through a sliding window and over the first `sinks` rows; at: int32 [n_tokens],
+        the row that each token's window goes by (None: its own)."""
+        pq, sq, po, so, heads = self._q(q, out, seqs, "out")
+        words, (pw, nw) = 0 if mask is None else mask.shape[1], _work(work, self.device)
+        check(lib().tie_hip_window_attention(self.ref, layer, seqs.ref, pq, sq, heads, scale, window, sinks,
+                                             _array(at, "int32", (seqs.n_tokens,), "at", self.device),
+                                             _array(mask, "int64", (seqs.n_tokens, words), "mask", self.device), words, po, so, pw,
+                                             nw, _current(stream, self.device)))
+
+    def window_attention_work_bytes(self, seqs, n_heads):
+        return lib().tie_hip_window_attention_work_bytes(self.ref, seqs.ref, n_heads)
+
     def attention_work_bytes(self, seqs, n_heads):
         return lib().tie_hip_tree_attention_work_bytes(self.ref, seqs.ref, n_heads)
 
@@ -647,6 +697,65 @@ class KVCache:
         check(lib().tie_hip_kv_keep(self.ref, seqs.ref, _array(path, "int32", (seqs.n_seqs, path.shape[1]), "path", dev),
                                     path.shape[1], _array(n_keep, "int32", (seqs.n_seqs,), "n_keep", dev),
                                     _array(len_out, "int32", (seqs.n_seqs,), "len_out", dev), _current(stream, dev)))
+
+
+class KVPool:
+    """The free pages of a cache in the caller's tensors (tie_hip_kv_pool): a ring `free` [n_pages] and `state` [2], the place
+    of its first page and how many there are, both int32.  Stream as for KVCache."""
+
+    def __init__(self, free, state):
+        self.device, self.n_pages, self.keep_alive = free.get_device(), free.shape[0], (free, state)
+        self.desc = KVPoolDesc(self.n_pages, _array(free, "int32", (self.n_pages,), "free", self.device),
+                               _array(state, "int32", (2,), "state", self.device), None)
+
+    def plan(self, pages, lens, n_new, pages_out, first, pos=None, slot=None, n_tokens=None, state_out=None, window=0, sinks=0,
+             work=None, stream=None):
+        """tie_hip_kv_plan: the step's page table, ranges of token rows, positions and slots, and the pool behind it (state_out
+        None: in `state` itself).  n_tokens: the most token rows, where neither pos nor slot says it."""
+        dev, (n_seqs, max_pages) = self.device, pages.shape
+        if dev != _device:
+            _on_device(dev, dev, "free")
+        if n_tokens is None:
+            sized = pos if pos is not None else slot
+            if sized is None:
+                raise ValueError("n_tokens: wanted where there is neither pos nor slot")
+            n_tokens = sized.shape[0]
+        d, (pw, nw) = self.desc, _work(work, dev)
+        pool = KVPoolDesc(d.n_pages, d.free, d.state, d.state if state_out is None else _array(state_out, "int32", (2,), "state_out", dev))
+        check(lib().tie_hip_kv_plan(ctypes.byref(pool), n_seqs, max_pages, n_tokens,
+                                    _array(pages, "int32", (n_seqs, max_pages), "pages", dev),
+                                    _array(lens, "int32", (n_seqs,), "lens", dev), _array(n_new, "int32", (n_seqs,), "n_new", dev),
+                                    window, sinks, _array(pages_out, "int32", (n_seqs, max_pages), "pages_out", dev),
+                                    _array(first, "int32", (n_seqs + 1,), "first", dev),
+                                    _array(pos, "int32", (n_tokens,), "pos", dev), _array(slot, "int32", (n_tokens,), "slot", dev),
+                                    pw, nw, _current(stream, dev)))
+
+
+def kv_plan_work_bytes(n_seqs):
+    return lib().tie_hip_kv_plan_work_bytes(n_seqs)
+
+
+def token_logprobs_work_bytes(vocab, n_tokens, n_top):
+    return lib().tie_hip_token_logprobs_work_bytes(vocab, n_tokens, n_top)
+
+
+def token_logprobs(logits, tokens=None, logprob=None, rank=None, entropy=None, top_tokens=None, top_logprobs=None, temperature=1.0,
+                   work=None, stream=None):
+    """tie_hip_token_logprobs: for each row of logits the log-probability and rank of its token, the entropy, and the likeliest
+    tokens (top_tokens [n][n_top] int32 with top_logprobs); the outputs that are given are written.  Stream as for KVCache."""
+    n, dev = logits.shape[0], logits.get_device()
+    if dev != _device:
+        _on_device(dev, dev, "logits")
+    pl, sl, vocab = _rows(logits, "logits", dev)
+    n_top, (pw, nw) = 0 if top_tokens is None else top_tokens.shape[1], _work(work, dev)
+    if (top_tokens is None) != (top_logprobs is None):
+        raise ValueError("top_tokens and top_logprobs go together")
+    check(lib().tie_hip_token_logprobs(pl, sl, vocab, n, _array(tokens, "int32", (n,), "tokens", dev), temperature, n_top,
+                                       _array(logprob, "float32", (n,), "logprob", dev), _array(rank, "int32", (n,), "rank", dev),
+                                       _array(entropy, "float32", (n,), "entropy", dev),
+                                       _array(top_tokens, "int32", (n, n_top), "top_tokens", dev),
+                                       _array(top_logprobs, "float32", (n, n_top), "top_logprobs", dev), pw, nw,
+                                       _current(stream, dev)))
 
 
 def verify_tree_work_bytes(vocab, n_tokens, max_children, with_draft):

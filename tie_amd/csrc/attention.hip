@@ -127,6 +127,11 @@ __device__ __forceinline__ float pow2_below(float x)
 // (a workgroup) for each.  Every workgroup finds the cut by itself from
 // the lengths on the device, so that neither a copy to the host nor a launch
 // for a plan stands before the attention and captured calls follow the lengths.
+__device__ __forceinline__ int div_up(int a, int b)
+{
+	return (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b);
+}
+
 struct Cut {
 	int cap;   // units that run at once: at most so many where tiles are cut
 	int full;  // so many tiles are not cut
@@ -148,8 +153,37 @@ __device__ __forceinline__ int wave_sum(int x)
 	return (int)wave_total((double)x);
 }
 
-__device__ __forceinline__ void seq_work(const KvSeqs &s, int b, int group, int rows, int &t0, int &n, int &len, int &tiles,
-					 int &pages)
+// The first row that a token at row `stand` sees through a window, 0 or more.
+__device__ __forceinline__ int window_low(int stand, int window)
+{
+	const long long low = (long long)stand - window + 1;
+	return low > 0 ? (int)low : 0;
+}
+
+// The pages of a tile that sees nothing below row `low` but the first rows: page i
+// of them is page i of the sequence below `sinks`, else i + skip.  all: the pages of
+// the sequence up to the last that the tile sees.
+struct Span {
+	int sinks, skip, pages;
+	__device__ __forceinline__ int page(int i) const
+	{
+		return i < sinks ? i : i + skip;
+	}
+};
+
+__device__ __forceinline__ Span window_span(int low, int sinks, int all)
+{
+	const int from = min(low / PAGE, all);
+	Span w;
+	w.sinks = min(div_up(sinks, PAGE), from);
+	w.skip = from - w.sinks;
+	w.pages = all - w.skip;
+	return w;
+}
+
+template <bool WIN>
+__device__ __forceinline__ void seq_work(const KvSeqs &s, const AttnArgs &a, int b, int group, int rows, int &t0, int &n, int &len,
+					 int &tiles, int &pages)
 {
 	t0 = n = len = tiles = pages = 0;
 	if (b >= s.n_seqs)
@@ -160,11 +194,17 @@ __device__ __forceinline__ void seq_work(const KvSeqs &s, int b, int group, int 
 		return;
 	tiles = (int)(((long long)n * group + rows - 1) / rows);
 	pages = seq_fits(s, len, n) ? (len + n + PAGE - 1) / PAGE : 1;
-}
-
-__device__ __forceinline__ int div_up(int a, int b)
-{
-	return (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b);
+	if (WIN && seq_fits(s, len, n)) {
+		// what the first tile sees, and no tile more than these: its tokens' windows
+		// together, on one page more than they fill
+		const int all = pages;
+		pages = window_span(window_low(len, a.window), a.sinks, all).pages;
+		if (tiles > 1 && !a.mask) {
+			const long long span = (long long)a.window + (rows + group - 2) / group;
+			const long long most = div_up(a.sinks, PAGE) + span / PAGE + 2;
+			pages = (int)(most < all ? most : all);
+		}
+	}
 }
 
 // Parts of a tile for a grain of its pages, so that no more than cap units come
@@ -176,7 +216,9 @@ __device__ __forceinline__ int tile_parts(const Cut &cut, int pages, float rate)
 	return p < 2 || grains <= cut.alone ? 1 : p < most ? p : most;
 }
 
-__device__ __forceinline__ float part_rate(const KvSeqs &s, int kvh, int group, const Cut &cut, int tiles0, int pages0)
+template <bool WIN>
+__device__ __forceinline__ float part_rate(const KvSeqs &s, const AttnArgs &a, int kvh, int group, const Cut &cut, int tiles0,
+					   int pages0)
 {
 	if (cut.whole)
 		return 0.0f;
@@ -185,7 +227,7 @@ __device__ __forceinline__ float part_rate(const KvSeqs &s, int kvh, int group, 
 		double x = f(tiles0, pages0);
 		for (int b = 64 + lane; b < s.n_seqs; b += 64) {
 			int t0, n, len, tiles, pages;
-			seq_work(s, b, group, cut.rows, t0, n, len, tiles, pages);
+			seq_work<WIN>(s, a, b, group, cut.rows, t0, n, len, tiles, pages);
 			x += f(tiles, pages);
 		}
 		return s.n_seqs > 1 ? wave_total(x) : of_lane(x, 0);
@@ -206,12 +248,13 @@ __device__ __forceinline__ float part_rate(const KvSeqs &s, int kvh, int group, 
 // The unit of workgroup `index`; false past the last.  Units of a sequence:
 // kv heads innermost (workgroups go to the dies in turn: a die then has few
 // heads' pages in its L2), then parts, then tiles.
-__device__ __forceinline__ bool find_unit(const KvSeqs &s, int kvh, int group, const Cut &cut, int index, Unit &u)
+template <bool WIN>
+__device__ __forceinline__ bool find_unit(const KvSeqs &s, const AttnArgs &a, int kvh, int group, const Cut &cut, int index, Unit &u)
 {
 	const int lane = threadIdx.x & 63;
 	int t0, n, len, tiles, pages;
-	seq_work(s, lane, group, cut.rows, t0, n, len, tiles, pages);
-	const float rate = part_rate(s, kvh, group, cut, tiles, pages);
+	seq_work<WIN>(s, a, lane, group, cut.rows, t0, n, len, tiles, pages);
+	const float rate = part_rate<WIN>(s, a, kvh, group, cut, tiles, pages);
 	int before = 0;
 	for (int b0 = 0;;) {
 		const int parts = tiles ? tile_parts(cut, pages, rate) : 0, mine = tiles * parts * kvh;
@@ -244,15 +287,16 @@ __device__ __forceinline__ bool find_unit(const KvSeqs &s, int kvh, int group, c
 		b0 += 64;
 		if (b0 >= s.n_seqs)
 			return false;
-		seq_work(s, b0 + lane, group, cut.rows, t0, n, len, tiles, pages);
+		seq_work<WIN>(s, a, b0 + lane, group, cut.rows, t0, n, len, tiles, pages);
 	}
 }
 
-// The first page of the unit's part, and behind its last.
-__device__ __forceinline__ void part_pages(const Cut &cut, const Unit &u, int pages, int &p0, int &p1)
+// The first page of the unit's part, and behind its last.  all: the pages that the
+// tile's parts share out.
+__device__ __forceinline__ void part_pages(const Cut &cut, const Unit &u, int all, int pages, int &p0, int &p1)
 {
 	// (in grains where a part has few of them, else to the page)
-	const int all = (u.len + u.n + PAGE - 1) / PAGE, grain = all / u.parts < 4 * cut.grain ? cut.grain : 1;
+	const int grain = all / u.parts < 4 * cut.grain ? cut.grain : 1;
 	const int grains = div_up(all, grain), q = grains / u.parts, r = grains % u.parts;
 	p0 = (u.part * q + min(u.part, r)) * grain;
 	p1 = min(pages, p0 + (q + (u.part < r)) * grain);
@@ -280,6 +324,56 @@ __device__ __forceinline__ uint64_t sees(const AttnArgs &a, const Unit &u, int n
 		w |= m[word + 1] << (64 - sh);
 	w &= below((long long)u.n - rel); // no bit names a node that is not there
 	return w | below(-(long long)rel);
+}
+
+// The same through a window whose lowest row is `low`: committed rows below it are
+// not seen but the first a.sinks; of the sequence's own tokens the mask's stand as
+// they are, and a causal row's go by the window too.
+template <bool WIN>
+__device__ __forceinline__ uint64_t sees_through(const AttnArgs &a, const Unit &u, int node, int low, int start)
+{
+	uint64_t w = sees(a, u, node, start);
+	if (WIN && w) {
+		auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
+		uint64_t near = ~below(low - start) | below(a.sinks - start);
+		if (a.mask)
+			near |= ~below(u.len - start);
+		w &= near;
+	}
+	return w;
+}
+
+// The lowest row that a token sees, but for the first ones.
+__device__ __forceinline__ int low_of(const AttnArgs &a, const Unit &u, int node)
+{
+	return window_low(a.at ? a.at[u.t0 + node] : u.len + node, a.window);
+}
+
+// min and max over the wave
+__device__ __forceinline__ int wave_least(int x)
+{
+#pragma unroll
+	for (int k = 1; k < 64; k <<= 1)
+		x = min(x, __shfl_xor(x, k));
+	return __builtin_amdgcn_readfirstlane(x);
+}
+
+// The least and the largest `low` of a tile's tokens, nodes n0 .. n1.
+__device__ __forceinline__ void tile_lows(const AttnArgs &a, const Unit &u, int n0, int n1, int &least, int &most)
+{
+	if (!a.at) {
+		least = window_low(u.len + n0, a.window);
+		most = window_low(u.len + n1, a.window);
+		return;
+	}
+	int lo = 0x7fffffff, hi = 0;
+	for (int i = n0 + (int)(threadIdx.x & 63); i <= n1; i += 64) {
+		const int x = low_of(a, u, i);
+		lo = min(lo, x);
+		hi = max(hi, x);
+	}
+	least = wave_least(lo);
+	most = -wave_least(-hi);
 }
 
 // Results of a part, for each row of its tile: O [HD], the maximum, the sum.
@@ -612,7 +706,7 @@ __device__ __forceinline__ void get_pair(const uint64_t *p, float &x, float &y)
 	y = __uint_as_float((uint32_t)(v >> 32));
 }
 
-template <int HD, bool I8>
+template <int HD, bool I8, bool WIN>
 __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, float *part,
 								       int *count)
 {
@@ -623,7 +717,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 	extern __shared__ __attribute__((aligned(16))) float lds[];
 	const int group = a.n_heads / c.kvh;
 	Unit u;
-	if (!find_unit(s, c.kvh, group, cut, blockIdx.x, u))
+	if (!find_unit<WIN>(s, a, c.kvh, group, cut, blockIdx.x, u))
 		return;
 	const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -633,16 +727,28 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 	const int node = row / group < u.n ? row / group : -1;
 	// (causal: nothing behind the tile's last token is seen)
 	const int last = a.mask ? u.n : min(u.n, (u.tile * R + R - 1) / group + 1);
-	const int pages = bad ? 0 : (u.len + last + PAGE - 1) / PAGE;
+	int pages = bad ? 0 : (u.len + last + PAGE - 1) / PAGE, shared = (u.len + u.n + PAGE - 1) / PAGE;
+	Span span = {0, 0, 0};
+	int low = 0;
+	if (WIN) {
+		int least, most;
+		const int n0 = u.tile * R / group, n1 = min(u.n, (u.tile * R + R - 1) / group + 1) - 1;
+		tile_lows(a, u, n0, n1, least, most);
+		low = node < 0 ? 0 : low_of(a, u, node);
+		// (a mask names its own tokens whatever the window)
+		span = window_span(a.mask ? min(least, u.len) : least, a.sinks, pages);
+		shared = pages = span.pages;
+	}
 	int p0, p1;
-	part_pages(cut, u, pages, p0, p1);
+	part_pages(cut, u, shared, pages, p0, p1);
 	const int steps = (p1 - p0) * SP;
 
 	u4 kr[KT][KL], vr[MT];
 	float ks = 0.0f, vs = 0.0f; // int8: the scales of the lane's row
 	size_t at = 0; // of the page whose V is in (or on its way to) vr
 	auto page = [&](int step) {
-		const int id = __builtin_amdgcn_readfirstlane(page_of(s, c.n_pages, u.b, (p0 + step / SP) * PAGE));
+		const int p = WIN ? span.page(p0 + step / SP) : p0 + step / SP;
+		const int id = __builtin_amdgcn_readfirstlane(page_of(s, c.n_pages, u.b, p * PAGE));
 		bad = bad || id < 0;
 		return (size_t)(id < 0 ? 0 : id) * c.kvh + u.head;
 	};
@@ -683,8 +789,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attn_few_kernel(KvLayer c, 
 	float up = V_UP;
 
 	for (int step = wave; step < steps; step += WK) {
-		const int start = (p0 + step / SP) * PAGE, row0 = step % SP * 32, end = u.len + u.n - start - row0;
-		const uint64_t vis = sees(a, u, node, start) >> row0;
+		const int start = (WIN ? span.page(p0 + step / SP) : p0 + step / SP) * PAGE, row0 = step % SP * 32;
+		const int end = u.len + u.n - start - row0;
+		const uint64_t vis = sees_through<WIN>(a, u, node, low, start) >> row0;
 		constexpr uint64_t all = KT == 4 ? ~0ull : 0xffffffffull;
 		const bool whole = __all((vis & all) == all || node < 0);
 		const bool more = step + WK < steps;
@@ -887,17 +994,17 @@ constexpr int MANY_WAVES = 4;
 // that, and is 0.6 us slower this way).
 struct PageIds {
 	int first, ids; // pages first .. first + 63
-	__device__ __forceinline__ void get(const KvSeqs &s, const Unit &u, int p)
+	__device__ __forceinline__ void get(const KvSeqs &s, const Unit &u, const Span &w, int p)
 	{
 		first = p;
-		const int at = p + (int)(threadIdx.x & 63);
+		const int at = w.page(p + (int)(threadIdx.x & 63));
 		ids = at < s.max_pages ? s.pages[(size_t)u.b * s.max_pages + at] : -1;
 	}
 	// the number of page p, p not below the last one asked for; bad: it is none
-	__device__ __forceinline__ int of(const KvSeqs &s, const Unit &u, int n_pages, int p, bool &bad)
+	__device__ __forceinline__ int of(const KvSeqs &s, const Unit &u, const Span &w, int n_pages, int p, bool &bad)
 	{
 		if (p - first >= 64)
-			get(s, u, p);
+			get(s, u, w, p);
 		const int id = __builtin_amdgcn_readlane(ids, p - first);
 		const bool ok = id >= 0 && id < n_pages;
 		bad = bad || !ok;
@@ -905,7 +1012,7 @@ struct PageIds {
 	}
 };
 
-template <int HD, bool I8, int RG>
+template <int HD, bool I8, int RG, bool WIN>
 __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, float *part)
 {
 	constexpr int KS = HD / 32, MT = HD / 16, R = 32 * RG, NT = 2, KT = 2, E = I8 ? 1 : 2;
@@ -919,23 +1026,32 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 	int index = blockIdx.x;
 	if (cut.whole && (int)gridDim.x <= cut.cap && index >= cut.cap / 2)
 		index = (int)gridDim.x - 1 - (index - cut.cap / 2);
-	if (!find_unit(s, c.kvh, group, cut, index, u))
+	if (!find_unit<WIN>(s, a, c.kvh, group, cut, index, u))
 		return;
 	const int tid = threadIdx.x, lane = tid & 63, n16 = lane & 15, g = lane >> 4;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	bool bad = !seq_fits(s, u.len, u.n);
 
 	const int last = a.mask ? u.n : min(u.n, (u.tile * R + R - 1) / group + 1);
-	const int pages = bad ? 0 : (u.len + last + PAGE - 1) / PAGE;
-	int p0, p1;
-	part_pages(cut, u, pages, p0, p1);
+	int pages = bad ? 0 : (u.len + last + PAGE - 1) / PAGE, shared = (u.len + u.n + PAGE - 1) / PAGE;
 	const int all_below = u.len + (a.mask ? 0 : u.tile * R / group + 1); // rows below it every query of the tile sees
+	Span span = {0, 0, 0};
+	int all_above = 0; // (a window: and from it on)
+	if (WIN) {
+		int least;
+		const int n0 = u.tile * R / group, n1 = min(u.n, (u.tile * R + R - 1) / group + 1) - 1;
+		tile_lows(a, u, n0, n1, least, all_above);
+		span = window_span(a.mask ? min(least, u.len) : least, a.sinks, pages);
+		shared = pages = span.pages;
+	}
+	int p0, p1;
+	part_pages(cut, u, shared, pages, p0, p1);
 	PageIds ids;
-	ids.get(s, u, p0);
+	ids.get(s, u, span, p0);
 	u4 codes[I8 ? NL : 1];
 	float sr = 0.0f;
 	auto page = [&](int p) {
-		return (size_t)ids.of(s, u, c.n_pages, p, bad) * c.kvh + u.head;
+		return (size_t)ids.of(s, u, span, c.n_pages, p, bad) * c.kvh + u.head;
 	};
 	// where a K row's and a V column's pieces lie
 	auto kx = [](int row) { return ((row & 3) | (row >> 3 & 3) << 2) & (KP - 1); };
@@ -1037,12 +1153,12 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 	__syncthreads();
 
 	for (int p = p0; p < p1; p++) {
-		const int b = (p - p0) & 1, start = p * PAGE, end = u.len + u.n - start;
+		const int b = (p - p0) & 1, start = (WIN ? span.page(p) : p) * PAGE, end = u.len + u.n - start;
 		const bool more = p + 1 < p1;
 		const size_t next = more ? page(p + 1) : at;
 		if (!I8 && more)
 			get(next, b ^ 1); // (all waves left that buffer at the last barrier)
-		const bool seen_all = start + PAGE <= all_below;
+		const bool seen_all = start + PAGE <= all_below && (!WIN || start >= all_above || start + PAGE <= a.sinks);
 		uint64_t vis[NT];
 #pragma unroll
 		for (int t = 0; t < NT; t++)
@@ -1050,7 +1166,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 		if (!seen_all)
 #pragma unroll
 			for (int t = 0; t < NT; t++)
-				vis[t] = sees(a, u, node[t], start);
+				vis[t] = sees_through<WIN>(a, u, node[t], WIN && node[t] >= 0 ? low_of(a, u, node[t]) : 0, start);
 		// a page that not all of the tile sees: f16 values that are not finite
 		// are taken out first (see guard_values), and come back below
 		if (!I8 && !seen_all) {
@@ -1261,7 +1377,7 @@ __global__ __launch_bounds__(64 * MANY_WAVES, 2) void attn_many_kernel(KvLayer c
 // at once.  Bound by the parts' bytes and the chain of steps: 26 tokens of 64 heads
 // in 18 parts (16 MB) 8.9 us, of which 2 find the parts.
 constexpr int JOIN_HEADS = 8;
-template <int HD>
+template <int HD, bool WIN>
 __global__ __launch_bounds__(JOIN_HEADS *HD / 4) void attn_join_kernel(KvLayer c, KvSeqs s, AttnArgs a, Cut cut, int units,
 								       const float *part)
 {
@@ -1275,15 +1391,15 @@ __global__ __launch_bounds__(JOIN_HEADS *HD / 4) void attn_join_kernel(KvLayer c
 	// the sequence's units: those of the sequences before it come first
 	const int lane = threadIdx.x & 63;
 	int t0, n, len, tiles, pages;
-	seq_work(s, lane, group, cut.rows, t0, n, len, tiles, pages);
-	const float rate = part_rate(s, c.kvh, group, cut, tiles, pages);
+	seq_work<WIN>(s, a, lane, group, cut.rows, t0, n, len, tiles, pages);
+	const float rate = part_rate<WIN>(s, a, c.kvh, group, cut, tiles, pages);
 	int before = 0;
 	for (int b0 = 0; b0 <= b; b0 += 64) {
 		if (b0)
-			seq_work(s, b0 + lane, group, cut.rows, t0, n, len, tiles, pages);
+			seq_work<WIN>(s, a, b0 + lane, group, cut.rows, t0, n, len, tiles, pages);
 		before += s.n_seqs > 1 ? wave_sum(b0 + lane < b && tiles ? tiles * tile_parts(cut, pages, rate) * c.kvh : 0) : 0;
 	}
-	seq_work(s, b, group, cut.rows, t0, n, len, tiles, pages);
+	seq_work<WIN>(s, a, b, group, cut.rows, t0, n, len, tiles, pages);
 	const int parts = tile_parts(cut, pages, rate);
 	if (parts == 1)
 		return;
@@ -1367,7 +1483,14 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 {
 	const size_t group = a.n_heads / c.kvh, rows = (size_t)s.n_tokens * group;
 	Shape h;
-	h.few = few_of(c, s.max_pages, rows, s.n_seqs);
+	// (what is known here of the pages that a tile sees: the table's columns, or the
+	// window's)
+	size_t columns = s.max_pages;
+	if (a.window) {
+		const size_t seen = ((size_t)a.sinks + PAGE - 1) / PAGE + ((size_t)a.window + PAGE - 2) / PAGE + 1;
+		columns = seen < columns ? seen : columns;
+	}
+	h.few = few_of(c, (int)columns, rows, s.n_seqs);
 	// many: 128 rows where such tiles fill the card (4096 tokens of 32 heads 240
 	// us, by 64 rows 257), or 64: as many units and half the parts' bytes, less
 	// left of tiles that a mask or a sequence's end cuts (1000 tokens over 2000
@@ -1417,8 +1540,9 @@ size_t attention_work_bytes(const KvLayer &c, const KvSeqs &s, const AttnArgs &a
 	for (size_t tile = 64; tile <= 128; tile *= 2) {
 		const size_t r = most_rows(tile, MANY_FULL);
 		// (one sequence's rows are the first that this kernel takes, and it takes
-		// more than FEW_ROWS for each sequence)
-		if (few_of(c, s.max_pages, r, 1) || (tile == 128 && r * c.kvh < (size_t)MANY_FULL * 128))
+		// more than FEW_ROWS for each sequence; with a window it takes them for the
+		// window's sake, which another call may have otherwise)
+		if ((!a.window && few_of(c, s.max_pages, r, 1)) || (tile == 128 && r * c.kvh < (size_t)MANY_FULL * 128))
 			continue;
 		const size_t by_rows = (r - 1) / FEW_ROWS, v = values(r, seqs < by_rows ? seqs : by_rows, tile, MANY_CAP);
 		most = most > v ? most : v;
@@ -1426,23 +1550,23 @@ size_t attention_work_bytes(const KvLayer &c, const KvSeqs &s, const AttnArgs &a
 	return WORK_COUNTERS * sizeof(int) + most * sizeof(float);
 }
 
-template <int HD, bool I8>
+template <int HD, bool I8, bool WIN>
 static hipError_t go(const Shape &h, const KvLayer &c, const KvSeqs &s, const AttnArgs &a, int *count, hipStream_t st)
 {
 	float *part = reinterpret_cast<float *>(count + WORK_COUNTERS);
 	if (h.few) {
 		const size_t lds = (size_t)FEW_WAVES * FEW_ROWS * part_row(HD) * sizeof(float);
-		const hipError_t e = ensure_lds_limit((const void *)attn_few_kernel<HD, I8>, lds);
+		const hipError_t e = ensure_lds_limit((const void *)attn_few_kernel<HD, I8, WIN>, lds);
 		if (e != hipSuccess)
 			return e;
-		tie_launch(attn_few_kernel<HD, I8>, dim3(h.units), dim3(64 * FEW_WAVES), lds, st, c, s, a, h.cut,
+		tie_launch(attn_few_kernel<HD, I8, WIN>, dim3(h.units), dim3(64 * FEW_WAVES), lds, st, c, s, a, h.cut,
 			   part, count);
 		return hipGetLastError();
 	}
-	tie_launch(h.cut.rows == 64 ? attn_many_kernel<HD, I8, 2> : attn_many_kernel<HD, I8, 4>, dim3(h.units), dim3(64 * MANY_WAVES),
-		   0, st, c, s, a, h.cut, part);
+	tie_launch(h.cut.rows == 64 ? attn_many_kernel<HD, I8, 2, WIN> : attn_many_kernel<HD, I8, 4, WIN>, dim3(h.units),
+		   dim3(64 * MANY_WAVES), 0, st, c, s, a, h.cut, part);
 	if (!h.cut.whole)
-		tie_launch(attn_join_kernel<HD>, dim3((size_t)s.n_tokens * ((a.n_heads + JOIN_HEADS - 1) / JOIN_HEADS)),
+		tie_launch(attn_join_kernel<HD, WIN>, dim3((size_t)s.n_tokens * ((a.n_heads + JOIN_HEADS - 1) / JOIN_HEADS)),
 			   dim3(JOIN_HEADS * HD / 4), 0, st, c, s, a, h.cut, (int)h.units, (const float *)part);
 	return hipGetLastError();
 }
@@ -1451,9 +1575,13 @@ hipError_t launch_attention(const KvLayer &c, const KvSeqs &s, const AttnArgs &a
 {
 	const Shape h = attn_shape(c, s, a);
 	int *count = reinterpret_cast<int *>(work);
-	if (c.hd == 128)
-		return c.i8 ? go<128, true>(h, c, s, a, count, st) : go<128, false>(h, c, s, a, count, st);
-	return c.i8 ? go<64, true>(h, c, s, a, count, st) : go<64, false>(h, c, s, a, count, st);
+	auto by_window = [&](auto win) {
+		constexpr bool W = decltype(win)::value;
+		if (c.hd == 128)
+			return c.i8 ? go<128, true, W>(h, c, s, a, count, st) : go<128, false, W>(h, c, s, a, count, st);
+		return c.i8 ? go<64, true, W>(h, c, s, a, count, st) : go<64, false, W>(h, c, s, a, count, st);
+	};
+	return a.window ? by_window(std::true_type()) : by_window(std::false_type());
 }
 
 } // namespace tie

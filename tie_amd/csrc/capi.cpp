@@ -1479,18 +1479,24 @@ static bool rows_overlap(int T, const float *a, size_t sa, size_t wa, const floa
 			return rc_;       \
 	} while (0)
 
-extern "C" int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
-				 size_t q_stride, const float *k, size_t k_stride, const float *v, size_t v_stride, int n_heads,
-				 const float *q_norm, const float *k_norm, float eps, float theta, const int32_t *pos,
-				 float *q_out, size_t q_out_stride, void *stream)
+// n_axes 0: one position for all pairs (axis is not looked at)
+static int append_call(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q, size_t q_stride,
+		       const float *k, size_t k_stride, const float *v, size_t v_stride, int n_heads, const float *q_norm,
+		       const float *k_norm, float eps, float theta, const int32_t *pos, int n_axes, const uint8_t *axis,
+		       float *q_out, size_t q_out_stride, void *stream)
 {
-	std::lock_guard<std::recursive_mutex> lk(g.mu);
-	clear_error();
 	KvLayer l;
 	KvSeqs s;
+	AppendArgs a;
 	TIE_TRY(check_cache(cache, layer, 1, l));
 	TIE_TRY(check_seqs(seqs, s));
 	TIE_TRY(check_heads(l, n_heads));
+	for (int i = 0; n_axes && i < l.hd / 2; i++) {
+		if (axis[i] >= n_axes)
+			return set_error(TIE_HIP_EINVAL, "axis[%d]=%d outside [0, %d)", i, axis[i], n_axes);
+		a.axis[i / 32] |= (uint64_t)axis[i] << i % 32 * 2;
+	}
+	a.axes = n_axes ? n_axes : 1;
 	if (!(theta > 0.0f) || !(theta <= 3.4e38f) || !(eps >= 0.0f))
 		return set_error(TIE_HIP_EINVAL, "theta=%g must be positive and finite, eps=%g not negative", theta, eps);
 	const size_t wq = (size_t)n_heads * l.hd, wk = (size_t)l.kvh * l.hd;
@@ -1507,7 +1513,6 @@ extern "C" int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const
 	TIE_TRY(ensure_init());
 	if (none)
 		return TIE_HIP_OK;
-	AppendArgs a;
 	a.q = q;
 	a.k = k;
 	a.v = v;
@@ -1528,6 +1533,33 @@ extern "C" int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const
 	prof_end(st);
 	HIP_TRY(e);
 	return TIE_HIP_OK;
+}
+
+extern "C" int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
+				 size_t q_stride, const float *k, size_t k_stride, const float *v, size_t v_stride, int n_heads,
+				 const float *q_norm, const float *k_norm, float eps, float theta, const int32_t *pos,
+				 float *q_out, size_t q_out_stride, void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	return append_call(cache, layer, seqs, q, q_stride, k, k_stride, v, v_stride, n_heads, q_norm, k_norm, eps, theta, pos, 0,
+			   nullptr, q_out, q_out_stride, stream);
+}
+
+extern "C" int tie_hip_kv_append_axes(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
+				      size_t q_stride, const float *k, size_t k_stride, const float *v, size_t v_stride,
+				      int n_heads, const float *q_norm, const float *k_norm, float eps, float theta,
+				      const int32_t *pos, int n_axes, const uint8_t *axis, float *q_out, size_t q_out_stride,
+				      void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	if (n_axes < 1 || n_axes > TIE_HIP_MAX_AXES || !axis)
+		return set_error(TIE_HIP_EINVAL, "n_axes=%d outside [1, %d], or null axis", n_axes, TIE_HIP_MAX_AXES);
+	if (!pos && seqs && seqs->n_tokens > 0)
+		return set_error(TIE_HIP_EINVAL, "null pos");
+	return append_call(cache, layer, seqs, q, q_stride, k, k_stride, v, v_stride, n_heads, q_norm, k_norm, eps, theta, pos,
+			   n_axes, axis, q_out, q_out_stride, stream);
 }
 
 extern "C" int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_layers, const tie_hip_kv_seqs *seqs,
@@ -1600,12 +1632,25 @@ extern "C" size_t tie_hip_tree_attention_work_bytes(const tie_hip_kv_cache *cach
 	return attention_work_bytes(l, s, a);
 }
 
-extern "C" int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
-				      size_t q_stride, int n_heads, float scale, const uint64_t *mask, int mask_words,
-				      float *out, size_t out_stride, void *work, size_t work_bytes, void *stream)
+extern "C" size_t tie_hip_window_attention_work_bytes(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, int n_heads)
 {
 	std::lock_guard<std::recursive_mutex> lk(g.mu);
 	clear_error();
+	KvLayer l;
+	KvSeqs s;
+	if (check_cache(cache, 0, 1, l) || check_seqs(seqs, s) || check_heads(l, n_heads) || s.n_seqs == 0)
+		return 0;
+	AttnArgs a = {};
+	a.n_heads = n_heads;
+	a.window = 1; // (whatever it is)
+	return attention_work_bytes(l, s, a);
+}
+
+// a: the window, its first rows and the tokens' places (a.window 0: none)
+static int attention_call(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q, size_t q_stride,
+			  int n_heads, float scale, AttnArgs a, const uint64_t *mask, int mask_words, float *out,
+			  size_t out_stride, void *work, size_t work_bytes, void *stream)
+{
 	KvLayer l;
 	KvSeqs s;
 	TIE_TRY(check_cache(cache, layer, 1, l));
@@ -1630,7 +1675,6 @@ extern "C" int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, 
 	TIE_TRY(ensure_init());
 	if (none)
 		return TIE_HIP_OK;
-	AttnArgs a;
 	a.q = q;
 	a.q_stride = q_stride;
 	a.out = out;
@@ -1642,8 +1686,181 @@ extern "C" int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, 
 	hipStream_t st = stream_of(stream);
 	void *mem = nullptr;
 	TIE_TRY(aux_scratch(st, work, work_bytes, attention_work_bytes(l, s, a), &mem));
-	prof_begin("attention", st);
+	prof_begin(a.window ? "window_attention" : "attention", st);
 	const hipError_t e = launch_attention(l, s, a, mem, st);
+	prof_end(st);
+	HIP_TRY(e);
+	return TIE_HIP_OK;
+}
+
+extern "C" int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
+				      size_t q_stride, int n_heads, float scale, const uint64_t *mask, int mask_words,
+				      float *out, size_t out_stride, void *work, size_t work_bytes, void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	return attention_call(cache, layer, seqs, q, q_stride, n_heads, scale, AttnArgs(), mask, mask_words, out, out_stride, work,
+			      work_bytes, stream);
+}
+
+extern "C" int tie_hip_window_attention(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
+					size_t q_stride, int n_heads, float scale, int window, int sinks, const int32_t *at,
+					const uint64_t *mask, int mask_words, float *out, size_t out_stride, void *work,
+					size_t work_bytes, void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	if (window < 1 || sinks < 0)
+		return set_error(TIE_HIP_EINVAL, "window=%d < 1 or sinks=%d < 0", window, sinks);
+	AttnArgs a;
+	a.window = window;
+	a.sinks = sinks;
+	a.at = at;
+	return attention_call(cache, layer, seqs, q, q_stride, n_heads, scale, a, mask, mask_words, out, out_stride, work, work_bytes,
+			      stream);
+}
+
+static int check_plan(int n_seqs)
+{
+	if (n_seqs < 0 || n_seqs > 65535)
+		return set_error(TIE_HIP_EINVAL, "n_seqs=%d outside [0, 65535]", n_seqs);
+	return TIE_HIP_OK;
+}
+
+extern "C" size_t tie_hip_kv_plan_work_bytes(int n_seqs)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	return check_plan(n_seqs) ? 0 : plan_work_bytes(n_seqs);
+}
+
+extern "C" int tie_hip_kv_plan(const tie_hip_kv_pool *pool, int n_seqs, int max_pages, int n_tokens, const int32_t *pages,
+			       const int32_t *len, const int32_t *n_new, int window, int sinks, int32_t *pages_out, int32_t *first,
+			       int32_t *pos, int32_t *slot, void *work, size_t work_bytes, void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	if (!pool || !pool->free || !pool->state || !pool->state_out)
+		return set_error(TIE_HIP_EINVAL, "null pool, free, state or state_out");
+	if (pool->n_pages < 1 || pool->n_pages > MAX_PAGES)
+		return set_error(TIE_HIP_EINVAL, "n_pages=%d outside [1, %d]", pool->n_pages, MAX_PAGES);
+	TIE_TRY(check_plan(n_seqs));
+	if (max_pages < 1 || max_pages > 0x7fffffff / PAGE)
+		return set_error(TIE_HIP_EINVAL, "max_pages=%d outside [1, %d]", max_pages, 0x7fffffff / PAGE);
+	if (n_tokens < 0 || window < 0 || sinks < 0)
+		return set_error(TIE_HIP_EINVAL, "n_tokens=%d, window=%d or sinks=%d < 0", n_tokens, window, sinks);
+	if (!first || (n_seqs > 0 && (!pages || !len || !n_new || !pages_out)))
+		return set_error(TIE_HIP_EINVAL, "null first, pages, len, n_new or pages_out");
+	{
+		const size_t nb = (size_t)n_seqs * 4, np = nb * max_pages, nt = (size_t)n_tokens * 4, nr = (size_t)pool->n_pages * 4;
+		const void *outs[6] = {pages_out, first, pos, slot, pool->free, pool->state_out}, *ins[4] = {pages, len, n_new, pool->state};
+		const size_t no[6] = {np, nb + 4, pos ? nt : 0, slot ? nt : 0, nr, 8}, ni[4] = {np, nb, nb, 8};
+		for (int o = 0; o < 6; o++) {
+			for (int i = 0; i < 4; i++)
+				if (!(outs[o] == ins[i] && (o == 0 ? i == 0 : o == 5 && i == 3)) && overlap(outs[o], no[o], ins[i], ni[i]))
+					return set_error(TIE_HIP_EINVAL, "an output overlaps an input (pages_out may be pages, "
+									 "state_out may be state)");
+			for (int i = 0; i < o; i++)
+				if (overlap(outs[o], no[o], outs[i], no[i]))
+					return set_error(TIE_HIP_EINVAL, "two of pages_out, first, pos, slot, free and state_out overlap");
+		}
+	}
+	CallersDevice back;
+	TIE_TRY(ensure_init());
+	PlanArgs a;
+	a.pages = pages;
+	a.len = len;
+	a.n_new = n_new;
+	a.pages_out = pages_out;
+	a.ring = pool->free;
+	a.state = pool->state;
+	a.state_out = pool->state_out;
+	a.n_pages = pool->n_pages;
+	a.n_seqs = n_seqs;
+	a.max_pages = max_pages;
+	a.n_tokens = n_tokens;
+	a.window = window;
+	a.sinks = sinks;
+	a.first = first;
+	a.pos = pos;
+	a.slot = slot;
+	hipStream_t st = stream_of(stream);
+	void *mem = nullptr;
+	TIE_TRY(aux_scratch(st, work, work_bytes, plan_work_bytes(n_seqs), &mem));
+	prof_begin("kv_plan", st);
+	const hipError_t e = launch_plan(a, mem, st);
+	prof_end(st);
+	HIP_TRY(e);
+	return TIE_HIP_OK;
+}
+
+static int check_logprobs(int vocab, int n_tokens, int n_top)
+{
+	if (vocab < 1 || vocab > (1 << 24) || n_tokens < 0 || n_tokens > (1 << 24))
+		return set_error(TIE_HIP_EINVAL, "vocab=%d outside [1, 2^24] or n_tokens=%d outside [0, 2^24]", vocab, n_tokens);
+	if (n_top < 0 || n_top > LOGPROB_TOP)
+		return set_error(TIE_HIP_EINVAL, "n_top=%d outside [0, %d]", n_top, LOGPROB_TOP);
+	return TIE_HIP_OK;
+}
+
+extern "C" size_t tie_hip_token_logprobs_work_bytes(int vocab, int n_tokens, int n_top)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	return check_logprobs(vocab, n_tokens, n_top) ? 0 : logprobs_work_bytes(vocab, n_tokens, n_top);
+}
+
+extern "C" int tie_hip_token_logprobs(const float *logits, size_t logits_stride, int vocab, int n_tokens, const int32_t *tokens,
+				      float temperature, int n_top, float *logprob, int32_t *rank, float *entropy,
+				      int32_t *top_tokens, float *top_logprobs, void *work, size_t work_bytes, void *stream)
+{
+	std::lock_guard<std::recursive_mutex> lk(g.mu);
+	clear_error();
+	TIE_TRY(check_logprobs(vocab, n_tokens, n_top));
+	if (logits_stride < (size_t)vocab)
+		return set_error(TIE_HIP_EINVAL, "logits_stride=%zu is below vocab=%d", logits_stride, vocab);
+	if (!(temperature >= 1e-6f) || !(temperature <= 1e6f))
+		return set_error(TIE_HIP_EINVAL, "temperature=%g outside [1e-6, 1e6]", temperature);
+	if (n_tokens > 0 && (!logits || (n_top && (!top_tokens || !top_logprobs))))
+		return set_error(TIE_HIP_EINVAL, "null logits/top_tokens/top_logprobs");
+	if (!tokens && (logprob || rank))
+		return set_error(TIE_HIP_EINVAL, "logprob and rank are of tokens, which is null");
+	{
+		// (rows are read while others' results are written)
+		const size_t nt = (size_t)n_tokens * 4;
+		const void *outs[5] = {logprob, rank, entropy, top_tokens, top_logprobs};
+		const size_t no[5] = {logprob ? nt : 0, rank ? nt : 0, entropy ? nt : 0, n_top ? nt * n_top : 0, n_top ? nt * n_top : 0};
+		for (int o = 0; o < 5; o++) {
+			if (overlap(outs[o], no[o], logits, row_span(n_tokens, logits_stride, vocab)) ||
+			    overlap(outs[o], no[o], tokens, tokens ? nt : 0))
+				return set_error(TIE_HIP_EINVAL, "an output overlaps an input");
+			for (int i = 0; i < o; i++)
+				if (overlap(outs[o], no[o], outs[i], no[i]))
+					return set_error(TIE_HIP_EINVAL, "two outputs overlap");
+		}
+	}
+	CallersDevice back;
+	TIE_TRY(ensure_init());
+	if (n_tokens == 0)
+		return TIE_HIP_OK;
+	LogprobArgs a;
+	a.logits = logits;
+	a.stride = logits_stride;
+	a.vocab = vocab;
+	a.n_rows = n_tokens;
+	a.n_top = n_top;
+	a.tokens = tokens;
+	a.temperature = temperature;
+	a.logprob = logprob;
+	a.entropy = entropy;
+	a.rank = rank;
+	a.top_tokens = top_tokens;
+	a.top_logprobs = top_logprobs;
+	hipStream_t st = stream_of(stream);
+	void *mem = nullptr;
+	TIE_TRY(aux_scratch(st, work, work_bytes, logprobs_work_bytes(vocab, n_tokens, n_top), &mem));
+	prof_begin("logprobs", st);
+	const hipError_t e = launch_logprobs(a, mem, st);
 	prof_end(st);
 	HIP_TRY(e);
 	return TIE_HIP_OK;

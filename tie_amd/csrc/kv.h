@@ -43,22 +43,29 @@ struct AppendArgs {
 	const int32_t *pos;           // [n_tokens], or null: the cache row
 	int n_heads;
 	double eps, log2_theta;
+	// several axes: pos [axes][n_tokens], and two bits for each pair of a head that name its axis
+	int axes = 1;
+	uint64_t axis[2] = {0, 0};
 };
 
 struct AttnArgs {
-	const float *q;
-	size_t q_stride;
-	float *out;
-	size_t o_stride;
-	const uint64_t *mask; // [n_tokens][mask_words], or null: causal
-	int mask_words, n_heads;
-	float scale;
+	const float *q = nullptr;
+	size_t q_stride = 0;
+	float *out = nullptr;
+	size_t o_stride = 0;
+	const uint64_t *mask = nullptr; // [n_tokens][mask_words], or null: causal
+	int mask_words = 0, n_heads = 0;
+	float scale = 0.0f;
+	// a window: rows below `sinks`, and above the row that the token stands at less `window`
+	int window = 0, sinks = 0;
+	const int32_t *at = nullptr; // [n_tokens], or null: the token's own row
 };
 
 hipError_t launch_kv_append(const KvLayer &c, const KvSeqs &s, const AppendArgs &a, hipStream_t st);
 hipError_t launch_kv_read(const KvLayer &c, int n_layers, const KvSeqs &s, float *k_out, float *v_out, hipStream_t st);
 hipError_t launch_kv_keep(const KvLayer &c, int n_layers, const KvSeqs &s, const int32_t *path, int max_path,
 			  const int32_t *n_keep, int32_t *len_out, hipStream_t st);
+// (a.window 0: none)
 size_t attention_work_bytes(const KvLayer &c, const KvSeqs &s, const AttnArgs &a);
 hipError_t launch_attention(const KvLayer &c, const KvSeqs &s, const AttnArgs &a, void *work, hipStream_t st);
 
@@ -74,6 +81,36 @@ struct VerifyArgs {
 constexpr int VERIFY_KIDS = 16; // children of a node that are tried, at most
 size_t verify_work_bytes(const VerifyArgs &a, bool with_draft);
 hipError_t launch_verify(const VerifyArgs &a, void *work, hipStream_t st);
+
+// The pages of a step (plan.hip).
+struct PlanArgs {
+	const int32_t *pages, *len, *n_new; // [n_seqs][max_pages], [n_seqs], [n_seqs]
+	int32_t *pages_out;                 // may be pages
+	int32_t *ring;                      // [n_pages]
+	const int32_t *state;               // [2]
+	int32_t *state_out;                 // may be state
+	int n_pages, n_seqs, max_pages, n_tokens, window, sinks;
+	int32_t *first;      // [n_seqs + 1]
+	int32_t *pos, *slot; // [n_tokens], or null
+};
+size_t plan_work_bytes(int n_seqs);
+hipError_t launch_plan(const PlanArgs &a, void *work, hipStream_t st);
+
+// Log-probabilities of tokens (logprobs.hip).
+struct LogprobArgs {
+	const float *logits;
+	size_t stride;
+	int vocab, n_rows, n_top;
+	const int32_t *tokens; // [n_rows], or null
+	float temperature;
+	float *logprob, *entropy; // [n_rows], or null
+	int32_t *rank;            // [n_rows], or null
+	int32_t *top_tokens;      // [n_rows][n_top]
+	float *top_logprobs;      // [n_rows][n_top]
+};
+constexpr int LOGPROB_TOP = 64; // alternatives, at most
+size_t logprobs_work_bytes(int vocab, int n_rows, int n_top);
+hipError_t launch_logprobs(const LogprobArgs &a, void *work, hipStream_t st);
 
 #if defined(__HIPCC__)
 // x moved across lanes by a DPP control; lanes that get nothing: `none`

@@ -79,8 +79,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 	const bool fits = seq_fits(s, len, n);
 	const int row = fits ? len + (t - t0) : 0;
 	const int page = fits ? page_of(s, c.n_pages, b, row) : -1, r = row % PAGE;
+	const int32_t *pos = a.pos + t;
+	if (a.axes > 1) // (as the pair's axis says: a load for each lane then)
+		pos += (size_t)(a.axis[i / 32] >> i % 32 * 2 & 3) * s.n_tokens;
 	// (no row: no position)
-	const double at = a.pos ? (double)a.pos[t] : fits ? (double)row : __builtin_nan("");
+	const double at = a.pos ? (double)*pos : fits ? (double)row : __builtin_nan("");
 	double cs, sn;
 	sincos(at * exp2((double)i * (-2.0 / HD) * a.log2_theta), &sn, &cs);
 	for (int u = 0; u < per_wave; u++) {
