@@ -4,15 +4,17 @@
 // With x_i = l_i - m, m the largest logit, and T the temperature
 //   Z = sum exp(x_i / T),  log p(i) = x_i / T - log Z,
 //   entropy = -sum p log p = log Z - sum x_i exp(x_i / T) / (T Z).
-// Each lane keeps its own running m with its two sums in 64 bits; they are
-// brought to one m when lanes are joined.  Exponentials are F32 (an ulp each, so that
-// the sums are good to 1e-7 of themselves whatever their length).
+// Each wave keeps a running m (which moves a few times in a row) and each lane its two
+// sums in 64 bits; they are brought to one m when waves are joined.  Exponentials are F32 (an ulp each, so that
+// the sums are good to 1e-7 of themselves whatever their length; the largest logit's
+// is exactly 1, so that a sure token's small logarithm keeps its digits).
 //
-// The n likeliest: a wave keeps the 64 largest so far sorted over its lanes, as
-// 64-bit keys (the logit's order, then the lower index first).  A logit is a
-// candidate if it reaches the n-th of them; candidates gather in LDS and are sorted and
-// merged 64 at a time.  The first bound is the n-th largest of the lanes' own
-// maxima, which n logits reach for certain: then few others do.
+// The n likeliest: each thread keeps the largest of its logits.  n threads have one
+// that reaches the n-th largest of those maxima, so no logit below it is among the n
+// largest, and few threads have more than one that reaches it (n threads of 256 hold the
+// n + n^2 / 512 largest, as a mean): only the chunk that a maximum came from is read
+// again, and all chunks of a thread whose second best chunk reaches it too.  What
+// reaches the bound is sorted, 64 at a time where equal logits bring more.
 //
 // A workgroup has a row, or a part of one where there are few rows; the last
 // of a row's parts to finish joins them.
@@ -21,7 +23,8 @@
 namespace tie {
 
 constexpr int LP_THREADS = 256, LP_WAVES = LP_THREADS / 64, LP_E = 16, LP_CHUNK = LP_THREADS * LP_E;
-constexpr float NONE = -3.402823466e38f; // the lowest finite value
+constexpr int LP_LIST = 1024; // (chunk, thread) whose logits are read again, at most: else all of the threads'
+constexpr float LOWEST = -3.402823466e38f;
 
 // One part's result.
 struct LpPart {
@@ -31,9 +34,9 @@ struct LpPart {
 };
 
 struct LpWork {
-	LpPart *part;  // [rows][parts]
-	uint64_t *top; // [rows][parts][n]
-	int *count;    // [rows]
+	LpPart *part; // [rows][parts]
+	float *most;  // [rows][parts][LP_THREADS] the threads' largest logits
+	int *count;   // [rows]
 };
 
 static int lp_parts(int vocab, int rows)
@@ -43,7 +46,7 @@ static int lp_parts(int vocab, int rows)
 	return rows > WORK_COUNTERS || want < 2 ? 1 : want < chunks ? want : chunks;
 }
 
-static size_t carve_logprobs(int rows, int parts, int n, uint8_t *base, LpWork *w)
+static size_t carve_logprobs(size_t parts, int n, uint8_t *base, LpWork *w)
 {
 	size_t off = WORK_COUNTERS * sizeof(int);
 	auto take = [&](size_t bytes) {
@@ -52,8 +55,8 @@ static size_t carve_logprobs(int rows, int parts, int n, uint8_t *base, LpWork *
 		return base + o;
 	};
 	LpWork v;
-	v.part = (LpPart *)take((size_t)rows * parts * sizeof(LpPart));
-	v.top = (uint64_t *)take((size_t)rows * parts * n * 8);
+	v.part = (LpPart *)take(parts * sizeof(LpPart));
+	v.most = (float *)take(n ? parts * LP_THREADS * sizeof(float) : 0);
 	v.count = (int *)base;
 	if (w)
 		*w = v;
@@ -66,7 +69,7 @@ size_t logprobs_work_bytes(int vocab, int rows, int n)
 {
 	const int chunks = (vocab + LP_CHUNK - 1) / LP_CHUNK, r = rows < 1024 ? rows : 1024;
 	const size_t most = (size_t)r * chunks < 2047 ? (size_t)r * chunks : 2047;
-	return carve_logprobs(1, (int)most, n, nullptr, nullptr);
+	return carve_logprobs(most, n, nullptr, nullptr);
 }
 
 // what one workgroup writes for another of the same launch goes past the dies' caches
@@ -77,6 +80,15 @@ __device__ __forceinline__ void put64(void *p, uint64_t x)
 __device__ __forceinline__ uint64_t get64(const void *p)
 {
 	return __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ void put32(float *p, float x)
+{
+	__hip_atomic_store((uint32_t *)p, __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get32(const float *p)
+{
+	return __uint_as_float(__hip_atomic_load((const uint32_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
 __device__ __forceinline__ uint64_t key_of(float l, int i)
@@ -127,66 +139,36 @@ __device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b)
 	return x;
 }
 
-// the same of floats: sorted, the largest in lane 0
-__device__ __forceinline__ float sort_floats(float x)
-{
-	const int lane = threadIdx.x & 63;
-#pragma unroll
-	for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-		for (int k = size / 2; k > 0; k >>= 1) {
-			const float y = __shfl_xor(x, k);
-			x = ((lane & size) == 0) == ((lane & k) == 0) ? __builtin_fmaxf(x, y) : __builtin_fminf(x, y);
-		}
-	return x;
-}
-
 // A wave's n largest so far.
 struct Best {
-	uint64_t key = 0;    // the lane's, sorted; 0: none
-	uint64_t bound = 0;  // the n-th: candidates are above it
-	float least = NONE;  // its logit
-	int n = 0, held = 0; // candidates that wait in `wait`
+	uint64_t key = 0;   // the lane's, sorted; 0: none
+	uint64_t bound = 0; // candidates are above it: the n-th, or one that n others reach
+	int n = 0, held = 0;      // candidates that wait in `wait`
 	uint64_t *wait = nullptr; // [128]
 
 	__device__ __forceinline__ void merge()
 	{
 		const int lane = threadIdx.x & 63;
-		uint64_t x = lane < held ? wait[lane] : 0;
-		const uint64_t rest = 64 + lane < held ? wait[64 + lane] : 0;
+		const uint64_t x = lane < held ? wait[lane] : 0, rest = 64 + lane < held ? wait[64 + lane] : 0;
 		if (held > 64)
 			wait[lane] = rest;
 		held = held > 64 ? held - 64 : 0;
 		key = merge64(key, sort64(x));
 		const uint64_t last = shfl64(key, n - 1);
-		if (last > bound) {
-			bound = last;
-			least = __builtin_fmaxf(least, logit_of(last));
-		}
+		bound = last > bound ? last : bound;
 	}
-	// the wave's logits x[0 .. E) of indexes i[e]
-	template <typename I> __device__ __forceinline__ void offer(const float (&x)[LP_E], float most, I index)
+	// the keys of the lanes that `in` says
+	__device__ __forceinline__ void offer(bool in, uint64_t k)
 	{
-		if (!__any(most >= least))
+		const unsigned long long set = __ballot(in && k > bound);
+		if (!set)
 			return;
-		// (n lanes have a logit that reaches the n-th of their maxima)
-		if (bound == 0)
-			least = __builtin_fmaxf(least, __shfl(sort_floats(most), n - 1));
-		const int lane = threadIdx.x & 63;
-#pragma unroll
-		for (int e = 0; e < LP_E; e++) {
-			const uint64_t k = key_of(x[e], index(e));
-			const bool in = x[e] >= least && k > bound;
-			const unsigned long long set = __ballot(in);
-			if (!set)
-				continue;
-			if (in)
-				wait[held + __popcll(set & ((1ull << lane) - 1))] = k;
-			held += __popcll(set);
-			__builtin_amdgcn_wave_barrier();
-			if (held >= 64)
-				merge();
-		}
+		if (set >> (threadIdx.x & 63) & 1)
+			wait[held + __popcll(set & ((1ull << (threadIdx.x & 63)) - 1))] = k;
+		held += __popcll(set);
+		__builtin_amdgcn_wave_barrier();
+		if (held >= 64)
+			merge();
 	}
 };
 
@@ -197,32 +179,26 @@ struct Sums {
 	float m = -__builtin_inff();
 };
 
-// b's sums added to a's (rate: log2 e / T)
-__device__ __forceinline__ void add(Sums &a, double s, double t, float m, double rate)
+// b's sums added to a's
+__device__ __forceinline__ void add(Sums &a, const Sums &b, double rate)
 {
-	const float most = __builtin_fmaxf(a.m, m);
+	const float most = __builtin_fmaxf(a.m, b.m);
 	if (most == -__builtin_inff()) {
-		a.s += s; // (0, or NaN)
+		a.s += b.s; // (0, or NaN)
 		return;
 	}
-	const double da = a.m == -__builtin_inff() ? 0.0 : (double)a.m - most, db = m == -__builtin_inff() ? 0.0 : (double)m - most;
-	const double fa = exp2(da * rate), fb = exp2(db * rate);
-	const double s0 = a.s * fa, s1 = s * fb;
-	a.t = a.t * fa + da * s0 + t * fb + db * s1;
-	a.s = s0 + s1;
+	const double da = a.m == -__builtin_inff() ? 0.0 : (double)a.m - most, db = b.m == -__builtin_inff() ? 0.0 : (double)b.m - most;
+	const double fa = exp2(da * rate), fb = exp2(db * rate), sa = a.s * fa, sb = b.s * fb;
+	a.t = a.t * fa + da * sa + b.t * fb + db * sb;
+	a.s = sa + sb;
 	a.m = most;
 }
 
-// over the wave
+// over the wave: one m for all of them first
 __device__ __forceinline__ void join_lanes(Sums &a, double rate)
 {
 	const float most = wave_max(a.m);
-	if (most == -__builtin_inff()) {
-		a.s = wave_total(a.s);
-		a.t = 0.0;
-		return;
-	}
-	const double d = a.m == -__builtin_inff() ? 0.0 : (double)a.m - most, f = exp2(d * rate), s = a.s * f;
+	const double d = a.m > -__builtin_inff() ? (double)a.m - most : 0.0, f = exp2(d * rate), s = a.s * f;
 	a.t = wave_total(a.t * f + d * s);
 	a.s = wave_total(s);
 	a.m = most;
@@ -232,178 +208,345 @@ struct LpShared {
 	uint64_t wait[LP_WAVES][128];
 	uint64_t top[LP_WAVES][64];
 	double s[LP_WAVES], t[LP_WAVES];
-	float m[LP_WAVES];
-	int above[LP_WAVES], flag;
+	float m[LP_WAVES], most[LP_THREADS];
+	int above[LP_WAVES], held[LP_WAVES], list[LP_LIST], listed, flag;
 };
 
-// The waves' results joined, in the first wave.
-__device__ __forceinline__ void join_waves(LpShared &sh, Sums &a, int &above, Best &best, double rate)
+// The waves' results joined, in all of them.
+__device__ __forceinline__ void join_waves(LpShared &sh, Sums &a, int &above, double rate)
 {
 	const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-	join_lanes(a, rate);
-	above = (int)wave_total((double)above);
+	a.s = wave_total(a.s); // (the wave's m is one)
+	a.t = wave_total(a.t);
 	if (lane == 0) {
 		sh.s[wave] = a.s;
 		sh.t[wave] = a.t;
 		sh.m[wave] = a.m;
 		sh.above[wave] = above;
 	}
-	sh.top[wave][lane] = best.key;
 	__syncthreads();
-	if (wave)
-		return;
-	for (int w = 1; w < LP_WAVES; w++) {
-		add(a, sh.s[w], sh.t[w], sh.m[w], rate);
-		above += sh.above[w];
-		if (best.n)
-			best.key = merge64(best.key, sh.top[w][lane]);
-	}
+	a = Sums();
+	if (lane < LP_WAVES)
+		a.s = sh.s[lane], a.t = sh.t[lane], a.m = sh.m[lane];
+	join_lanes(a, rate);
+	above = (sh.above[0] + sh.above[1]) + (sh.above[2] + sh.above[3]);
 }
 
-// The row's outputs (a wave).
-__device__ __forceinline__ void write_row(const LogprobArgs &a, int row, const Sums &d, int above, uint64_t key)
+// A row's distribution, for its outputs.
+struct Row {
+	bool good; // there is one
+	double m, inv, logz;
+	__device__ __forceinline__ float log_p(float l) const
+	{
+		return (float)(((double)l - m) * inv - logz);
+	}
+};
+
+// The place-th of a row's alternatives: a key, or 0 for none.
+__device__ __forceinline__ void write_top(const LogprobArgs &a, int row, const Row &r, int place, uint64_t key)
+{
+	const size_t o = (size_t)row * a.n_top + place;
+	const bool is = r.good && key != 0;
+	a.top_tokens[o] = is ? (int)~(uint32_t)key : -1;
+	a.top_logprobs[o] = !r.good ? __builtin_nanf("") : is ? r.log_p(logit_of(key)) : -__builtin_inff();
+}
+
+// The chunks of a part.
+__device__ __forceinline__ int chunk_from(int chunks, int part, int parts)
+{
+	return (int)((long long)chunks * part / parts);
+}
+
+// What n of the threads' maxima sh.most reach and hardly more (a wave, each for itself), as
+// the upper half of a key: the n-th largest to its sign, exponent and 11 bits, bit by bit
+// from the top, counted in the waves' masks.
+__device__ __forceinline__ uint32_t nth_most(const LpShared &sh, int n)
 {
 	const int lane = threadIdx.x & 63;
-	const bool good = d.m > -__builtin_inff() && d.m < __builtin_inff() && d.s < (double)__builtin_inff(); // (no NaN among them)
-	const double inv = 1.0 / (double)a.temperature, logz = log(d.s);
-	if (lane == 0) {
-		if (a.tokens) {
-			const int token = a.tokens[row];
-			const bool is = good && token >= 0 && token < a.vocab;
-			const float l = is ? a.logits[(size_t)row * a.stride + token] : 0.0f;
-			if (a.logprob)
-				a.logprob[row] = is ? (float)(((double)l - d.m) * inv - logz) : __builtin_nanf("");
-			if (a.rank)
-				a.rank[row] = is ? above : -1;
+	uint32_t v[LP_WAVES], t = 0;
+#pragma unroll
+	for (int i = 0; i < LP_WAVES; i++)
+		v[i] = (uint32_t)(key_of(sh.most[i * 64 + lane], 0) >> 32);
+#pragma unroll
+	for (int bit = 31; bit >= 12; bit--) {
+		const uint32_t c = t | 1u << bit;
+		int count = 0;
+#pragma unroll
+		for (int i = 0; i < LP_WAVES; i++)
+			count += __popcll(__ballot(v[i] >= c));
+		t = count >= n ? c : t;
+	}
+	return t;
+}
+
+// The n likeliest of a row whose threads' maxima are known: a thread's largest logit, the
+// chunk that it is of, and the largest of its other chunks (parts: `mosts` has each part's).
+__device__ __forceinline__ void likeliest(const LogprobArgs &a, LpShared &sh, int row, const Row &r, const float *l, const float *mosts,
+					  int parts, float most, int most_at, float second, bool vec)
+{
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int chunks = (a.vocab + LP_CHUNK - 1) / LP_CHUNK;
+	sh.most[tid] = most;
+	if (tid == 0)
+		sh.listed = 0;
+	__syncthreads();
+	// (none at -infinity)
+	uint32_t nth = nth_most(sh, a.n_top);
+	const uint32_t lowest = (uint32_t)(key_of(LOWEST, 0) >> 32);
+	nth = nth > lowest ? nth : lowest;
+	auto reaches = [&](float x) { return x > -__builtin_inff() && (uint32_t)(key_of(x, 0) >> 32) >= nth; };
+	Best best;
+	best.n = a.n_top;
+	best.wait = sh.wait[wave];
+	best.bound = (uint64_t)nth << 32; // (no key's lower half is 0)
+	// the logits of `count` pairs of chunk and thread again, 16 of a pair: each wave 64
+	// pieces of four at a time
+	auto read_again = [&](int count, auto pair) {
+		for (int p0 = wave * 64; p0 < count * 4; p0 += LP_THREADS * 2) {
+			float x[2][4];
+			int at[2];
+#pragma unroll
+			for (int u = 0; u < 2; u++) {
+				const int p = p0 + u * LP_THREADS + lane;
+				int c = -1, thread = 0;
+				if (p < count * 4)
+					pair(p / 4, c, thread);
+				at[u] = c < 0 ? a.vocab : c * LP_CHUNK + (p % 4 * LP_THREADS + thread) * 4;
+				if (vec && at[u] + 4 <= a.vocab) {
+					const float4 v = *reinterpret_cast<const float4 *>(l + at[u]);
+					x[u][0] = v.x, x[u][1] = v.y, x[u][2] = v.z, x[u][3] = v.w;
+				} else {
+#pragma unroll
+					for (int e = 0; e < 4; e++)
+						x[u][e] = at[u] + e < a.vocab ? l[at[u] + e] : -__builtin_inff();
+				}
+			}
+#pragma unroll
+			for (int u = 0; u < 2; u++)
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					best.offer(reaches(x[u][e]), key_of(x[u][e], at[u] + e));
 		}
-		if (a.entropy)
-			a.entropy[row] = good ? (float)(logz - d.t * inv / d.s) : __builtin_nanf("");
+	};
+	auto put = [&](int c) {
+		const int i = atomicAdd(&sh.listed, 1);
+		if (i < LP_LIST)
+			sh.list[i] = c * LP_THREADS + tid;
+	};
+	if (reaches(most)) {
+		if (parts == 1) {
+			put(most_at);
+			for (int c = 0; reaches(second) && c < chunks; c++)
+				if (c != most_at)
+					put(c);
+		} else {
+			for (int q = 0; q < parts; q++)
+				if (reaches(get32(mosts + (size_t)q * LP_THREADS + tid)))
+					for (int c = chunk_from(chunks, q, parts); c < chunk_from(chunks, q + 1, parts); c++)
+						put(c);
+		}
 	}
-	if (lane < a.n_top) {
-		const size_t o = (size_t)row * a.n_top + lane;
-		const bool is = good && key != 0;
-		a.top_tokens[o] = is ? (int)~(uint32_t)key : -1;
-		a.top_logprobs[o] = !good ? __builtin_nanf("") : is ? (float)(((double)logit_of(key) - d.m) * inv - logz) : -__builtin_inff();
+	__syncthreads();
+	if (sh.listed <= LP_LIST)
+		read_again(sh.listed, [&](int i, int &c, int &thread) {
+			c = sh.list[i] / LP_THREADS;
+			thread = sh.list[i] % LP_THREADS;
+		});
+	else // (equal logits)
+		for (int q = 0; q < chunks; q++)
+			read_again(LP_THREADS, [&](int i, int &c, int &thread) {
+				c = reaches(sh.most[i]) ? q : -1;
+				thread = i;
+			});
+	// where all candidates wait still and are one wave's lot, they are sorted once
+	const bool merged = best.key != 0; // (in lane 0 if in any)
+	if (lane == 0)
+		sh.held[wave] = merged ? 1000 : best.held;
+	__syncthreads();
+	int total = 0, from = 0, w0 = 0;
+	for (int w = 0; w < LP_WAVES; w++) {
+		if (lane >= total) {
+			w0 = w;
+			from = total;
+		}
+		total += sh.held[w];
 	}
+	if (total <= 64) {
+		// (each candidate's place: how many are larger)
+		const uint64_t key = lane < total ? sh.wait[w0][lane - from] : 0;
+		int place = 0;
+		for (int i = 0; i < total; i++) {
+			const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), i) << 32 |
+					       (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key, i);
+			place += other > key;
+		}
+		if (wave == 0 && (lane < total ? place : lane) < a.n_top)
+			write_top(a, row, r, lane < total ? place : lane, key);
+		return;
+	}
+	while (best.held > 0)
+		best.merge();
+	sh.top[wave][lane] = best.key;
+	__syncthreads();
+	if (wave == 0)
+		for (int w = 1; w < LP_WAVES; w++)
+			best.key = merge64(best.key, sh.top[w][lane]);
+	if (wave == 0 && lane < a.n_top)
+		write_top(a, row, r, lane, best.key);
 }
 
 __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, LpWork w, int parts)
 {
 	__shared__ LpShared sh;
-	const int row = (uint32_t)blockIdx.x / (uint32_t)parts, part = (uint32_t)blockIdx.x % (uint32_t)parts, tid = threadIdx.x, lane = tid & 63;
-	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int row = (uint32_t)blockIdx.x / (uint32_t)parts, part = (uint32_t)blockIdx.x % (uint32_t)parts, tid = threadIdx.x;
+	const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const float *l = a.logits + (size_t)row * a.stride;
 	const int chunks = (a.vocab + LP_CHUNK - 1) / LP_CHUNK;
-	const int c0 = (int)((long long)chunks * part / parts), c1 = (int)((long long)chunks * (part + 1) / parts);
-	const int token = a.tokens ? a.tokens[row] : -1;
-	const bool is_token = token >= 0 && token < a.vocab;
-	const float mine = is_token ? l[token] : __builtin_inff();
+	const int c0 = chunk_from(chunks, part, parts), c1 = chunk_from(chunks, part + 1, parts);
 	const bool vec = ((uintptr_t)l & 15) == 0;
-	const double rate = 1.4426950408889634 / (double)a.temperature;
-	const float rate_hi = (float)rate, rate_lo = (float)(rate - (double)rate_hi);
-	const float far = -200.0f / rate_hi; // from there on exp() is 0
-	Sums d;
-	Best best;
-	best.n = a.n_top;
-	best.wait = sh.wait[wave];
-	int above = 0;
-	for (int c = c0; c < c1; c++) {
-		const int base = c * LP_CHUNK;
-		float x[LP_E];
-		auto index = [&](int e) { return base + (e / 4 * LP_THREADS + tid) * 4 + e % 4; };
-		if (vec && base + LP_CHUNK <= a.vocab) {
+	auto index = [&](int c, int e) { return c * LP_CHUNK + (e / 4 * LP_THREADS + tid) * 4 + e % 4; };
+	auto get = [&](int c, float (&x)[LP_E]) {
+		if (vec && (c + 1) * LP_CHUNK <= a.vocab) {
 #pragma unroll
 			for (int e = 0; e < LP_E; e += 4) {
-				const float4 v = reinterpret_cast<const float4 *>(l + base)[e / 4 * LP_THREADS + tid];
+				const float4 v = reinterpret_cast<const float4 *>(l + (size_t)c * LP_CHUNK)[e / 4 * LP_THREADS + tid];
 				x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
 			}
 		} else {
 #pragma unroll
 			for (int e = 0; e < LP_E; e++)
-				x[e] = index(e) < a.vocab ? l[index(e)] : -__builtin_inff();
+				x[e] = index(c, e) < a.vocab ? l[index(c, e)] : -__builtin_inff();
 		}
+	};
+	float next[LP_E];
+	get(c0, next);
+	const int token = a.tokens ? a.tokens[row] : -1;
+	const bool is_token = token >= 0 && token < a.vocab;
+	const float mine = is_token ? l[token] : __builtin_inff();
+	const double rate = 1.4426950408889634 / (double)a.temperature;
+	const float rate32 = (float)rate;
+	const float far = -200.0f / rate32; // from there on exp() is 0
+	Sums d;
+	int above = 0, most_at = 0;
+	float largest = -__builtin_inff(), second = largest;
+	for (int c = c0; c < c1; c++) {
+		float x[LP_E];
+#pragma unroll
+		for (int e = 0; e < LP_E; e++)
+			x[e] = next[e];
+		if (c + 1 < c1)
+			get(c + 1, next);
 		float most = x[0];
 #pragma unroll
 		for (int e = 1; e < LP_E; e++)
 			most = __builtin_fmaxf(most, x[e]);
-		if (a.n_top)
-			best.offer(x, most, index);
+		// (equal logits count where they come before the token: not in chunks behind its own)
+		if (a.rank) {
+			if ((c + 1) * LP_CHUNK <= token) {
 #pragma unroll
-		for (int e = 0; e < LP_E; e++)
-			above += x[e] > mine || (x[e] == mine && index(e) < token);
+				for (int e = 0; e < LP_E; e++)
+					above += __popcll(__ballot(x[e] >= mine));
+			} else if (c * LP_CHUNK > token) {
+#pragma unroll
+				for (int e = 0; e < LP_E; e++)
+					above += __popcll(__ballot(x[e] > mine));
+			} else {
+#pragma unroll
+				for (int e = 0; e < LP_E; e++)
+					above += __popcll(__ballot(x[e] > mine || (x[e] == mine && index(c, e) < token)));
+			}
+		}
+		second = __builtin_fmaxf(second, __builtin_fminf(largest, most));
+		most_at = most > largest ? c : most_at;
+		largest = __builtin_fmaxf(largest, most);
 		if (__any(most > d.m)) {
-			const float m = __builtin_fmaxf(d.m, most);
-			if (d.m > -__builtin_inff() && m > d.m) {
+			const float m = wave_max(largest);
+			if (d.m > -__builtin_inff()) {
 				const double by = (double)d.m - m, f = exp2(by * rate);
 				d.s *= f;
 				d.t = d.t * f + by * d.s;
 			}
 			d.m = m;
 		}
-		const float base_m = d.m == -__builtin_inff() ? 0.0f : d.m;
+		const float m = d.m == -__builtin_inff() ? 0.0f : d.m;
 #pragma unroll
 		for (int e = 0; e < LP_E; e++) {
-			float y = x[e] - base_m;
-			y = y < far ? far : y; // (NaN stays)
-			const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(y, rate_lo, y * rate_hi));
+			const float y = x[e] - m, p = __builtin_amdgcn_exp2f(y * rate32);
 			d.s += (double)p;
-			d.t = __builtin_fma((double)y, (double)p, d.t);
+			// (y of -infinity, whose p is 0)
+			d.t = __builtin_fma((double)__builtin_fmaxf(y, far), (double)p, d.t);
 		}
 	}
-	while (best.held > 0)
-		best.merge();
-	join_waves(sh, d, above, best, rate);
-	if (parts == 1) {
-		if (wave == 0)
-			write_row(a, row, d, above, best.key);
-		return;
-	}
-	LpPart *to = w.part + (size_t)row * parts;
-	uint64_t *tops = w.top + (size_t)row * parts * a.n_top;
-	if (wave == 0) {
-		if (lane == 0) {
+	join_waves(sh, d, above, rate);
+	float *mosts = w.most + (size_t)row * parts * LP_THREADS;
+	if (parts > 1) {
+		LpPart *to = w.part + (size_t)row * parts;
+		if (tid == 0) {
 			put64(&to[part].s, (uint64_t)__double_as_longlong(d.s));
 			put64(&to[part].t, (uint64_t)__double_as_longlong(d.t));
 			put64(&to[part].m, (uint64_t)__float_as_uint(d.m) | (uint64_t)(uint32_t)above << 32);
 		}
-		if (lane < a.n_top)
-			put64(tops + (size_t)part * a.n_top + lane, best.key);
+		if (a.n_top)
+			put32(mosts + (size_t)part * LP_THREADS + tid, largest);
 		// the last of the row's parts joins them: what the parts wrote is there once the
-		// writer's stores are done, which it waits for before it counts
+		// writers' stores are done, which each waits for before its workgroup counts
 		asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-		if (lane == 0) {
+		__syncthreads();
+		if (tid == 0) {
 			const int got = __hip_atomic_fetch_add(w.count + row, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 			sh.flag = got == parts - 1;
 			if (got == parts - 1)
 				__hip_atomic_store(w.count + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 		}
+		__syncthreads();
+		if (!sh.flag)
+			return;
+		// a lane a part, the same in all waves; and a thread a column of the maxima
+		d = Sums();
+		above = 0;
+		for (int q = lane; q < parts; q += 64) {
+			Sums b;
+			b.s = __longlong_as_double((long long)get64(&to[q].s));
+			b.t = __longlong_as_double((long long)get64(&to[q].t));
+			const uint64_t v = get64(&to[q].m);
+			b.m = __uint_as_float((uint32_t)v);
+			above += (int)(v >> 32);
+			if (q == lane)
+				d = b;
+			else
+				add(d, b, rate);
+		}
+		largest = -__builtin_inff();
+		if (a.n_top) {
+#pragma unroll 8
+			for (int q = 0; q < parts; q++)
+				largest = __builtin_fmaxf(largest, get32(mosts + (size_t)q * LP_THREADS + tid));
+		}
+		join_lanes(d, rate);
+		above = (int)wave_total((double)above);
 	}
-	__syncthreads();
-	if (!sh.flag)
-		return;
-	// a lane a part
-	Sums all;
-	int sum = 0;
-	for (int q = tid; q < parts; q += LP_THREADS) {
-		const double s = __longlong_as_double((long long)get64(&to[q].s)), t = __longlong_as_double((long long)get64(&to[q].t));
-		const uint64_t v = get64(&to[q].m);
-		add(all, s, t, __uint_as_float((uint32_t)v), rate);
-		sum += (int)(v >> 32);
+	Row r;
+	r.good = d.m > -__builtin_inff() && d.m < __builtin_inff() && d.s < (double)__builtin_inff(); // (no NaN among them)
+	r.m = d.m;
+	r.inv = 1.0 / (double)a.temperature;
+	r.logz = log(d.s);
+	if (tid == LP_THREADS - 64) { // (the last wave's: the first writes the alternatives)
+		if (a.logprob)
+			a.logprob[row] = r.good && is_token ? r.log_p(mine) : __builtin_nanf("");
+		if (a.rank)
+			a.rank[row] = r.good && is_token ? above : -1;
+		if (a.entropy)
+			a.entropy[row] = r.good ? (float)(r.logz - d.t * r.inv / d.s) : __builtin_nanf("");
 	}
-	best.key = 0;
 	if (a.n_top)
-		for (int q = wave; q < parts; q += LP_WAVES)
-			best.key = merge64(best.key, lane < a.n_top ? get64(tops + (size_t)q * a.n_top + lane) : 0);
-	join_waves(sh, all, sum, best, rate);
-	if (wave == 0)
-		write_row(a, row, all, sum, best.key);
+		likeliest(a, sh, row, r, l, mosts, parts, largest, most_at, second, vec);
 }
 
 hipError_t launch_logprobs(const LogprobArgs &a, void *work, hipStream_t st)
 {
 	const int parts = lp_parts(a.vocab, a.n_rows);
 	LpWork w;
-	carve_logprobs(a.n_rows, parts, a.n_top, (uint8_t *)work, &w);
+	carve_logprobs(parts > 1 ? (size_t)a.n_rows * parts : 0, a.n_top, (uint8_t *)work, &w);
 	tie_launch(logprobs_kernel, dim3((uint32_t)a.n_rows * parts), dim3(LP_THREADS), 0, st, a, w, parts);
 	return hipGetLastError();
 }
