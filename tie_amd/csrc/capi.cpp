@@ -1850,7 +1850,8 @@ extern "C" int tie_hip_token_logprobs(const float *logits, size_t logits_stride,
 	a.n_rows = n_tokens;
 	a.n_top = n_top;
 	a.tokens = tokens;
-	a.temperature = temperature;
+	a.rate = 1.4426950408889634 / (double)temperature;
+	a.inv = 1.0 / (double)temperature;
 	a.logprob = logprob;
 	a.entropy = entropy;
 	a.rank = rank;

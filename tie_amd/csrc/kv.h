@@ -102,7 +102,7 @@ struct LogprobArgs {
 	size_t stride;
 	int vocab, n_rows, n_top;
 	const int32_t *tokens; // [n_rows], or null
-	float temperature;
+	double rate, inv; // log2 e / temperature, 1 / temperature
 	float *logprob, *entropy; // [n_rows], or null
 	int32_t *rank;            // [n_rows], or null
 	int32_t *top_tokens;      // [n_rows][n_top]

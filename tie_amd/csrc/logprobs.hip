@@ -22,6 +22,8 @@
 
 namespace tie {
 
+typedef float f4 __attribute__((ext_vector_type(4)));
+
 constexpr int LP_THREADS = 256, LP_WAVES = LP_THREADS / 64, LP_E = 16, LP_CHUNK = LP_THREADS * LP_E;
 constexpr int LP_LIST = 1024; // (chunk, thread) whose logits are read again, at most: else all of the threads'
 constexpr float LOWEST = -3.402823466e38f;
@@ -119,9 +121,9 @@ __device__ __forceinline__ uint64_t swap64(uint64_t x, int k, bool larger)
 __device__ __forceinline__ uint64_t sort64(uint64_t x)
 {
 	const int lane = threadIdx.x & 63;
-#pragma unroll
+#pragma unroll 1
 	for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
+#pragma unroll 1
 		for (int k = size / 2; k > 0; k >>= 1)
 			x = swap64(x, k, ((lane & size) == 0) == ((lane & k) == 0));
 	return x;
@@ -133,7 +135,7 @@ __device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b)
 	const int lane = threadIdx.x & 63;
 	const uint64_t r = shfl64(b, 63 - lane);
 	uint64_t x = a > r ? a : r;
-#pragma unroll
+#pragma unroll 1
 	for (int k = 32; k > 0; k >>= 1)
 		x = swap64(x, k, (lane & k) == 0);
 	return x;
@@ -177,59 +179,64 @@ struct Best {
 struct Sums {
 	double s = 0.0, t = 0.0;
 	float m = -__builtin_inff();
-};
-
-// b's sums added to a's
-__device__ __forceinline__ void add(Sums &a, const Sums &b, double rate)
-{
-	const float most = __builtin_fmaxf(a.m, b.m);
-	if (most == -__builtin_inff()) {
-		a.s += b.s; // (0, or NaN)
-		return;
+	// to another m, not below its own (rate: log2 e / T)
+	__device__ __forceinline__ void move(float to, double rate)
+	{
+		const double by = m > -__builtin_inff() ? (double)m - to : 0.0, f = exp2(by * rate);
+		s *= f;
+		t = t * f + by * s;
+		m = to;
 	}
-	const double da = a.m == -__builtin_inff() ? 0.0 : (double)a.m - most, db = b.m == -__builtin_inff() ? 0.0 : (double)b.m - most;
-	const double fa = exp2(da * rate), fb = exp2(db * rate), sa = a.s * fa, sb = b.s * fb;
-	a.t = a.t * fa + da * sa + b.t * fb + db * sb;
-	a.s = sa + sb;
-	a.m = most;
-}
-
-// over the wave: one m for all of them first
-__device__ __forceinline__ void join_lanes(Sums &a, double rate)
-{
-	const float most = wave_max(a.m);
-	const double d = a.m > -__builtin_inff() ? (double)a.m - most : 0.0, f = exp2(d * rate), s = a.s * f;
-	a.t = wave_total(a.t * f + d * s);
-	a.s = wave_total(s);
-	a.m = most;
-}
+};
 
 struct LpShared {
 	uint64_t wait[LP_WAVES][128];
 	uint64_t top[LP_WAVES][64];
 	double s[LP_WAVES], t[LP_WAVES];
 	float m[LP_WAVES], most[LP_THREADS];
-	int above[LP_WAVES], held[LP_WAVES], list[LP_LIST], listed, flag;
+	int above, held[LP_WAVES], list[LP_LIST], listed, flag;
 };
 
-// The waves' results joined, in all of them.
-__device__ __forceinline__ void join_waves(LpShared &sh, Sums &a, int &above, double rate)
+// The threads' sums joined, in all of them.
+__device__ __forceinline__ void join_threads(LpShared &sh, Sums &d, double rate)
 {
 	const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-	a.s = wave_total(a.s); // (the wave's m is one)
-	a.t = wave_total(a.t);
+	const float m = wave_max(d.m);
+	if (lane == 0)
+		sh.m[wave] = m;
+	__syncthreads();
+	d.move(__builtin_fmaxf(__builtin_fmaxf(sh.m[0], sh.m[1]), __builtin_fmaxf(sh.m[2], sh.m[3])), rate);
+	d.s = wave_total(d.s);
+	d.t = wave_total(d.t);
 	if (lane == 0) {
-		sh.s[wave] = a.s;
-		sh.t[wave] = a.t;
-		sh.m[wave] = a.m;
-		sh.above[wave] = above;
+		sh.s[wave] = d.s;
+		sh.t[wave] = d.t;
 	}
 	__syncthreads();
-	a = Sums();
-	if (lane < LP_WAVES)
-		a.s = sh.s[lane], a.t = sh.t[lane], a.m = sh.m[lane];
-	join_lanes(a, rate);
-	above = (sh.above[0] + sh.above[1]) + (sh.above[2] + sh.above[3]);
+	d.s = (sh.s[0] + sh.s[1]) + (sh.s[2] + sh.s[3]);
+	d.t = (sh.t[0] + sh.t[1]) + (sh.t[2] + sh.t[3]);
+}
+
+// The logarithm of a sum that is 1 or more, with the digits of what it has above 1: of 2^k
+// f, f from 2/3 to 4/3, k log 2 + 2 artanh((f - 1) / (f + 1)), by its series up to the 17th power
+// (0.2^19 / 19 = 3e-15).
+__device__ __forceinline__ double log_of(double s)
+{
+	int k = (int)(__double_as_longlong(s) >> 52) - 1023;
+	double f = __builtin_amdgcn_ldexp(s, -k); // [1, 2)
+	if (f > 4.0 / 3.0) {
+		f *= 0.5;
+		k++;
+	}
+	const double over = f + 1.0;
+	double inv = __builtin_amdgcn_rcp(over); // (2^-26)
+	inv = __builtin_fma(__builtin_fma(-over, inv, 1.0), inv, inv);
+	const double r = (f - 1.0) * inv, r2 = r * r;
+	double y = 2.0 / 17.0;
+#pragma unroll
+	for (int i = 15; i > 0; i -= 2)
+		y = __builtin_fma(y, r2, 2.0 / i);
+	return __builtin_fma((double)k, 0.69314718055994531, y * r);
 }
 
 // A row's distribution, for its outputs.
@@ -251,23 +258,34 @@ __device__ __forceinline__ void write_top(const LogprobArgs &a, int row, const R
 	a.top_logprobs[o] = !r.good ? __builtin_nanf("") : is ? r.log_p(logit_of(key)) : -__builtin_inff();
 }
 
-// The chunks of a part.
+// The first chunk of a part (of 2^24 logits there are 2^12).
 __device__ __forceinline__ int chunk_from(int chunks, int part, int parts)
 {
-	return (int)((long long)chunks * part / parts);
+	return (int)((uint32_t)chunks * (uint32_t)part / (uint32_t)parts);
 }
 
 // What n of the threads' maxima sh.most reach and hardly more (a wave, each for itself), as
-// the upper half of a key: the n-th largest to its sign, exponent and 11 bits, bit by bit
-// from the top, counted in the waves' masks.
+// the upper half of a key, to its sign, exponent and 11 bits: bit by bit from the top,
+// counted in the wave's masks.  Up to 32 of them: by the lanes' maxima of four
+// threads (64 lanes' hold the n + n^2 / 128 largest, as a mean).
 __device__ __forceinline__ uint32_t nth_most(const LpShared &sh, int n)
 {
 	const int lane = threadIdx.x & 63;
-	uint32_t v[LP_WAVES], t = 0;
+	uint32_t v[LP_WAVES], t = 0, top = 0;
 #pragma unroll
-	for (int i = 0; i < LP_WAVES; i++)
+	for (int i = 0; i < LP_WAVES; i++) {
 		v[i] = (uint32_t)(key_of(sh.most[i * 64 + lane], 0) >> 32);
-#pragma unroll
+		top = max(top, v[i]);
+	}
+	if (n <= 32) {
+#pragma unroll 4
+		for (int bit = 31; bit >= 12; bit--) {
+			const uint32_t c = t | 1u << bit;
+			t = __popcll(__ballot(top >= c)) >= n ? c : t;
+		}
+		return t;
+	}
+#pragma unroll 1
 	for (int bit = 31; bit >= 12; bit--) {
 		const uint32_t c = t | 1u << bit;
 		int count = 0;
@@ -279,16 +297,27 @@ __device__ __forceinline__ uint32_t nth_most(const LpShared &sh, int n)
 	return t;
 }
 
-// The n likeliest of a row whose threads' maxima are known: a thread's largest logit, the
-// chunk that it is of, and the largest of its other chunks (parts: `mosts` has each part's).
-__device__ __forceinline__ void likeliest(const LogprobArgs &a, LpShared &sh, int row, const Row &r, const float *l, const float *mosts,
-					  int parts, float most, int most_at, float second, bool vec)
+// A thread's largest logit so far, the chunk (or part) that it is of, and the largest of
+// its others.
+struct Mosts {
+	float most = -__builtin_inff(), second = most;
+	int at = 0;
+	__device__ __forceinline__ void add(float x, int where)
+	{
+		second = __builtin_fmaxf(second, __builtin_fminf(most, x));
+		at = x > most ? where : at;
+		most = __builtin_fmaxf(most, x);
+	}
+};
+
+// The n likeliest of a row whose threads' maxima are known (where there are parts: of
+// all of them, by part).
+__device__ __forceinline__ void likeliest(const LogprobArgs &a, LpShared &sh, int row, const Row &r, const float *l, int parts,
+					  const Mosts &t, bool vec)
 {
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int chunks = (a.vocab + LP_CHUNK - 1) / LP_CHUNK;
-	sh.most[tid] = most;
-	if (tid == 0)
-		sh.listed = 0;
+	sh.most[tid] = t.most;
 	__syncthreads();
 	// (none at -infinity)
 	uint32_t nth = nth_most(sh, a.n_top);
@@ -299,65 +328,48 @@ __device__ __forceinline__ void likeliest(const LogprobArgs &a, LpShared &sh, in
 	best.n = a.n_top;
 	best.wait = sh.wait[wave];
 	best.bound = (uint64_t)nth << 32; // (no key's lower half is 0)
-	// the logits of `count` pairs of chunk and thread again, 16 of a pair: each wave 64
-	// pieces of four at a time
-	auto read_again = [&](int count, auto pair) {
-		for (int p0 = wave * 64; p0 < count * 4; p0 += LP_THREADS * 2) {
-			float x[2][4];
-			int at[2];
-#pragma unroll
-			for (int u = 0; u < 2; u++) {
-				const int p = p0 + u * LP_THREADS + lane;
-				int c = -1, thread = 0;
-				if (p < count * 4)
-					pair(p / 4, c, thread);
-				at[u] = c < 0 ? a.vocab : c * LP_CHUNK + (p % 4 * LP_THREADS + thread) * 4;
-				if (vec && at[u] + 4 <= a.vocab) {
-					const float4 v = *reinterpret_cast<const float4 *>(l + at[u]);
-					x[u][0] = v.x, x[u][1] = v.y, x[u][2] = v.z, x[u][3] = v.w;
-				} else {
-#pragma unroll
-					for (int e = 0; e < 4; e++)
-						x[u][e] = at[u] + e < a.vocab ? l[at[u] + e] : -__builtin_inff();
-				}
-			}
-#pragma unroll
-			for (int u = 0; u < 2; u++)
-#pragma unroll
-				for (int e = 0; e < 4; e++)
-					best.offer(reaches(x[u][e]), key_of(x[u][e], at[u] + e));
-		}
-	};
-	auto put = [&](int c) {
-		const int i = atomicAdd(&sh.listed, 1);
-		if (i < LP_LIST)
+	if (reaches(t.most)) {
+		// (the chunks of one place: a chunk, or a part)
+		const bool all = reaches(t.second);
+		const int from = all ? 0 : parts == 1 ? t.at : chunk_from(chunks, t.at, parts);
+		const int to = all ? chunks : parts == 1 ? t.at + 1 : chunk_from(chunks, t.at + 1, parts);
+		int i = atomicAdd(&sh.listed, to - from);
+		for (int c = from; c < to && i < LP_LIST; c++, i++)
 			sh.list[i] = c * LP_THREADS + tid;
-	};
-	if (reaches(most)) {
-		if (parts == 1) {
-			put(most_at);
-			for (int c = 0; reaches(second) && c < chunks; c++)
-				if (c != most_at)
-					put(c);
-		} else {
-			for (int q = 0; q < parts; q++)
-				if (reaches(get32(mosts + (size_t)q * LP_THREADS + tid)))
-					for (int c = chunk_from(chunks, q, parts); c < chunk_from(chunks, q + 1, parts); c++)
-						put(c);
-		}
 	}
 	__syncthreads();
-	if (sh.listed <= LP_LIST)
-		read_again(sh.listed, [&](int i, int &c, int &thread) {
-			c = sh.list[i] / LP_THREADS;
-			thread = sh.list[i] % LP_THREADS;
-		});
-	else // (equal logits)
-		for (int q = 0; q < chunks; q++)
-			read_again(LP_THREADS, [&](int i, int &c, int &thread) {
-				c = reaches(sh.most[i]) ? q : -1;
-				thread = i;
-			});
+	// the logits of the listed pairs of chunk and thread again, 16 of a pair, four to a
+	// lane (equal logits may bring more pairs than the list holds: then those of all
+	// threads that have one, chunk by chunk).  One place that sorts: what is not in
+	// the instruction cache yet costs more than the loop
+	const bool all = sh.listed > LP_LIST;
+	const int pairs = all ? LP_THREADS : sh.listed;
+#pragma unroll 1
+	for (int q = 0; q < (all ? chunks : 1); q++)
+#pragma unroll 1
+		for (int p0 = wave * 64; p0 < pairs * 4; p0 += LP_THREADS) {
+			const int p = p0 + lane;
+			int at = a.vocab;
+			if (p < pairs * 4) {
+				const int pair = all ? q * LP_THREADS + p / 4 : sh.list[p / 4], thread = pair % LP_THREADS;
+				if (!all || reaches(sh.most[thread]))
+					at = pair / LP_THREADS * LP_CHUNK + (p % 4 * LP_THREADS + thread) * 4;
+			}
+			float x[4];
+			if (vec && at + 4 <= a.vocab) {
+				const float4 v = *reinterpret_cast<const float4 *>(l + at);
+				x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+			} else {
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					x[e] = at + e < a.vocab ? l[at + e] : -__builtin_inff();
+			}
+#pragma unroll 1
+			for (int e = 0; e < 4; e++) {
+				best.offer(reaches(x[0]), key_of(x[0], at + e));
+				x[0] = x[1], x[1] = x[2], x[2] = x[3];
+			}
+		}
 	// where all candidates wait still and are one wave's lot, they are sorted once
 	const bool merged = best.key != 0; // (in lane 0 if in any)
 	if (lane == 0)
@@ -389,6 +401,7 @@ __device__ __forceinline__ void likeliest(const LogprobArgs &a, LpShared &sh, in
 	sh.top[wave][lane] = best.key;
 	__syncthreads();
 	if (wave == 0)
+#pragma unroll 1
 		for (int w = 1; w < LP_WAVES; w++)
 			best.key = merge64(best.key, sh.top[w][lane]);
 	if (wave == 0 && lane < a.n_top)
@@ -405,11 +418,12 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 	const int c0 = chunk_from(chunks, part, parts), c1 = chunk_from(chunks, part + 1, parts);
 	const bool vec = ((uintptr_t)l & 15) == 0;
 	auto index = [&](int c, int e) { return c * LP_CHUNK + (e / 4 * LP_THREADS + tid) * 4 + e % 4; };
+	// (past the caches: nothing is read twice soon; 2047 rows of 151936 233 us without)
 	auto get = [&](int c, float (&x)[LP_E]) {
 		if (vec && (c + 1) * LP_CHUNK <= a.vocab) {
 #pragma unroll
 			for (int e = 0; e < LP_E; e += 4) {
-				const float4 v = reinterpret_cast<const float4 *>(l + (size_t)c * LP_CHUNK)[e / 4 * LP_THREADS + tid];
+				const f4 v = __builtin_nontemporal_load(reinterpret_cast<const f4 *>(l + (size_t)c * LP_CHUNK) + e / 4 * LP_THREADS + tid);
 				x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
 			}
 		} else {
@@ -423,12 +437,12 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 	const int token = a.tokens ? a.tokens[row] : -1;
 	const bool is_token = token >= 0 && token < a.vocab;
 	const float mine = is_token ? l[token] : __builtin_inff();
-	const double rate = 1.4426950408889634 / (double)a.temperature;
+	const double rate = a.rate;
 	const float rate32 = (float)rate;
 	const float far = -200.0f / rate32; // from there on exp() is 0
 	Sums d;
-	int above = 0, most_at = 0;
-	float largest = -__builtin_inff(), second = largest;
+	Mosts t;
+	int above = 0;
 	for (int c = c0; c < c1; c++) {
 		float x[LP_E];
 #pragma unroll
@@ -456,18 +470,9 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 					above += __popcll(__ballot(x[e] > mine || (x[e] == mine && index(c, e) < token)));
 			}
 		}
-		second = __builtin_fmaxf(second, __builtin_fminf(largest, most));
-		most_at = most > largest ? c : most_at;
-		largest = __builtin_fmaxf(largest, most);
-		if (__any(most > d.m)) {
-			const float m = wave_max(largest);
-			if (d.m > -__builtin_inff()) {
-				const double by = (double)d.m - m, f = exp2(by * rate);
-				d.s *= f;
-				d.t = d.t * f + by * d.s;
-			}
-			d.m = m;
-		}
+		t.add(most, c);
+		if (__any(most > d.m))
+			d.move(wave_max(t.most), rate);
 		const float m = d.m == -__builtin_inff() ? 0.0f : d.m;
 #pragma unroll
 		for (int e = 0; e < LP_E; e++) {
@@ -477,69 +482,97 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 			d.t = __builtin_fma((double)__builtin_fmaxf(y, far), (double)p, d.t);
 		}
 	}
-	join_waves(sh, d, above, rate);
+	// the threads joined; then, where there are parts, the parts by the last of them to
+	// finish, by the same code: it is in the instruction cache then (what is not costs 0.2 us for
+	// each 128 bytes of it, and bounds the short calls)
+	if (tid == 0) {
+		sh.above = 0;
+		sh.listed = 0;
+	}
 	float *mosts = w.most + (size_t)row * parts * LP_THREADS;
-	if (parts > 1) {
-		LpPart *to = w.part + (size_t)row * parts;
+	LpPart *to = w.part + (size_t)row * parts;
+#pragma unroll 1
+	for (bool whole = parts == 1;; whole = true) {
+		join_threads(sh, d, rate);
+		if (whole)
+			break;
+		if (lane == 0)
+			atomicAdd(&sh.above, above);
+		if (a.n_top)
+			put32(mosts + (size_t)part * LP_THREADS + tid, t.most);
 		if (tid == 0) {
 			put64(&to[part].s, (uint64_t)__double_as_longlong(d.s));
 			put64(&to[part].t, (uint64_t)__double_as_longlong(d.t));
-			put64(&to[part].m, (uint64_t)__float_as_uint(d.m) | (uint64_t)(uint32_t)above << 32);
 		}
-		if (a.n_top)
-			put32(mosts + (size_t)part * LP_THREADS + tid, largest);
-		// the last of the row's parts joins them: what the parts wrote is there once the
-		// writers' stores are done, which each waits for before its workgroup counts
+		__syncthreads();
+		if (tid == 0)
+			put64(&to[part].m, (uint64_t)__float_as_uint(d.m) | (uint64_t)(uint32_t)sh.above << 32);
+		// what the parts wrote is there once the writers' stores are done, which each waits
+		// for before its workgroup counts
 		asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 		__syncthreads();
 		if (tid == 0) {
 			const int got = __hip_atomic_fetch_add(w.count + row, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 			sh.flag = got == parts - 1;
+			sh.above = 0;
 			if (got == parts - 1)
 				__hip_atomic_store(w.count + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 		}
 		__syncthreads();
 		if (!sh.flag)
 			return;
-		// a lane a part, the same in all waves; and a thread a column of the maxima
+		// a thread a part, and a column of the maxima
 		d = Sums();
 		above = 0;
-		for (int q = lane; q < parts; q += 64) {
-			Sums b;
-			b.s = __longlong_as_double((long long)get64(&to[q].s));
-			b.t = __longlong_as_double((long long)get64(&to[q].t));
+		for (int q = tid; q < parts; q += LP_THREADS) {
+			const double ps = __longlong_as_double((long long)get64(&to[q].s)), pt = __longlong_as_double((long long)get64(&to[q].t));
 			const uint64_t v = get64(&to[q].m);
-			b.m = __uint_as_float((uint32_t)v);
+			const float m = __uint_as_float((uint32_t)v), most = __builtin_fmaxf(d.m, m);
+			Sums b;
+			b.s = ps, b.t = pt, b.m = m;
 			above += (int)(v >> 32);
-			if (q == lane)
-				d = b;
-			else
-				add(d, b, rate);
+			if (q >= LP_THREADS) { // (a thread's second part)
+				d.move(most, rate);
+				b.move(most, rate);
+			}
+			d.s += b.s, d.t += b.t, d.m = most;
 		}
-		largest = -__builtin_inff();
-		if (a.n_top) {
-#pragma unroll 8
-			for (int q = 0; q < parts; q++)
-				largest = __builtin_fmaxf(largest, get32(mosts + (size_t)q * LP_THREADS + tid));
+		t = Mosts();
+		for (int q0 = 0; a.n_top && q0 < parts; q0 += 8) {
+			float x[8];
+#pragma unroll
+			for (int i = 0; i < 8; i++)
+				x[i] = get32(mosts + (size_t)min(q0 + i, parts - 1) * LP_THREADS + tid);
+#pragma unroll
+			for (int i = 0; i < 8; i++)
+				if (q0 + i < parts)
+					t.add(x[i], q0 + i);
 		}
-		join_lanes(d, rate);
-		above = (int)wave_total((double)above);
 	}
+	// (of parts a thread's own, else a wave's)
+	if (parts > 1 ? above != 0 : lane == 0)
+		atomicAdd(&sh.above, above);
 	Row r;
 	r.good = d.m > -__builtin_inff() && d.m < __builtin_inff() && d.s < (double)__builtin_inff(); // (no NaN among them)
 	r.m = d.m;
-	r.inv = 1.0 / (double)a.temperature;
-	r.logz = log(d.s);
-	if (tid == LP_THREADS - 64) { // (the last wave's: the first writes the alternatives)
+	r.inv = a.inv;
+	r.logz = log_of(d.s);
+	if (a.n_top)
+		likeliest(a, sh, row, r, l, parts, t, vec);
+	else
+		__syncthreads();
+	// (behind all barriers, which wait for stores; by the last wave: the first has written the alternatives)
+	if (tid == LP_THREADS - 64) {
 		if (a.logprob)
 			a.logprob[row] = r.good && is_token ? r.log_p(mine) : __builtin_nanf("");
 		if (a.rank)
-			a.rank[row] = r.good && is_token ? above : -1;
-		if (a.entropy)
-			a.entropy[row] = r.good ? (float)(r.logz - d.t * r.inv / d.s) : __builtin_nanf("");
+			a.rank[row] = r.good && is_token ? sh.above : -1;
+		if (a.entropy) {
+			double inv = __builtin_amdgcn_rcp(d.s); // (2^-26)
+			inv = __builtin_fma(__builtin_fma(-d.s, inv, 1.0), inv, inv);
+			a.entropy[row] = r.good ? (float)(r.logz - d.t * r.inv * inv) : __builtin_nanf("");
+		}
 	}
-	if (a.n_top)
-		likeliest(a, sh, row, r, l, mosts, parts, largest, most_at, second, vec);
 }
 
 hipError_t launch_logprobs(const LogprobArgs &a, void *work, hipStream_t st)
