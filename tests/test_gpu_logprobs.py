@@ -104,6 +104,14 @@ def test_rows_in_parts_and_whole(N, V, n):
     check(some(rng, N, V), rng.integers(0, V, N), 1.0, n, work=True)
 
 
+def test_a_row_of_more_parts_than_a_workgroup_has_threads():
+    rng = np.random.default_rng(2)
+    l = some(rng, 1, 9000001)
+    check(l, np.array([8999999]), 1.0, 20, work=True)
+    l[0, rng.integers(0, 9000001, 5)] = 30.0
+    check(l, np.array([77]), 0.5, 3)
+
+
 @pytest.mark.parametrize("V", [100, 5000, 30000])
 def test_equal_logits(V):
     """The lowest index first among equals: rows of one value, of few values, of -0 and 0, with the token anywhere."""

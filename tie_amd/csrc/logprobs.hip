@@ -25,6 +25,7 @@ namespace tie {
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int LP_THREADS = 256, LP_WAVES = LP_THREADS / 64, LP_E = 16, LP_CHUNK = LP_THREADS * LP_E;
+constexpr int LP_AT_ONCE = 384; // workgroups
 constexpr int LP_LIST = 1024; // (chunk, thread) whose logits are read again, at most: else all of the threads'
 constexpr float LOWEST = -3.402823466e38f;
 
@@ -41,11 +42,16 @@ struct LpWork {
 	int *count;   // [rows]
 };
 
+// A row's parts: enough workgroups for a CU and a half each (a hand-over costs 5 us and the
+// last part's chain 6: 400 rows of 151936 by a workgroup each 49 us, by three 64; 61
+// by seven 22.5, by 17 25 and by five 24.6), and one chunk each, but 16 or more only
+// for rows of more than 8 chunks each (8 rows of 151936 by 16 workgroups each 16.0 us, by 38
+// 19; one 13.5 and 13.6).
 static int lp_parts(int vocab, int rows)
 {
-	// as many workgroups as run at once (four on a CU)
-	const int chunks = (vocab + LP_CHUNK - 1) / LP_CHUNK, want = (1024 + rows - 1) / rows;
-	return rows > WORK_COUNTERS || want < 2 ? 1 : want < chunks ? want : chunks;
+	const int chunks = (vocab + LP_CHUNK - 1) / LP_CHUNK, want = (LP_AT_ONCE + rows - 1) / rows;
+	const int most = chunks < 16 ? chunks : chunks / 8 < 16 ? 16 : chunks / 8;
+	return want < most ? want : most;
 }
 
 static size_t carve_logprobs(size_t parts, int n, uint8_t *base, LpWork *w)
@@ -65,13 +71,12 @@ static size_t carve_logprobs(size_t parts, int n, uint8_t *base, LpWork *w)
 	return off;
 }
 
-// Enough for every call of no more logits, rows and alternatives: rows * parts is at most
-// 1024 + rows, where there are parts.
+// Enough for every call of no more logits, rows and alternatives: where there are parts,
+// there are fewer than 2 LP_AT_ONCE.
 size_t logprobs_work_bytes(int vocab, int rows, int n)
 {
-	const int chunks = (vocab + LP_CHUNK - 1) / LP_CHUNK, r = rows < 1024 ? rows : 1024;
-	const size_t most = (size_t)r * chunks < 2047 ? (size_t)r * chunks : 2047;
-	return carve_logprobs(most, n, nullptr, nullptr);
+	const size_t chunks = ((size_t)vocab + LP_CHUNK - 1) / LP_CHUNK, all = (rows < LP_AT_ONCE ? rows : LP_AT_ONCE) * chunks;
+	return carve_logprobs(all < 2 * LP_AT_ONCE ? all : 2 * LP_AT_ONCE, n, nullptr, nullptr);
 }
 
 // what one workgroup writes for another of the same launch goes past the dies' caches
@@ -538,13 +543,13 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 			d.s += b.s, d.t += b.t, d.m = most;
 		}
 		t = Mosts();
-		for (int q0 = 0; a.n_top && q0 < parts; q0 += 8) {
-			float x[8];
+		for (int q0 = 0; a.n_top && q0 < parts; q0 += 16) {
+			float x[16];
 #pragma unroll
-			for (int i = 0; i < 8; i++)
+			for (int i = 0; i < 16; i++)
 				x[i] = get32(mosts + (size_t)min(q0 + i, parts - 1) * LP_THREADS + tid);
 #pragma unroll
-			for (int i = 0; i < 8; i++)
+			for (int i = 0; i < 16; i++)
 				if (q0 + i < parts)
 					t.add(x[i], q0 + i);
 		}
