@@ -22,12 +22,15 @@
 
 namespace tie {
 
-constexpr int PLAN_BLOCK = 16; // requests of a workgroup
+constexpr int PLAN_BLOCK = 16; // requests of a workgroup, one to a wave
+constexpr int PLAN_THREADS = 64 * PLAN_BLOCK;
 constexpr int PLAN_SMALL = 64; // requests that one workgroup takes alone
 
 struct PlanCounts {
 	int need, want, away; // pages to take, token rows, pages to give back
 	int held;             // pages of its new rows that the table names already
+	int away0;            // the first column whose page goes back
+	int len;
 };
 
 struct PlanWork {
@@ -58,69 +61,68 @@ size_t plan_work_bytes(int n_seqs)
 	return carve_plan(n_seqs, nullptr, nullptr);
 }
 
-// What a request asks for, from its length and count alone.
-struct Request {
-	int len, want;
-	int c0, c1; // columns of its new rows' pages: all but the first may be taken from the ring
-	int fresh0; // from this one on
-	int r0, r1; // columns whose pages go back
-};
-
-__device__ __forceinline__ Request request(const PlanArgs &a, int b)
-{
-	Request r;
-	r.len = a.len[b];
-	const int n = a.n_new[b];
-	const bool good = r.len >= 0 && n >= 0 && (long long)r.len + n <= (long long)a.max_pages * PAGE;
-	r.want = good ? n : 0;
-	r.c0 = r.want ? r.len / PAGE : 0;
-	r.c1 = r.want ? (r.len + r.want - 1) / PAGE + 1 : 0;
-	r.fresh0 = r.want ? r.c0 + (r.len % PAGE != 0) : 0;
-	r.r0 = r.r1 = 0;
-	if (n < 0) { // ended
-		r.r1 = a.max_pages;
-	} else if (a.window) {
-		// (a page whose last row is below the window of the next token, at row len)
-		const long long low = (long long)r.len - a.window + 1;
-		r.r0 = a.sinks / PAGE + (a.sinks % PAGE != 0);
-		r.r1 = low > 0 ? min((int)(low / PAGE), a.max_pages) : 0;
+// The columns of a request's new rows: from c0 on, of which all but the first may be
+// taken from the ring, those from `fresh` on.
+struct Columns {
+	int c0, c1, fresh;
+	__device__ __forceinline__ Columns(int len, int want)
+	{
+		c0 = want ? len / PAGE : 0;
+		c1 = want ? (len + want - 1) / PAGE + 1 : 0;
+		fresh = want ? c0 + (len % PAGE != 0) : 0;
 	}
-	return r;
-}
+};
 
 __device__ __forceinline__ bool is_page(const PlanArgs &a, int id)
 {
 	return id >= 0 && id < a.n_pages;
 }
 
-// A wave: the counts of request b, and its row of the table copied.
+// A wave: the counts of request b, and its row of the table copied.  Columns are loaded
+// PLAN_AHEAD times 64 at a time.
+constexpr int PLAN_AHEAD = 8;
 __device__ __forceinline__ PlanCounts count_request(const PlanArgs &a, int b)
 {
-	const Request r = request(a, b);
 	const int32_t *row = a.pages + (size_t)b * a.max_pages;
 	int32_t *out = a.pages_out + (size_t)b * a.max_pages;
-	const int lane = threadIdx.x & 63;
-	const bool copy = out != row;
-	PlanCounts n = {0, r.want, 0, 0};
-	auto look = [&](int from, int to) {
-		for (int c0 = from; c0 < to; c0 += 64) {
-			const int c = c0 + lane;
-			const int id = c < to ? row[c] : -1;
-			if (copy && c < to)
-				out[c] = id;
-			const bool page = is_page(a, id);
-			n.held += __popcll(__ballot(page && c >= r.fresh0 && c < r.c1));
-			n.away += __popcll(__ballot(page && c >= r.r0 && c < r.r1));
-		}
-	};
-	if (copy) {
-		look(0, a.max_pages);
-	} else {
-		// (the two ranges do not meet)
-		look(r.r0, r.r1);
-		look(r.fresh0, r.c1);
+	const int lane = threadIdx.x & 63, len = a.len[b], more = a.n_new[b];
+	const bool copy = out != row, good = len >= 0 && more >= 0 && (long long)len + more <= (long long)a.max_pages * PAGE;
+	PlanCounts n = {0, good ? more : 0, 0, 0, 0, len};
+	const Columns c(len, n.want);
+	// the columns whose pages go back: all of one that ended; else those whose last row is
+	// below the window of the next token, at row len
+	int r0 = 0, r1 = more < 0 ? a.max_pages : 0;
+	if (a.window && more >= 0) {
+		const long long low = (long long)len - a.window + 1;
+		r0 = a.sinks / PAGE + (a.sinks % PAGE != 0);
+		r1 = low > 0 ? min((int)(low / PAGE), a.max_pages) : 0;
 	}
-	n.need = r.c1 - r.fresh0 - n.held;
+	// (in place: the two ranges, which do not meet, and what lies between them)
+	const int from = copy ? 0 : r0 < r1 ? r0 : c.fresh, to = copy ? a.max_pages : c.c1 > c.fresh ? c.c1 : r1;
+#pragma unroll 1
+	for (int c0 = from; c0 < to; c0 += 64 * PLAN_AHEAD) {
+		int id[PLAN_AHEAD];
+#pragma unroll
+		for (int i = 0; i < PLAN_AHEAD; i++) {
+			const int x = c0 + i * 64 + lane;
+			id[i] = x < to ? row[x] : -1;
+		}
+#pragma unroll
+		for (int i = 0; i < PLAN_AHEAD; i++) {
+			const int x = c0 + i * 64 + lane;
+			if (c0 + i * 64 >= to)
+				break;
+			if (copy && x < to)
+				out[x] = id[i];
+			const bool page = is_page(a, id[i]);
+			n.held += __popcll(__ballot(page && x >= c.fresh && x < c.c1));
+			const unsigned long long away = __ballot(page && x >= r0 && x < r1);
+			if (away && n.away == 0)
+				n.away0 = c0 + i * 64 + __builtin_ctzll(away);
+			n.away += __popcll(away);
+		}
+	}
+	n.need = c.c1 - c.fresh - n.held;
 	return n;
 }
 
@@ -145,57 +147,64 @@ __device__ __forceinline__ int ring_at(const PlanArgs &a, const Ring &r, int i)
 	return (int)(at < a.n_pages ? at : at - a.n_pages < a.n_pages ? at - a.n_pages : at - 2 * (long long)a.n_pages);
 }
 
-// A wave: what request b gets, its columns' chunks y, y + ny, ... of 64.  need0, want0,
-// away0: the sums over the requests before it.
-__device__ __forceinline__ void fill_request(const PlanArgs &a, int b, const PlanCounts &n, const Ring &ring, double need0,
-					     double want0, double away0, int y, int ny)
+// The table's entries of a request's columns that may be named already, from `at` on: a
+// lane each.
+__device__ __forceinline__ int named(const PlanArgs &a, int b, const PlanCounts &n, const Columns &c, int at)
 {
-	const Request r = request(a, b);
+	const int col = at + (int)(threadIdx.x & 63);
+	return col < (n.held ? c.c1 : c.fresh) ? a.pages[(size_t)b * a.max_pages + col] : -1;
+}
+
+// A wave: what request b gets, its columns' chunks y, y + ny, ... of 64, the first of which
+// has the entries id (see named()).  need0, want0, away0: the sums over the requests before it.
+__device__ __forceinline__ void fill_request(const PlanArgs &a, int b, const PlanCounts &n, const Ring &ring, double need0,
+					     double want0, double away0, int y, int ny, int id)
+{
 	const int32_t *row = a.pages + (size_t)b * a.max_pages;
 	int32_t *out = a.pages_out + (size_t)b * a.max_pages;
 	const int lane = threadIdx.x & 63;
-	if (r.want && need0 + n.need <= ring.free && want0 + r.want <= a.n_tokens) {
-		const int t0 = (int)want0 - r.len; // token row of cache row 0
+	if (n.want && need0 + n.need <= ring.free && want0 + n.want <= a.n_tokens) {
+		const Columns k(n.len, n.want);
+		const int t0 = (int)want0 - n.len, end = n.len + n.want; // (token row of cache row 0)
 		// (where the table names some of the pages, the ones before are counted in turn)
 		const bool all_fresh = n.held == 0;
 		int taken = 0;
-		for (int c = r.c0 + (all_fresh ? y * 64 : 0); c < r.c1 && (all_fresh || y == 0); c += all_fresh ? ny * 64 : 64) {
+		for (int c = k.c0 + (all_fresh ? y * 64 : 0); c < k.c1 && (all_fresh || y == 0);) {
 			const int col = c + lane;
-			int id = -1;
-			if (col < r.c1 && (!all_fresh || col < r.fresh0))
-				id = row[col];
-			const bool fresh = col >= r.fresh0 && col < r.c1 && !is_page(a, id);
+			const bool fresh = col >= k.fresh && col < k.c1 && !is_page(a, id);
 			const unsigned long long set = __ballot(fresh);
-			const int rank = all_fresh ? col - r.fresh0 : taken + __popcll(set & ((1ull << lane) - 1));
+			const int rank = all_fresh ? col - k.fresh : taken + __popcll(set & ((1ull << lane) - 1));
 			if (fresh) {
 				id = a.ring[ring_at(a, ring, (int)need0 + rank)];
 				out[col] = id;
 			}
 			taken += __popcll(set);
-			if (!a.pos && !a.slot)
-				continue;
-			const int from = max(r.len, c * PAGE), to = (int)min((long long)r.len + r.want, ((long long)c + 64) * PAGE);
-			for (int x0 = from; x0 < to; x0 += 64) {
-				const int x = x0 + lane, page = __shfl(id, x / PAGE - c);
-				if (x < to) {
-					if (a.pos)
-						a.pos[t0 + x] = x;
-					if (a.slot)
-						a.slot[t0 + x] = is_page(a, page) ? page * PAGE + x % PAGE : -1;
+			const int from = max(n.len, c * PAGE), to = (int)min((long long)end, ((long long)c + 64) * PAGE);
+			if (a.pos || a.slot)
+				for (int x0 = from; x0 < to; x0 += 64) {
+					const int x = x0 + lane, page = __shfl(id, x / PAGE - c);
+					if (x < to) {
+						if (a.pos)
+							a.pos[t0 + x] = x;
+						if (a.slot)
+							a.slot[t0 + x] = is_page(a, page) ? page * PAGE + x % PAGE : -1;
+					}
 				}
-			}
+			c += all_fresh ? ny * 64 : 64;
+			id = named(a, b, n, k, c);
 		}
 	}
 	if (y)
 		return;
+	// (the first n.away pages from the first of them on)
 	int gone = 0;
-	for (int c = r.r0; c < r.r1; c += 64) {
-		const int col = c + lane, id = col < r.r1 ? row[col] : -1;
-		const bool away = is_page(a, id);
+	for (int c = n.away0; gone < n.away; c += 64) {
+		const int col = c + lane, page = col < a.max_pages ? row[col] : -1;
+		const bool away = is_page(a, page);
 		const unsigned long long set = __ballot(away);
-		const double place = away0 + gone + __popcll(set & ((1ull << lane) - 1));
-		if (away && place < ring.room) {
-			a.ring[ring_at(a, ring, ring.free + (int)place)] = id;
+		const int at = gone + __popcll(set & ((1ull << lane) - 1));
+		if (away && at < n.away && away0 + at < ring.room) {
+			a.ring[ring_at(a, ring, ring.free + (int)away0 + at)] = page;
 			out[col] = -1;
 		}
 		gone += __popcll(set);
@@ -222,32 +231,28 @@ __device__ __forceinline__ void finish_plan(const PlanArgs &a, const Ring &ring,
 	}
 }
 
-__global__ __launch_bounds__(256) void plan_count_kernel(PlanArgs a, PlanWork w)
+__global__ __launch_bounds__(PLAN_THREADS) void plan_count_kernel(PlanArgs a, PlanWork w)
 {
-	__shared__ double sum[4][3];
-	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-	double need = 0.0, want = 0.0, away = 0.0;
-	for (int i = wave; i < PLAN_BLOCK; i += 4) {
-		const int b = blockIdx.x * PLAN_BLOCK + i;
-		if (b >= a.n_seqs)
-			break;
-		const PlanCounts n = count_request(a, b);
+	__shared__ PlanCounts counts[PLAN_BLOCK];
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, b = blockIdx.x * PLAN_BLOCK + wave;
+	PlanCounts n = {0, 0, 0, 0, 0, 0};
+	if (b < a.n_seqs) {
+		n = count_request(a, b);
 		if (lane == 0)
 			w.counts[b] = n;
-		need += n.need;
-		want += n.want;
-		away += n.away;
 	}
-	if (lane == 0) {
-		sum[wave][0] = need;
-		sum[wave][1] = want;
-		sum[wave][2] = away;
-	}
+	if (lane == 0)
+		counts[wave] = n;
 	__syncthreads();
-	if (threadIdx.x < 3)
-		w.sums[blockIdx.x * 3 + threadIdx.x] = (sum[0][threadIdx.x] + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x]);
-	if (blockIdx.x == 0 && threadIdx.x < 2)
-		w.state[threadIdx.x] = a.state[threadIdx.x];
+	if (wave == 0) {
+		const bool on = lane < PLAN_BLOCK;
+		const double need = wave_total(on ? counts[lane % PLAN_BLOCK].need : 0.0), want = wave_total(on ? counts[lane % PLAN_BLOCK].want : 0.0),
+			     away = wave_total(on ? counts[lane % PLAN_BLOCK].away : 0.0);
+		if (lane < 3)
+			w.sums[blockIdx.x * 3 + lane] = lane == 0 ? need : lane == 1 ? want : away;
+		if (blockIdx.x == 0 && lane < 2)
+			w.state[lane] = a.state[lane];
+	}
 }
 
 __device__ __forceinline__ double of_last(double x)
@@ -255,21 +260,24 @@ __device__ __forceinline__ double of_last(double x)
 	return of_lane(x, 63);
 }
 
-// The sums over the requests before block `block` (a wave, whole numbers in 64-bit
-// floats), and of those that are served where the sums pass what there is: cut is set
-// then, and every request from there on gets nothing.
+// of requests b0 .. b0 + n - 1, a lane each
+__device__ __forceinline__ PlanCounts counts_at(const PlanCounts *counts, int b0, int n)
+{
+	const int lane = threadIdx.x & 63;
+	return lane < n ? counts[b0 + lane] : PlanCounts{0, 0, 0, 0, 0, 0};
+}
+
+// The sums over the requests so far (in 64-bit floats: whole numbers of up to 2^53), and of
+// those that are served where the sums pass what there is: cut is set then, and every
+// request from there on gets nothing.
 struct Before {
 	double need, want, away;
 	bool cut;
 };
 
-__device__ __forceinline__ void add_requests(const PlanArgs &a, const PlanCounts *counts, int b0, int n, const Ring &ring, Before &s,
-					     double &my_need, double &my_want, double &my_away, PlanCounts &mine)
+__device__ __forceinline__ void add_requests(const PlanArgs &a, const PlanCounts &mine, const Ring &ring, Before &s, double &my_need,
+					     double &my_want, double &my_away)
 {
-	const int lane = threadIdx.x & 63;
-	mine = PlanCounts{0, 0, 0, 0};
-	if (lane < n)
-		mine = counts[b0 + lane];
 	const double need = running_of<64>((double)mine.need), want = running_of<64>((double)mine.want),
 		     away = running_of<64>((double)mine.away);
 	my_need = s.need + (need - mine.need);
@@ -290,18 +298,35 @@ __device__ __forceinline__ void add_requests(const PlanArgs &a, const PlanCounts
 	}
 }
 
-__global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a, PlanWork w)
+// of lane i
+__device__ __forceinline__ PlanCounts counts_of(const PlanCounts &c, int i)
+{
+	auto of = [&](int x) { return __builtin_amdgcn_readlane(x, i); };
+	return PlanCounts{of(c.need), of(c.want), of(c.away), of(c.held), of(c.away0), of(c.len)};
+}
+
+__global__ __launch_bounds__(PLAN_THREADS) void plan_fill_kernel(PlanArgs a, PlanWork w)
 {
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, block = blockIdx.x;
+	// (the loads that wait for nothing first: the counts, and the table by them)
+	const int b0 = block * PLAN_BLOCK, m = min(PLAN_BLOCK, a.n_seqs - b0);
+	const PlanCounts mine = counts_at(w.counts, b0, m);
 	const Ring ring = ring_of(a, w.state);
+	double sum0[3] = {0.0, 0.0, 0.0};
+	if (lane < block)
+		for (int i = 0; i < 3; i++)
+			sum0[i] = w.sums[lane * 3 + i];
+	const PlanCounts own = counts_of(mine, wave);
+	const Columns k(own.len, own.want);
+	const int id = wave < m ? named(a, b0 + wave, own, k, k.c0 + (own.held ? 0 : (int)blockIdx.y * 64)) : -1;
 	Before s = {0.0, 0.0, 0.0, false};
 	// the blocks before this one, 64 at a time; the one that the cut lies in is looked at
 	for (int k0 = 0; k0 < block; k0 += 64) {
 		const int k = k0 + lane;
-		double x[3] = {0.0, 0.0, 0.0};
-		if (k < block)
+		double x[3] = {sum0[0], sum0[1], sum0[2]};
+		if (k0)
 			for (int i = 0; i < 3; i++)
-				x[i] = w.sums[k * 3 + i];
+				x[i] = k < block ? w.sums[k * 3 + i] : 0.0;
 		const double need = running_of<64>(x[0]), want = running_of<64>(x[1]), away = running_of<64>(x[2]);
 		const double away_before = s.away;
 		if (!s.cut) {
@@ -311,8 +336,7 @@ __global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a, PlanWork w)
 				s.need += of_lane(need - x[0], l);
 				s.want += of_lane(want - x[1], l);
 				double d0, d1, d2;
-				PlanCounts mine;
-				add_requests(a, w.counts, b0, min(PLAN_BLOCK, a.n_seqs - b0), ring, s, d0, d1, d2, mine);
+				add_requests(a, counts_at(w.counts, b0, min(PLAN_BLOCK, a.n_seqs - b0)), ring, s, d0, d1, d2);
 			} else {
 				s.need += of_last(need);
 				s.want += of_last(want);
@@ -320,26 +344,19 @@ __global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a, PlanWork w)
 		}
 		s.away = away_before + of_last(away);
 	}
-	const int b0 = block * PLAN_BLOCK, m = min(PLAN_BLOCK, a.n_seqs - b0);
 	double need, want, away;
-	PlanCounts mine;
 	const bool cut_before = s.cut;
 	const double want_at = s.want;
-	add_requests(a, w.counts, b0, m, ring, s, need, want, away, mine);
-	for (int i = wave; i < m; i += 4) {
-		PlanCounts n;
-		n.need = __builtin_amdgcn_readlane(mine.need, i);
-		n.want = __builtin_amdgcn_readlane(mine.want, i);
-		n.away = __builtin_amdgcn_readlane(mine.away, i);
-		n.held = __builtin_amdgcn_readlane(mine.held, i);
+	add_requests(a, mine, ring, s, need, want, away);
+	if (wave < m) {
 		// (past the cut: sums that nothing fits)
-		const double over = cut_before ? __builtin_inf() : of_lane(need, i);
-		fill_request(a, b0 + i, n, ring, over, of_lane(want, i), of_lane(away, i), blockIdx.y, gridDim.y);
+		const double over = cut_before ? __builtin_inf() : of_lane(need, wave);
+		fill_request(a, b0 + wave, own, ring, over, of_lane(want, wave), of_lane(away, wave), blockIdx.y, gridDim.y, id);
 	}
 	if (blockIdx.y == 0 && wave == 0 && lane < m)
 		a.first[b0 + lane] = (int)(cut_before ? want_at : want < s.want ? want : s.want);
 	if (block == (int)gridDim.x - 1)
-		finish_plan(a, ring, w.state, s.need, s.want, s.away, blockIdx.y * 256 + threadIdx.x, gridDim.y * 256);
+		finish_plan(a, ring, w.state, s.need, s.want, s.away, blockIdx.y * PLAN_THREADS + threadIdx.x, gridDim.y * PLAN_THREADS);
 }
 
 // Few requests: all of it in one workgroup.
@@ -359,17 +376,15 @@ __global__ __launch_bounds__(1024) void plan_small_kernel(PlanArgs a)
 	const Ring ring = ring_of(a, state);
 	Before s = {0.0, 0.0, 0.0, false};
 	double need, want, away;
-	PlanCounts mine;
-	add_requests(a, counts, 0, a.n_seqs, ring, s, need, want, away, mine);
+	const PlanCounts mine = counts_at(counts, 0, a.n_seqs);
+	add_requests(a, mine, ring, s, need, want, away);
 	// all waves on a few requests: each takes some of their chunks
 	const int per = a.n_seqs < 16 ? 16 / max(a.n_seqs, 1) : 1;
 	for (int i = wave / per; i < a.n_seqs; i += 16 / per) {
-		PlanCounts n;
-		n.need = __builtin_amdgcn_readlane(mine.need, i);
-		n.want = __builtin_amdgcn_readlane(mine.want, i);
-		n.away = __builtin_amdgcn_readlane(mine.away, i);
-		n.held = __builtin_amdgcn_readlane(mine.held, i);
-		fill_request(a, i, n, ring, of_lane(need, i), of_lane(want, i), of_lane(away, i), wave % per, per);
+		const PlanCounts own = counts_of(mine, i);
+		const Columns k(own.len, own.want);
+		const int id = named(a, i, own, k, k.c0 + (own.held ? 0 : wave % per * 64));
+		fill_request(a, i, own, ring, of_lane(need, i), of_lane(want, i), of_lane(away, i), wave % per, per, id);
 	}
 	if (wave == 0 && lane < a.n_seqs)
 		a.first[lane] = (int)(want < s.want ? want : s.want);
@@ -385,8 +400,8 @@ hipError_t launch_plan(const PlanArgs &a, void *work, hipStream_t st)
 	PlanWork w;
 	carve_plan(a.n_seqs, (uint8_t *)work, &w);
 	const int blocks = (a.n_seqs + PLAN_BLOCK - 1) / PLAN_BLOCK, chunks = (a.n_tokens + 64 * PAGE - 1) / (64 * PAGE);
-	tie_launch(plan_count_kernel, dim3(blocks), dim3(256), 0, st, a, w);
-	tie_launch(plan_fill_kernel, dim3(blocks, chunks < 1 ? 1 : chunks < 16 ? chunks : 16), dim3(256), 0, st, a, w);
+	tie_launch(plan_count_kernel, dim3(blocks), dim3(PLAN_THREADS), 0, st, a, w);
+	tie_launch(plan_fill_kernel, dim3(blocks, chunks < 1 ? 1 : chunks < 4 ? chunks : 4), dim3(PLAN_THREADS), 0, st, a, w);
 	return hipGetLastError();
 }
 
