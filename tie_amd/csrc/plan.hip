@@ -35,7 +35,7 @@ struct PlanCounts {
 
 struct PlanWork {
 	PlanCounts *counts; // [n_seqs]
-	double *sums;       // [blocks][3] of need, want and away
+	uint32_t *sums;     // [blocks][3] of need, want and away
 	int *state;         // the ring's, as the call found it (it may be updated in place)
 };
 
@@ -49,7 +49,7 @@ static size_t carve_plan(int n_seqs, uint8_t *base, PlanWork *w)
 	};
 	PlanWork v;
 	v.counts = (PlanCounts *)take((size_t)n_seqs * sizeof(PlanCounts));
-	v.sums = (double *)take(((size_t)n_seqs + PLAN_BLOCK - 1) / PLAN_BLOCK * 3 * sizeof(double));
+	v.sums = (uint32_t *)take(((size_t)n_seqs + PLAN_BLOCK - 1) / PLAN_BLOCK * 3 * sizeof(uint32_t));
 	v.state = (int *)take(2 * sizeof(int));
 	if (w)
 		*w = v;
@@ -59,6 +59,34 @@ static size_t carve_plan(int n_seqs, uint8_t *base, PlanWork *w)
 size_t plan_work_bytes(int n_seqs)
 {
 	return carve_plan(n_seqs, nullptr, nullptr);
+}
+
+// Sums that stay at 2^32 - 1 when they pass it: every number and limit here is below 2^31,
+// so they are exact where they matter and too large where not.
+__device__ __forceinline__ uint32_t plus(uint32_t x, uint32_t y)
+{
+	return __builtin_elementwise_add_sat(x, y);
+}
+
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t plus_dpp(uint32_t x)
+{
+	return plus(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false));
+}
+
+// the running sum over the wave, as running_of() makes it
+__device__ __forceinline__ uint32_t running_sum(uint32_t x)
+{
+	x = plus_dpp<0x111, 0xf>(x);
+	x = plus_dpp<0x112, 0xf>(x);
+	x = plus_dpp<0x114, 0xf>(x);
+	x = plus_dpp<0x118, 0xf>(x);
+	x = plus_dpp<0x142, 0xa>(x);
+	return plus_dpp<0x143, 0xc>(x);
+}
+
+__device__ __forceinline__ uint32_t sum_at(uint32_t x, int lane)
+{
+	return (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
 }
 
 // The columns of a request's new rows: from c0 on, of which all but the first may be
@@ -157,13 +185,13 @@ __device__ __forceinline__ int named(const PlanArgs &a, int b, const PlanCounts 
 
 // A wave: what request b gets, its columns' chunks y, y + ny, ... of 64, the first of which
 // has the entries id (see named()).  need0, want0, away0: the sums over the requests before it.
-__device__ __forceinline__ void fill_request(const PlanArgs &a, int b, const PlanCounts &n, const Ring &ring, double need0,
-					     double want0, double away0, int y, int ny, int id)
+__device__ __forceinline__ void fill_request(const PlanArgs &a, int b, const PlanCounts &n, const Ring &ring, uint32_t need0,
+					     uint32_t want0, uint32_t away0, int y, int ny, int id)
 {
 	const int32_t *row = a.pages + (size_t)b * a.max_pages;
 	int32_t *out = a.pages_out + (size_t)b * a.max_pages;
 	const int lane = threadIdx.x & 63;
-	if (n.want && need0 + n.need <= ring.free && want0 + n.want <= a.n_tokens) {
+	if (n.want && plus(need0, n.need) <= (uint32_t)ring.free && plus(want0, n.want) <= (uint32_t)a.n_tokens) {
 		const Columns k(n.len, n.want);
 		const int t0 = (int)want0 - n.len, end = n.len + n.want; // (token row of cache row 0)
 		// (where the table names some of the pages, the ones before are counted in turn)
@@ -203,7 +231,7 @@ __device__ __forceinline__ void fill_request(const PlanArgs &a, int b, const Pla
 		const bool away = is_page(a, page);
 		const unsigned long long set = __ballot(away);
 		const int at = gone + __popcll(set & ((1ull << lane) - 1));
-		if (away && at < n.away && away0 + at < ring.room) {
+		if (away && at < n.away && plus(away0, at) < (uint32_t)ring.room) {
 			a.ring[ring_at(a, ring, ring.free + (int)away0 + at)] = page;
 			out[col] = -1;
 		}
@@ -213,8 +241,8 @@ __device__ __forceinline__ void fill_request(const PlanArgs &a, int b, const Pla
 
 // What is known when all requests are summed: the last range's end, the token rows
 // behind it and the ring's new state.
-__device__ __forceinline__ void finish_plan(const PlanArgs &a, const Ring &ring, const int *state, double need, double want, double away,
-					    int thread, int threads)
+__device__ __forceinline__ void finish_plan(const PlanArgs &a, const Ring &ring, const int *state, uint32_t need, uint32_t want,
+					    uint32_t away, int thread, int threads)
 {
 	for (int t = (int)want + thread; t < a.n_tokens; t += threads) {
 		if (a.pos)
@@ -224,11 +252,18 @@ __device__ __forceinline__ void finish_plan(const PlanArgs &a, const Ring &ring,
 	}
 	if (thread == 0) {
 		const bool none = ring.room == 0 && ring.free == 0; // (no ring)
-		const int back = (int)(away < ring.room ? away : ring.room);
+		const int back = (int)min(away, (uint32_t)ring.room);
 		a.first[a.n_seqs] = (int)want;
 		a.state_out[0] = none ? state[0] : ring_at(a, ring, (int)need);
 		a.state_out[1] = none ? state[1] : ring.free - (int)need + back;
 	}
+}
+
+// of requests b0 .. b0 + n - 1, a lane each
+__device__ __forceinline__ PlanCounts counts_at(const PlanCounts *counts, int b0, int n)
+{
+	const int lane = threadIdx.x & 63;
+	return lane < n ? counts[b0 + lane] : PlanCounts{0, 0, 0, 0, 0, 0};
 }
 
 __global__ __launch_bounds__(PLAN_THREADS) void plan_count_kernel(PlanArgs a, PlanWork w)
@@ -245,58 +280,46 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_count_kernel(PlanArgs a, Pl
 		counts[wave] = n;
 	__syncthreads();
 	if (wave == 0) {
-		const bool on = lane < PLAN_BLOCK;
-		const double need = wave_total(on ? counts[lane % PLAN_BLOCK].need : 0.0), want = wave_total(on ? counts[lane % PLAN_BLOCK].want : 0.0),
-			     away = wave_total(on ? counts[lane % PLAN_BLOCK].away : 0.0);
-		if (lane < 3)
-			w.sums[blockIdx.x * 3 + lane] = lane == 0 ? need : lane == 1 ? want : away;
+		const PlanCounts c = counts_at(counts, 0, PLAN_BLOCK);
+		const uint32_t need = running_sum(c.need), want = running_sum(c.want), away = running_sum(c.away);
+		if (lane == 63) {
+			w.sums[blockIdx.x * 3] = need;
+			w.sums[blockIdx.x * 3 + 1] = want;
+			w.sums[blockIdx.x * 3 + 2] = away;
+		}
 		if (blockIdx.x == 0 && lane < 2)
 			w.state[lane] = a.state[lane];
 	}
 }
 
-__device__ __forceinline__ double of_last(double x)
-{
-	return of_lane(x, 63);
-}
-
-// of requests b0 .. b0 + n - 1, a lane each
-__device__ __forceinline__ PlanCounts counts_at(const PlanCounts *counts, int b0, int n)
-{
-	const int lane = threadIdx.x & 63;
-	return lane < n ? counts[b0 + lane] : PlanCounts{0, 0, 0, 0, 0, 0};
-}
-
-// The sums over the requests so far (in 64-bit floats: whole numbers of up to 2^53), and of
-// those that are served where the sums pass what there is: cut is set then, and every
-// request from there on gets nothing.
+// The sums over the requests so far, and of those that are served where the sums pass
+// what there is: cut is set then, and every request from there on gets nothing.
 struct Before {
-	double need, want, away;
-	bool cut;
-};
-
-__device__ __forceinline__ void add_requests(const PlanArgs &a, const PlanCounts &mine, const Ring &ring, Before &s, double &my_need,
-					     double &my_want, double &my_away)
-{
-	const double need = running_of<64>((double)mine.need), want = running_of<64>((double)mine.want),
-		     away = running_of<64>((double)mine.away);
-	my_need = s.need + (need - mine.need);
-	my_want = s.want + (want - mine.want);
-	my_away = s.away + (away - mine.away);
-	s.away += of_last(away);
-	if (s.cut)
-		return;
-	const unsigned long long over = __ballot(s.need + need > ring.free || s.want + want > a.n_tokens);
-	if (over) {
-		const int l = __builtin_ctzll(over);
-		s.need = of_lane(my_need, l);
-		s.want = of_lane(my_want, l);
-		s.cut = true;
-	} else {
-		s.need += of_last(need);
-		s.want += of_last(want);
+	uint32_t need = 0, want = 0, away = 0;
+	bool cut = false;
+	// the first lane where the running sums pass what there is, 64: none
+	__device__ __forceinline__ int over(const PlanArgs &a, const Ring &ring, uint32_t more_need, uint32_t more_want) const
+	{
+		const unsigned long long set = __ballot(plus(need, more_need) > (uint32_t)ring.free || plus(want, more_want) > (uint32_t)a.n_tokens);
+		return set ? __builtin_ctzll(set) : 64;
 	}
-}
+	// a lane's counts added; the sums before each of them
+	__device__ __forceinline__ void add(const PlanArgs &a, const Ring &ring, const PlanCounts &mine, uint32_t &my_need, uint32_t &my_want,
+					    uint32_t &my_away)
+	{
+		const uint32_t n = running_sum(mine.need), w = running_sum(mine.want), g = running_sum(mine.away);
+		my_need = plus(need, n - mine.need);
+		my_want = plus(want, w - mine.want);
+		my_away = plus(away, g - mine.away);
+		away = plus(away, sum_at(g, 63));
+		if (cut)
+			return;
+		const int l = over(a, ring, n, w);
+		cut = l < 64;
+		need = cut ? sum_at(my_need, l & 63) : plus(need, sum_at(n, 63));
+		want = cut ? sum_at(my_want, l & 63) : plus(want, sum_at(w, 63));
+	}
+};
 
 // of lane i
 __device__ __forceinline__ PlanCounts counts_of(const PlanCounts &c, int i)
@@ -312,49 +335,48 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_fill_kernel(PlanArgs a, Pla
 	const int b0 = block * PLAN_BLOCK, m = min(PLAN_BLOCK, a.n_seqs - b0);
 	const PlanCounts mine = counts_at(w.counts, b0, m);
 	const Ring ring = ring_of(a, w.state);
-	double sum0[3] = {0.0, 0.0, 0.0};
+	uint32_t sum0[3] = {0, 0, 0};
 	if (lane < block)
 		for (int i = 0; i < 3; i++)
 			sum0[i] = w.sums[lane * 3 + i];
 	const PlanCounts own = counts_of(mine, wave);
 	const Columns k(own.len, own.want);
 	const int id = wave < m ? named(a, b0 + wave, own, k, k.c0 + (own.held ? 0 : (int)blockIdx.y * 64)) : -1;
-	Before s = {0.0, 0.0, 0.0, false};
+	Before s;
 	// the blocks before this one, 64 at a time; the one that the cut lies in is looked at
 	for (int k0 = 0; k0 < block; k0 += 64) {
 		const int k = k0 + lane;
-		double x[3] = {sum0[0], sum0[1], sum0[2]};
+		uint32_t x[3] = {sum0[0], sum0[1], sum0[2]};
 		if (k0)
 			for (int i = 0; i < 3; i++)
-				x[i] = k < block ? w.sums[k * 3 + i] : 0.0;
-		const double need = running_of<64>(x[0]), want = running_of<64>(x[1]), away = running_of<64>(x[2]);
-		const double away_before = s.away;
+				x[i] = k < block ? w.sums[k * 3 + i] : 0;
+		const uint32_t need = running_sum(x[0]), want = running_sum(x[1]), away = plus(s.away, sum_at(running_sum(x[2]), 63));
 		if (!s.cut) {
-			const unsigned long long over = __ballot(s.need + need > ring.free || s.want + want > a.n_tokens);
-			if (over) {
-				const int l = __builtin_ctzll(over), b0 = (k0 + l) * PLAN_BLOCK;
-				s.need += of_lane(need - x[0], l);
-				s.want += of_lane(want - x[1], l);
-				double d0, d1, d2;
-				add_requests(a, counts_at(w.counts, b0, min(PLAN_BLOCK, a.n_seqs - b0)), ring, s, d0, d1, d2);
+			const int l = s.over(a, ring, need, want);
+			if (l < 64) {
+				const int from = (k0 + l) * PLAN_BLOCK;
+				s.need = plus(s.need, sum_at(need - x[0], l));
+				s.want = plus(s.want, sum_at(want - x[1], l));
+				uint32_t none[3];
+				s.add(a, ring, counts_at(w.counts, from, min(PLAN_BLOCK, a.n_seqs - from)), none[0], none[1], none[2]);
 			} else {
-				s.need += of_last(need);
-				s.want += of_last(want);
+				s.need = plus(s.need, sum_at(need, 63));
+				s.want = plus(s.want, sum_at(want, 63));
 			}
 		}
-		s.away = away_before + of_last(away);
+		s.away = away;
 	}
-	double need, want, away;
+	uint32_t need, want, away;
 	const bool cut_before = s.cut;
-	const double want_at = s.want;
-	add_requests(a, mine, ring, s, need, want, away);
+	const uint32_t want_at = s.want;
+	s.add(a, ring, mine, need, want, away);
 	if (wave < m) {
 		// (past the cut: sums that nothing fits)
-		const double over = cut_before ? __builtin_inf() : of_lane(need, wave);
-		fill_request(a, b0 + wave, own, ring, over, of_lane(want, wave), of_lane(away, wave), blockIdx.y, gridDim.y, id);
+		fill_request(a, b0 + wave, own, ring, cut_before ? ~0u : sum_at(need, wave), sum_at(want, wave), sum_at(away, wave), blockIdx.y,
+			     gridDim.y, id);
 	}
 	if (blockIdx.y == 0 && wave == 0 && lane < m)
-		a.first[b0 + lane] = (int)(cut_before ? want_at : want < s.want ? want : s.want);
+		a.first[b0 + lane] = (int)(cut_before ? want_at : min(want, s.want));
 	if (block == (int)gridDim.x - 1)
 		finish_plan(a, ring, w.state, s.need, s.want, s.away, blockIdx.y * PLAN_THREADS + threadIdx.x, gridDim.y * PLAN_THREADS);
 }
@@ -374,20 +396,20 @@ __global__ __launch_bounds__(1024) void plan_small_kernel(PlanArgs a)
 	}
 	__syncthreads();
 	const Ring ring = ring_of(a, state);
-	Before s = {0.0, 0.0, 0.0, false};
-	double need, want, away;
+	Before s;
+	uint32_t need, want, away;
 	const PlanCounts mine = counts_at(counts, 0, a.n_seqs);
-	add_requests(a, mine, ring, s, need, want, away);
+	s.add(a, ring, mine, need, want, away);
 	// all waves on a few requests: each takes some of their chunks
 	const int per = a.n_seqs < 16 ? 16 / max(a.n_seqs, 1) : 1;
 	for (int i = wave / per; i < a.n_seqs; i += 16 / per) {
 		const PlanCounts own = counts_of(mine, i);
 		const Columns k(own.len, own.want);
 		const int id = named(a, i, own, k, k.c0 + (own.held ? 0 : wave % per * 64));
-		fill_request(a, i, own, ring, of_lane(need, i), of_lane(want, i), of_lane(away, i), wave % per, per, id);
+		fill_request(a, i, own, ring, sum_at(need, i), sum_at(want, i), sum_at(away, i), wave % per, per, id);
 	}
 	if (wave == 0 && lane < a.n_seqs)
-		a.first[lane] = (int)(want < s.want ? want : s.want);
+		a.first[lane] = (int)min(want, s.want);
 	finish_plan(a, ring, state, s.need, s.want, s.away, threadIdx.x, 1024);
 }
 
