@@ -133,6 +133,8 @@ __device__ __forceinline__ int div_up(int a, int b)
 }
 
 struct Cut {
+	// (grain, least and rows are powers of two: shifts where divisions would be a third of
+	// the kernels' instructions, which are not in the cache when a call begins)
 	int cap;   // units that run at once: at most so many where tiles are cut
 	int full;  // so many tiles are not cut
 	int grain; // pages that are not cut
@@ -192,7 +194,7 @@ __device__ __forceinline__ void seq_work(const KvSeqs &s, const AttnArgs &a, int
 	seq_tokens(s, b, t0, n);
 	if (n == 0)
 		return;
-	tiles = (int)(((long long)n * group + rows - 1) / rows);
+	tiles = (int)(((long long)n * group + rows - 1) >> __builtin_ctz(rows));
 	pages = seq_fits(s, len, n) ? (len + n + PAGE - 1) / PAGE : 1;
 	if (WIN && seq_fits(s, len, n)) {
 		// what the first tile sees, and no tile more than these: its tokens' windows
@@ -207,12 +209,18 @@ __device__ __forceinline__ void seq_work(const KvSeqs &s, const AttnArgs &a, int
 	}
 }
 
+// x / 2^k, rounded up, for a divisor of 2^k
+__device__ __forceinline__ int shift_up(int x, int by)
+{
+	return (int)(((uint32_t)x + (uint32_t)by - 1) >> __builtin_ctz(by));
+}
+
 // Parts of a tile for a grain of its pages, so that no more than cap units come
 // (0: whole tiles; so where the tiles alone fill the card).  The first block of
 // 64 sequences is in the wave's lanes already.
 __device__ __forceinline__ int tile_parts(const Cut &cut, int pages, float rate)
 {
-	const int grains = div_up(pages, cut.grain), most = grains / cut.least, p = (int)((float)grains * rate + 0.5f);
+	const int grains = shift_up(pages, cut.grain), most = grains >> __builtin_ctz(cut.least), p = (int)((float)grains * rate + 0.5f);
 	return p < 2 || grains <= cut.alone ? 1 : p < most ? p : most;
 }
 
@@ -236,7 +244,7 @@ __device__ __forceinline__ float part_rate(const KvSeqs &s, const AttnArgs &a, i
 	if (over([](int t, int) { return t; }) * kvh >= cut.full)
 		return 0.0f;
 	// the nearest number to each tile's share; a little less where those are too many
-	float rate = (float)(cap / over([&](int t, int p) { return (double)t * div_up(p, cut.grain); }));
+	float rate = (float)(cap / over([&](int t, int p) { return (double)t * shift_up(p, cut.grain); }));
 	for (int i = 0; i < 16; i++) {
 		if (over([&](int t, int p) { return t * tile_parts(cut, p, rate); }) <= cap)
 			return rate;
@@ -297,7 +305,7 @@ __device__ __forceinline__ void part_pages(const Cut &cut, const Unit &u, int al
 {
 	// (in grains where a part has few of them, else to the page)
 	const int grain = all / u.parts < 4 * cut.grain ? cut.grain : 1;
-	const int grains = div_up(all, grain), q = grains / u.parts, r = grains % u.parts;
+	const int grains = shift_up(all, grain), q = grains / u.parts, r = grains % u.parts;
 	p0 = (u.part * q + min(u.part, r)) * grain;
 	p1 = min(pages, p0 + (q + (u.part < r)) * grain);
 }
