@@ -1499,6 +1499,15 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 		columns = seen < columns ? seen : columns;
 	}
 	h.few = few_of(c, (int)columns, rows, s.n_seqs);
+	// Through a window a tile has few pages, so that reading them again for each 16 rows
+	// costs less than the other kernel's second launch, as long as no CU has two tiles (100
+	// f16 tokens over a window of 200 15 us, by the other kernel 23; 48 tokens of 64 heads over
+	// 1000 24.5 and 28; 200 int8 tokens over 200 58 and 27).  f16: up to 640 KB of them (26 tokens
+	// of four sequences, 8 kv heads of 64, over 2000 22.5 and 26, over 4000 36 and 31); int8,
+	// whose codes the other kernel converts first: to 1280 (32 tokens of four sequences over 4000
+	// 37.5 both, 26 of one 30 and 36).
+	if (a.window && rows * c.kvh <= (size_t)FEW_CAP * FEW_ROWS && columns * PAGE * c.hd * 2 <= (c.i8 ? 1280u : 320u) * 1024)
+		h.few = true;
 	// many: 128 rows where such tiles fill the card (4096 tokens of 32 heads 240
 	// us, by 64 rows 257), or 64: as many units and half the parts' bytes, less
 	// left of tiles that a mask or a sequence's end cuts (1000 tokens over 2000
@@ -1519,6 +1528,13 @@ static Shape attn_shape(const KvLayer &c, const KvSeqs &s, const AttnArgs &a)
 	const size_t tiles = (rows + seqs * (h.cut.rows - 1)) / h.cut.rows;
 	// as many tiles as fill the card are not cut: no parts, no join
 	h.cut.whole = rows / h.cut.rows * c.kvh >= (size_t)h.cut.full;
+	// Nor are tiles that a window leaves few pages: a cut saves the pages of all but one part,
+	// at 2 us each (int8 more), and the join costs 10 us.  f16: 200 tokens of 32 heads over 200 21.7
+	// us (cut 28.0), over 500 27.8 (28.3), 175 of 64 in eight sequences over 700 34.5 (42.8);
+	// int8: 70 of 64 in four over 300 27.2 (27.4), over 500 32.5 (29.5).
+	const size_t all = tiles * c.kvh;
+	if (a.window && !h.few && all < MANY_CAP && columns * (MANY_CAP - all) <= (size_t)(c.i8 ? 6 : 10) * MANY_CAP)
+		h.cut.whole = 1;
 	// (a share that is rounded down can make one more part)
 	h.units = (h.cut.whole ? 0 : h.cut.cap + c.kvh) + tiles * c.kvh;
 	// (not with a kv head for every 8 rows or more, and then: whole tiles)
