@@ -85,3 +85,63 @@ def test_one_position_on_all_axes_is_append():
         got.append([out.cpu().numpy()] + c.back())
     for a, b in zip(*got):
         assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+
+
+@pytest.mark.parametrize("kind,H,kvh,hd", [("i8", 4, 2, 128), ("f16", 4, 2, 64), ("i8", 3, 3, 64), ("f16", 2, 1, 128)])
+@pytest.mark.parametrize("n_seqs,most", [(3, 500), (40, 60), (150, 11), (700, 3)])
+@pytest.mark.parametrize("plain", [False, True])
+def test_many_tokens_of_many_sequences(kind, H, kvh, hd, n_seqs, most, plain):
+    """Rows that begin anywhere in a page, sequences without tokens, rows of no sequence, a page that is none, lengths that do
+    not fit, values that are not finite: the cache to the byte, and the queries of all sequences whose rows fit."""
+    import torch
+    rng = np.random.default_rng(n_seqs + hd)
+    lens, counts = rng.integers(0, 200, n_seqs).tolist(), rng.integers(0, most + 1, n_seqs).tolist()
+    counts[-1] += max(0, 600 - sum(counts))
+    c = kv_ref.Cache(rng, kind, kvh, hd, lens, counts, fill=False)
+    T, pad = sum(counts), 21
+    x = rng.standard_normal((T + pad, (H + 2 * kvh) * hd)).astype(np.float32)
+    x[rng.integers(0, T, 5), -3] = [np.inf, np.nan, -np.inf, 1e6, -7e4]
+    pos = rng.integers(0, 3000, (2, T + pad)).astype(np.int32)
+    axes = rng.integers(0, 2, hd // 2).tolist()
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    b_len, b_page = (int(np.argsort(counts)[-1 - i]) for i in (1, 2))
+    lens[b_len] = 64 * c.table.shape[1] if n_seqs % 2 else -1
+    gone = -(-(lens[b_page] + counts[b_page]) // 64) - 1
+    c.table[b_page, gone] = -5
+    kv = c.gpu()
+    seqs = tie_amd.KVSeqs(torch.from_numpy(c.table).cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), torch.from_numpy(first).cuda(),
+                          T + pad)
+    xd, pd = torch.from_numpy(x).cuda(), torch.from_numpy(pos).cuda()
+    q_out = torch.full((T + pad, H, hd), -7.0, device="cuda")
+    parts = (xd[:, : H * hd], xd[:, H * hd: (H + kvh) * hd], xd[:, (H + kvh) * hd:], q_out)
+    if plain:
+        kv.append(0, seqs, *parts, pd[0].contiguous())
+        pos, axes = pos[:1], [0] * (hd // 2)
+    else:
+        kv.append_axes(0, seqs, *parts, pd, axes)
+    torch.cuda.synchronize()
+    x = x.reshape(T + pad, H + 2 * kvh, hd)
+    got = q_out.cpu().numpy()
+    assert (got[T:] == -7.0).all()
+    np.testing.assert_allclose(got[:T], rotate(x[:T, :H], None, pos[:, :T], axes, 1e-6, 1e6), rtol=2.0 ** -23, atol=1e-8)
+    k, v = rotate(x[:T, H: H + kvh], None, pos[:, :T], axes, 1e-6, 1e6).astype(np.float32), x[:T, H + kvh:]
+    for b, (n, m) in enumerate(zip(lens, counts)):
+        if b == b_len:
+            continue
+        t = first[b]
+        m = min(m, gone * 64 - n) if b == b_page else m
+        if m <= 0:
+            continue
+        for j in range(m):
+            p, r = c.place(b, n + j)
+            if kind == "f16":
+                c.k[0, p, :, r] = kv_ref.held_f16(k[t + j])
+                c.v[0, p, :, :, r] = np.where(np.isnan(v[t + j]), np.float16(np.nan), kv_ref.held_f16(v[t + j]))
+            else:
+                bad = ~np.isfinite(v[t + j]).all(-1)
+                kc, ks = kv_ref.codes(k[t + j])
+                vc, vs = kv_ref.codes(np.where(bad[:, None], np.float32(0), v[t + j]))
+                c.k[0, p, :, r], c.ks[0, p, :, r], c.v[0, p, :, :, r], c.vs[0, p, :, r] = kc, ks, vc, np.where(bad, np.nan, vs)
+    for mine, theirs in zip(c.back(), (c.k, c.v, c.ks, c.vs)):
+        if theirs is not None:
+            assert np.array_equal(mine, theirs, equal_nan=mine.dtype != np.int8)

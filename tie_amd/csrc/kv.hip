@@ -1,6 +1,8 @@
 // kv.hip -- the cache around the attention: norm and rotation of queries and
 // keys with the quantised write (append), reading back, and moving the
 // accepted path's rows (keep).
+#include <type_traits>
+
 #include "kv.h"
 
 namespace tie {
@@ -35,10 +37,13 @@ __device__ __forceinline__ _Float16 half_of(float x)
 // chain of steps (position, angle, sincos; row, norm, code), 3.6 us (on the default
 // stream 4.1).  Many: by the bytes, the 64-bit arithmetic (about 60 instructions
 // for 64 pairs) and the V columns' pieces (a row's values lie PAGE apart) together:
-// 2048 tokens of 40 heads 22.5 us, 3.5 TB/s; 20 to 21.5 without any one of them.
+// 7479 tokens of 56 heads of 64 from memory (200 MB) 66 us, 3.0 TB/s; 50 without the
+// stores, 60 without the arithmetic, 33 without both.  U: heads whose rows are under
+// way at once (4 where a wave has so many: 75 to 69 us; 8 72), and there the queries go
+// past the caches (66).
 constexpr int DIES = 8;
 
-template <int HD, bool I8>
+template <int HD, bool I8, int U>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, AppendArgs a, int per_wave)
 {
 	constexpr int L = HD / 2, G = 64 / L; // lanes of a head, heads of a wave at a time
@@ -60,16 +65,19 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 		       : kv < c.kvh ? a.k + (size_t)t * a.k_stride + (size_t)kv * HD
 				    : a.v + (size_t)t * a.v_stride + (size_t)(kv - c.kvh) * HD;
 	};
-	// the first head's row and the norms' weights are requested before the
+	// the first heads' rows and the norms' weights are requested before the
 	// position is known
-	float n0 = 0.0f, n1 = 0.0f;
+	float n0[U] = {}, n1[U] = {};
 	auto fetch = [&](int u) {
-		int kv;
-		const int h = u * G + part;
-		if (h < n_all) {
-			const float *p = source(h, kv);
-			n0 = p[i];
-			n1 = p[i + L];
+#pragma unroll
+		for (int j = 0; j < U; j++) {
+			int kv;
+			const int h = (u + 4 * j) * G + part;
+			if (h < n_all) {
+				const float *p = source(h, kv);
+				n0[j] = p[i];
+				n1[j] = p[i + L];
+			}
 		}
 	};
 	fetch(u0);
@@ -86,16 +94,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 	const double at = a.pos ? (double)*pos : fits ? (double)row : __builtin_nan("");
 	double cs, sn;
 	sincos(at * exp2((double)i * (-2.0 / HD) * a.log2_theta), &sn, &cs);
-	for (int u = 0; u < per_wave; u++) {
-		const int h = (u0 + 4 * u) * G + part;
-		if ((u0 + 4 * u) * G >= n_all)
-			break;
+	auto unit = [&](int u, float x0, float x1) {
+		const int h = u * G + part;
 		const bool on = h < n_all;
 		const int kv = h - a.n_heads, head = kv < 0 ? h : kv < c.kvh ? kv : kv - c.kvh;
 		const bool is_q = kv < 0, is_v = kv >= c.kvh;
-		float x0 = n0, x1 = n1;
-		if (u + 1 < per_wave)
-			fetch(u0 + 4 * (u + 1));
 		if (!__all(is_v)) {
 			double y0 = x0, y1 = x1;
 			if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
@@ -112,11 +115,16 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 		}
 		if (on && is_q) {
 			float *o = a.q_out + (size_t)t * a.qo_stride + (size_t)head * HD;
-			o[i] = x0;
-			o[i + L] = x1;
+			if (U == 1) {
+				o[i] = x0;
+				o[i + L] = x1;
+			} else { // (past the caches, which lose it before it is read)
+				__builtin_nontemporal_store(x0, o + i);
+				__builtin_nontemporal_store(x1, o + i + L);
+			}
 		}
 		if (__all(is_q))
-			continue;
+			return;
 		// (every lane of a head takes part in its row's largest magnitude)
 		float scale = 0.0f;
 		if (I8) {
@@ -129,7 +137,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 			scale = bad ? __builtin_nanf("") : most / 127.0f;
 		}
 		if (!on || is_q || page < 0)
-			continue;
+			return;
 		const size_t at = (size_t)page * c.kvh + head; // this page's rows of this kv head
 		if (I8 && i == 0)
 			(is_v ? c.vs : c.ks)[at * PAGE + r] = scale;
@@ -144,6 +152,22 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 			o[e0] = half_of(x0);
 			o[e1] = half_of(x1);
 		}
+	};
+	for (int u = 0; u < per_wave; u += U) {
+		float x0[U], x1[U];
+#pragma unroll
+		for (int j = 0; j < U; j++) {
+			x0[j] = n0[j];
+			x1[j] = n1[j];
+		}
+		if (u + U < per_wave)
+			fetch(u0 + 4 * (u + U));
+#pragma unroll
+		for (int j = 0; j < U; j++) {
+			if (u + j >= per_wave || (u0 + 4 * (u + j)) * G >= n_all)
+				return;
+			unit(u0 + 4 * (u + j), x0[j], x1[j]);
+		}
 	}
 }
 
@@ -157,10 +181,14 @@ hipError_t launch_kv_append(const KvLayer &c, const KvSeqs &s, const AppendArgs 
 	per = per > (units + 3) / 4 ? (units + 3) / 4 : per;
 	const dim3 grid((s.n_tokens + DIES - 1) / DIES * DIES, (units + 4 * per - 1) / (4 * per));
 	auto go = [&](auto kern) { tie_launch(kern, grid, dim3(256), 0, st, c, s, a, per); };
-	if (c.hd == 128)
-		c.i8 ? go(kv_append_kernel<128, true>) : go(kv_append_kernel<128, false>);
-	else
-		c.i8 ? go(kv_append_kernel<64, true>) : go(kv_append_kernel<64, false>);
+	auto by_units = [&](auto units_ahead) {
+		constexpr int U = decltype(units_ahead)::value;
+		if (c.hd == 128)
+			c.i8 ? go(kv_append_kernel<128, true, U>) : go(kv_append_kernel<128, false, U>);
+		else
+			c.i8 ? go(kv_append_kernel<64, true, U>) : go(kv_append_kernel<64, false, U>);
+	};
+	per < 4 ? by_units(std::integral_constant<int, 1>()) : by_units(std::integral_constant<int, 4>());
 	return hipGetLastError();
 }
 
