@@ -445,8 +445,8 @@ int tie_hip_kv_plan(const tie_hip_kv_pool *pool, int n_seqs, int max_pages, int 
  * Any output may be NULL (the top ones with n_top 0), tokens NULL with logprob and
  * rank.  A row with a logit of NaN or +infinity, or with none above -infinity, has no
  * distribution: NaN, rank and top tokens -1.  A token outside [0, vocab): NaN and
- * rank -1.  temperature from 1e-6 to 1e6; rows of `vocab` (at most 2^24), logits_stride
- * floats apart.  Sums in 64 bits of exponentials in 32.  No output may share memory
+ * rank -1.  temperature from 1e-6 to 1e6; at most 2^23 rows of `vocab` (at most 2^24),
+ * logits_stride floats apart.  Sums in 64 bits of exponentials in 32.  No output may share memory
  * with an input or another output.  work as for tie_hip_verify_tree. */
 size_t tie_hip_token_logprobs_work_bytes(int vocab, int n_tokens, int n_top);
 int tie_hip_token_logprobs(const float *logits, size_t logits_stride, int vocab, int n_tokens, const int32_t *tokens,

@@ -212,3 +212,29 @@ def test_no_page_is_lost_or_given_twice():
         free = [int(want_r[(want_s[0] + i) % P]) for i in range(want_s[1])]
         assert sorted(held + free) == list(range(P)), step
         n = np.where(m < 0, 0, n + np.diff(want_f)).astype(np.int32)
+
+
+def test_sums_that_pass_32_bits():
+    """Requests that ask for 2^26 rows each, 70 of them: nothing fits, or what stands before them."""
+    import torch
+    i32 = dict(dtype=torch.int32, device="cuda")
+    B, M = 70, 1 << 20
+    table, lens, new = torch.full((B, M), -1, **i32), torch.zeros(B, **i32), torch.full((B,), 1 << 26, **i32)
+    ring, state = torch.arange(50, **i32), torch.tensor([48, 50], **i32)
+    pool, first, pos = tie_amd.KVPool(ring, state), torch.zeros(B + 1, **i32), torch.zeros(100, **i32)
+    after = torch.zeros(2, **i32)
+    for small in (0, 3):
+        new[:small] = 30
+        pool.plan(table, lens, new, table, first, pos=pos, state_out=after)
+        torch.cuda.synchronize()
+        assert first.tolist() == [30 * min(b, small) for b in range(B + 1)]
+        assert after.tolist() == [(48 + small) % 50, 50 - small]
+        assert pos.tolist() == list(range(30)) * small + [-1] * (100 - 30 * small)
+    assert table[:4, 0].tolist() == [48, 49, 0, -1] and (table[:, 1:] == -1).all()
+    # as many token rows as an int names: the first request does not lie within its row of the table, the second (64
+    # rows) and the third (30) have their pages already, and the fourth wants more than there are
+    new[:2] = torch.tensor([0x7fffffff - 63, 64], **i32)
+    pool.plan(table, lens, new, table, first, n_tokens=0x7fffffff, state_out=after)
+    torch.cuda.synchronize()
+    assert first.tolist() == [0, 0, 64] + [94] * (B - 2)
+    assert after.tolist() == [48, 50]

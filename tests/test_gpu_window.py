@@ -275,3 +275,111 @@ def test_replayed_graph_follows_the_lengths():
         want, tol = expect(c, q, 0.09, visible(now, [1] * 3, window, sinks))
         assert (np.abs(out.cpu().numpy() - want) <= tol).all()
         _ = torch.randn(1000, device="cuda").sum().item()
+
+
+@pytest.mark.parametrize("kind", ["f16", "i8"])
+@pytest.mark.parametrize("H,n", [(8, 5), (16, 500)])
+def test_whole_tiles_that_see_nothing(kind, H, n):
+    """Every token stands past its window and the mask names none, or (causal) all stand ahead of their rows: zeros."""
+    rng = np.random.default_rng(n)
+    c = kv_ref.Cache(rng, kind, 2, 128, [400], [n])
+    q, at = queries(rng, c, H), np.full(n, 100000, np.int32)
+    assert (run(c, q, 70, 0, at, np.zeros((n, 1), np.uint64)) == 0).all()
+    assert (run(c, q, 70, 0, at) == 0).all()
+    rows = visible(c.lens, c.counts, 70, 3, at)
+    got = run(c, q, 70, 3, at)
+    k, v = c.rows(0, 0, 0, 3)
+    for t in (0, n // 2, n - 1):
+        assert rows[t] == [0, 1, 2]
+        for h in range(H):
+            kk, vv = k[:, h // (H // 2)], v[:, h // (H // 2)]
+            s = kk @ q[t, h].astype(np.float64) * 0.09
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            assert (np.abs(got[t, h] - w @ vv) <= kv_ref.tolerance(q[t, h].astype(np.float64), kk, vv, w, 0.09)).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "i8"])
+@pytest.mark.parametrize("H,n", [(8, 30), (16, 400)])
+def test_ranges_that_are_none(kind, H, n):
+    """Ranges that fall, overlap, begin below 0 or end past the rows: rows of no sequence stay as they are, and sequences
+    whose ranges lie apart from the others' keep their results."""
+    import torch
+    rng = np.random.default_rng(n)
+    lens, counts = [200, 70, 300, 90], [n, 6, 4, 9]
+    c = kv_ref.Cache(rng, kind, 2, 64, lens, counts)
+    q, T = queries(rng, c, H), sum(counts)
+    want = run(c, q, 100, 4)
+    kv = c.gpu()
+    qd = torch.from_numpy(q).cuda()
+    for first in ([0, n, n + 6, n + 10, T + 1], [0, n, n + 6, n + 10, 0x7fffffff], [0, n, n + 6, n + 4, T], [0, n, -0x80000000, n + 10, T],
+                  [5, 0, 3, -2, 7], [T, T, T, T, T], [-5, n, n + 6, n + 10, T]):
+        seqs = tie_amd.KVSeqs(torch.from_numpy(c.table).cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+                              torch.tensor(first, dtype=torch.int32).cuda(), T)
+        out = torch.full((T + 3, H, 64), -7.0, device="cuda")
+        kv.window_attention(0, seqs, qd, out[:T], 0.09, 100, sinks=4)
+        torch.cuda.synchronize()
+        got = out.cpu().numpy()
+        assert (got[T:] == -7.0).all()
+        if first[0] == 0 and first[1] == n:
+            tol = 1e-5 * (1 + np.abs(want[:n]).max())
+            assert (np.abs(got[:n] - want[:n]) <= tol).all(), first
+        if first[4] > T:
+            assert (got[n + 10: T] == -7.0).all()
+
+
+def test_the_streams_own_memory_is_for_calls_it_has_seen():
+    """Without work memory a capture is refused where the stream's has to grow, and taken once the call has run there."""
+    import torch
+    rng = np.random.default_rng(2)
+    c = kv_ref.Cache(rng, "f16", 2, 64, [700, 100], [40, 3])
+    kv, seqs = c.gpu(), c.seqs()
+    q = queries(rng, c, 8)
+    qd, out = torch.from_numpy(q).cuda(), torch.zeros(43, 8, 64, device="cuda")
+    l, lp = torch.randn(3, 9000, device="cuda"), torch.zeros(3, device="cuda")
+    tok = torch.zeros(3, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+
+    def calls():
+        kv.window_attention(0, seqs, qd, out, 0.09, 100, sinks=4)
+        tie_amd.token_logprobs(l, tok, lp)
+
+    torch.cuda.synchronize()
+    tie_amd.stream_release(side.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(tie_amd.TieError) as e:
+        with kv_ref.capture(graph, side):
+            calls()
+    assert e.value.code == tie_amd.EINVAL
+    with torch.cuda.stream(side):
+        calls()
+    torch.cuda.synchronize()
+    want, want_lp = out.clone(), lp.clone()
+    graph = torch.cuda.CUDAGraph()
+    with kv_ref.capture(graph, side):
+        calls()
+    for _ in range(3):
+        out.zero_(), lp.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lp, want_lp)
+
+
+def test_two_streams_at_once():
+    """Calls of one size on two streams, each with its stream's memory: the results of calls one behind another."""
+    import torch
+    rng = np.random.default_rng(7)
+    cs = [kv_ref.Cache(rng, "i8", 2, 128, [5000], [1]) for _ in range(2)]
+    qs = [queries(rng, c, 8) for c in cs]
+    want = [run(c, q, 4500, 4) for c, q in zip(cs, qs)]
+    kvs, seqs = [c.gpu() for c in cs], [c.seqs() for c in cs]
+    qd, outs = [torch.from_numpy(q).cuda() for q in qs], [torch.zeros(1, 8, 128, device="cuda") for _ in cs]
+    streams = [torch.cuda.Stream() for _ in cs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in (0, 1):
+            kvs[i].window_attention(0, seqs[i], qd[i], outs[i], 0.09, 4500, sinks=4, stream=streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert np.array_equal(outs[i].cpu().numpy(), want[i])

@@ -61,7 +61,7 @@ def test_caches_and_sequences(call):
             dict(lens=None), dict(new=None), dict(out=None), dict(first=None), dict(out=A + 4), dict(out=A + 1024 - 4),
             dict(first=A + 4096), dict(pos=A + 20480, slot=A + 20484), dict(first=A + 1024 - 12), dict(pos=A + 2048 + 8),
             dict(state_out=A + 12292), dict(free=A + 4096 + 56), dict(state_out=A + 2048), dict(slot=A)]),
-    (logprobs, [dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(n=-1), dict(n=(1 << 24) + 1), dict(stride=99), dict(temp=0.0),
+    (logprobs, [dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(n=-1), dict(n=(1 << 23) + 1), dict(stride=99), dict(temp=0.0),
                 dict(temp=-1.0), dict(temp=NAN), dict(temp=INF), dict(temp=1e7), dict(top=-1), dict(top=65), dict(logits=None),
                 dict(tt=None), dict(tl=None), dict(tokens=None), dict(tokens=None, rank=None), dict(lp=A + 1996), dict(rank=A + 4096),
                 dict(ent=A + 8192 + 16), dict(tl=A + 20480 + 56)]),

@@ -1796,8 +1796,9 @@ extern "C" int tie_hip_kv_plan(const tie_hip_kv_pool *pool, int n_seqs, int max_
 
 static int check_logprobs(int vocab, int n_tokens, int n_top)
 {
-	if (vocab < 1 || vocab > (1 << 24) || n_tokens < 0 || n_tokens > (1 << 24))
-		return set_error(TIE_HIP_EINVAL, "vocab=%d outside [1, 2^24] or n_tokens=%d outside [0, 2^24]", vocab, n_tokens);
+	// (a launch has fewer than 2^32 threads)
+	if (vocab < 1 || vocab > (1 << 24) || n_tokens < 0 || n_tokens > (1 << 23))
+		return set_error(TIE_HIP_EINVAL, "vocab=%d outside [1, 2^24] or n_tokens=%d outside [0, 2^23]", vocab, n_tokens);
 	if (n_top < 0 || n_top > LOGPROB_TOP)
 		return set_error(TIE_HIP_EINVAL, "n_top=%d outside [0, %d]", n_top, LOGPROB_TOP);
 	return TIE_HIP_OK;

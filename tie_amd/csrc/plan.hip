@@ -226,7 +226,7 @@ __device__ __forceinline__ void fill_request(const PlanArgs &a, int b, const Pla
 		return;
 	// (the first n.away pages from the first of them on)
 	int gone = 0;
-	for (int c = n.away0; gone < n.away; c += 64) {
+	for (int c = n.away0; gone < n.away && c < a.max_pages; c += 64) {
 		const int col = c + lane, page = col < a.max_pages ? row[col] : -1;
 		const bool away = is_page(a, page);
 		const unsigned long long set = __ballot(away);
@@ -244,12 +244,14 @@ __device__ __forceinline__ void fill_request(const PlanArgs &a, int b, const Pla
 __device__ __forceinline__ void finish_plan(const PlanArgs &a, const Ring &ring, const int *state, uint32_t need, uint32_t want,
 					    uint32_t away, int thread, int threads)
 {
-	for (int t = (int)want + thread; t < a.n_tokens; t += threads) {
-		if (a.pos)
-			a.pos[t] = -1;
-		if (a.slot)
-			a.slot[t] = -1;
-	}
+	// (n_tokens may be as large as an int: the counter is wider)
+	if (a.pos || a.slot)
+		for (size_t t = (size_t)want + thread; t < (size_t)a.n_tokens; t += threads) {
+			if (a.pos)
+				a.pos[t] = -1;
+			if (a.slot)
+				a.slot[t] = -1;
+		}
 	if (thread == 0) {
 		const bool none = ring.room == 0 && ring.free == 0; // (no ring)
 		const int back = (int)min(away, (uint32_t)ring.room);
@@ -421,7 +423,7 @@ hipError_t launch_plan(const PlanArgs &a, void *work, hipStream_t st)
 	}
 	PlanWork w;
 	carve_plan(a.n_seqs, (uint8_t *)work, &w);
-	const int blocks = (a.n_seqs + PLAN_BLOCK - 1) / PLAN_BLOCK, chunks = (a.n_tokens + 64 * PAGE - 1) / (64 * PAGE);
+	const int blocks = (a.n_seqs + PLAN_BLOCK - 1) / PLAN_BLOCK, chunks = a.n_tokens / (64 * PAGE) + 1;
 	tie_launch(plan_count_kernel, dim3(blocks), dim3(PLAN_THREADS), 0, st, a, w);
 	tie_launch(plan_fill_kernel, dim3(blocks, chunks < 1 ? 1 : chunks < 4 ? chunks : 4), dim3(PLAN_THREADS), 0, st, a, w);
 	return hipGetLastError();
