@@ -133,8 +133,8 @@ __device__ __forceinline__ int div_up(int a, int b)
 }
 
 struct Cut {
-	// (grain, least and rows are powers of two: shifts where divisions would be a third of
-	// the kernels' instructions, which are not in the cache when a call begins)
+	// (grain, least and rows are powers of two: shifts, where 64-bit divisions are a sixth of
+	// the kernels' instructions, on the way to a unit's first page)
 	int cap;   // units that run at once: at most so many where tiles are cut
 	int full;  // so many tiles are not cut
 	int grain; // pages that are not cut

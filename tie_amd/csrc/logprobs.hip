@@ -345,8 +345,8 @@ __device__ __forceinline__ void likeliest(const LogprobArgs &a, LpShared &sh, in
 	__syncthreads();
 	// the logits of the listed pairs of chunk and thread again, 16 of a pair, four to a
 	// lane (equal logits may bring more pairs than the list holds: then those of all
-	// threads that have one, chunk by chunk).  One place that sorts: what is not in
-	// the instruction cache yet costs more than the loop
+	// threads that have one, chunk by chunk).  One place that sorts, in a loop: a copy for
+	// each of the logits is 100 KB of code
 	const bool all = sh.listed > LP_LIST;
 	const int pairs = all ? LP_THREADS : sh.listed;
 #pragma unroll 1
@@ -488,8 +488,7 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 		}
 	}
 	// the threads joined; then, where there are parts, the parts by the last of them to
-	// finish, by the same code: it is in the instruction cache then (what is not costs 0.2 us for
-	// each 128 bytes of it, and bounds the short calls)
+	// finish, by the same code
 	if (tid == 0) {
 		sh.above = 0;
 		sh.listed = 0;
