@@ -78,7 +78,7 @@ def check(c, q, window, sinks, at=None, mask=None, work=None):
     assert not bad.any(), (np.argwhere(bad)[:4], got[bad][:4], want[bad][:4], tol[bad][:4])
 
 
-HEADS = [(8, 2, 128), (10, 2, 64), (3, 3, 64), (24, 1, 128)]
+HEADS = [(8, 2, 128), (10, 2, 64), (3, 3, 64), (20, 1, 128)]
 WINDOWS = [(1, 0), (1, 1), (5, 64), (64, 0), (65, 70), (100, 3), (130, 300), (1 << 20, 0), (0x7fffffff, 0x7fffffff)]
 
 

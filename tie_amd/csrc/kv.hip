@@ -171,8 +171,168 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 	}
 }
 
+// The sum, and the maximum, over the eight lanes of a head of 64, in all of them.
+__device__ __forceinline__ double head_sum(double x)
+{
+	x = x + dpp<0xb1, 0xf>(0.0, x); // lane ^ 1
+	x = x + dpp<0x4e, 0xf>(0.0, x); // lane ^ 2
+	return x + dpp<0x141, 0xf>(0.0, x); // the other four, mirrored
+}
+__device__ __forceinline__ float head_max(float x)
+{
+	x = __builtin_fmaxf(x, dpp<0xb1, 0xf>(0.0f, x));
+	x = __builtin_fmaxf(x, dpp<0x4e, 0xf>(0.0f, x));
+	return __builtin_fmaxf(x, dpp<0x141, 0xf>(0.0f, x));
+}
+
+// Many tokens of heads of 64 in 16-byte aligned rows: the same with a wave to a token
+// and four pairs to a lane, so that a norm's sum and root serve eight heads at a time, not
+// two, and rows go by 16 bytes a lane: 7479 tokens of 56 heads 56 us, 3.5 TB/s (by
+// the kernel above 66; int8 64 and 75), 4096 32 (38), 2048 19 either way; 44 without
+// V's pieces.  (Of heads of 128, where it is four against one: 8192 f16 tokens of 40 83 and
+// 87.5, 4096 int8 ones 54 and 48.)
+constexpr int MANY_TOKENS = 2500;
+template <bool I8>
+__global__ __launch_bounds__(256) void kv_append_rows_kernel(KvLayer c, KvSeqs s, AppendArgs a)
+{
+	constexpr int HD = 64, L = HD / 2, LN = HD / 8, G = 64 / LN; // lanes of a head, heads at a time
+	const int lane = threadIdx.x & 63, i = lane % LN * 4, part = lane / LN;
+	const int t = (blockIdx.x % DIES * (gridDim.x / DIES) + blockIdx.x / DIES) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	if (t >= s.n_tokens)
+		return;
+	int t0, n;
+	const int b = seq_of_token(s, t, t0, n);
+	if (b < 0)
+		return;
+	const int n_all = a.n_heads + 2 * c.kvh, units = (n_all + G - 1) / G;
+	constexpr int U = 3; // units whose rows are under way
+	f4 next[U][2];
+	auto fetch = [&](int u, f4 (&x)[2]) {
+		const int h = u * G + part, kv = h - a.n_heads;
+		if (h >= n_all)
+			return;
+		const float *p = kv < 0 ? a.q + (size_t)t * a.q_stride + (size_t)h * HD
+			       : kv < c.kvh ? a.k + (size_t)t * a.k_stride + (size_t)kv * HD
+					    : a.v + (size_t)t * a.v_stride + (size_t)(kv - c.kvh) * HD;
+		x[0] = __builtin_nontemporal_load(reinterpret_cast<const f4 *>(p + i));
+		x[1] = __builtin_nontemporal_load(reinterpret_cast<const f4 *>(p + i + L));
+	};
+#pragma unroll
+	for (int j = 0; j < U; j++) {
+		next[j][0] = next[j][1] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+		fetch(j, next[j]);
+	}
+	float wq[8], wk[8];
+#pragma unroll
+	for (int e = 0; e < 8; e++) {
+		const int at = e < 4 ? i + e : i + L + e - 4;
+		wq[e] = a.q_norm ? a.q_norm[at] : 1.0f;
+		wk[e] = a.k_norm ? a.k_norm[at] : 1.0f;
+	}
+	const int len = s.len[b];
+	const bool fits = seq_fits(s, len, n);
+	const int row = fits ? len + (t - t0) : 0;
+	const int page = fits ? page_of(s, c.n_pages, b, row) : -1, r = row % PAGE;
+	double cs[4], sn[4];
+#pragma unroll
+	for (int e = 0; e < 4; e++) {
+		const int32_t *pos = a.pos + t;
+		if (a.axes > 1)
+			pos += (size_t)(a.axis[(i + e) / 32] >> (i + e) % 32 * 2 & 3) * s.n_tokens;
+		const double at = a.pos ? (double)*pos : fits ? (double)row : __builtin_nan("");
+		sincos(at * exp2((double)(i + e) * (-2.0 / HD) * a.log2_theta), &sn[e], &cs[e]);
+	}
+	auto unit = [&](int u, const f4 (&in)[2]) {
+		const int h = u * G + part, kv = h - a.n_heads, head = kv < 0 ? h : kv < c.kvh ? kv : kv - c.kvh;
+		const bool on = h < n_all, is_q = kv < 0, is_v = kv >= c.kvh;
+		float x[8];
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			x[e] = in[e / 4][e % 4];
+		if (!__all(is_v)) {
+			double y[8];
+#pragma unroll
+			for (int e = 0; e < 8; e++)
+				y[e] = x[e];
+			if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
+				double ss = y[0] * y[0];
+#pragma unroll
+				for (int e = 1; e < 8; e++)
+					ss = __builtin_fma(y[e], y[e], ss);
+				const double f = rsqrt(__builtin_fma(head_sum(ss), 1.0 / HD, a.eps));
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+					y[e] *= f * (double)(is_q ? wq[e] : wk[e]);
+			}
+#pragma unroll
+			for (int e = 0; e < 4; e++) {
+				const float z0 = (float)__builtin_fma(y[e], cs[e], -(y[e + 4] * sn[e])), z1 = (float)__builtin_fma(y[e + 4], cs[e], y[e] * sn[e]);
+				x[e] = is_v ? x[e] : z0;
+				x[e + 4] = is_v ? x[e + 4] : z1;
+			}
+		}
+		if (on && is_q) { // (past the caches, which lose it before it is read)
+			f4 *o = reinterpret_cast<f4 *>(a.q_out + (size_t)t * a.qo_stride + (size_t)head * HD + i);
+			__builtin_nontemporal_store((f4){x[0], x[1], x[2], x[3]}, o);
+			__builtin_nontemporal_store((f4){x[4], x[5], x[6], x[7]}, o + L / 4);
+		}
+		if (__all(is_q))
+			return;
+		float scale = 0.0f;
+		if (I8) {
+			float big = 0.0f;
+#pragma unroll
+			for (int e = 0; e < 8; e++) // (NaN as infinity)
+				big = __builtin_fabsf(x[e]) < __builtin_inff() ? __builtin_fmaxf(big, __builtin_fabsf(x[e])) : __builtin_inff();
+			big = head_max(big);
+			scale = big < __builtin_inff() ? big / 127.0f : __builtin_nanf("");
+		}
+		if (!on || is_q || page < 0)
+			return;
+		const size_t at = (size_t)page * c.kvh + head; // this page's rows of this kv head
+		if (I8 && i == 0)
+			(is_v ? c.vs : c.ks)[at * PAGE + r] = scale;
+		typedef typename std::conditional<I8, int8_t, _Float16>::type T;
+		typedef T T4 __attribute__((ext_vector_type(4)));
+		T z[8];
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			z[e] = I8 ? (T)code_of(x[e], scale) : (T)half_of(x[e]);
+		if (is_v) {
+			T *o = reinterpret_cast<T *>(c.v) + (at * HD + i) * PAGE + r;
+#pragma unroll
+			for (int e = 0; e < 8; e++)
+				o[(e < 4 ? e : e - 4 + L) * PAGE] = z[e];
+		} else {
+			T4 *o = reinterpret_cast<T4 *>(reinterpret_cast<T *>(c.k) + (at * PAGE + r) * HD + i);
+			o[0] = (T4){z[0], z[1], z[2], z[3]};
+			o[L / 4] = (T4){z[4], z[5], z[6], z[7]};
+		}
+	};
+	for (int u = 0; u < units; u += U) {
+		f4 x[U][2];
+#pragma unroll
+		for (int j = 0; j < U; j++) {
+			x[j][0] = next[j][0];
+			x[j][1] = next[j][1];
+			fetch(u + U + j, next[j]);
+		}
+#pragma unroll
+		for (int j = 0; j < U; j++)
+			if (u + j < units)
+				unit(u + j, x[j]);
+	}
+}
+
 hipError_t launch_kv_append(const KvLayer &c, const KvSeqs &s, const AppendArgs &a, hipStream_t st)
 {
+	const bool aligned = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out |
+			       (a.q_stride | a.k_stride | a.v_stride | a.qo_stride) * 4) & 15) == 0;
+	if (c.hd == 64 && s.n_tokens >= MANY_TOKENS && aligned) {
+		const dim3 groups(((s.n_tokens + 3) / 4 + DIES - 1) / DIES * DIES);
+		tie_launch(c.i8 ? kv_append_rows_kernel<true> : kv_append_rows_kernel<false>, groups, dim3(256), 0, st, c, s, a);
+		return hipGetLastError();
+	}
 	const int units = (a.n_heads + 2 * c.kvh + 128 / c.hd - 1) / (128 / c.hd); // a wave's share at a time: a head of 128, two of 64
 	// a wave takes one unit where there are few tokens, else as many as leave
 	// 4096 waves: the angles' cosines are the same for all of them
