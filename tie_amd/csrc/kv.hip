@@ -43,7 +43,7 @@ __device__ __forceinline__ _Float16 half_of(float x)
 // past the caches (66).
 constexpr int DIES = 8;
 
-template <int HD, bool I8, int U>
+template <int HD, bool I8, int U, bool AXES>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, AppendArgs a, int per_wave)
 {
 	constexpr int L = HD / 2, G = 64 / L; // lanes of a head, heads of a wave at a time
@@ -87,11 +87,12 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 	const bool fits = seq_fits(s, len, n);
 	const int row = fits ? len + (t - t0) : 0;
 	const int page = fits ? page_of(s, c.n_pages, b, row) : -1, r = row % PAGE;
-	const int32_t *pos = a.pos + t;
-	if (a.axes > 1) // (as the pair's axis says: a load for each lane then)
-		pos += (size_t)(a.axis[i / 32] >> i % 32 * 2 & 3) * s.n_tokens;
-	// (no row: no position)
-	const double at = a.pos ? (double)*pos : fits ? (double)row : __builtin_nan("");
+	// (no row: no position; several axes: a load for each lane, by the pair's)
+	double at = fits ? (double)row : __builtin_nan("");
+	if (AXES && a.axes > 1)
+		at = (double)a.pos[(size_t)(a.axis[i / 32] >> i % 32 * 2 & 3) * s.n_tokens + t];
+	else if (a.pos)
+		at = (double)a.pos[t];
 	double cs, sn;
 	sincos(at * exp2((double)i * (-2.0 / HD) * a.log2_theta), &sn, &cs);
 	auto unit = [&](int u, float x0, float x1) {
@@ -341,14 +342,20 @@ hipError_t launch_kv_append(const KvLayer &c, const KvSeqs &s, const AppendArgs 
 	per = per > (units + 3) / 4 ? (units + 3) / 4 : per;
 	const dim3 grid((s.n_tokens + DIES - 1) / DIES * DIES, (units + 4 * per - 1) / (4 * per));
 	auto go = [&](auto kern) { tie_launch(kern, grid, dim3(256), 0, st, c, s, a, per); };
-	auto by_units = [&](auto units_ahead) {
+	auto by = [&](auto units_ahead, auto axes) {
 		constexpr int U = decltype(units_ahead)::value;
+		constexpr bool A = decltype(axes)::value;
 		if (c.hd == 128)
-			c.i8 ? go(kv_append_kernel<128, true, U>) : go(kv_append_kernel<128, false, U>);
+			c.i8 ? go(kv_append_kernel<128, true, U, A>) : go(kv_append_kernel<128, false, U, A>);
 		else
-			c.i8 ? go(kv_append_kernel<64, true, U>) : go(kv_append_kernel<64, false, U>);
+			c.i8 ? go(kv_append_kernel<64, true, U, A>) : go(kv_append_kernel<64, false, U, A>);
 	};
-	per < 4 ? by_units(std::integral_constant<int, 1>()) : by_units(std::integral_constant<int, 4>());
+	if (per >= 4)
+		by(std::integral_constant<int, 4>(), std::true_type());
+	else if (a.axes > 1)
+		by(std::integral_constant<int, 1>(), std::true_type());
+	else // (0.1 us of one token's 4 without the choice)
+		by(std::integral_constant<int, 1>(), std::false_type());
 	return hipGetLastError();
 }
 
