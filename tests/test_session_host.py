@@ -162,3 +162,17 @@ def test_the_binding_names_the_stream(monkeypatch):
                 lambda: tie_amd.token_logprobs(torch.zeros(2, 50, dtype=torch.float16), two, torch.zeros(2))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("bad", [32, np.zeros(4, np.int64), np.zeros(16, np.int16), [0] * 31 + [256], [0] * 31 + [-1], [0.0] * 32])
+def test_axes_that_are_not_one_small_number_for_each_pair(bad):
+    """(32 is not 32 zeros, and an array's numbers are looked at, not its memory)"""
+    import torch
+    k = torch.zeros(1, 2, 2, 64, 64, dtype=torch.float16)
+    c, s = tie_amd.KVCache(k, k.clone()), tie_amd.KVSeqs(torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
+    q, kv = torch.zeros(2, 256), torch.zeros(2, 128)
+    with pytest.raises((ValueError, TypeError)):
+        c.append_axes(0, s, q, kv, kv, q, torch.zeros(3, 2, dtype=torch.int32), bad)
+    with pytest.raises(tie_amd.TieError):
+        c.append_axes(0, s, q, kv, kv, q, None, PAIRS)
+    assert "n_axes" in tie_amd.last_error()

@@ -646,13 +646,13 @@ class KVCache:
     def append_axes(self, layer, seqs, q, k, v, q_out, pos, axes, q_norm=None, k_norm=None, eps=1e-6, theta=1e6, stream=None):
         """tie_hip_kv_append_axes: append with pos [n_axes][n_tokens]; axes: the axis of each of a head's head_dim / 2 pairs
         (small whole numbers, or bytes)."""
-        n, dev, axes = seqs.n_tokens, self.device, bytes(axes)
+        n, dev, axes = seqs.n_tokens, self.device, axes if type(axes) is bytes else bytes(iter(axes))
         if len(axes) != self.head_dim // 2:
             raise ValueError("axes: one for each of %d pairs is wanted (got %d)" % (self.head_dim // 2, len(axes)))
         pq, sq, po, so, heads = self._q(q, q_out, seqs, "q_out")
         pk, sk, _ = _rows(k, "k", dev, self.width, n)
         pv, sv, _ = _rows(v, "v", dev, self.width, n)
-        n_axes = pos.shape[0]
+        n_axes = 0 if pos is None else pos.shape[0]
         check(lib().tie_hip_kv_append_axes(self.ref, layer, seqs.ref, pq, sq, pk, sk, pv, sv, heads,
                                            _array(q_norm, "float32", self.head_shape, "q_norm", dev),
                                            _array(k_norm, "float32", self.head_shape, "k_norm", dev), eps, theta,
