@@ -21,6 +21,11 @@
 // The maximum m is a reference only: it moves when some weight would pass
 // 2^MOVE, so most steps need no exchange between lanes and leave O alone.  (int8:
 // when some weight times its row's V scale would pass f16; see weigh8.)
+//
+// Through a window (WIN) a tile walks the pages of the first rows and those from its
+// lowest visible row on, and masks what lies beside them: the same kernels, with
+// the same bounds (61 f16 tokens over 4096 rows of up to 30000, 481 MB: 92 us, 5.2 TB/s;
+// a chunk of 4096 over 1024, 69 GFLOP: 142 us).
 #include <type_traits>
 
 #include "kv.h"
@@ -122,16 +127,16 @@ __device__ __forceinline__ float pow2_below(float x)
 	return __uint_as_float(__float_as_uint(x) & 0x7f800000u);
 }
 
-// How the work of a call is cut: sequence b has tiles(b) row tiles for each kv
-// head, each over pages(b) pages, in parts of as many pages -- one unit of work
-// (a workgroup) for each.  Every workgroup finds the cut by itself from
-// the lengths on the device, so that neither a copy to the host nor a launch
-// for a plan stands before the attention and captured calls follow the lengths.
 __device__ __forceinline__ int div_up(int a, int b)
 {
 	return (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b);
 }
 
+// How the work of a call is cut: sequence b has tiles(b) row tiles for each kv
+// head, each over pages(b) pages, in parts of as many pages -- one unit of work
+// (a workgroup) for each.  Every workgroup finds the cut by itself from
+// the lengths on the device, so that neither a copy to the host nor a launch
+// for a plan stands before the attention and captured calls follow the lengths.
 struct Cut {
 	// (grain, least and rows are powers of two: shifts, where 64-bit divisions are a sixth of
 	// the kernels' instructions, on the way to a unit's first page)

@@ -34,8 +34,7 @@ __device__ __forceinline__ _Float16 half_of(float x)
 // cosine and sine stay with it.  All of it in 64 bits up to the one rounding to
 // F32: positions reach where a 32-bit angle is off by a thousandth, and a key's
 // code must not depend on the order of a 32-bit sum.  One token: bound by its
-// chain of steps (position, angle, sincos; row, norm, code), 3.6 us (on the default
-// stream 4.1).  Many: by the bytes, the 64-bit arithmetic (about 60 instructions
+// chain of steps (position, angle, sincos; row, norm, code), 4.3 us.  Many: by the bytes, the 64-bit arithmetic (about 60 instructions
 // for 64 pairs) and the V columns' pieces (a row's values lie PAGE apart) together:
 // 7479 tokens of 56 heads of 64 from memory (200 MB) 66 us, 3.0 TB/s; 50 without the
 // stores, 60 without the arithmetic, 33 without both.  U: heads whose rows are under

@@ -5,9 +5,9 @@
 //   Z = sum exp(x_i / T),  log p(i) = x_i / T - log Z,
 //   entropy = -sum p log p = log Z - sum x_i exp(x_i / T) / (T Z).
 // Each wave keeps a running m (which moves a few times in a row) and each lane its two
-// sums in 64 bits; they are brought to one m when waves are joined.  Exponentials are F32 (an ulp each, so that
-// the sums are good to 1e-7 of themselves whatever their length; the largest logit's
-// is exactly 1, so that a sure token's small logarithm keeps its digits).
+// sums in 64 bits; they are brought to one m when waves are joined.  Exponentials are
+// F32 (an ulp each, so that the sums are good to 1e-7 of themselves whatever their length;
+// the largest logit's is exactly 1, so that a sure token's small logarithm keeps its digits).
 //
 // The n likeliest: each thread keeps the largest of its logits.  n threads have one
 // that reaches the n-th largest of those maxima, so no logit below it is among the n
@@ -17,7 +17,9 @@
 // reaches the bound is sorted, 64 at a time where equal logits bring more.
 //
 // A workgroup has a row, or a part of one where there are few rows; the last
-// of a row's parts to finish joins them.
+// of a row's parts to finish joins them.  Many rows: bound by memory (2047 of 151936
+// 202 us, 6.1 TB/s); few: by the row's chain of steps (one of 32000 9.3 us, 61 of
+// 151936 21.7, of which the logits 6.4).
 #include "kv.h"
 
 namespace tie {
@@ -44,9 +46,9 @@ struct LpWork {
 
 // A row's parts: enough workgroups for a CU and a half each (a hand-over costs 5 us and the
 // last part's chain 6: 400 rows of 151936 by a workgroup each 49 us, by three 64; 61
-// by seven 22.5, by 17 25 and by five 24.6), and one chunk each, but 16 or more only
-// for rows of more than 8 chunks each (8 rows of 151936 by 16 workgroups each 16.0 us, by 38
-// 19; one 13.5 and 13.6).
+// by seven 22.5, by 17 25 and by five 24.6), a chunk or more to each, and more than 16 only where
+// each has eight chunks (8 rows of 151936 by 16 workgroups each 16.0 us, by 38 19; one 13.5
+// and 13.6).
 static int lp_parts(int vocab, int rows)
 {
 	const int chunks = (vocab + LP_CHUNK - 1) / LP_CHUNK, want = (LP_AT_ONCE + rows - 1) / rows;
