@@ -62,8 +62,10 @@ size_t plan_work_bytes(int n_seqs)
 	return carve_plan(n_seqs, nullptr, nullptr);
 }
 
-// Sums that stay at 2^32 - 1 when they pass it: every number and limit here is below 2^31,
-// so they are exact where they matter and too large where not.
+// Sums that stay at 2^32 - 1 when they pass it.  A limit is below 2^31, and so is one request's
+// count: a sum that fits is exact, and so is the one that first does not, less that request.
+// A block's sum may have stayed at 2^32 - 1 itself: it says that the block does not fit, and
+// nothing is taken off it or off a sum that holds it.
 __device__ __forceinline__ uint32_t plus(uint32_t x, uint32_t y)
 {
 	return __builtin_elementwise_add_sat(x, y);
@@ -358,8 +360,9 @@ __global__ __launch_bounds__(PLAN_THREADS) void plan_fill_kernel(PlanArgs a, Pla
 			const int l = s.over(a, ring, need, want);
 			if (l < 64) {
 				const int from = (k0 + l) * PLAN_BLOCK;
-				s.need = plus(s.need, sum_at(need - x[0], l));
-				s.want = plus(s.want, sum_at(want - x[1], l));
+				// (before that block: the sums up to the lane before)
+				s.need = plus(s.need, l ? sum_at(need, l - 1) : 0);
+				s.want = plus(s.want, l ? sum_at(want, l - 1) : 0);
 				uint32_t none[3];
 				s.add(a, ring, counts_at(w.counts, from, min(PLAN_BLOCK, a.n_seqs - from)), none[0], none[1], none[2]);
 			} else {
