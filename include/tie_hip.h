@@ -306,8 +306,8 @@ typedef struct tie_hip_kv_seqs {
  *             position), NULL: the token's cache row (a query without one, as
  *             its sequence's length is none, is NaN)
  * in 64 bits, rounded once.  The queries go to q_out (which may be q, with the
- * same stride, or other columns of the same matrix), keys and values to the
- * cache. */
+ * same stride, or other columns of the same matrix; it shares no memory with k, v,
+ * pos or the sequences' arrays), keys and values to the cache. */
 int tie_hip_kv_append(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q, size_t q_stride,
 		      const float *k, size_t k_stride, const float *v, size_t v_stride, int n_heads, const float *q_norm,
 		      const float *k_norm, float eps, float theta, const int32_t *pos, float *q_out, size_t q_out_stride,
@@ -339,7 +339,8 @@ int tie_hip_kv_read(const tie_hip_kv_cache *cache, int layer, int n_layers, cons
  * the words are not seen).  mask NULL: token i sees tokens 0 .. i (a prompt's
  * chunk, a chain, a single token).  A row that sees nothing gives 0.
  *   q    [n_tokens] rows of n_heads heads (as tie_hip_kv_append leaves them)
- *   out  the same shape (may be q, with the same stride)
+ *   out  the same shape (may be q, with the same stride; it shares no memory with
+ *        the mask or the sequences' arrays)
  *   work work_bytes of device memory, 16-byte aligned, at least
  *        tie_hip_tree_attention_work_bytes, filled with zeros before the first
  *        call that gets it and after anything else has written to it (calls
@@ -375,8 +376,8 @@ int tie_hip_tree_attention(const tie_hip_kv_cache *cache, int layer, const tie_h
  * that lie behind the window.
  * Pages that hold no row that a token sees are not looked at: their entries in
  * the page table may be none, as tie_hip_kv_plan leaves them.
- * window at least 1, sinks 0 or more; everything else, scratch memory included, as
- * for tie_hip_tree_attention.  The work bytes are enough for any window. */
+ * window at least 1, sinks 0 or more; out shares no memory with at either; everything
+ * else, scratch memory included, as for tie_hip_tree_attention.  The work bytes are enough for any window. */
 size_t tie_hip_window_attention_work_bytes(const tie_hip_kv_cache *cache, const tie_hip_kv_seqs *seqs, int n_heads);
 int tie_hip_window_attention(const tie_hip_kv_cache *cache, int layer, const tie_hip_kv_seqs *seqs, const float *q,
 			     size_t q_stride, int n_heads, float scale, int window, int sinks, const int32_t *at,

@@ -1470,6 +1470,18 @@ static bool rows_overlap(int T, const float *a, size_t sa, size_t wa, const floa
 	return off < wa * 4 || off + wb * 4 > (size_t)row;
 }
 
+// Whether T rows of `w` floats share memory with n bytes from p; what lies in the gaps
+// between the rows does not.
+static bool rows_meet(int T, const float *a, size_t stride, size_t w, const void *p, size_t n)
+{
+	if (!overlap(a, row_span(T, stride, w), p, n))
+		return false;
+	if ((uintptr_t)p <= (uintptr_t)a)
+		return true;
+	const size_t row = stride * 4, off = ((uintptr_t)p - (uintptr_t)a) % row; // p's place behind a row's begin
+	return off < w * 4 || off + n > row;
+}
+
 } // namespace tie
 
 #define TIE_TRY(expr)                     \
@@ -1509,6 +1521,9 @@ static int append_call(const tie_hip_kv_cache *cache, int layer, const tie_hip_k
 	if ((!(q_out == q && q_out_stride == q_stride) && rows_overlap(T, q_out, q_out_stride, wq, q, q_stride, wq)) ||
 	    rows_overlap(T, q_out, q_out_stride, wq, k, k_stride, wk) || rows_overlap(T, q_out, q_out_stride, wq, v, v_stride, wk))
 		return set_error(TIE_HIP_EINVAL, "q_out overlaps an input (it may be q itself, with q's stride)");
+	// (positions are read while other tokens' queries are written; in place they would lie in q's own values)
+	if (q_out != q && pos && rows_meet(T, q_out, q_out_stride, wq, pos, (size_t)a.axes * T * sizeof *pos))
+		return set_error(TIE_HIP_EINVAL, "q_out overlaps pos");
 	CallersDevice back;
 	TIE_TRY(ensure_init());
 	if (none)
@@ -1671,6 +1686,12 @@ static int attention_call(const tie_hip_kv_cache *cache, int layer, const tie_hi
 	if (!(out == q && out_stride == q_stride) &&
 	    rows_overlap(s.n_tokens, out, out_stride, w, q, q_stride, w))
 		return set_error(TIE_HIP_EINVAL, "out overlaps q (it may be q itself, with q's stride)");
+	// (both are read while other rows' results are written)
+	const size_t T = s.n_tokens;
+	if (mask && rows_meet(s.n_tokens, out, out_stride, w, mask, T * mask_words * sizeof *mask))
+		return set_error(TIE_HIP_EINVAL, "out overlaps mask");
+	if (a.at && rows_meet(s.n_tokens, out, out_stride, w, a.at, T * sizeof *a.at))
+		return set_error(TIE_HIP_EINVAL, "out overlaps at");
 	CallersDevice back;
 	TIE_TRY(ensure_init());
 	if (none)
