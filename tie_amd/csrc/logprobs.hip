@@ -6,8 +6,12 @@
 //   entropy = -sum p log p = log Z - sum x_i exp(x_i / T) / (T Z).
 // Each wave keeps a running m (which moves a few times in a row) and each lane its two
 // sums in 64 bits; they are brought to one m when waves are joined.  Exponentials are
-// F32 (an ulp each, so that the sums are good to 1e-7 of themselves whatever their length;
-// the largest logit's is exactly 1, so that a sure token's small logarithm keeps its digits).
+// F32, of arguments x / T in 64 bits whose rest beside a whole power of two is rounded to
+// 23 bits: each is off by at most 1.4 2^-23 of itself however far x is (2^-24 log 2 of the
+// rest, an ulp of v_exp_f32), and so are the sums whatever their length.  (An argument rounded
+// to F32 is off by half a unit in its last place, which equal and near logits have in common:
+// 1.2e-6 of exponentials at x = -20, and no sum averages it out.)  The largest
+// logit's is exactly 1, so that a sure token's small logarithm keeps its digits.
 //
 // The n likeliest: each thread keeps the largest of its logits.  n threads have one
 // that reaches the n-th largest of those maxima, so no logit below it is among the n
@@ -19,7 +23,7 @@
 // A workgroup has a row, or a part of one where there are few rows; the last
 // of a row's parts to finish joins them.  Many rows: bound by memory (2047 of 151936
 // 202 us, 6.1 TB/s); few: by the row's chain of steps (one of 32000 9.3 us, 61 of
-// 151936 21.7, of which the logits 6.4).
+// 151936 21.5, of which the logits 6.4).
 #include "kv.h"
 
 namespace tie {
@@ -189,9 +193,11 @@ struct Sums {
 	// to another m, not below its own (rate: log2 e / T)
 	__device__ __forceinline__ void move(float to, double rate)
 	{
-		const double by = m > -__builtin_inff() ? (double)m - to : 0.0, f = exp2(by * rate);
-		s *= f;
-		t = t * f + by * s;
+		if (m > -__builtin_inff() && m < to) {
+			const double by = (double)m - to, f = exp2(by * rate);
+			s *= f;
+			t = t * f + by * s;
+		}
 		m = to;
 	}
 };
@@ -444,12 +450,15 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 	const int token = a.tokens ? a.tokens[row] : -1;
 	const bool is_token = token >= 0 && token < a.vocab;
 	const float mine = is_token ? l[token] : __builtin_inff();
-	const double rate = a.rate;
-	const float rate32 = (float)rate;
-	const float far = -200.0f / rate32; // from there on exp() is 0
+	const double rate = a.rate, far = -127.0 / rate;
+	const double grid = 0x1.8p29 - 1.0; // added to z, it leaves z - 1 in units of 2^-23 in the lower half
+	// x > mine, and x < mine, are the signs of differences (of zeros +0), where mine is above -infinity
+	const bool signs = mine > -__builtin_inff();
+	const float mine_up = mine + 0.0f, mine_down = mine == 0.0f ? -0.0f : mine;
 	Sums d;
 	Mosts t;
 	int above = 0;
+	bool nan = false;
 	for (int c = c0; c < c1; c++) {
 		float x[LP_E];
 #pragma unroll
@@ -460,35 +469,49 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 		float most = x[0];
 #pragma unroll
 		for (int e = 1; e < LP_E; e++)
-			most = __builtin_fmaxf(most, x[e]);
-		// (equal logits count where they come before the token: not in chunks behind its own)
+			most = __builtin_elementwise_maximum(most, x[e]); // (NaN if any is)
+		nan = nan || most != most;
+		// (equal logits count where they come before the token: not in chunks behind its own.
+		// By signs: 400 rows of 151936 55 us, by comparisons whose masks are counted 59)
 		if (a.rank) {
-			if ((c + 1) * LP_CHUNK <= token) {
+			if (signs && (c + 1) * LP_CHUNK <= token) {
+				above += LP_E;
 #pragma unroll
 				for (int e = 0; e < LP_E; e++)
-					above += __popcll(__ballot(x[e] >= mine));
-			} else if (c * LP_CHUNK > token) {
+					above -= (int)(__float_as_uint(x[e] - mine_down) >> 31);
+			} else if (signs && c * LP_CHUNK > token) {
 #pragma unroll
 				for (int e = 0; e < LP_E; e++)
-					above += __popcll(__ballot(x[e] > mine));
+					above += (int)(__float_as_uint(mine_up - x[e]) >> 31);
 			} else {
 #pragma unroll
 				for (int e = 0; e < LP_E; e++)
-					above += __popcll(__ballot(x[e] > mine || (x[e] == mine && index(c, e) < token)));
+					above += (int)(x[e] > mine) | ((int)(x[e] == mine) & (int)(index(c, e) < token));
 			}
 		}
 		t.add(most, c);
 		if (__any(most > d.m))
 			d.move(wave_max(t.most), rate);
-		const float m = d.m == -__builtin_inff() ? 0.0f : d.m;
+		const double m = d.m == -__builtin_inff() ? 0.0 : (double)d.m;
 #pragma unroll
 		for (int e = 0; e < LP_E; e++) {
-			const float y = x[e] - m, p = __builtin_amdgcn_exp2f(y * rate32);
-			d.s += (double)p;
-			// (y of -infinity, whose p is 0)
-			d.t = __builtin_fma((double)__builtin_fmaxf(y, far), (double)p, d.t);
+			// 2^z = 2^n 2^f: w holds n - 1 in its upper 9 bits and f in the lower 23, which are 1 + f's
+			// mantissa; the exponential of that, from 2 on, gets n - 1 added to its exponent.  (Whole
+			// numbers at twice the 64-bit rate: 2047 rows of 151936 202 us, with whole and rest of z by
+			// 64-bit sums 214.  z of -127, -infinity and NaN give 0, z above that and below -126 less
+			// than 2^-126)
+			const double y = __builtin_fmax((double)x[e] - m, far);
+			const uint32_t w = (uint32_t)__double_as_longlong(__builtin_fma(y, rate, grid));
+			const float e2 = __builtin_amdgcn_exp2f(__uint_as_float((w & 0x7fffffu) | 0x3f800000u));
+			const double p = (double)__uint_as_float(__float_as_uint(e2) + (w & 0xff800000u));
+			d.s += p;
+			d.t = __builtin_fma(y, p, d.t);
 		}
 	}
+	if (nan)
+		d.s = __builtin_nan("");
+	if (a.rank)
+		above = (int)wave_total((double)above);
 	// the threads joined; then, where there are parts, the parts by the last of them to
 	// finish, by the same code
 	if (tid == 0) {
