@@ -21,9 +21,9 @@
 // reaches the bound is sorted, 64 at a time where equal logits bring more.
 //
 // A workgroup has a row, or a part of one where there are few rows; the last
-// of a row's parts to finish joins them.  Many rows: bound by memory (2047 of 151936
-// 202 us, 6.1 TB/s); few: by the row's chain of steps (one of 32000 9.3 us, 61 of
-// 151936 21.5, of which the logits 6.4).
+// of a row's parts to finish joins them.  Many rows: bound by memory and the 64-bit arithmetic
+// at once (2047 of 151936 207 us, 6.0 TB/s; 203 with exponentials of F32 arguments); few: by the
+// row's chain of steps (one of 32000 8.9 us, 61 of 151936 22.4, of which the logits 6.4).
 #include "kv.h"
 
 namespace tie {
@@ -31,7 +31,7 @@ namespace tie {
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int LP_THREADS = 256, LP_WAVES = LP_THREADS / 64, LP_E = 16, LP_CHUNK = LP_THREADS * LP_E;
-constexpr int LP_AT_ONCE = 384; // workgroups
+constexpr int LP_AT_ONCE = 384, LP_PARTS = 1024; // workgroups where rows are few, parts of a call at most
 constexpr int LP_LIST = 1024; // (chunk, thread) whose logits are read again, at most: else all of the threads'
 constexpr float LOWEST = -3.402823466e38f;
 
@@ -48,15 +48,18 @@ struct LpWork {
 	int *count;   // [rows]
 };
 
-// A row's parts: enough workgroups for a CU and a half each (a hand-over costs 5 us and the
-// last part's chain 6: 400 rows of 151936 by a workgroup each 49 us, by three 64; 61
-// by seven 22.5, by 17 25 and by five 24.6), a chunk or more to each, and more than 16 only where
-// each has eight chunks (8 rows of 151936 by 16 workgroups each 16.0 us, by 38 19; one 13.5
-// and 13.6).
+// A row's parts.  Fewer than 64 rows: enough workgroups for a CU and a half each, a chunk or more
+// to each, and more than 16 only where each has eight chunks (a hand-over costs 5 us and the last
+// part's chain 6: 61 rows of 151936 by seven 22.4 us, by five 25.2; 32 by twelve 19.8, by 16 20.8;
+// 8 by 16 15.8, by eight 17.7; one 13.7).  64 to 170: just under two workgroups to a CU (100 rows
+// by five 26.7, by four 30; 128 by four 29.8, by three 34).  To 341: three parts (200 rows 41, by
+// two 44; 300 52, by two 55; by one 39 and 54, but rows that are not 16-byte aligned, of 128257, 46
+// against 37).  Then two (383 58, by one 55, unaligned 54 and 63), and whole rows where those fill
+// the card (384 by one 55, by three 65).
 static int lp_parts(int vocab, int rows)
 {
-	const int chunks = (vocab + LP_CHUNK - 1) / LP_CHUNK, want = (LP_AT_ONCE + rows - 1) / rows;
-	const int most = chunks < 16 ? chunks : chunks / 8 < 16 ? 16 : chunks / 8;
+	const int chunks = (vocab + LP_CHUNK - 1) / LP_CHUNK, most = chunks < 16 ? chunks : chunks / 8 < 16 ? 16 : chunks / 8;
+	const int want = rows >= 64 && rows <= 170 ? 512 / rows : rows > 170 && rows <= 341 ? 3 : (LP_AT_ONCE + rows - 1) / rows;
 	return want < most ? want : most;
 }
 
@@ -77,12 +80,11 @@ static size_t carve_logprobs(size_t parts, int n, uint8_t *base, LpWork *w)
 	return off;
 }
 
-// Enough for every call of no more logits, rows and alternatives: where there are parts,
-// there are fewer than 2 LP_AT_ONCE.
+// Enough for every call of no more logits, rows and alternatives.
 size_t logprobs_work_bytes(int vocab, int rows, int n)
 {
-	const size_t chunks = ((size_t)vocab + LP_CHUNK - 1) / LP_CHUNK, all = (rows < LP_AT_ONCE ? rows : LP_AT_ONCE) * chunks;
-	return carve_logprobs(all < 2 * LP_AT_ONCE ? all : 2 * LP_AT_ONCE, n, nullptr, nullptr);
+	const size_t chunks = ((size_t)vocab + LP_CHUNK - 1) / LP_CHUNK, all = rows * chunks;
+	return carve_logprobs(all < LP_PARTS ? all : LP_PARTS, n, nullptr, nullptr);
 }
 
 // what one workgroup writes for another of the same launch goes past the dies' caches
@@ -472,8 +474,9 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 			most = __builtin_elementwise_maximum(most, x[e]); // (NaN if any is)
 		nan = nan || most != most;
 		// (equal logits count where they come before the token: not in chunks behind its own.
-		// By signs: 400 rows of 151936 55 us, by comparisons whose masks are counted 59)
-		if (a.rank) {
+		// By signs: 400 rows of 151936 55 us, by comparisons whose masks are counted 59.  A
+		// likely token has few chunks with a logit before it)
+		if (a.rank && __any(most >= mine)) {
 			if (signs && (c + 1) * LP_CHUNK <= token) {
 				above += LP_E;
 #pragma unroll
@@ -497,8 +500,8 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 		for (int e = 0; e < LP_E; e++) {
 			// 2^z = 2^n 2^f: w holds n - 1 in its upper 9 bits and f in the lower 23, which are 1 + f's
 			// mantissa; the exponential of that, from 2 on, gets n - 1 added to its exponent.  (Whole
-			// numbers at twice the 64-bit rate: 2047 rows of 151936 202 us, with whole and rest of z by
-			// 64-bit sums 214.  z of -127, -infinity and NaN give 0, z above that and below -126 less
+			// numbers at twice the 64-bit rate: 2047 rows of 151936 207 us, with whole and rest of z by
+			// 64-bit sums 218; 203 without the clamp.  z of -127, -infinity and NaN give 0, z above that and below -126 less
 			// than 2^-126)
 			const double y = __builtin_fmax((double)x[e] - m, far);
 			const uint32_t w = (uint32_t)__double_as_longlong(__builtin_fma(y, rate, grid));
