@@ -34,12 +34,14 @@ __device__ __forceinline__ _Float16 half_of(float x)
 // cosine and sine stay with it.  All of it in 64 bits up to the one rounding to
 // F32: positions reach where a 32-bit angle is off by a thousandth, and a key's
 // code must not depend on the order of a 32-bit sum.  One token: bound by its
-// chain of steps (position, angle, sincos; row, norm, code), 4.3 us.  Many: by the bytes, the 64-bit arithmetic (about 60 instructions
-// for 64 pairs) and the V columns' pieces (a row's values lie PAGE apart) together:
-// 7479 tokens of 56 heads of 64 from memory (200 MB) 66 us, 3.0 TB/s; 50 without the
-// stores, 60 without the arithmetic, 33 without both.  U: heads whose rows are under
-// way at once (4 where a wave has so many: 75 to 69 us; 8 72), and there the queries go
-// past the caches (66).
+// chain of steps (position, angle, sincos; row, norm, code), 4.1 to 4.3 us.  Many: by the bytes,
+// the 64-bit arithmetic (about 60 instructions for 64 pairs) and the V columns' pieces (a
+// row's values lie PAGE apart) together: from memory 8192 tokens of 40 heads of 128 (319 MB)
+// 85 us, 3.8 TB/s, 8000 of 72 as int8 (566 MB) 115, 4.9; 7479 of 56 heads of 64 whose rows are not
+// 16-byte aligned (200 MB) 65, 3.1.  (Those, aligned, 66: 50 without the stores, 60 without the
+// arithmetic, 33 without both; kv_append_rows_kernel below takes them now.)  U: heads whose rows
+// are under way at once: four where a wave has so many (8192 tokens 94 us by one, 86.5 by two,
+// 86 by eight), and there the queries go past the caches.
 constexpr int DIES = 8;
 
 template <int HD, bool I8, int U, bool AXES>
@@ -92,6 +94,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 		at = (double)a.pos[(size_t)(a.axis[i / 32] >> i % 32 * 2 & 3) * s.n_tokens + t];
 	else if (a.pos)
 		at = (double)a.pos[t];
+	// (the cache's addresses early: chosen by is_v they would be loaded behind the codes, at the end
+	// of one token's chain)
+	uint8_t *ck = c.k, *cv = c.v;
+	float *ks = c.ks, *vs = c.vs;
+	asm volatile("" : "+s"(ck), "+s"(cv), "+s"(ks), "+s"(vs));
 	double cs, sn;
 	sincos(at * exp2((double)i * (-2.0 / HD) * a.log2_theta), &sn, &cs);
 	auto unit = [&](int u, float x0, float x1) {
@@ -140,15 +147,15 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvLayer c, KvSeqs s, App
 			return;
 		const size_t at = (size_t)page * c.kvh + head; // this page's rows of this kv head
 		if (I8 && i == 0)
-			(is_v ? c.vs : c.ks)[at * PAGE + r] = scale;
+			(is_v ? vs : ks)[at * PAGE + r] = scale;
 		const size_t e0 = at * PAGE * HD + (is_v ? (size_t)i * PAGE + r : (size_t)r * HD + i);
 		const size_t e1 = e0 + (is_v ? (size_t)L * PAGE : (size_t)L);
 		if (I8) {
-			int8_t *o = reinterpret_cast<int8_t *>(is_v ? c.v : c.k);
+			int8_t *o = reinterpret_cast<int8_t *>(is_v ? cv : ck);
 			o[e0] = code_of(x0, scale);
 			o[e1] = code_of(x1, scale);
 		} else {
-			_Float16 *o = reinterpret_cast<_Float16 *>(is_v ? c.v : c.k);
+			_Float16 *o = reinterpret_cast<_Float16 *>(is_v ? cv : ck);
 			o[e0] = half_of(x0);
 			o[e1] = half_of(x1);
 		}
