@@ -22,8 +22,8 @@
 //
 // A workgroup has a row, or a part of one where there are few rows; the last
 // of a row's parts to finish joins them.  Many rows: bound by memory and the 64-bit arithmetic
-// at once (2047 of 151936 207 us, 6.0 TB/s; 203 with exponentials of F32 arguments); few: by the
-// row's chain of steps (one of 32000 8.9 us, 61 of 151936 22.4, of which the logits 6.4).
+// at once (2047 of 151936 202 to 210 us from card to card, 6.0 TB/s; with exponentials of F32
+// arguments 201 to 204); few: by the row's chain of steps (one of 32000 8.9 us, 61 of 151936 22.4, of which the logits 6.4).
 #include "kv.h"
 
 namespace tie {
@@ -500,9 +500,9 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_kernel(LogprobArgs a, 
 		for (int e = 0; e < LP_E; e++) {
 			// 2^z = 2^n 2^f: w holds n - 1 in its upper 9 bits and f in the lower 23, which are 1 + f's
 			// mantissa; the exponential of that, from 2 on, gets n - 1 added to its exponent.  (Whole
-			// numbers at twice the 64-bit rate: 2047 rows of 151936 207 us, with whole and rest of z by
-			// 64-bit sums 218; 203 without the clamp.  z of -127, -infinity and NaN give 0, z above that and below -126 less
-			// than 2^-126)
+			// numbers at twice the 64-bit rate: 2047 rows of 151936 207 us where whole and rest of z by
+			// 64-bit sums take 218; 203 without the clamp.  z of -127, -infinity and NaN give 0, z above
+			// that and below -126 less than 2^-126)
 			const double y = __builtin_fmax((double)x[e] - m, far);
 			const uint32_t w = (uint32_t)__double_as_longlong(__builtin_fma(y, rate, grid));
 			const float e2 = __builtin_amdgcn_exp2f(__uint_as_float((w & 0x7fffffu) | 0x3f800000u));
